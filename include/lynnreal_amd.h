@@ -323,6 +323,34 @@ int lr_adaln_table(const void* temb, int temb_is_bf16, int apply_silu, const voi
                    const void* bias, void* out, int64_t rows, int64_t in_features,
                    int64_t out_features, void* stream);
 
+/* Rows x [rows, width] (bf16, fp16 or fp32: LR_DTYPE_*) to MXFP4. Each 32
+ * columns (the last block filled up with zeros) share a scale 2^e, e =
+ * max(floor(log2(absmax)) - 2, -127), and hold E2M1 codes of x / 2^e, rounded
+ * to nearest, ties to the even code, saturating at 6. A block with a NaN or an
+ * infinity gets the scale byte 255 (NaN) and codes 0.
+ *   codes  [rows, 16 * ceil(width / 32)], the even column in a byte's low half
+ *   scales [ceil(rows / 64), ceil(width / 256), 512] bytes e + 127: byte
+ *          (16 * (b % 4) + r % 16) * 8 + 2 * (r / 16 % 4) + b / 4 % 2 of tile
+ *          (r / 64, b / 8) is row r, block b. Blocks past the last: 0. Rows past
+ *          the last are left as they were or 0.
+ * codes and scales 16-byte aligned. */
+int lr_quantize_rows_mxfp4(const void* x, int dtype, int64_t rows, int64_t width, void* codes, void* scales,
+                           void* stream);
+
+/* The values that such codes and scales stand for, out [rows, width] of `dtype`:
+ * exact in bf16 and fp32, rounded from fp32 in fp16. out 16-byte aligned. */
+int lr_dequantize_rows_mxfp4(const void* codes, const void* scales, int dtype, int64_t rows, int64_t width,
+                             void* out, void* stream);
+
+/* Product of MXFP4 rows a [m, k] and b [n, k] (codes and scales as above):
+ *   y[i, j] = bf16(sum over blocks, in fp32, + bias[j])
+ * then LR_EPI_BF16 (y), LR_EPI_GELU_TANH or LR_EPI_GATED_RESIDUAL as in
+ * lr_int8_gemm. bias bf16 [n] or NULL; out bf16 [m, n]. k at most 2^23. */
+int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, const void* b_scale, int64_t m, int64_t n,
+                  int64_t k, const void* bias, void* out, int epilogue, const void* residual, const void* table,
+                  int64_t table_rows, int64_t table_width, const int64_t* indices, int64_t sequence,
+                  int gate_slot, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

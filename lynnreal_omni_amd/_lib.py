@@ -63,6 +63,9 @@ SIGNATURES = {
     "lr_flash_restore": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _F32, _P],
     "lr_flash_nearest_anchor": [_P, _I64, _P, _I64, _P, _I64, _P, _P],
     "lr_adaln_table": [_P, _I32, _I32, _P, _P, _P, _I64, _I64, _I64, _P],
+    "lr_quantize_rows_mxfp4": [_P, _I32, _I64, _I64, _P, _P, _P],
+    "lr_dequantize_rows_mxfp4": [_P, _P, _I32, _I64, _I64, _P, _P],
+    "lr_mxfp4_gemm": [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I32, _P, _P, _I64, _I64, _P, _I64, _I32, _P],
     "lr_device_supported": [_I32],
     "lr_abi_version": [],
 }
@@ -144,6 +147,17 @@ def call(name: str, *args) -> None:
     status = fn(*args)
     if status:
         raise_for(status, name)
+
+
+def launch(t: torch.Tensor, name: str, *args) -> None:
+    """call(name, *args, stream) on t's device and the caller's current stream
+    there, whichever device is current: the default stream's handle is the same
+    on every device, so a launch takes the current one."""
+    if t.get_device() == torch.cuda.current_device():
+        call(name, *args, stream(t))
+        return
+    with torch.cuda.device(t.get_device()):
+        call(name, *args, stream(t))
 
 
 _checked_devices: dict[int, bool] = {}

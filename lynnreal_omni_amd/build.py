@@ -50,7 +50,7 @@ def hipcc() -> str:
 # Per-file flags. The GEMM keeps at most 128 accumulators per wave and wants
 # them in VGPRs: with the default heuristic LLVM puts MFMA accumulators in
 # AGPRs and copies them between AGPRs and VGPRs inside the k-loop.
-FILE_FLAGS = {"gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("gemm.hip", "mxfp4_gemm.hip")}
 
 
 def _compile(src: pathlib.Path, extra: list[str]) -> pathlib.Path:

@@ -9,6 +9,8 @@ and never modified.
 Arithmetic (all fp32 with the reference's bf16 rounding points):
   quantize_rows        s = max(absmax, 1e-8)/127; q = clamp(rint(x/s), +-127)
                        (the torch path, model/int8.py:66-67)
+  quantize_rows_mxfp4  2^e and E2M1 codes for each 32 values (new), and
+  dequantize_rows_mxfp4  the values they stand for
   int8_epilogue        bf16((acc*as)*ws + bias)               kernels.py:27-38
   _rms_adaln(_quant)   RMSNorm*gamma -> bf16, *bf16(1+scale) -> bf16,
                        +shift -> bf16 (-> INT8)               kernels.py:48-128
@@ -33,6 +35,7 @@ import torch
 
 from . import _lib
 from .int8_gemm import _ROW_DTYPES as _QUANT_DTYPES
+from .mxfp4_gemm import _operand, code_bytes, scale_shape
 
 
 def _bf16(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -91,6 +94,48 @@ def quantize_rows(value):
         _lib.call("lr_quantize_rows_typed", value.data_ptr(), dtype, rows, width, output.data_ptr(),
                   scales.data_ptr(), _lib.stream(value))
     return output, scales
+
+
+def quantize_rows_mxfp4(value):
+    """MXFP4 of bf16, fp16 or fp32 rows [rows, width]: codes uint8 [rows, 16 *
+    ceil(width / 32)] (two per byte, the even column in the low half) and E8M0
+    scales in the tile order of the matrix instruction (mxfp4_gemm.untile_scales
+    gives them as [rows, blocks]). Scale exponent floor(log2(absmax)) - 2,
+    nearest code with ties to even, saturating; the last block is filled up with
+    zeros; a block with a NaN or an infinity gets the scale byte 255 (NaN)."""
+    if value.dim() != 2:
+        raise ValueError(f"value must be [rows, width], got {tuple(value.shape)}")
+    rows, width = value.shape
+    dtype = _QUANT_DTYPES.get(value.dtype)
+    if dtype is None:
+        raise RuntimeError(f"value: dtype {value.dtype} is not supported by the HIP quantizer")
+    value = value.contiguous()
+    _lib.check_device(value)
+    codes = value.new_empty((rows, code_bytes(width)), dtype=torch.uint8)
+    scales = value.new_empty(scale_shape(rows, width), dtype=torch.uint8)
+    _lib.launch(value, "lr_quantize_rows_mxfp4", value.data_ptr(), dtype, rows, width, codes.data_ptr(),
+                scales.data_ptr())
+    return codes, scales
+
+
+def dequantize_rows_mxfp4(codes, scales, width=None, dtype=torch.bfloat16):
+    """The values [rows, width] that quantize_rows_mxfp4's codes and scales stand
+    for, in bf16 or fp32 (exact) or fp16 (rounded). width defaults to all
+    columns, 32 per block."""
+    _operand(codes, scales, "codes")
+    rows, full = codes.shape[0], 2 * codes.shape[1]
+    width = full if width is None else int(width)
+    if code_bytes(width) != codes.shape[1]:
+        raise ValueError(f"width {width} does not make {codes.shape[1] // 16} blocks")
+    kind = _QUANT_DTYPES.get(dtype)
+    if kind is None:
+        raise RuntimeError(f"dtype {dtype} is not supported by the HIP dequantizer")
+    _lib.check_device(codes)
+    _lib.same_device(codes, scales=scales)
+    out = torch.empty((rows, width), device=codes.device, dtype=dtype)
+    _lib.launch(codes, "lr_dequantize_rows_mxfp4", codes.data_ptr(), scales.data_ptr(), kind, rows, width,
+                out.data_ptr())
+    return out
 
 
 def int8_epilogue(accumulator, activation_scale, weight_scale, bias):

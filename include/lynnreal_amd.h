@@ -351,6 +351,34 @@ int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, const void*
                   int64_t table_rows, int64_t table_width, const int64_t* indices, int64_t sequence,
                   int gate_slot, void* stream);
 
+/* Softmax attention, out = softmax(scale * Q K^T) V, with fp32 scores, maxima,
+ * sums and accumulators; the probabilities are rounded to the inputs' type.
+ *   q, out: `heads` heads; k, v: `kv_heads` heads, which heads / kv_heads query
+ *   heads in a row share; bf16 or fp16 (LR_DTYPE_*), head_dim 32, 64 or 128,
+ *   dense along it. strides, nine numbers in host memory: from one token, head
+ *   and sequence of q to the next in elements, then of k, then of v; multiples of
+ *   8, those between keys and between values below 2^23; pointers 16-byte aligned.
+ *   out is dense: [.., heads, head_dim].
+ * Dense batch (cu_q, cu_k NULL): `sequences` sequences of q_rows tokens and
+ *   k_rows keys; with key_lengths int32 [sequences], sequence i has its first
+ *   key_lengths[i] keys only (what lies behind them is not read).
+ * Packed (cu_q, cu_k int32 [sequences + 1], nondecreasing, on the device):
+ *   sequence i has tokens cu_q[i] .. cu_q[i + 1] - 1 of the q_rows in all, and
+ *   keys cu_k[i] .. of the k_rows; the sequence strides are not used. Rows of no
+ *   sequence become 0. Values are clamped to the rows.
+ * causal: a token sees the keys up to its own place counted from the end, that
+ *   is the last token all keys. A token that sees no key gives 0.
+ * scale_bits: the fp32 bits of the scale, positive and finite.
+ * splits > 1 cuts a sequence's keys for as many workgroups, joined in order by a
+ *   second kernel; needs a workspace of splits * rows * (head_dim + 2) * 4 bytes,
+ *   rows = heads * q_rows (* sequences for a dense batch), 16-byte aligned.
+ *   lr_attention_splits gives the count that fills the GPU. */
+int lr_attention_splits(int64_t sequences, int64_t q_rows, int64_t k_rows, int packed, int heads, int kv_heads);
+int lr_attention(const void* q, const void* k, const void* v, void* out, int dtype, int64_t sequences,
+                 int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int head_dim, const int64_t* strides,
+                 const int32_t* cu_q, const int32_t* cu_k, const int32_t* key_lengths, int causal,
+                 int scale_bits, void* workspace, int64_t workspace_bytes, int splits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

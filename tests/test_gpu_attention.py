@@ -1,0 +1,245 @@
+"""GPU parity of the attention with the formula in 64 bits.
+
+Tolerance. With P the exact softmax row and eps = finfo(dtype).eps / 2 the half
+step of the inputs' type: rounding each weight to the type moves the output by at
+most eps * sum P |v|; the fp32 scores (D + 2 additions and products, each off by
+at most 2^-23 of sum |q k| * scale where the matrix unit truncates) and the
+exponential (an error of 2^-22 and, through its argument, the score's) move a
+weight by the factor 2 * ds + 2^-21 with ds = (D + 2) * 2^-23 * scale * sum |q k|;
+the sums over the keys, of weights and of weighted values, add at most 2^-24 and
+2^-23 per key; and the output is rounded once: eps * |o|.
+fp16 weights are kept as fractions of at least 2^-31 of a row's largest, below
+which they round by 2^-32 of it at most: that much times sum |v|.
+"""
+import math
+
+import pytest
+import torch
+
+from lynnreal_omni_amd import _lib
+from lynnreal_omni_amd import attention as A
+
+pytestmark = pytest.mark.gpu
+
+
+def formula(q, k, v, scale, seen):
+    """float64 [heads, rows, dim] outputs and their bounds; seen: bool [rows, keys]."""
+    dtype = q.dtype
+    group = q.shape[1] // k.shape[1]
+    q, k, v = (t.double().cpu().transpose(0, 1) for t in (q, k, v))
+    k, v = k.repeat_interleave(group, 0), v.repeat_interleave(group, 0)
+    s = q @ k.transpose(1, 2) * scale
+    size = (q.abs() @ k.abs().transpose(1, 2) * scale)
+    s = s.masked_fill(~seen, -math.inf)
+    m = s.amax(-1, keepdim=True) if s.shape[-1] else s.new_full((*s.shape[:2], 1), -math.inf)
+    p = torch.where(seen, torch.exp(s - m.clamp_min(-1e300)), 0.0)
+    total = p.sum(-1, keepdim=True)
+    p = torch.where(total > 0, p / total.clamp_min(1e-300), 0.0)
+    eps = torch.finfo(dtype).eps / 2
+    ds = (q.shape[-1] + 2) * 2.0 ** -23 * torch.where(seen, size, 0.0).amax(-1, keepdim=True) if s.shape[-1] else 0.0
+    o = p @ v
+    pv = p @ v.abs()
+    bound = eps * o.abs() + (eps + 2 * ds + 2.0 ** -21 + 3 * 2.0 ** -24 * s.shape[-1]) * pv * 1.01
+    # fp16 weights far below the largest, and outputs below the normal numbers.
+    bound = bound + 2.0 ** -32 * (seen.double() @ v.abs()) + torch.finfo(dtype).smallest_normal * eps
+    return o.transpose(0, 1), bound.transpose(0, 1)
+
+
+def check(got, o, bound):
+    off = (got.double().cpu() - o).abs() - bound
+    assert not got.isnan().any()
+    assert off.numel() == 0 or off.max() <= 0, f"off by {off.max()} past the bound of {bound.flatten()[off.argmax()]}"
+
+
+def tensors(n_q, n_k, heads, kv_heads, dim, dtype, seed, scale=1.5):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(n_q, heads, dim, generator=g) * scale
+    k, v = (torch.randn(n_k, kv_heads, dim, generator=g) for _ in range(2))
+    return tuple(t.to(dtype).cuda() for t in (q, k, v))
+
+
+def mask(rows, keys, causal):
+    seen = torch.ones(rows, keys, dtype=torch.bool)
+    return seen.tril(keys - rows) if causal else seen
+
+
+CASES = [(1, 1, 1, 1, 32), (1, 1, 4, 2, 64), (1, 2, 2, 1, 128), (5, 5, 3, 3, 64), (31, 33, 2, 2, 128),
+         (64, 64, 2, 2, 32), (65, 63, 4, 2, 64), (130, 257, 2, 1, 128), (200, 40, 2, 2, 128), (7, 1000, 6, 2, 64),
+         (1, 4097, 8, 2, 128), (2, 700, 7, 1, 128), (300, 300, 1, 1, 32), (513, 513, 2, 2, 128), (3, 0, 2, 2, 64),
+         (33, 2500, 14, 2, 32), (257, 1025, 3, 1, 64)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("rows,keys,heads,kv_heads,dim", CASES)
+def test_one_sequence(rows, keys, heads, kv_heads, dim, causal, dtype):
+    q, k, v = tensors(rows, keys, heads, kv_heads, dim, dtype, rows + keys)
+    got = A.attention(q[None], k[None], v[None], causal=causal)
+    check(got[0], *formula(q, k, v, dim ** -0.5, mask(rows, keys, causal)))
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 20.0])
+def test_scales(scale):
+    """From a nearly flat softmax to one that a single key takes."""
+    q, k, v = tensors(70, 300, 2, 2, 64, torch.bfloat16, 3)
+    check(A.attention(q[None], k[None], v[None], scale=scale)[0], *formula(q, k, v, scale, mask(70, 300, False)))
+
+
+def test_growing_maximum():
+    """Scores that rise from tile to tile, so that the running maximum moves often."""
+    q, k, v = tensors(64, 1024, 2, 2, 64, torch.bfloat16, 4)
+    k = (k * torch.linspace(0.1, 6, 1024, device="cuda")[:, None, None]).bfloat16()
+    for keys in (k, k.flip(0)):
+        keys = keys.contiguous()
+        check(A.attention(q[None], keys[None], v[None])[0], *formula(q, keys, v, 64 ** -0.5, mask(64, 1024, False)))
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_views_of_a_fused_projection(dim):
+    g = torch.Generator().manual_seed(dim)
+    fused = torch.randn(2, 150, (6 + 2 * 2) * dim, generator=g).bfloat16().cuda()
+    q, k, v = (t.unflatten(-1, (-1, dim)) for t in fused.split([6 * dim, 2 * dim, 2 * dim], -1))
+    got = A.attention(q, k, v, causal=True)
+    for b in range(2):
+        check(got[b], *formula(q[b], k[b], v[b], dim ** -0.5, mask(150, 150, True)))
+    heads_first = q.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(A.attention(heads_first, k, v, causal=True), got)
+    odd = torch.zeros(2, 150, 6, dim + 1, dtype=torch.bfloat16, device="cuda")[..., :dim].copy_(q)
+    assert torch.equal(A.attention(odd, k, v, causal=True), got)
+
+
+LENGTHS = [[5], [0, 3, 0], [1, 1, 1, 1], [64, 128, 1, 63, 65], [300, 0, 17, 129], [33] * 9, [700, 2]]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths", LENGTHS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (3, 3, 128), (5, 1, 32)])
+def test_packed(lengths, heads, kv_heads, dim, causal, dtype):
+    """Sequences behind each other, with rows before the first and behind the last,
+    and NaN in the rows of no sequence."""
+    before, after = 3, 70
+    total = sum(lengths) + before + after
+    q, k, v = tensors(total, total, heads, kv_heads, dim, dtype, total)
+    cu = (torch.tensor([0] + lengths).cumsum(0) + before)
+    for t in (k, v):
+        t[:before], t[total - after:] = float("nan"), float("inf")
+    got = A.attention_packed(q, k, v, cu.cuda(), causal=causal)
+    assert (got[:before] == 0).all() and (got[total - after:] == 0).all()
+    for a, b in zip(cu.tolist(), cu.tolist()[1:]):
+        check(got[a:b], *formula(q[a:b], k[a:b], v[a:b], dim ** -0.5, mask(b - a, b - a, causal)))
+    # The sequences alone: the same bits, whatever lies around them.
+    alone = A.attention_packed(*(t[before:total - after].contiguous() for t in (q, k, v)),
+                               (cu - before).to(torch.int32).cuda(), causal=causal)
+    assert torch.equal(alone, got[before:total - after])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_with_other_keys(causal):
+    """A few new tokens per sequence over longer, shorter and missing keys."""
+    q_len, k_len = [1, 4, 3, 0, 2], [700, 2, 0, 9, 300]
+    q, _, _ = tensors(sum(q_len), 1, 8, 2, 128, torch.bfloat16, 1)
+    _, k, v = tensors(1, sum(k_len), 8, 2, 128, torch.bfloat16, 2)
+    cu = [torch.tensor([0] + x, device="cuda").cumsum(0) for x in (q_len, k_len)]
+    got = A.attention_packed(q, k, v, *cu, causal=causal)
+    a = b = 0
+    for x, y in zip(q_len, k_len):
+        check(got[a:a + x], *formula(q[a:a + x], k[b:b + y], v[b:b + y], 128 ** -0.5, mask(x, y, causal)))
+        a, b = a + x, b + y
+
+
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 64), (8, 2, 128), (7, 1, 128), (64, 1, 32)])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_cache(new, heads, kv_heads, dim, kind):
+    """New tokens over padded caches: NaN behind the valid keys is not read."""
+    lengths, size = [1, 64, 999, 130, 0, 2000], 2000
+    g = torch.Generator().manual_seed(heads)
+    q = (torch.randn(6, new, heads, dim, generator=g) * 1.5).half().cuda()
+    k, v = (torch.randn(6, size, kv_heads, dim, generator=g).half().cuda() for _ in range(2))
+    for i, n in enumerate(lengths):
+        k[i, n:], v[i, n:] = float("nan"), float("inf")
+    given = torch.tensor(lengths, device="cuda", dtype=kind)
+    for causal in (True, False):
+        got = A.attention(q, k, v, causal=causal, key_lengths=given)
+        for i, n in enumerate(lengths):
+            check(got[i], *formula(q[i], k[i, :n], v[i, :n], dim ** -0.5, mask(new, n, causal)))
+    far = torch.tensor([2 ** 40 if kind == torch.int64 else 2 ** 31 - 1] * 5 + [-5], device="cuda", dtype=kind)
+    k.nan_to_num_(0.0), v.nan_to_num_(0.0, 0.0, 0.0)
+    got = A.attention(q, k, v, key_lengths=far)
+    assert torch.equal(got[:5], A.attention(q[:5], k[:5], v[:5], key_lengths=torch.full_like(far[:5], size)))
+    assert (got[5] == 0).all()
+
+
+def test_masked_scores_may_be_anything():
+    """NaN and infinite keys after a token's own place do not reach it."""
+    q, k, v = tensors(100, 100, 2, 2, 64, torch.bfloat16, 9)
+    want = A.attention(q[None], k[None], v[None], causal=True)
+    k[60:80], k[80:] = float("nan"), float("inf")
+    got = A.attention(q[None], k[None], v[None], causal=True)
+    assert torch.equal(got[:, :60], want[:, :60])
+    assert got[:, 60:].isnan().all()
+
+
+def test_lists_that_lead_outside_are_clamped():
+    q, k, v = tensors(40, 40, 2, 2, 64, torch.bfloat16, 6)
+    cu = torch.tensor([0, 10, 40], device="cuda", dtype=torch.int32)
+    want = A.attention_packed(q, k, v, cu)
+    assert torch.equal(A.attention_packed(q, k, v, torch.tensor([-7, 10, 4000], device="cuda")), want)
+
+
+def test_long_rows_of_a_cache_past_32_bits():
+    """Keys whose offsets pass 2^31 bytes, through the batch and the token stride."""
+    size, heads, dim = 1 << 18, 8, 128
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k = torch.randn(5, size, heads, dim, device="cuda", generator=g, dtype=torch.bfloat16)
+    v = torch.randn(5, size, heads, dim, device="cuda", generator=g, dtype=torch.bfloat16)
+    q = torch.randn(5, 1, heads, dim, device="cuda", generator=g, dtype=torch.bfloat16)
+    n = torch.full((5,), 300, device="cuda", dtype=torch.int32)
+    got = A.attention(q, k, v, key_lengths=n)
+    check(got[4], *formula(q[4], k[4, :300], v[4, :300], dim ** -0.5, mask(1, 300, False)))
+    one = A.attention(q[4:], k[4:], v[4:])[0]
+    check(one[:, 7:], *formula(q[4, :, 7:], k[4, :, 7:], v[4, :, 7:], dim ** -0.5, mask(1, size, False)))
+
+
+def test_streams_and_graphs():
+    """Split keys on two streams at once; two captured calls, replayed between eager ones."""
+    q, k, v = tensors(2, 5000, 8, 2, 128, torch.bfloat16, 8)
+    q2, k2, v2 = tensors(2, 5000, 8, 2, 128, torch.bfloat16, 18)
+    ins = [[t[None].clone() for t in x] for x in ((q, k, v), (q2, k2, v2))]
+    assert _lib.load().lr_attention_splits(1, 2, 5000, 0, 8, 2) > 1
+    want = [A.attention(*x) for x in ins]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    here, there = [], []
+    for _ in range(20):
+        here.append(A.attention(*ins[0]))
+        with torch.cuda.stream(side):
+            there.append(A.attention(*ins[1]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[0]) for x in here) and all(torch.equal(x, want[1]) for x in there)
+    graphs, outs, live = [], [], [[t.clone() for t in x] for x in ins]
+    for x in live:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(A.attention(*x))
+        graphs.append(g)
+    for turn in range(3):
+        for i in range(2):
+            for t, u in zip(live[i], ins[(i + turn) % 2]):
+                t.copy_(u)
+        for g in graphs:
+            g.replay()
+        A.attention(*ins[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[(i + turn) % 2]) for i in range(2))
+
+
+def test_empty_calls():
+    q, k, v = tensors(4, 4, 2, 2, 64, torch.bfloat16, 1)
+    assert A.attention(q[None, :0], k[None], v[None]).shape == (1, 0, 2, 64)
+    assert A.attention(q[None][:0], k[None][:0], v[None][:0]).shape == (0, 4, 2, 64)
+    assert (A.attention(q[None], k[None, :0], v[None, :0]) == 0).all()
+    none = torch.zeros(1, device="cuda", dtype=torch.int32)
+    assert (A.attention_packed(q, k, v, none) == 0).all()
+    assert A.attention_packed(q[:0], k[:0], v[:0], none).shape == (0, 2, 64)

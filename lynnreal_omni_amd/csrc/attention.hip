@@ -20,6 +20,8 @@
 // the multiplication of o.
 #include <math.h>
 
+#include <type_traits>
+
 #include "lr_device.h"
 #include "lr_runtime.h"
 
@@ -71,6 +73,7 @@ __device__ __forceinline__ int64_t first_row(const AttnArgs& p, int64_t i) {
 template <typename T> struct Mfma;
 template <> struct Mfma<__bf16> {
   typedef v8bf V;
+  static constexpr float kShift = 0.0f;
   static __device__ __forceinline__ v16f mul(const V& a, const V& b, const v16f& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -78,6 +81,8 @@ template <> struct Mfma<__bf16> {
 };
 template <> struct Mfma<_Float16> {
   typedef v8h V;
+  // p is kept 2^7 larger: its subnormals then begin at 2^-31 of a row's largest.
+  static constexpr float kShift = 7.0f;
   static __device__ __forceinline__ v16f mul(const V& a, const V& b, const v16f& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -104,42 +109,40 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, void* lds, ui
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)lds, 16, voffset, 0, 0, 0);
 }
 
-constexpr int kKeys = 64;        // keys per tile
+template <typename V8>
+__device__ __forceinline__ V8 tr_pair(const char* a0, const char* a1) {
+  const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t)a0);
+  const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t)a1);
+  return __builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+constexpr int kKeys = 64;        // keys per tile of a prompt
 constexpr float kSlack = 8.0f;   // log2
 
-// Rows of a workgroup: 32 * QB per wave. Keys in tiles of 64 through a ring of S
-// slots in LDS (K rows, then V rows), by 16-byte DMA. A row's 16-byte chunk c lies
-// in slot c ^ 2 * (row / (256 / row bytes) % (row bytes / 32)): eight rows' equal
-// 32-byte columns are on distinct banks, which is what both reads need.
-template <typename T, int D, int QB, int WAVES, int S>
-__global__ __launch_bounds__(64 * WAVES, 1) void attention(AttnArgs p) {
-  typedef typename Mfma<T>::V V8;
-  constexpr int BM = 32 * QB * WAVES;
-  constexpr int ROW = 2 * D;                     // bytes of a row
-  constexpr int CH = ROW / 16;                   // chunks per row
-  constexpr int RPB = 256 / ROW, PAIRS = ROW / 32;
-  constexpr int TILE = kKeys * ROW, SLOT = 2 * TILE;
-  constexpr int DMAS = TILE / 1024 / WAVES;      // per wave, operand and tile
-  constexpr int KD = D / 16, DB = D / 32;
-  static_assert(TILE / 1024 % WAVES == 0, "DMA split");
-  __shared__ __attribute__((aligned(1024))) char smem[S * SLOT];
-  // fp16 p is kept 2^7 larger: its subnormals then begin at 2^-31 of a row's largest.
-  constexpr float kShift = __is_same(T, _Float16) ? 7.0f : 0.0f;
+// What a workgroup works on: its split, sequence, rows [r0, r0 + BM) of the
+// sequence's (row r: token r / pack, head hd * pack + r % pack), and key tiles.
+struct Item {
+  Seq s;
+  int64_t rows, r0;
+  int split, hd, kv_head;
+  int sure;     // keys that every row of the workgroup sees
+  int t0, t1;   // its tiles of KEYS keys
+};
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int half = lane >> 5, col = lane & 31;
+template <int BM, int KEYS>
+__device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
   // Tiles of a head lie together, and each XCD (workgroups are dealt to them in
   // turn) takes a contiguous run, so that its L2 serves a head's keys once.
   const int64_t total = p.tiles * (p.heads / p.pack) * p.splits;
   const int64_t pid = blockIdx.x;
   const int64_t per = total >> 3, rest = total & 7, xcd = pid & 7;
   const int64_t lid = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3);
-  const int split = (int)(lid % p.splits);
+  it.split = (int)(lid % p.splits);
   int64_t tile = lid / p.splits % p.tiles;
-  const int hd = (int)(lid / p.splits / p.tiles);   // head, or key head where heads share rows
-  const int kv_head = p.pack > 1 ? hd : hd / p.group;
-
+  it.hd = (int)(lid / p.splits / p.tiles);   // head, or key head where heads share rows
+  it.kv_head = p.pack > 1 ? it.hd : it.hd / p.group;
   Seq s = {};
+  int64_t tiles;   // of the sequence
   if (p.cu_q) {
     // Sequence i has the tile slots from first_row(i) * pack / BM + i on: at least
     // as many as its rows need, and its own.
@@ -153,54 +156,148 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention(AttnArgs p) {
     s.q0 = first_row(p, lo);
     s.qn = (int)clamp64(first_row(p, lo + 1) - s.q0, 0, p.q_rows);
     tile = slot - (s.q0 * p.pack / BM + lo);
+    tiles = ((int64_t)s.qn * p.pack + BM - 1) / BM;
     if (lo > 0 && lo <= p.n) {
       s.k0 = clamp64(p.cu_k[lo - 1], 0, p.k_rows);
       s.kn = (int)clamp64(clamp64(p.cu_k[lo], 0, p.k_rows) - s.k0, 0, p.k_rows);
     }
+    if (tile >= tiles) return false;
   } else {
-    const int64_t per_seq = p.tiles / p.n;
-    s.b = tile / per_seq;
-    tile -= s.b * per_seq;
+    tiles = p.tiles / p.n;
+    s.b = tile / tiles;
+    tile -= s.b * tiles;
     s.qn = (int)p.q_rows;
     s.kn = (int)(p.lengths ? clamp64(p.lengths[s.b], 0, p.k_rows) : p.k_rows);
-    // Causal: the last tiles see the most keys and go first.
-    if (p.causal) tile = per_seq - 1 - tile;
   }
-  const int64_t rows = (int64_t)s.qn * p.pack;
-  const int64_t r0 = tile * BM;
-  if (r0 >= rows) return;
-
-  // This wave's query rows: row r is token r / pack, head hd * pack + r % pack.
-  int tok[QB], head[QB];
-  int64_t qoff[QB];
-  int limit[QB];  // keys that the row sees
-#pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    const int64_t r = r0 + wave * 32 * QB + 32 * b + col;
-    const int64_t rc = r < rows ? r : rows - 1;
-    tok[b] = (int)(p.pack == 1 ? rc : rc / p.pack);
-    head[b] = p.pack == 1 ? hd : hd * p.pack + (int)(rc - (int64_t)tok[b] * p.pack);
-    qoff[b] = s.b * p.qb + (s.q0 + tok[b]) * p.qt + head[b] * p.qh;
-    limit[b] = p.causal ? min(s.kn, max(0, s.kn - s.qn + tok[b] + 1)) : s.kn;
-  }
-  V8 q[QB][KD];
-#pragma unroll
-  for (int b = 0; b < QB; ++b)
-#pragma unroll
-    for (int d = 0; d < KD; ++d)
-      q[b][d] = *reinterpret_cast<const V8*>(p.q + qoff[b] + 16 * d + 8 * half);
-
-  // Key tiles [t0, t1) of this split; the last one that any row of the workgroup sees.
-  const int64_t last = r0 + BM <= rows ? r0 + BM - 1 : rows - 1;
+  // Causal: the last tiles see the most keys and go first.
+  if (p.causal) tile = tiles - 1 - tile;
+  it.s = s;
+  it.rows = (int64_t)s.qn * p.pack;
+  it.r0 = tile * BM;
+  const int64_t last = it.r0 + BM <= it.rows ? it.r0 + BM - 1 : it.rows - 1;
   const int last_tok = (int)(p.pack == 1 ? last : last / p.pack);
-  const int first_tok = (int)(p.pack == 1 ? r0 : r0 / p.pack);
+  const int first_tok = (int)(p.pack == 1 ? it.r0 : it.r0 / p.pack);
   const int seen = p.causal ? min(s.kn, max(0, s.kn - s.qn + last_tok + 1)) : s.kn;
-  const int sure = p.causal ? min(s.kn, max(0, s.kn - s.qn + first_tok + 1)) : s.kn;  // seen by every row
-  const int tiles_k = (seen + kKeys - 1) / kKeys;
-  const int t0 = (int)((int64_t)tiles_k * split / p.splits), t1 = (int)((int64_t)tiles_k * (split + 1) / p.splits);
+  it.sure = p.causal ? min(s.kn, max(0, s.kn - s.qn + first_tok + 1)) : s.kn;
+  const int tiles_k = (seen + KEYS - 1) / KEYS;
+  it.t0 = (int)((int64_t)tiles_k * it.split / p.splits);
+  it.t1 = (int)((int64_t)tiles_k * (it.split + 1) / p.splits);
+  return true;
+}
 
-  const uint16_t* const kbase = p.k + s.b * p.kb + s.k0 * p.kt + kv_head * p.kh;
-  const uint16_t* const vbase = p.v + s.b * p.vb + s.k0 * p.vt + kv_head * p.vh;
+// The query row of a lane (column `col` of a wave's 32 rows from `r` on).
+struct QueryRow {
+  int64_t r, off;   // off: of its first element in q
+  int tok, head, limit;   // limit: keys that it sees
+  __device__ __forceinline__ QueryRow(const AttnArgs& p, const Item& it, int64_t row) : r(row) {
+    const int64_t rc = row < it.rows ? row : it.rows - 1;
+    tok = (int)(p.pack == 1 ? rc : rc / p.pack);
+    head = p.pack == 1 ? it.hd : it.hd * p.pack + (int)(rc - (int64_t)tok * p.pack);
+    off = it.s.b * p.qb + (it.s.q0 + tok) * p.qt + head * p.qh;
+    limit = p.causal ? min(it.s.kn, max(0, it.s.kn - it.s.qn + tok + 1)) : it.s.kn;
+  }
+};
+
+// Moves m to the new maximum x where some row of the wave exceeds it by more than
+// the slack (or has its first key); returns what the exponent subtracts.
+template <int DB>
+__device__ __forceinline__ float move_max(float x, float& m, float& l, v16f (&o)[DB], float c, float shift) {
+  if (__any((x - m) * c > kSlack || (m == -INFINITY && x > -INFINITY))) {
+    const float mn = fmaxf(m, x);
+    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+  }
+  return m == -INFINITY ? 0.0f : m * c - shift;
+}
+
+// o / l, or a split's o, m and l; lane holds columns 32 * d + 8 * g + 4 * half + 0..3 of its row.
+template <typename T, int D>
+__device__ __forceinline__ void store_row(const AttnArgs& p, const Item& it, const QueryRow& qr, float m, float l,
+                                          const v16f (&o)[D / 32], int half) {
+  const float sum = add_partner(l);
+  if (qr.r >= it.rows) return;
+  const int64_t row = (it.s.b * p.q_rows + it.s.q0 + qr.tok) * p.heads + qr.head;
+  if (p.splits > 1) {
+    const int64_t all = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;
+    float* const po = p.part + (it.split * all + row) * D;
+    float* const ml = p.part + (int64_t)p.splits * all * D + (it.split * all + row) * 2;
+    if (half == 0) {
+      ml[0] = m;
+      ml[1] = sum;
+    }
+    if (sum == 0.0f) return;   // without keys of this row: left out of the join by its l
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(po + 32 * d + 8 * g + 4 * half) =
+            make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    return;
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint16_t* const po = p.out + row * D;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<uint2*>(po + 32 * d + 8 * g + 4 * half) =
+          make_uint2(Mfma<T>::pack(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
+                     Mfma<T>::pack(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+}
+
+// ------------------------------------------------------------- prompts ----
+// Four waves of 32 rows; keys in tiles of 64 through two slots of LDS (K rows,
+// then V rows), by 16-byte DMA. A row's 16-byte chunk c lies in slot c ^ 2 * (row
+// / (256 / row bytes) % (row bytes / 32)): eight rows' equal 32-byte columns are
+// on distinct banks, which is what both reads need.
+//
+// A trip computes the scores of tile t + 1 while those of tile t become
+// probabilities, then the second product of tile t while the maxima of tile t + 1
+// form: the matrix instructions of each phase are independent of its vector work.
+// The compiler would move the exponentials behind the first product (the fences
+// and the empty asm keep them between its instructions). Two workgroups share a
+// CU (256 registers, 64 KB), so that one wave's vector phase runs under the
+// other's matrix phase; the second product's priority is raised.
+// Measured, 56 heads of 128, 12605 tokens, bf16: without the pipeline and with one
+// wave per SIMD 6.5 ms; two waves per SIMD 4.42; pipelined 4.25; two tiles per
+// trip (no copies of the scores, constant LDS slots) and the priority 4.10-4.14
+// ms, 1100-1110 TFLOP/s. There the clock is down to 1.69 GHz and the matrix units
+// are 62% busy: the chip's power is the bound, as for a large bf16 matrix product
+// (1505 TFLOP/s on the same card). 64 rows per wave and one wave per SIMD halves
+// the LDS reads and was slower (869 against 734 us on 8 heads), reading V by asm
+// blocks with their waits too (4.32 ms), sums by a dot product with ones level.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
+  typedef typename Mfma<T>::V V8;
+  constexpr int BM = 128, WAVES = 4;
+  constexpr int ROW = 2 * D;                     // bytes of a row
+  constexpr int CH = ROW / 16;                   // chunks per row
+  constexpr int RPB = 256 / ROW, PAIRS = ROW / 32;
+  constexpr int TILE = kKeys * ROW, SLOT = 2 * TILE;
+  constexpr int DMAS = TILE / 1024 / WAVES;      // per wave, operand and tile
+  constexpr int KD = D / 16, DB = D / 32;
+  static_assert(TILE / 1024 % WAVES == 0, "DMA split");
+  __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
+  constexpr float kShift = Mfma<T>::kShift;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, col = lane & 31;
+  Item it;
+  if (!find_item<BM, kKeys>(p, it)) return;
+  const Seq s = it.s;
+  const int t0 = it.t0, t1 = it.t1;
+  const QueryRow qr(p, it, it.r0 + wave * 32 + col);
+  V8 q[KD];
+#pragma unroll
+  for (int d = 0; d < KD; ++d) q[d] = *reinterpret_cast<const V8*>(p.q + qr.off + 16 * d + 8 * half);
+
+  const uint16_t* const kbase = p.k + s.b * p.kb + s.k0 * p.kt + it.kv_head * p.kh;
+  const uint16_t* const vbase = p.v + s.b * p.vb + s.k0 * p.vt + it.kv_head * p.vh;
   // DMA i of this wave: 1 KB of the tile's rows.
   uint32_t koff[DMAS], voff[DMAS];
 #pragma unroll
@@ -210,193 +307,320 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention(AttnArgs p) {
     koff[i] = (uint32_t)(row * p.kt * 2 + c * 16);
     voff[i] = (uint32_t)(row * p.vt * 2 + c * 16);
   }
-  auto issue = [&](int t) {
+  auto issue = [&](int t, int v) {
     if (t >= t1) return;
-    char* const slot = smem + t % S * SLOT;
+    char* const slot = smem + ((t - t0) & 1) * SLOT + v * TILE;
     const int left = min(kKeys, s.kn - t * kKeys);  // rows past the sequence's keys read as zero
-    const __amdgpu_buffer_rsrc_t rk =
-        row_rsrc(kbase + (int64_t)t * kKeys * p.kt, ((int64_t)(left - 1) * p.kt + D) * 2);
-    const __amdgpu_buffer_rsrc_t rv =
-        row_rsrc(vbase + (int64_t)t * kKeys * p.vt, ((int64_t)(left - 1) * p.vt + D) * 2);
+    const int64_t stride = v ? p.vt : p.kt;
+    const __amdgpu_buffer_rsrc_t r =
+        row_rsrc((v ? vbase : kbase) + (int64_t)t * kKeys * stride, ((int64_t)(left - 1) * stride + D) * 2);
 #pragma unroll
-    for (int i = 0; i < DMAS; ++i)
-      dma16(rk, slot + (wave * DMAS + i) * 1024, koff[i]);
-#pragma unroll
-    for (int i = 0; i < DMAS; ++i)
-      dma16(rv, slot + TILE + (wave * DMAS + i) * 1024, voff[i]);
+    for (int i = 0; i < DMAS; ++i) dma16(r, slot + (wave * DMAS + i) * 1024, v ? voff[i] : koff[i]);
   };
 
-  v16f o[QB][DB];
-  float m[QB], l[QB];
+  v16f o[DB], s0[2], s1[2];
+  float m = -INFINITY, l = 0.0f, mx, off;
+  uint32_t pk[4][4];
 #pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    m[b] = -INFINITY;
-    l[b] = 0.0f;
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  // Fragment reads. K: d = g / 2, rows 32 * (g % 2) + col, columns 16 * d + 8 *
+  // half. V^T: 16 keys kc = g / DB, column 32 * (g % DB) + col, keys 16 * kc + 4 *
+  // half + (0..3, 8..11).
+  const int krow = col * ROW, kswz = (col / RPB % PAIRS) * 2;
+  auto kfrag = [&](const char* ks, int g) -> V8 {
+    return *reinterpret_cast<const V8*>(ks + (g & 1) * 32 * ROW + krow + ((2 * (g >> 1) + half) ^ kswz) * 16);
+  };
+  const int i16 = lane & 15;
+  const int vr = 4 * half + (i16 >> 2);
+  auto vfrag = [&](const char* vs, int g) -> V8 {
+    const int kc = g / DB, d = g % DB;
+    const int c = 4 * d + 2 * ((lane >> 4) & 1) + (i16 >> 1 & 1);
+    const int sub = (i16 & 1) * 8;
+    return tr_pair<V8>(vs + (16 * kc + vr) * ROW + (c ^ (vr / RPB % PAIRS) * 2) * 16 + sub,
+                       vs + (16 * kc + 8 + vr) * ROW + (c ^ ((vr + 8) / RPB % PAIRS) * 2) * 16 + sub);
+  };
+  constexpr int NQ = 2 * KD, NV = 4 * DB;   // matrix instructions of the two products
+  constexpr int NP = 16, NP1 = 12;          // pairs of keys per lane; those under the first product
+  auto pair = [&](v16f (&sc)[2], int j) {
+    const int kc = j >> 2, w = j & 3, e = (kc & 1) * 8 + 2 * w;
+    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kc >> 1][e], p.c, -off));
+    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kc >> 1][e + 1], p.c, -off));
+    l += p0 + p1;
+    pk[kc][w] = Mfma<T>::pack(p0, p1);
+    asm volatile("" : "+v"(pk[kc][w]), "+v"(l));
+  };
+  auto masked = [&](v16f (&nx)[2], int t) {
+    if ((t + 1) * kKeys <= it.sure) return;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[b][d][e] = 0.0f;
-  }
-
-  issue(t0);
-#pragma unroll 1
-  for (int t = t0; t < t1; ++t) {
-    __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);  // vmcnt(0): tile t has landed
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = t * kKeys + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3);
+        nx[kb][e] = key < qr.limit ? nx[kb][e] : -INFINITY;
+      }
+  };
+  auto score = [&](v16f (&nx)[2], const V8& kf, int g) {
+    if (g < 2) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) nx[g][e] = 0.0f;
+    }
+    nx[g & 1] = Mfma<T>::mul(kf, q[g >> 1], nx[g & 1]);
+  };
+  // Publishes what every wave's DMAs have fetched, and frees the slots that they
+  // go to next: behind it every wave is done with tile t - 1.
+  auto publish = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);  // vmcnt(0)
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    issue(t + 1);  // into the slot that every wave left before the barrier
-    const char* const ks = smem + t % S * SLOT;
-    const char* const vs = ks + TILE;
-    v16f sc[QB][2];
+  };
+  // Tile t, in slot `par`, with the scores sc; those of tile t + 1 go to nx.
+  auto body = [&](v16f (&sc)[2], v16f (&nx)[2], int t, const int par, auto has_next) {
+    constexpr bool NEXT = decltype(has_next)::value;
+    const char* const ks = smem + (par ^ 1) * SLOT;
+    const char* const vs = smem + par * SLOT + TILE;
+    V8 kf[4], vf[4];
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (NEXT) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+      for (int g = 0; g < 3; ++g) kf[g] = kfrag(ks, g);
 #pragma unroll
-      for (int b = 0; b < QB; ++b)
+      for (int g = 0; g < NQ; ++g) {
+        if (g + 3 < NQ) kf[(g + 3) & 3] = kfrag(ks, g + 3);
+        else vf[(g + 3 - NQ) & 3] = vfrag(vs, g + 3 - NQ);
+        score(nx, kf[g & 3], g);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[b][kb][e] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < KD; ++d) {
-        const int row = 32 * kb + col;
-        const V8 kf = *reinterpret_cast<const V8*>(ks + row * ROW +
-                                                   ((2 * d + half) ^ (row / RPB % PAIRS) * 2) * 16);
-#pragma unroll
-        for (int b = 0; b < QB; ++b) sc[b][kb] = Mfma<T>::mul(kf, q[b][d], sc[b][kb]);
+        for (int j = 0; j < NP1; ++j)
+          if (j * NQ / NP1 == g) pair(sc, j);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      masked(nx, t + 1);
+      mx = -INFINITY;
+    } else {
+#pragma unroll
+      for (int g = 0; g < 3; ++g) vf[g] = vfrag(vs, g);
+#pragma unroll
+      for (int j = 0; j < NP1; ++j) pair(sc, j);
     }
-    if ((t + 1) * kKeys > sure) {
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int b = 0; b < QB; ++b)
+    for (int g = 0; g < NV; ++g) {
+      const int kc = g / DB;
+      if (g + 3 < NV) vf[(g + 3) & 3] = vfrag(vs, g + 3);
+      const uint4 pw = make_uint4(pk[kc][0], pk[kc][1], pk[kc][2], pk[kc][3]);
+      o[g % DB] = Mfma<T>::mul(vf[g & 3], __builtin_bit_cast(V8, pw), o[g % DB]);
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+      for (int j = NP1; j < NP; ++j)
+        if ((j - NP1) * (NV / 2) / (NP - NP1) == g) pair(sc, j);
+      if constexpr (NEXT) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = t * kKeys + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3);
-            sc[b][kb][e] = key < limit[b] ? sc[b][kb][e] : -INFINITY;
-          }
-    }
-    uint32_t pk[QB][2][8];
-#pragma unroll
-    for (int b = 0; b < QB; ++b) {
-      float mx = fmaxf(sc[b][0][0], sc[b][1][0]);
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(sc[b][0][e], sc[b][1][e]));
-      mx = max_with_partner(mx);
-      if (__any((mx - m[b]) * p.c > kSlack || (m[b] == -INFINITY && mx > -INFINITY))) {
-        const float mn = fmaxf(m[b], mx);
-        const float alpha = m[b] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[b] - mn) * p.c);
-        m[b] = mn;
-        l[b] *= alpha;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[b][d][e] *= alpha;
+        for (int j = 0; j < 16; ++j)
+          if (j * NV / 16 == g) mx = fmaxf(fmaxf(mx, nx[j >> 3][2 * j & 15]), nx[j >> 3][(2 * j & 15) + 1]);
       }
-      const float off = m[b] == -INFINITY ? 0.0f : m[b] * p.c - kShift;
-      float sum = 0.0f;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][kb][e], p.c, -off));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][kb][e + 1], p.c, -off));
-          sum += p0 + p1;
-          pk[b][kb][e >> 1] = Mfma<T>::pack(p0, p1);
-        }
-      l[b] += sum;
+      __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int kc = 0; kc < 4; ++kc) {  // 16 keys
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        // Lane's column 32 * d + col; its keys 16 * kc + 4 * half + (0..3, 8..11).
-        const int i16 = lane & 15;
-        const int row = 16 * kc + 4 * half + (i16 >> 2);
-        const int c = 4 * d + 2 * ((lane >> 4) & 1) + (i16 >> 1 & 1);
-        const int sub = (i16 & 1) * 8;
-        const char* const a0 = vs + row * ROW + (c ^ (row / RPB % PAIRS) * 2) * 16 + sub;
-        const char* const a1 = vs + (row + 8) * ROW + (c ^ ((row + 8) / RPB % PAIRS) * 2) * 16 + sub;
-        const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t)a0);
-        const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t)a1);
-        const V8 vf = __builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int b = 0; b < QB; ++b) {
-          const uint4 pw = make_uint4(pk[b][kc >> 1][(kc & 1) * 4], pk[b][kc >> 1][(kc & 1) * 4 + 1],
-                                      pk[b][kc >> 1][(kc & 1) * 4 + 2], pk[b][kc >> 1][(kc & 1) * 4 + 3]);
-          o[b][d] = Mfma<T>::mul(vf, __builtin_bit_cast(V8, pw), o[b][d]);
-        }
-      }
-    }
-  }
+  };
+  auto advance = [&]() { off = move_max<DB>(max_with_partner(mx), m, l, o, p.c, kShift); };
 
-  // o / l; lane holds columns 32 * d + 8 * g + 4 * half + 0..3 of its row.
+  if (t0 < t1) {
+    // K(t + 1) and V(t) are used together; K(t0) alone first.
+    issue(t0, 0);
+    publish();
+    issue(t0 + 1, 0);
+    issue(t0, 1);
 #pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    const int64_t r = r0 + wave * 32 * QB + 32 * b + col;
-    const float sum = add_partner(l[b]);
-    if (r >= rows) continue;
-    const int64_t row = (s.b * p.q_rows + s.q0 + tok[b]) * p.heads + head[b];
-    if (p.splits > 1) {
-      const int64_t all = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;
-      float* const po = p.part + (split * all + row) * D;
-      float* const ml = p.part + (int64_t)p.splits * all * D + (split * all + row) * 2;
-      if (half == 0) {
-        ml[0] = m[b];
-        ml[1] = sum;
-      }
-      // A split without keys of this row is left out of the sum by its l of 0.
-      if (sum != 0.0f) {
+    for (int g = 0; g < NQ; ++g) score(s0, kfrag(smem, g), g);
+    masked(s0, t0);
+    mx = -INFINITY;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4*>(po + 32 * d + 8 * g + 4 * half) =
-                make_float4(o[b][d][4 * g], o[b][d][4 * g + 1], o[b][d][4 * g + 2], o[b][d][4 * g + 3]);
-      }
-      continue;
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s0[kb][e]);
+    auto step = [&](v16f (&sc)[2], v16f (&nx)[2], int t, const int par) {
+      advance();
+      publish();
+      issue(t + 2, 0);
+      issue(t + 1, 1);
+      body(sc, nx, t, par, std::true_type{});
+    };
+    int t = t0;
+#pragma unroll 1
+    for (; t + 2 < t1; t += 2) {
+      step(s0, s1, t, 0);
+      step(s1, s0, t + 1, 1);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint16_t* const po = p.out + row * D;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<uint2*>(po + 32 * d + 8 * g + 4 * half) =
-            make_uint2(Mfma<T>::pack(o[b][d][4 * g] * inv, o[b][d][4 * g + 1] * inv),
-                       Mfma<T>::pack(o[b][d][4 * g + 2] * inv, o[b][d][4 * g + 3] * inv));
+    if (t + 1 < t1) {
+      step(s0, s1, t, 0);
+      advance();
+      publish();
+      body(s1, s0, t1 - 1, 1, std::false_type{});
+    } else {
+      advance();
+      publish();
+      body(s0, s1, t1 - 1, 0, std::false_type{});
+    }
   }
+  store_row<T, D>(p, it, qr, m, l, o, half);
 }
 
-// Joins the splits of a row: weights 2^(c (m_s - max m)), in split order.
+// ---------------------------------------------------------- few queries ----
+// One wave, 32 rows (the heads that share a key head, times the new tokens), a
+// part of the keys. What counts is the stream of keys and values, so nothing is
+// shared and no barrier is met: tiles of 32 keys come straight into registers, K
+// as the first product's fragments (lane: key l % 32, 16 bytes), V row-major in
+// 16-byte pieces that pass through the wave's own LDS for the transposing read.
+// The next tile's loads are in flight while this one is worked on, of eight waves
+// per CU.
+template <typename T, int D>
+__global__ __launch_bounds__(64, 2) void attention_few(AttnArgs p) {
+  typedef typename Mfma<T>::V V8;
+  constexpr int BM = 32, KEYS = 32;
+  constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32;
+  constexpr int KD = D / 16, DB = D / 32;
+  constexpr int NVL = KEYS * ROW / 1024;   // 16-byte loads of V per lane and tile
+  __shared__ __attribute__((aligned(1024))) char smem[KEYS * ROW];
+  constexpr float kShift = Mfma<T>::kShift;
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  Item it;
+  if (!find_item<BM, KEYS>(p, it)) return;
+  const Seq s = it.s;
+  const QueryRow qr(p, it, it.r0 + col);
+  V8 q[KD];
+#pragma unroll
+  for (int d = 0; d < KD; ++d) q[d] = *reinterpret_cast<const V8*>(p.q + qr.off + 16 * d + 8 * half);
+  const uint16_t* const kbase = p.k + s.b * p.kb + s.k0 * p.kt + it.kv_head * p.kh;
+  const uint16_t* const vbase = p.v + s.b * p.vb + s.k0 * p.vt + it.kv_head * p.vh;
+  const uint32_t koff = (uint32_t)(col * p.kt * 2 + 16 * half);
+  uint32_t voff[NVL];
+#pragma unroll
+  for (int i = 0; i < NVL; ++i) voff[i] = (uint32_t)((i * 64 + lane) / CH * p.vt * 2 + (i * 64 + lane) % CH * 16);
+  uint4 kr[KD], vr_[NVL];
+  auto load = [&](int t) {
+    const int left = min(KEYS, s.kn - t * KEYS);  // rows past the sequence's keys read as zero
+    const __amdgpu_buffer_rsrc_t rk =
+        row_rsrc(kbase + (int64_t)t * KEYS * p.kt, ((int64_t)(left - 1) * p.kt + D) * 2);
+    const __amdgpu_buffer_rsrc_t rv =
+        row_rsrc(vbase + (int64_t)t * KEYS * p.vt, ((int64_t)(left - 1) * p.vt + D) * 2);
+#pragma unroll
+    for (int d = 0; d < KD; ++d) kr[d] = buf_load16(rk, koff + 32 * d);
+#pragma unroll
+    for (int i = 0; i < NVL; ++i) vr_[i] = buf_load16(rv, voff[i]);
+  };
+  v16f o[DB];
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  const int i16 = lane & 15, vrow = 4 * half + (i16 >> 2);
+  if (it.t0 < it.t1) load(it.t0);
+#pragma unroll 1
+  for (int t = it.t0; t < it.t1; ++t) {
+    v16f sc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < KD; ++d) sc = Mfma<T>::mul(__builtin_bit_cast(V8, kr[d]), q[d], sc);
+#pragma unroll
+    for (int i = 0; i < NVL; ++i) {
+      const int row = (i * 64 + lane) / CH, c = (i * 64 + lane) % CH ^ (row / RPB % PAIRS) * 2;
+      *reinterpret_cast<uint4*>(smem + row * ROW + c * 16) = vr_[i];
+    }
+    if (t + 1 < it.t1) load(t + 1);
+    if ((t + 1) * KEYS > it.sure) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        sc[e] = t * KEYS + 8 * (e >> 2) + 4 * half + (e & 3) < qr.limit ? sc[e] : -INFINITY;
+    }
+    float mx = sc[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+    const float off = move_max<DB>(max_with_partner(mx), m, l, o, p.c, kShift);
+    uint32_t pk[8];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.c, -off));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e + 1], p.c, -off));
+      l += p0 + p1;
+      pk[e >> 1] = Mfma<T>::pack(p0, p1);
+    }
+    // The wave's own writes are done before its reads: LDS operations of a wave
+    // stay in order.
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const int c = 4 * d + 2 * ((lane >> 4) & 1) + (i16 >> 1 & 1);
+        const int row = 16 * kc + vrow, sub = (i16 & 1) * 8;
+        const V8 vf = tr_pair<V8>(smem + row * ROW + (c ^ (row / RPB % PAIRS) * 2) * 16 + sub,
+                                  smem + (row + 8) * ROW + (c ^ ((row + 8) / RPB % PAIRS) * 2) * 16 + sub);
+        const uint4 pw = make_uint4(pk[4 * kc], pk[4 * kc + 1], pk[4 * kc + 2], pk[4 * kc + 3]);
+        o[d] = Mfma<T>::mul(vf, __builtin_bit_cast(V8, pw), o[d]);
+      }
+    asm volatile("" ::: "memory");
+  }
+  store_row<T, D>(p, it, qr, m, l, o, half);
+}
+
+// Joins the splits of a row: weights 2^(c (m_s - max m)). A workgroup per row: D / 4
+// threads hold a split's columns, and the groups of them take every G-th split,
+// then are added in order, so that the result does not depend on timing.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_splits(const float* __restrict__ part, uint16_t* __restrict__ out,
                                                    int64_t rows, int splits, float c) {
-  constexpr int LANES = D / 4;  // threads of a row, four columns each
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-  const int at = threadIdx.x % LANES * 4;
-  if (row >= rows) return;
-  const float* const ml = part + (int64_t)splits * rows * D;
+  constexpr int LANES = D / 4, G = 256 / LANES;
+  __shared__ float weight[256];
+  __shared__ float4 sums[G][LANES];
+  const int64_t row = blockIdx.x;
+  const float2* const ml = reinterpret_cast<const float2*>(part + (int64_t)splits * rows * D);
+  const int t = threadIdx.x, at = t % LANES, g = t / LANES;
+  // Every wave finds the maximum and the sum by itself (at most 256 splits).
+  float2 v[4];
   float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) {
-    const float2 v = *reinterpret_cast<const float2*>(ml + (s * rows + row) * 2);
-    if (v.y != 0.0f) m = fmaxf(m, v.x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = 64 * i + (t & 63);
+    v[i] = s < splits ? ml[s * rows + row] : make_float2(0.0f, 0.0f);
+    if (v[i].y != 0.0f) m = fmaxf(m, v[i].x);
   }
-  float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < splits; ++s) {
-    const float2 v = *reinterpret_cast<const float2*>(ml + (s * rows + row) * 2);
-    if (v.y == 0.0f) continue;
-    const float w = __builtin_amdgcn_exp2f((v.x - m) * c);
-    const float4 x = *reinterpret_cast<const float4*>(part + (s * rows + row) * D + at);
-    l += w * v.y;
-    o[0] += w * x.x;
-    o[1] += w * x.y;
-    o[2] += w * x.z;
-    o[3] += w * x.w;
+  m = wave_max(m);
+  float l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float w = v[i].y != 0.0f ? __builtin_amdgcn_exp2f((v[i].x - m) * c) : 0.0f;
+    weight[64 * i + (t & 63)] = w;   // the same value from each wave
+    l += w * v[i].y;
+  }
+  l = wave_tree_sum(l);
+  __syncthreads();
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = g; s < splits; s += G) {
+    const float w = weight[s];
+    if (w == 0.0f) continue;   // not written where the split had no keys
+    const float4 x = *reinterpret_cast<const float4*>(part + (s * rows + row) * D + 4 * at);
+    o.x += w * x.x;
+    o.y += w * x.y;
+    o.z += w * x.z;
+    o.w += w * x.w;
+  }
+  sums[g][at] = o;
+  __syncthreads();
+  if (g != 0) return;
+#pragma unroll
+  for (int i = 1; i < G; ++i) {
+    const float4 x = sums[i][at];
+    o.x += x.x;
+    o.y += x.y;
+    o.z += x.z;
+    o.w += x.w;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<uint2*>(out + row * D + at) =
-      make_uint2(Mfma<T>::pack(o[0] * inv, o[1] * inv), Mfma<T>::pack(o[2] * inv, o[3] * inv));
+  *reinterpret_cast<uint2*>(out + row * D + 4 * at) =
+      make_uint2(Mfma<T>::pack(o.x * inv, o.y * inv), Mfma<T>::pack(o.z * inv, o.w * inv));
 }
 
 // How a call is laid over the GPU.
@@ -410,14 +634,14 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, bool packed, int heads, int
   const int64_t mean_q = packed ? (n > 0 ? q_rows / n : 0) : q_rows;   // rows per sequence
   const int64_t mean_k = packed ? (n > 0 ? k_rows / n : 0) : k_rows;
   Plan pl;
-  const bool few = mean_q * group <= 64;
-  pl.pack = few ? group : 1;
-  pl.rows = few && mean_q * group <= 32 ? 32 : 128;
+  // Query heads share a tile's rows where their tokens leave most of it empty.
+  pl.pack = mean_q * group <= 128 ? group : 1;
+  pl.rows = mean_q * pl.pack <= 32 ? 32 : 128;
   const int64_t slots = kMaxBlocks;
   pl.tiles = packed ? q_rows * pl.pack / pl.rows + n + 2
                     : n * ((q_rows * pl.pack + pl.rows - 1) / pl.rows);
   const int64_t work = pl.tiles * (heads / pl.pack);
-  const int64_t want = pl.rows == 32 ? 4 * compute_units() : compute_units();
+  const int64_t want = (pl.rows == 32 ? 8 : 2) * compute_units();
   int64_t s = work > 0 ? want / work : 1;
   const int64_t most = mean_k / 256;   // at least 256 keys each
   s = s < most ? s : most;
@@ -430,13 +654,13 @@ template <typename T, int D>
 int launch(AttnArgs p, const Plan& pl, hipStream_t s) {
   const int64_t grid = pl.tiles * (p.heads / pl.pack) * pl.splits;
   LR_REQUIRE(grid <= kMaxBlocks, "attention: %lld workgroups are not supported", (long long)grid);
-  if (pl.rows == 32) attention<T, D, 1, 1, 2><<<(unsigned)grid, 64, 0, s>>>(p);
-  else attention<T, D, 1, 4, 2><<<(unsigned)grid, 256, 0, s>>>(p);
+  if (pl.rows == 32) attention_few<T, D><<<(unsigned)grid, 64, 0, s>>>(p);
+  else attention<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
   if (int rc = check_launch("attention")) return rc;
   if (pl.splits == 1) return LR_OK;
-  const int64_t rows = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads, blocks = (rows * (D / 4) + 255) / 256;
-  LR_REQUIRE(blocks <= kMaxBlocks, "attention: %lld rows are not supported", (long long)rows);
-  join_splits<T, D><<<(unsigned)blocks, 256, 0, s>>>(p.part, p.out, rows, pl.splits, p.c);
+  const int64_t rows = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;
+  LR_REQUIRE(rows <= kMaxBlocks, "attention: %lld rows are not supported", (long long)rows);
+  join_splits<T, D><<<(unsigned)rows, 256, 0, s>>>(p.part, p.out, rows, pl.splits, p.c);
   return check_launch("attention");
 }
 

@@ -167,7 +167,8 @@ def test_cache(new, heads, kv_heads, dim, kind):
     far = torch.tensor([2 ** 40 if kind == torch.int64 else 2 ** 31 - 1] * 5 + [-5], device="cuda", dtype=kind)
     k.nan_to_num_(0.0), v.nan_to_num_(0.0, 0.0, 0.0)
     got = A.attention(q, k, v, key_lengths=far)
-    assert torch.equal(got[:5], A.attention(q[:5], k[:5], v[:5], key_lengths=torch.full_like(far[:5], size)))
+    # (the same batch: the keys of another one may be split elsewhere)
+    assert torch.equal(got, A.attention(q, k, v, key_lengths=torch.tensor([size] * 5 + [0], device="cuda", dtype=kind)))
     assert (got[5] == 0).all()
 
 

@@ -351,6 +351,14 @@ int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, const void*
                   int64_t table_rows, int64_t table_width, const int64_t* indices, int64_t sequence,
                   int gate_slot, void* stream);
 
+/* lr_quantize_rows_mxfp4 of x [m, k] into the scratch, then lr_mxfp4_gemm of it.
+ * scratch: 16-byte aligned, the codes (m * 16 * ceil(k / 32) bytes, rounded up to
+ * a multiple of 256) and behind them ceil(m / 64) * ceil(k / 256) * 512 bytes. */
+int lr_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t n, int64_t k, void* scratch,
+                    int64_t scratch_bytes, const void* b, const void* b_scale, const void* bias, void* out,
+                    int epilogue, const void* residual, const void* table, int64_t table_rows, int64_t table_width,
+                    const int64_t* indices, int64_t sequence, int gate_slot, void* stream);
+
 /* Softmax attention, out = softmax(scale * Q K^T) V, with fp32 scores, maxima,
  * sums and accumulators; the probabilities are rounded to the inputs' type.
  *   q, out: `heads` heads; k, v: `kv_heads` heads, which heads / kv_heads query

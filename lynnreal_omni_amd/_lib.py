@@ -66,6 +66,8 @@ SIGNATURES = {
     "lr_quantize_rows_mxfp4": [_P, _I32, _I64, _I64, _P, _P, _P],
     "lr_dequantize_rows_mxfp4": [_P, _P, _I32, _I64, _I64, _P, _P],
     "lr_mxfp4_gemm": [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I32, _P, _P, _I64, _I64, _P, _I64, _I32, _P],
+    "lr_mxfp4_linear": [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _P, _I64,
+                        _I32, _P],
     "lr_attention_splits": [_I64, _I64, _I64, _I32, _I32, _I32],
     "lr_attention": [_P, _P, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _I32, _P, _I64,
                      _I32, _P],

@@ -813,3 +813,20 @@ extern "C" int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, 
              (epilogue != EPI_GATED || (aligned(residual, 16) && aligned(table, 16) && table_width % 8 == 0));
   return launch(p, epilogue, as_stream(stream));
 }
+
+extern "C" int lr_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t n, int64_t k, void* scratch,
+                               int64_t scratch_bytes, const void* b, const void* b_scale, const void* bias, void* out,
+                               int epilogue, const void* residual, const void* table, int64_t table_rows,
+                               int64_t table_width, const int64_t* indices, int64_t sequence, int gate_slot,
+                               void* stream) {
+  LR_REQUIRE(m >= 0 && n >= 0 && k > 0, "mxfp4_linear: bad shape m=%lld n=%lld k=%lld", (long long)m, (long long)n,
+             (long long)k);
+  const int64_t codes = (m * ((k + 31) / 32 * 16) + 255) / 256 * 256;
+  const int64_t need = codes + (m + 63) / 64 * mxfp4_scale_tiles(k) * 512;
+  LR_REQUIRE(m == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= need),
+             "mxfp4_linear: the scratch must be 16-byte aligned and hold %lld bytes", (long long)need);
+  char* const scales = static_cast<char*>(scratch) + codes;
+  if (int rc = lr_quantize_rows_mxfp4(x, dtype, m, k, scratch, m ? scales : nullptr, stream)) return rc;
+  return lr_mxfp4_gemm(scratch, scales, b, b_scale, m, n, k, bias, out, epilogue, residual, table, table_rows,
+                       table_width, indices, sequence, gate_slot, stream);
+}

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import kernels, mxfp4_gemm
+from . import mxfp4_gemm
 from .int8 import _concat_qkv
 from .mxfp4_gemm import BLOCK
 
@@ -91,10 +91,14 @@ class Mxfp4Linear(nn.Module):
         return y.view(*output_shape, self.out_features)
 
     def forward(self, value, **epilogue):
+        """Quantize the rows of value (bf16, fp16 or fp32) and project them to bf16
+        [.., out_features]. `epilogue`: mxfp4_matmul's keywords."""
         if value.shape[-1] != self.in_features:
             raise ValueError(f"the layer takes {self.in_features} features, got {value.shape[-1]}")
-        flat = value.reshape(-1, self.in_features)
-        return self.forward_codes(*kernels.quantize_rows_mxfp4(flat), value.shape[:-1], **epilogue)
+        buffers = self._buffers
+        y = mxfp4_gemm.linear_rows(value.reshape(-1, self.in_features), buffers["weight_codes"],
+                                   buffers["weight_scale"], buffers["bias"], **epilogue)
+        return y.view(*value.shape[:-1], self.out_features)
 
 
 @torch.no_grad()

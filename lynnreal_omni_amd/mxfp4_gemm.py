@@ -8,9 +8,12 @@ Inference only: the outputs carry no gradient.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
+from .int8_gemm import _ROW_DTYPES
 
 BLOCK = 32          # values that share a scale
 _TILE_ROWS, _TILE_BLOCKS = 64, 8
@@ -75,6 +78,36 @@ def _gated(m, n, residual, table, indices, gate_slot):
     return residual.reshape(m, n).contiguous(), table.contiguous(), indices, sequence
 
 
+def _epilogue(m, n, activation, residual, table, indices, gate_slot):
+    """(epilogue, residual, table, table rows, table width, indices, sequence, slot) of a call's keywords."""
+    if residual is not None:
+        if activation is not None:
+            raise ValueError("activation and gated residual epilogues are exclusive")
+        residual, table, indices, sequence = _gated(m, n, residual, table, indices, gate_slot)
+        width = table.shape[-1]
+        rows = table.numel() // width if width else 0
+        return _lib.EPI_GATED_RESIDUAL, residual, table, rows, width, indices, sequence, int(gate_slot)
+    if table is not None or indices is not None or gate_slot is not None:
+        raise ValueError("table, indices and gate_slot belong to a gated residual: residual is missing")
+    if activation is None:
+        return _PLAIN
+    if activation == "gelu_tanh":
+        return _GELU
+    raise ValueError(f"unsupported activation {activation!r}")
+
+
+_PLAIN = (_lib.EPI_BF16, None, None, 0, 0, None, 0, 0)
+_GELU = (_lib.EPI_GELU_TANH, None, None, 0, 0, None, 0, 0)
+
+
+def _bias(bias, n):
+    if bias is None:
+        return None
+    if bias.dtype != torch.bfloat16 or bias.numel() != n:
+        raise ValueError("bias must be bfloat16 with N entries")
+    return bias.contiguous()
+
+
 def mxfp4_matmul(a, b, a_scale, b_scale, bias=None, *, activation=None, residual=None, table=None, indices=None,
                  gate_slot=None):
     """bf16(A @ W.T + bias) of MXFP4 rows A [M, K] and W [N, K].
@@ -89,31 +122,58 @@ def mxfp4_matmul(a, b, a_scale, b_scale, bias=None, *, activation=None, residual
     _operand(b, b_scale, "b")
     if a.shape[1] != b.shape[1]:
         raise ValueError(f"a has {a.shape[1]} bytes of codes per row, b {b.shape[1]}")
+    if a.shape[1] == 0:
+        raise ValueError("a and b have no columns")
     _lib.check_device(a)
     _lib.same_device(a, b=b, a_scale=a_scale, b_scale=b_scale, bias=bias, residual=residual, table=table,
                      indices=indices)
     m, n = a.shape[0], b.shape[0]
-    if bias is not None:
-        if bias.dtype != torch.bfloat16 or bias.numel() != n:
-            raise ValueError("bias must be bfloat16 with N entries")
-        bias = bias.contiguous()
-    epilogue, sequence, slot, rows, width = _lib.EPI_BF16, 0, 0, 0, 0
-    if residual is not None:
-        if activation is not None:
-            raise ValueError("activation and gated residual epilogues are exclusive")
-        residual, table, indices, sequence = _gated(m, n, residual, table, indices, gate_slot)
-        epilogue, slot, width = _lib.EPI_GATED_RESIDUAL, int(gate_slot), table.shape[-1]
-        rows = table.numel() // width if width else 0
-    elif table is not None or indices is not None or gate_slot is not None:
-        raise ValueError("table, indices and gate_slot belong to a gated residual: residual is missing")
-    elif activation == "gelu_tanh":
-        epilogue = _lib.EPI_GELU_TANH
-    elif activation is not None:
-        raise ValueError(f"unsupported activation {activation!r}")
+    bias = _bias(bias, n)
+    epilogue, residual, table, rows, width, indices, sequence, slot = _epilogue(m, n, activation, residual, table,
+                                                                                indices, gate_slot)
     output = torch.empty((m, n), device=a.device, dtype=torch.bfloat16)
-    if a.shape[1] == 0:
-        raise ValueError("a and b have no columns")
     _lib.launch(a, "lr_mxfp4_gemm", a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), m, n,
                 2 * a.shape[1], _lib.ptr(bias), output.data_ptr(), epilogue, _lib.ptr(residual), _lib.ptr(table), rows,
                 width, _lib.ptr(indices), sequence, slot)
+    return output
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch(m, k):
+    """Bytes of lr_mxfp4_linear's scratch."""
+    codes = -(-m * code_bytes(k) // 256) * 256
+    tiles, blocks, size = scale_shape(m, k)
+    return codes + tiles * blocks * size
+
+
+def linear_rows(rows, b, b_scale, bias=None, *, activation=None, residual=None, table=None, indices=None,
+                gate_slot=None):
+    """mxfp4_matmul of kernels.quantize_rows_mxfp4(rows) and the weight, with one
+    allocation for codes and scales and one call for both kernels. At a few rows the
+    host bounds a layer: 21.7 us for the two functions one after the other."""
+    m, k = rows.shape
+    n = b.shape[0]
+    dtype = _ROW_DTYPES.get(rows.dtype)
+    if dtype is None:
+        raise RuntimeError(f"value: dtype {rows.dtype} is not supported by the HIP quantizer")
+    _operand(b, b_scale, "b")
+    if b.shape[1] != code_bytes(k) or k == 0:
+        raise ValueError(f"rows of {k} columns do not fit a weight of {2 * b.shape[1]}")
+    _lib.check_device(rows)
+    epilogue = _PLAIN
+    if activation is None and residual is None and table is None and indices is None and gate_slot is None:
+        _lib.same_device(rows, b=b, b_scale=b_scale, bias=bias)
+    else:
+        _lib.same_device(rows, b=b, b_scale=b_scale, bias=bias, residual=residual, table=table, indices=indices)
+        epilogue = _epilogue(m, n, activation, residual, table, indices, gate_slot)
+    if not rows.is_contiguous():
+        rows = rows.contiguous()
+    bias = _bias(bias, n)
+    nbytes = _scratch(m, k)
+    scratch = rows.new_empty(nbytes, dtype=torch.uint8)
+    output = rows.new_empty((m, n), dtype=torch.bfloat16)
+    kind, residual, table, table_rows, width, indices, sequence, slot = epilogue
+    _lib.launch(rows, "lr_mxfp4_linear", rows.data_ptr(), dtype, m, n, k, scratch.data_ptr(), nbytes, b.data_ptr(),
+                b_scale.data_ptr(), _lib.ptr(bias), output.data_ptr(), kind, _lib.ptr(residual), _lib.ptr(table),
+                table_rows, width, _lib.ptr(indices), sequence, slot)
     return output

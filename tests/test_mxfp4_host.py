@@ -75,6 +75,10 @@ def test_refusals():
         kernels.dequantize_rows_mxfp4(codes, scales, 32)                           # one block, codes of two
     with pytest.raises(ValueError):
         kernels.dequantize_rows_mxfp4(codes, scales[..., :256], 64)
+    for bad in [dict(activation="relu"), dict(gate_slot=1), dict(activation="gelu_tanh", residual=torch.zeros(3, 3))]:
+        with pytest.raises(ValueError):
+            mxfp4_gemm._epilogue(3, 3, **{**dict(activation=None, residual=None, table=None, indices=None,
+                                                 gate_slot=None), **bad})
     for args in [(codes[:, :20], codes, scales, scales), (codes, codes, scales[0], scales),
                  (codes.to(torch.int8), codes, scales, scales), (codes, codes[:, :16].contiguous(), scales, scales),
                  (codes.t().contiguous().t(), codes, scales, scales), (codes, codes, scales, scales)]:
@@ -97,3 +101,11 @@ def test_entry_points_refuse_without_a_gpu():
         assert lib.lr_quantize_rows_mxfp4(*bad) == _lib.LR_EINVAL, bad
     assert lib.lr_quantize_rows_mxfp4(None, 0, 0, 32, None, None, None) == _lib.LR_OK
     assert lib.lr_dequantize_rows_mxfp4(p, p, 0, 2, 32, p + 2, None) == _lib.LR_EINVAL
+    # codes of 3 rows of 64 columns: 96 bytes, kept as 256, and one tile of scales
+    linear = lambda **kw: lib.lr_mxfp4_linear(*{**dict(x=p, dtype=0, m=3, n=8, k=64, s=p, sb=768, b=p, bs=p, bias=None,  # noqa: E731
+                                                       out=p, epi=0, res=None, table=None, rows=0, width=0, idx=None,
+                                                       seq=0, slot=0, stream=None), **kw}.values())
+    for bad in [dict(sb=767), dict(s=None), dict(s=p + 8), dict(k=0), dict(dtype=9), dict(x=None)]:
+        assert linear(**bad) == _lib.LR_EINVAL, bad
+    assert linear(m=0, s=None, sb=0) == _lib.LR_OK
+    assert mxfp4_gemm._scratch(3, 64) == 768

@@ -51,7 +51,7 @@ struct AttnArgs {
   int pack;              // query heads that share a tile's rows (group or 1)
   int causal, splits;
   float c;               // scale * log2(e)
-  int64_t tiles;         // row tiles per head in all
+  int tiles, seq_tiles;  // row tiles per head in all, and of a dense batch's sequence
 };
 
 // A sequence's rows and keys. Values read from the device are clamped, so that
@@ -123,62 +123,71 @@ constexpr float kSlack = 8.0f;   // log2
 // sequence's (row r: token r / pack, head hd * pack + r % pack), and key tiles.
 struct Item {
   Seq s;
-  int64_t rows, r0;
+  int rows, r0;
   int split, hd, kv_head;
   int sure;     // keys that every row of the workgroup sees
   int t0, t1;   // its tiles of KEYS keys
 };
 
+// Everything fits 32 bits: workgroups are fewer than 2^24, rows than 2^31 (plan).
 template <int BM, int KEYS>
 __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
   // Tiles of a head lie together, and each XCD (workgroups are dealt to them in
   // turn) takes a contiguous run, so that its L2 serves a head's keys once.
-  const int64_t total = p.tiles * (p.heads / p.pack) * p.splits;
-  const int64_t pid = blockIdx.x;
-  const int64_t per = total >> 3, rest = total & 7, xcd = pid & 7;
-  const int64_t lid = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3);
-  it.split = (int)(lid % p.splits);
-  int64_t tile = lid / p.splits % p.tiles;
-  it.hd = (int)(lid / p.splits / p.tiles);   // head, or key head where heads share rows
+  const uint32_t total = gridDim.x, pid = blockIdx.x;
+  const uint32_t per = total >> 3, rest = total & 7, xcd = pid & 7;
+  const uint32_t lid = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3);
+  const uint32_t item = lid / (uint32_t)p.splits;
+  it.split = (int)(lid - item * p.splits);
+  it.hd = (int)(item / (uint32_t)p.tiles);   // head, or key head where heads share rows
+  int tile = (int)(item - it.hd * p.tiles);
   it.kv_head = p.pack > 1 ? it.hd : it.hd / p.group;
   Seq s = {};
-  int64_t tiles;   // of the sequence
+  int tiles;   // of the sequence
   if (p.cu_q) {
     // Sequence i has the tile slots from first_row(i) * pack / BM + i on: at least
     // as many as its rows need, and its own.
-    const int64_t slot = tile;
+    const int slot = tile;
+    auto start = [&](int64_t i) __attribute__((always_inline)) {
+      return (int)((uint32_t)(first_row(p, i) * p.pack) / BM) + (int)i;
+    };
     int64_t lo = 0, hi = p.n + 1;
     while (lo < hi) {
       const int64_t mid = (lo + hi + 1) >> 1;
-      if (first_row(p, mid) * p.pack / BM + mid <= slot) lo = mid;
+      if (start(mid) <= slot) lo = mid;
       else hi = mid - 1;
     }
     s.q0 = first_row(p, lo);
     s.qn = (int)clamp64(first_row(p, lo + 1) - s.q0, 0, p.q_rows);
-    tile = slot - (s.q0 * p.pack / BM + lo);
-    tiles = ((int64_t)s.qn * p.pack + BM - 1) / BM;
+    tile = slot - start(lo);
+    tiles = (int)((uint32_t)(s.qn * p.pack + BM - 1) / BM);
     if (lo > 0 && lo <= p.n) {
       s.k0 = clamp64(p.cu_k[lo - 1], 0, p.k_rows);
       s.kn = (int)clamp64(clamp64(p.cu_k[lo], 0, p.k_rows) - s.k0, 0, p.k_rows);
     }
     if (tile >= tiles) return false;
   } else {
-    tiles = p.tiles / p.n;
-    s.b = tile / tiles;
-    tile -= s.b * tiles;
+    tiles = p.seq_tiles;
+    const int b = (int)((uint32_t)tile / (uint32_t)tiles);
+    s.b = b;
+    tile -= b * tiles;
     s.qn = (int)p.q_rows;
-    s.kn = (int)(p.lengths ? clamp64(p.lengths[s.b], 0, p.k_rows) : p.k_rows);
+    s.kn = (int)(p.lengths ? clamp64(p.lengths[b], 0, p.k_rows) : p.k_rows);
   }
   // Causal: the last tiles see the most keys and go first.
   if (p.causal) tile = tiles - 1 - tile;
   it.s = s;
-  it.rows = (int64_t)s.qn * p.pack;
+  it.rows = s.qn * p.pack;
   it.r0 = tile * BM;
-  const int64_t last = it.r0 + BM <= it.rows ? it.r0 + BM - 1 : it.rows - 1;
-  const int last_tok = (int)(p.pack == 1 ? last : last / p.pack);
-  const int first_tok = (int)(p.pack == 1 ? it.r0 : it.r0 / p.pack);
-  const int seen = p.causal ? min(s.kn, max(0, s.kn - s.qn + last_tok + 1)) : s.kn;
-  it.sure = p.causal ? min(s.kn, max(0, s.kn - s.qn + first_tok + 1)) : s.kn;
+  it.sure = s.kn;
+  int seen = s.kn;
+  if (p.causal) {
+    const int last = min(it.r0 + BM, it.rows) - 1;
+    const int last_tok = p.pack == 1 ? last : (int)((uint32_t)last / (uint32_t)p.pack);
+    const int first_tok = p.pack == 1 ? it.r0 : (int)((uint32_t)it.r0 / (uint32_t)p.pack);
+    seen = min(s.kn, max(0, s.kn - s.qn + last_tok + 1));
+    it.sure = min(s.kn, max(0, s.kn - s.qn + first_tok + 1));
+  }
   const int tiles_k = (seen + KEYS - 1) / KEYS;
   it.t0 = (int)((int64_t)tiles_k * it.split / p.splits);
   it.t1 = (int)((int64_t)tiles_k * (it.split + 1) / p.splits);
@@ -187,12 +196,12 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
 
 // The query row of a lane (column `col` of a wave's 32 rows from `r` on).
 struct QueryRow {
-  int64_t r, off;   // off: of its first element in q
-  int tok, head, limit;   // limit: keys that it sees
-  __device__ __forceinline__ QueryRow(const AttnArgs& p, const Item& it, int64_t row) : r(row) {
-    const int64_t rc = row < it.rows ? row : it.rows - 1;
-    tok = (int)(p.pack == 1 ? rc : rc / p.pack);
-    head = p.pack == 1 ? it.hd : it.hd * p.pack + (int)(rc - (int64_t)tok * p.pack);
+  int64_t off;   // of its first element in q
+  int r, tok, head, limit;   // limit: keys that it sees
+  __device__ __forceinline__ QueryRow(const AttnArgs& p, const Item& it, int row) : r(row) {
+    const int rc = row < it.rows ? row : it.rows - 1;
+    tok = p.pack == 1 ? rc : (int)((uint32_t)rc / (uint32_t)p.pack);
+    head = p.pack == 1 ? it.hd : it.hd * p.pack + (rc - tok * p.pack);
     off = it.s.b * p.qb + (it.s.q0 + tok) * p.qt + head * p.qh;
     limit = p.causal ? min(it.s.kn, max(0, it.s.kn - it.s.qn + tok + 1)) : it.s.kn;
   }
@@ -467,23 +476,30 @@ __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
 }
 
 // ---------------------------------------------------------- few queries ----
-// One wave, 32 rows (the heads that share a key head, times the new tokens), a
-// part of the keys. What counts is the stream of keys and values, so nothing is
-// shared and no barrier is met: tiles of 32 keys come straight into registers, K
-// as the first product's fragments (lane: key l % 32, 16 bytes), V row-major in
-// 16-byte pieces that pass through the wave's own LDS for the transposing read.
-// The next tile's loads are in flight while this one is worked on, of eight waves
-// per CU.
+// 32 rows (the heads that share a key head, times the new tokens) and a part of the
+// keys per workgroup. What counts is the stream of keys and values, so its four waves
+// share nothing and meet no barrier until their ends: each takes every fourth tile of
+// 32 keys straight into registers, K as the first product's fragments (lane: key l %
+// 32, 16 bytes), V row-major in 16-byte pieces that pass through the wave's own LDS
+// for the transposing read; the next tile's loads are in flight while this one is
+// worked on. Then the waves' o, m and l are joined in LDS, in a fixed order.
+// Measured, one token of 56 heads over 131072 keys of 8 heads (537 MB): key tiles
+// through LDS DMA by single waves 208 us, straight to registers 123 us and 16 us for
+// joining 256 splits.
 template <typename T, int D>
-__global__ __launch_bounds__(64, 2) void attention_few(AttnArgs p) {
+__global__ __launch_bounds__(256, 2) void attention_few(AttnArgs p) {
   typedef typename Mfma<T>::V V8;
-  constexpr int BM = 32, KEYS = 32;
+  constexpr int BM = 32, KEYS = 32, WAVES = 4;
   constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32;
   constexpr int KD = D / 16, DB = D / 32;
   constexpr int NVL = KEYS * ROW / 1024;   // 16-byte loads of V per lane and tile
-  __shared__ __attribute__((aligned(1024))) char smem[KEYS * ROW];
+  constexpr int TILE = KEYS * ROW;         // a wave's V tile; two hold a wave's o
+  __shared__ __attribute__((aligned(1024))) char smem_all[WAVES * TILE];
+  __shared__ float2 ml[2][64];
   constexpr float kShift = Mfma<T>::kShift;
-  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, col = lane & 31;
+  char* const smem = smem_all + wave * TILE;
   Item it;
   if (!find_item<BM, KEYS>(p, it)) return;
   const Seq s = it.s;
@@ -516,9 +532,9 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttnArgs p) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
   const int i16 = lane & 15, vrow = 4 * half + (i16 >> 2);
-  if (it.t0 < it.t1) load(it.t0);
+  if (it.t0 + wave < it.t1) load(it.t0 + wave);
 #pragma unroll 1
-  for (int t = it.t0; t < it.t1; ++t) {
+  for (int t = it.t0 + wave; t < it.t1; t += WAVES) {
     v16f sc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
@@ -529,7 +545,7 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttnArgs p) {
       const int row = (i * 64 + lane) / CH, c = (i * 64 + lane) % CH ^ (row / RPB % PAIRS) * 2;
       *reinterpret_cast<uint4*>(smem + row * ROW + c * 16) = vr_[i];
     }
-    if (t + 1 < it.t1) load(t + 1);
+    if (t + WAVES < it.t1) load(t + WAVES);
     if ((t + 1) * KEYS > it.sure) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -563,7 +579,42 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttnArgs p) {
       }
     asm volatile("" ::: "memory");
   }
-  store_row<T, D>(p, it, qr, m, l, o, half);
+  // Wave 2 into 0 and 3 into 1, then 1 into 0: a wave's o takes 128 * D bytes, two tiles.
+#pragma unroll
+  for (int from = 2; from >= 1; --from) {
+    const int slot = from == 2 ? wave & 1 : 0;
+    float* const po = reinterpret_cast<float*>(smem_all + slot * 2 * TILE);
+    __syncthreads();   // the tiles, and what the round before left, have been read
+    if (wave >= from && wave < 2 * from) {
+      ml[slot][lane] = make_float2(m, l);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(po + ((d * 4 + g) * 64 + lane) * 4) =
+              make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    }
+    __syncthreads();
+    if (wave < from) {
+      const float2 other = ml[slot][lane];
+      const float mn = fmaxf(m, other.x);
+      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c);
+      const float b = other.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((other.x - mn) * p.c);
+      m = mn;
+      l = l * a + other.y * b;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 x = *reinterpret_cast<const float4*>(po + ((d * 4 + g) * 64 + lane) * 4);
+          o[d][4 * g] = o[d][4 * g] * a + x.x * b;
+          o[d][4 * g + 1] = o[d][4 * g + 1] * a + x.y * b;
+          o[d][4 * g + 2] = o[d][4 * g + 2] * a + x.z * b;
+          o[d][4 * g + 3] = o[d][4 * g + 3] * a + x.w * b;
+        }
+    }
+  }
+  if (wave == 0) store_row<T, D>(p, it, qr, m, l, o, half);
 }
 
 // Joins the splits of a row: weights 2^(c (m_s - max m)). A workgroup per row: D / 4
@@ -635,13 +686,13 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, bool packed, int heads, int
   const int64_t mean_k = packed ? (n > 0 ? k_rows / n : 0) : k_rows;
   Plan pl;
   // Query heads share a tile's rows where their tokens leave most of it empty.
-  pl.pack = mean_q * group <= 128 ? group : 1;
+  pl.pack = mean_q * group <= 128 && q_rows * group < (1LL << 31) ? group : 1;
   pl.rows = mean_q * pl.pack <= 32 ? 32 : 128;
   const int64_t slots = kMaxBlocks;
   pl.tiles = packed ? q_rows * pl.pack / pl.rows + n + 2
                     : n * ((q_rows * pl.pack + pl.rows - 1) / pl.rows);
   const int64_t work = pl.tiles * (heads / pl.pack);
-  const int64_t want = (pl.rows == 32 ? 8 : 2) * compute_units();
+  const int64_t want = 2 * compute_units();   // workgroups that are resident at once
   int64_t s = work > 0 ? want / work : 1;
   const int64_t most = mean_k / 256;   // at least 256 keys each
   s = s < most ? s : most;
@@ -654,7 +705,7 @@ template <typename T, int D>
 int launch(AttnArgs p, const Plan& pl, hipStream_t s) {
   const int64_t grid = pl.tiles * (p.heads / pl.pack) * pl.splits;
   LR_REQUIRE(grid <= kMaxBlocks, "attention: %lld workgroups are not supported", (long long)grid);
-  if (pl.rows == 32) attention_few<T, D><<<(unsigned)grid, 64, 0, s>>>(p);
+  if (pl.rows == 32) attention_few<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
   else attention<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
   if (int rc = check_launch("attention")) return rc;
   if (pl.splits == 1) return LR_OK;
@@ -736,7 +787,9 @@ extern "C" int lr_attention(const void* q, const void* k, const void* v, void* o
   Plan pl = plan(sequences, q_rows, k_rows, packed, heads, kv_heads);
   pl.splits = splits;
   p.pack = pl.pack;
-  p.tiles = pl.tiles;
+  LR_REQUIRE(pl.tiles < (1LL << 31), "attention: %lld row tiles are not supported", (long long)pl.tiles);
+  p.tiles = (int)pl.tiles;
+  p.seq_tiles = packed ? 0 : (int)(pl.tiles / sequences);
   p.splits = splits;
   if (splits > 1) {
     const int64_t rows = (packed ? 1 : sequences) * q_rows * heads;

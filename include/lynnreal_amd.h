@@ -379,9 +379,13 @@ int lr_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t n, int64_t k, v
  * scale_bits: the fp32 bits of the scale, positive and finite.
  * splits > 1 cuts a sequence's keys for as many workgroups, joined in order by a
  *   second kernel; needs a workspace of splits * rows * (head_dim + 2) * 4 bytes,
- *   rows = heads * q_rows (* sequences for a dense batch), 16-byte aligned.
- *   lr_attention_splits gives the count that fills the GPU. */
-int lr_attention_splits(int64_t sequences, int64_t q_rows, int64_t k_rows, int packed, int heads, int kv_heads);
+ *   rows = heads * q_rows (LR_ATTN_DENSE: * sequences), 16-byte aligned.
+ *   lr_attention_splits gives the count that fills the GPU; with key_lengths it
+ *   counts the pieces of all sequences, and only 1 or that count is taken. */
+#define LR_ATTN_DENSE 0   /* all sequences of one length */
+#define LR_ATTN_PACKED 1
+#define LR_ATTN_LENGTHS 2 /* a dense batch with key_lengths */
+int lr_attention_splits(int64_t sequences, int64_t q_rows, int64_t k_rows, int kind, int heads, int kv_heads);
 int lr_attention(const void* q, const void* k, const void* v, void* out, int dtype, int64_t sequences,
                  int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int head_dim, const int64_t* strides,
                  const int32_t* cu_q, const int32_t* cu_k, const int32_t* key_lengths, int causal,

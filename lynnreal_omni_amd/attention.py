@@ -26,6 +26,7 @@ from . import _lib
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _HEAD_DIMS = (32, 64, 128)
+_DENSE, _PACKED, _LENGTHS = range(3)
 
 
 def _rows(t):
@@ -42,8 +43,8 @@ def _rows(t):
 
 
 @functools.lru_cache(maxsize=4096)
-def _splits(sequences, q_rows, k_rows, packed, heads, kv_heads):
-    return int(_lib.load().lr_attention_splits(sequences, q_rows, k_rows, packed, heads, kv_heads))
+def _splits(sequences, q_rows, k_rows, kind, heads, kv_heads):
+    return int(_lib.load().lr_attention_splits(sequences, q_rows, k_rows, kind, heads, kv_heads))
 
 
 @functools.lru_cache(maxsize=64)
@@ -75,10 +76,11 @@ def _launch(query, key, value, out, sequences, q_rows, k_rows, cu_q, cu_k, lengt
     heads, dim = query.shape[-2:]
     kv_heads = key.shape[-2]
     packed = cu_q is not None
-    splits = _splits(sequences, q_rows, k_rows, int(packed), heads, kv_heads)
+    kind = _PACKED if packed else (_DENSE if lengths is None else _LENGTHS)
+    splits = _splits(sequences, q_rows, k_rows, kind, heads, kv_heads)
     ws, nbytes = None, 0
     if splits > 1:
-        nbytes = splits * (1 if packed else sequences) * q_rows * heads * (dim + 2) * 4
+        nbytes = splits * (sequences if kind == _DENSE else 1) * q_rows * heads * (dim + 2) * 4
         ws = _lib.workspace(query, nbytes)   # held until the launch
     strides = array("q")
     for t in (query, key, value):

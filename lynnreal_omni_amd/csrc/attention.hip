@@ -51,7 +51,8 @@ struct AttnArgs {
   int pack;              // query heads that share a tile's rows (group or 1)
   int causal, splits;
   float c;               // scale * log2(e)
-  int tiles, seq_tiles;  // row tiles per head in all, and of a dense batch's sequence
+  int tiles, seq_tiles;  // row tiles per head in all (pieces: of a sequence), and of a dense batch's sequence
+  int piece;             // least keys of a piece
 };
 
 // A sequence's rows and keys. Values read from the device are clamped, so that
@@ -118,13 +119,80 @@ __device__ __forceinline__ V8 tr_pair(const char* a0, const char* a1) {
 
 constexpr int kKeys = 64;        // keys per tile of a prompt
 constexpr float kSlack = 8.0f;   // log2
+constexpr int kMaxSplits = 256;  // of a sequence
+
+// Sum of v over the lanes up to this one: within rows of 16 lanes by shifts, then the
+// last lane of each row (and of each pair of rows) added to the rows behind it.
+__device__ __forceinline__ int wave_prefix_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// Few queries over sequences of different numbers of keys: all are cut into pieces of
+// one size, so that the longest is not what everybody waits for, in a list over the
+// sequences that every wave works out from the lengths by itself. With n sequences and
+// p.splits > n places, pieces of (keys in all) / (p.splits - n) keys fit the list.
+struct Pieces {
+  int chunk = 0;              // keys of a piece, a multiple of 64
+  int seq = -1, keys = 0;     // the sequence asked for (-1: the list ends before)
+  int first = 0, count = 0;   // its pieces
+  __device__ Pieces() {}
+  // Of sequence `want`, or where that is -1 the one that has piece `place`.
+  __device__ Pieces(const AttnArgs& p, int64_t want, int place) {
+    const int lane = threadIdx.x & 63;
+    auto length = [&](int64_t i) __attribute__((always_inline)) {
+      return i < p.n ? (int)clamp64(p.lengths[i], 0, p.k_rows) : 0;
+    };
+    // The smallest pieces that the list holds: from an even share up in steps, at the
+    // latest where n of the places are left for sequences' last pieces. Sums in fp32,
+    // in units of 64 keys: they may pass 32 bits (sequences of an expanded tensor
+    // share their keys); the counts that have to be exact are below 2^24.
+    auto units_of = [&](int size) __attribute__((always_inline)) {
+      float sum = 0.0f;
+      for (int64_t i = lane; i < p.n; i += 64)
+        sum += (float)((uint32_t)(((length(i) + 63) >> 6) + size - 1) / (uint32_t)size);
+      // The same in every lane; said so, since what depends on it addresses memory.
+      return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_tree_sum(sum))));
+    };
+    const float all = units_of(1) * 1.001f;
+    const int least = (int)((p.k_rows + 64 * kMaxSplits - 1) / (64 * kMaxSplits));   // of one sequence
+    const bool tight = p.splits < 2 * p.n;
+    const float share = all / (float)(tight ? p.splits - (int)p.n : p.splits);
+    int size = max(max(p.piece >> 6, least), share < 1.6e7f ? (int)share + (tight ? 1 : 0) : 1 << 24);
+    if (!tight)
+      while (units_of(size) > (float)p.splits) size += max(1, size >> 4);
+    chunk = __builtin_amdgcn_readfirstlane(size) * 64;
+    int before = 0;   // pieces of the sequences before this group of 64
+    for (int64_t base = 0; base < p.n; base += 64) {
+      const int mine = length(base + lane);
+      const int n = (int)((uint32_t)(mine + chunk - 1) / (uint32_t)chunk);
+      const int upto = wave_prefix_sum(n);   // pieces of this group's sequences up to the lane's
+      const bool here = want >= 0 ? base + lane == want : (before + upto > place && base + lane < p.n);
+      const uint64_t hit = __ballot(here);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        seq = (int)base + l;
+        keys = __builtin_amdgcn_readlane(mine, l);
+        count = __builtin_amdgcn_readlane(n, l);
+        first = before + __builtin_amdgcn_readlane(upto, l) - count;
+        return;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+};
 
 // What a workgroup works on: its split, sequence, rows [r0, r0 + BM) of the
 // sequence's (row r: token r / pack, head hd * pack + r % pack), and key tiles.
 struct Item {
   Seq s;
   int rows, r0;
-  int split, hd, kv_head;
+  int split, piece, hd, kv_head;   // piece: over all sequences (Pieces)
   int sure;     // keys that every row of the workgroup sees
   int t0, t1;   // its tiles of KEYS keys
 };
@@ -133,18 +201,37 @@ struct Item {
 template <int BM, int KEYS>
 __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
   // Tiles of a head lie together, and each XCD (workgroups are dealt to them in
-  // turn) takes a contiguous run, so that its L2 serves a head's keys once.
+  // turn) takes a contiguous run, so that its L2 serves a head's keys once. Splits
+  // share no keys: all heads of the same keys, which lie side by side, come first.
   const uint32_t total = gridDim.x, pid = blockIdx.x;
-  const uint32_t per = total >> 3, rest = total & 7, xcd = pid & 7;
-  const uint32_t lid = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3);
-  const uint32_t item = lid / (uint32_t)p.splits;
-  it.split = (int)(lid - item * p.splits);
-  it.hd = (int)(item / (uint32_t)p.tiles);   // head, or key head where heads share rows
-  int tile = (int)(item - it.hd * p.tiles);
+  int tile;
+  if (p.splits > 1) {
+    const uint32_t hds = (uint32_t)p.heads / (uint32_t)p.pack, item = pid / hds;
+    tile = (int)(item / (uint32_t)p.splits);
+    it.hd = (int)(pid - item * hds);
+    it.split = (int)(item - tile * p.splits);
+  } else {
+    const uint32_t per = total >> 3, rest = total & 7, xcd = pid & 7;
+    const uint32_t lid = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3);
+    it.split = 0;
+    it.hd = (int)(lid / (uint32_t)p.tiles);   // head, or key head where heads share rows
+    tile = (int)(lid - it.hd * p.tiles);
+  }
   it.kv_head = p.pack > 1 ? it.hd : it.hd / p.group;
   Seq s = {};
   int tiles;   // of the sequence
-  if (p.cu_q) {
+  Pieces pc = {};
+  const bool ragged = p.lengths && p.splits > 1;
+  if (ragged) {
+    pc = Pieces(p, -1, it.split);
+    if (pc.seq < 0) return false;
+    it.piece = it.split;
+    it.split -= pc.first;
+    tiles = p.tiles;
+    s.b = pc.seq;
+    s.qn = (int)p.q_rows;
+    s.kn = pc.keys;
+  } else if (p.cu_q) {
     // Sequence i has the tile slots from first_row(i) * pack / BM + i on: at least
     // as many as its rows need, and its own.
     const int slot = tile;
@@ -189,8 +276,9 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
     it.sure = min(s.kn, max(0, s.kn - s.qn + first_tok + 1));
   }
   const int tiles_k = (seen + KEYS - 1) / KEYS;
-  it.t0 = (int)((int64_t)tiles_k * it.split / p.splits);
-  it.t1 = (int)((int64_t)tiles_k * (it.split + 1) / p.splits);
+  const int chunk = ragged ? pc.chunk / KEYS : (tiles_k + p.splits - 1) / p.splits;
+  it.t0 = min(tiles_k, it.split * chunk);
+  it.t1 = min(tiles_k, it.t0 + chunk);
   return true;
 }
 
@@ -232,9 +320,10 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, const Item& it, con
   if (qr.r >= it.rows) return;
   const int64_t row = (it.s.b * p.q_rows + it.s.q0 + qr.tok) * p.heads + qr.head;
   if (p.splits > 1) {
-    const int64_t all = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;
-    float* const po = p.part + (it.split * all + row) * D;
-    float* const ml = p.part + (int64_t)p.splits * all * D + (it.split * all + row) * 2;
+    const int64_t all = (p.cu_q || p.lengths ? 1 : p.n) * p.q_rows * p.heads;   // rows of a split
+    const int64_t at = p.lengths ? it.piece * all + (int64_t)qr.tok * p.heads + qr.head : it.split * all + row;
+    float* const po = p.part + at * D;
+    float* const ml = p.part + (int64_t)p.splits * all * D + at * 2;
     if (half == 0) {
       ml[0] = m;
       ml[1] = sum;
@@ -486,10 +575,10 @@ __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
 // Measured, one token of 56 heads over 131072 keys of 8 heads (537 MB): key tiles
 // through LDS DMA by single waves 208 us, straight to registers 123 us and 16 us for
 // joining 256 splits.
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void attention_few(AttnArgs p) {
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void attention_few(AttnArgs p) {
   typedef typename Mfma<T>::V V8;
-  constexpr int BM = 32, KEYS = 32, WAVES = 4;
+  constexpr int BM = 32, KEYS = 32;
   constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32;
   constexpr int KD = D / 16, DB = D / 32;
   constexpr int NVL = KEYS * ROW / 1024;   // 16-byte loads of V per lane and tile
@@ -580,8 +669,9 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttnArgs p) {
     asm volatile("" ::: "memory");
   }
   // Wave 2 into 0 and 3 into 1, then 1 into 0: a wave's o takes 128 * D bytes, two tiles.
+  if (WAVES > 1 && it.t0 < it.t1) {
 #pragma unroll
-  for (int from = 2; from >= 1; --from) {
+  for (int from = WAVES / 2; from >= 1; from /= 2) {
     const int slot = from == 2 ? wave & 1 : 0;
     float* const po = reinterpret_cast<float*>(smem_all + slot * 2 * TILE);
     __syncthreads();   // the tiles, and what the round before left, have been read
@@ -614,6 +704,7 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttnArgs p) {
         }
     }
   }
+  }
   if (wave == 0) store_row<T, D>(p, it, qr, m, l, o, half);
 }
 
@@ -621,13 +712,23 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttnArgs p) {
 // threads hold a split's columns, and the groups of them take every G-th split,
 // then are added in order, so that the result does not depend on timing.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void join_splits(const float* __restrict__ part, uint16_t* __restrict__ out,
-                                                   int64_t rows, int splits, float c) {
+__global__ __launch_bounds__(256) void join_splits(AttnArgs p) {
   constexpr int LANES = D / 4, G = 256 / LANES;
   __shared__ float weight[256];
   __shared__ float4 sums[G][LANES];
   const int64_t row = blockIdx.x;
-  const float2* const ml = reinterpret_cast<const float2*>(part + (int64_t)splits * rows * D);
+  const int64_t rows = (p.cu_q || p.lengths ? 1 : p.n) * p.q_rows * p.heads;   // of a split
+  const float* const part = p.part;
+  const float2* const ml = reinterpret_cast<const float2*>(part + (int64_t)p.splits * rows * D);
+  // The row of its first split, and how many it has.
+  int64_t at0 = row;
+  int splits = p.splits;
+  if (p.lengths) {
+    const int64_t seq = row / rows;
+    const Pieces pc(p, seq, 0);
+    at0 = pc.first * rows + (row - seq * rows);
+    splits = pc.count;
+  }
   const int t = threadIdx.x, at = t % LANES, g = t / LANES;
   // Every wave finds the maximum and the sum by itself (at most 256 splits).
   float2 v[4];
@@ -635,14 +736,14 @@ __global__ __launch_bounds__(256) void join_splits(const float* __restrict__ par
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = 64 * i + (t & 63);
-    v[i] = s < splits ? ml[s * rows + row] : make_float2(0.0f, 0.0f);
+    v[i] = s < splits ? ml[at0 + s * rows] : make_float2(0.0f, 0.0f);
     if (v[i].y != 0.0f) m = fmaxf(m, v[i].x);
   }
   m = wave_max(m);
   float l = 0.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float w = v[i].y != 0.0f ? __builtin_amdgcn_exp2f((v[i].x - m) * c) : 0.0f;
+    const float w = v[i].y != 0.0f ? __builtin_amdgcn_exp2f((v[i].x - m) * p.c) : 0.0f;
     weight[64 * i + (t & 63)] = w;   // the same value from each wave
     l += w * v[i].y;
   }
@@ -652,7 +753,7 @@ __global__ __launch_bounds__(256) void join_splits(const float* __restrict__ par
   for (int s = g; s < splits; s += G) {
     const float w = weight[s];
     if (w == 0.0f) continue;   // not written where the split had no keys
-    const float4 x = *reinterpret_cast<const float4*>(part + (s * rows + row) * D + 4 * at);
+    const float4 x = *reinterpret_cast<const float4*>(part + (at0 + s * rows) * D + 4 * at);
     o.x += w * x.x;
     o.y += w * x.y;
     o.z += w * x.z;
@@ -670,17 +771,19 @@ __global__ __launch_bounds__(256) void join_splits(const float* __restrict__ par
     o.w += x.w;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<uint2*>(out + row * D + 4 * at) =
+  *reinterpret_cast<uint2*>(p.out + row * D + 4 * at) =
       make_uint2(Mfma<T>::pack(o.x * inv, o.y * inv), Mfma<T>::pack(o.z * inv, o.w * inv));
 }
 
 // How a call is laid over the GPU.
 struct Plan {
-  int pack, rows, splits;  // query heads per tile row space, rows per tile
-  int64_t tiles;           // row tiles per head in all
+  int pack, rows, waves, piece, splits;  // heads that share rows; a workgroup's rows, waves, least keys of a split
+  int64_t tiles, want;     // row tiles per head in all (pieces: of a sequence); workgroups to aim at
+  bool pieces = false;     // splits counts pieces of all sequences
 };
 
-Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, bool packed, int heads, int kv_heads) {
+Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int kind, int heads, int kv_heads) {
+  const bool packed = kind == LR_ATTN_PACKED;
   const int group = heads / kv_heads;
   const int64_t mean_q = packed ? (n > 0 ? q_rows / n : 0) : q_rows;   // rows per sequence
   const int64_t mean_k = packed ? (n > 0 ? k_rows / n : 0) : k_rows;
@@ -688,16 +791,33 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, bool packed, int heads, int
   // Query heads share a tile's rows where their tokens leave most of it empty.
   pl.pack = mean_q * group <= 128 && q_rows * group < (1LL << 31) ? group : 1;
   pl.rows = mean_q * pl.pack <= 32 ? 32 : 128;
-  const int64_t slots = kMaxBlocks;
   pl.tiles = packed ? q_rows * pl.pack / pl.rows + n + 2
                     : n * ((q_rows * pl.pack + pl.rows - 1) / pl.rows);
   const int64_t work = pl.tiles * (heads / pl.pack);
-  const int64_t want = 2 * compute_units();   // workgroups that are resident at once
-  int64_t s = work > 0 ? want / work : 1;
-  const int64_t most = mean_k / 256;   // at least 256 keys each
+  // The workgroups that are resident at once: two of four waves per CU, or eight of
+  // one. Single waves start and end faster, four joined leave fewer pieces to the
+  // second kernel: one token over eight caches of up to 5000 keys takes 23.3 us with
+  // single waves and 28.9 with four, over one of 131072 keys 123 us either way and
+  // then 16 or 5.8 us for the join. So four from 512 keys per wave up.
+  const int64_t cus = compute_units();
+  pl.waves = pl.rows == 32 && mean_k * work < 512 * 8 * cus ? 1 : 4;
+  pl.want = (pl.waves == 1 ? 8 : 2) * cus;
+  pl.piece = pl.waves == 1 ? 128 : 256;
+  int64_t s = work > 0 ? pl.want / work : 1;
+  const int64_t most = mean_k / pl.piece;
   s = s < most ? s : most;
-  pl.splits = (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
-  while (pl.splits > 1 && work * pl.splits > slots) --pl.splits;
+  pl.splits = (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
+  if (kind == LR_ATTN_LENGTHS && pl.splits > 1) {
+    // Places of a list of pieces over all sequences: as many as fill the GPU (one
+    // workgroup more would take a second round), n of them for the last pieces.
+    pl.pieces = true;
+    pl.tiles /= n;
+    const int64_t places = pl.want / (pl.tiles * (heads / pl.pack));
+    const int64_t all = n + n * (most < kMaxSplits ? most : kMaxSplits);
+    pl.splits = (int)(places > all ? all : (places > n ? places : n + 1));
+    return pl;
+  }
+  while (pl.splits > 1 && work * pl.splits > kMaxBlocks) --pl.splits;
   return pl;
 }
 
@@ -705,13 +825,14 @@ template <typename T, int D>
 int launch(AttnArgs p, const Plan& pl, hipStream_t s) {
   const int64_t grid = pl.tiles * (p.heads / pl.pack) * pl.splits;
   LR_REQUIRE(grid <= kMaxBlocks, "attention: %lld workgroups are not supported", (long long)grid);
-  if (pl.rows == 32) attention_few<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
+  if (pl.rows == 32 && pl.waves == 1) attention_few<T, D, 1><<<(unsigned)grid, 64, 0, s>>>(p);
+  else if (pl.rows == 32) attention_few<T, D, 4><<<(unsigned)grid, 256, 0, s>>>(p);
   else attention<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
   if (int rc = check_launch("attention")) return rc;
   if (pl.splits == 1) return LR_OK;
-  const int64_t rows = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;
+  const int64_t rows = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;   // of the output
   LR_REQUIRE(rows <= kMaxBlocks, "attention: %lld rows are not supported", (long long)rows);
-  join_splits<T, D><<<(unsigned)rows, 256, 0, s>>>(p.part, p.out, rows, pl.splits, p.c);
+  join_splits<T, D><<<(unsigned)rows, 256, 0, s>>>(p);
   return check_launch("attention");
 }
 
@@ -727,10 +848,10 @@ int by_dim(const AttnArgs& p, int dim, const Plan& pl, hipStream_t s) {
 
 using namespace lr;
 
-extern "C" int lr_attention_splits(int64_t sequences, int64_t q_rows, int64_t k_rows, int packed, int heads,
+extern "C" int lr_attention_splits(int64_t sequences, int64_t q_rows, int64_t k_rows, int kind, int heads,
                                    int kv_heads) {
   if (sequences <= 0 || q_rows <= 0 || k_rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 1;
-  return plan(sequences, q_rows, k_rows, packed != 0, heads, kv_heads).splits;
+  return plan(sequences, q_rows, k_rows, kind, heads, kv_heads).splits;
 }
 
 extern "C" int lr_attention(const void* q, const void* k, const void* v, void* out, int dtype, int64_t sequences,
@@ -759,7 +880,6 @@ extern "C" int lr_attention(const void* q, const void* k, const void* v, void* o
   // A tile's keys are addressed by 32-bit byte offsets from its first one.
   LR_REQUIRE(strides[3] < (1LL << 23) && strides[6] < (1LL << 23),
              "attention: strides of 2^23 and more between keys or values are not supported");
-  LR_REQUIRE(splits >= 1 && splits <= 256, "attention: %d splits", splits);
   AttnArgs p = {};
   p.q = static_cast<const uint16_t*>(q);
   p.k = static_cast<const uint16_t*>(k);
@@ -784,15 +904,24 @@ extern "C" int lr_attention(const void* q, const void* k, const void* v, void* o
   __builtin_memcpy(&scale, &scale_bits, sizeof scale);
   p.c = scale * 1.4426950408889634f;
   LR_REQUIRE(p.c > 0.0f && isfinite(p.c), "attention: the scale must be positive and finite");
-  Plan pl = plan(sequences, q_rows, k_rows, packed, heads, kv_heads);
+  Plan pl = plan(sequences, q_rows, k_rows, packed ? LR_ATTN_PACKED : (key_lengths ? LR_ATTN_LENGTHS : LR_ATTN_DENSE),
+                 heads, kv_heads);
+  LR_REQUIRE(splits >= 1 && (splits == 1 || splits <= (pl.splits > kMaxSplits ? pl.splits : kMaxSplits)),
+             "attention: %d splits", splits);
+  if (key_lengths && splits > 1)
+    LR_REQUIRE(pl.pieces && splits == pl.splits, "attention: with key lengths, 1 or the %d splits of lr_attention_splits",
+               pl.splits);
+  else if (pl.pieces)   // one split: whole sequences
+    pl.tiles *= sequences;
   pl.splits = splits;
   p.pack = pl.pack;
   LR_REQUIRE(pl.tiles < (1LL << 31), "attention: %lld row tiles are not supported", (long long)pl.tiles);
   p.tiles = (int)pl.tiles;
-  p.seq_tiles = packed ? 0 : (int)(pl.tiles / sequences);
+  p.seq_tiles = packed || (key_lengths && splits > 1) ? 0 : (int)(pl.tiles / sequences);
+  p.piece = pl.piece;
   p.splits = splits;
   if (splits > 1) {
-    const int64_t rows = (packed ? 1 : sequences) * q_rows * heads;
+    const int64_t rows = (packed || key_lengths ? 1 : sequences) * q_rows * heads;
     LR_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= splits * rows * (head_dim + 2) * 4,
                "attention: %d splits need a workspace of %lld bytes", splits,
                (long long)(splits * rows * (head_dim + 2) * 4));

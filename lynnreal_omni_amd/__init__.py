@@ -12,6 +12,10 @@ Drop-in modules with the reference's call surface:
   acceleration        fastest_available, optional_kernel_failure
                                                           (model/acceleration.py)
   flash_int8          the Flash W8A8 shard format loader  (model/flash_int8.py)
+Beside them, without a counterpart there:
+  mxfp4               Mxfp4Linear, quantize_transformer (4-bit projections)
+  mxfp4_gemm          mxfp4_matmul, tile_scales; kernels.quantize_rows_mxfp4
+  attention           attention, attention_packed, block_attention
 All compute runs in liblynnreal_amd.so (hand-written HIP for gfx950, C ABI in
 include/lynnreal_amd.h); there is no CPU or Triton fallback.
 """

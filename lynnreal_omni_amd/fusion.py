@@ -38,15 +38,16 @@ import torch
 
 from . import kernels as k
 from .int8 import Int8Linear
+from .mxfp4 import Mxfp4Linear
 
 
 @dataclass
 class ChainLayers:
-    """The four W8A8 projections of a block."""
-    to_qkv: Int8Linear
-    to_out: Int8Linear
-    up: Int8Linear
-    down: Int8Linear
+    """The four projections of a block, all W8A8 or all MXFP4."""
+    to_qkv: Int8Linear | Mxfp4Linear
+    to_out: Int8Linear | Mxfp4Linear
+    up: Int8Linear | Mxfp4Linear
+    down: Int8Linear | Mxfp4Linear
 
 
 @torch.inference_mode()
@@ -62,8 +63,12 @@ def projection_chain(hidden_states, layers: ChainLayers, norm1, norm2, table, in
 
     hidden_states bf16 [B, T, D]; attention_output bf16 [B, T, D] (stand-in for
     the attention result); table bf16 [R, 6D]; indices int64 [T].
-    attention_quantized: optional precomputed (q, s) of the QKV input.
+    attention_quantized: optional precomputed (q, s) of the QKV input (W8A8).
     """
+    if isinstance(layers.to_qkv, Mxfp4Linear):
+        if attention_quantized is not None:
+            raise ValueError("attention_quantized belongs to W8A8 layers")
+        return _mxfp4_chain(hidden_states, layers, norm1, norm2, table, indices, attention_output, ffn)
     shape = hidden_states.shape[:-1]
     q, s = attention_quantized or attention_input(hidden_states, norm1, table, indices)
     qkv = layers.to_qkv.forward_quantized(q, s, shape)
@@ -83,6 +88,21 @@ def projection_chain(hidden_states, layers: ChainLayers, norm1, norm2, table, in
     x2 = layers.down.forward_quantized(q3, s3, shape, residual=x1, table=table, indices=indices,
                                        gate_slot=5)
     return qkv, x1, x2
+
+
+def _mxfp4_chain(x, layers, norm1, norm2, table, indices, attention_output, ffn):
+    """projection_chain of MXFP4 layers: the norms write bf16, the layers quantize
+    their own inputs, GELU and the gated residuals run in the products' epilogues."""
+    qkv = layers.to_qkv(k._rms_adaln(x, norm1, table, indices, 0, 1))
+    x1 = layers.to_out(attention_output, residual=x, table=table, indices=indices, gate_slot=2)
+    h = k._rms_adaln(x1, norm2, table, indices, 3, 4)
+    if ffn == "gelu_tanh":
+        h = layers.up(h, activation="gelu_tanh")
+    elif ffn == "swiglu":
+        h = k._swiglu(layers.up(h))
+    else:
+        raise ValueError(f"unknown FFN activation {ffn!r}")
+    return qkv, x1, layers.down(h, residual=x1, table=table, indices=indices, gate_slot=5)
 
 
 # ----------------------------------------------------------------------------
@@ -114,7 +134,7 @@ def _diffusers_attention():
 
 
 def _fp32_attention(query, key, value, attention_mask, processor):
-    """Stand-in when diffusers is absent (attention is outside this package):
+    """Stand-in when diffusers is absent and enable_fusion was given no attention:
     scaled dot-product attention over [batch, sequence, heads, head_dim]
     computed in fp32 and returned in the query's dtype."""
     q, kk, v = (t.transpose(1, 2).float().contiguous() for t in (query, key, value))
@@ -133,7 +153,8 @@ class FusedAttention:
     from attn.to_qkv (or to_q/to_k/to_v); Q and K go through one
     kernels.qk_norm_rope launch on their strided views. `attention` (a
     callable (query, key, value, mask, processor) -> [B, S, H, Dh]) defaults
-    to diffusers' dispatch_attention_fn with the original processor's backend.
+    to diffusers' dispatch_attention_fn with the original processor's backend;
+    attention.block_attention is this package's own kernel.
     """
 
     def __init__(self, original, ordered_qk=False, attention=None):
@@ -220,6 +241,8 @@ def fused_block(self, hidden_states, temb, adaln_indices, rotary_emb, attention_
         out = down.forward_quantized(rows, scales, projected.shape[:-1], residual=hidden_states,
                                      table=table, indices=adaln_indices, gate_slot=5)
         return out
+    if isinstance(down, Mxfp4Linear):
+        return down(k._swiglu(projected), residual=hidden_states, table=table, indices=adaln_indices, gate_slot=5)
     if quant and hasattr(down, "forward_quantized"):
         rows, scales = k._swiglu_quant_int8(projected)
         output = down.forward_quantized(rows, scales, projected.shape[:-1])
@@ -268,8 +291,10 @@ def enable_fusion(transformer, fused_quant=False, attention=None):
     activation quantization into the norms and SwiGLU and marks every
     Int8Linear fused_ops; the residual + norm2 + quant kernel
     (residual_rms_quant) then runs as well (the reference limits it to Hopper;
-    here it is a gfx950 kernel). `attention` optionally replaces the attention
-    call of FusedAttention. Enabling again keeps the original native forward.
+    here it is a gfx950 kernel). Mxfp4Linear layers quantize their own inputs,
+    fused_quant or not. `attention` optionally replaces the attention call of
+    FusedAttention (attention.block_attention: the HIP kernel). Enabling again
+    keeps the original native forward.
     """
     blocks = list(transformer.transformer_blocks)
     if any(getattr(block, name, 1) != 1 for block in blocks for name in _DENSE_MATH):

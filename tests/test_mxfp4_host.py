@@ -109,3 +109,25 @@ def test_entry_points_refuse_without_a_gpu():
         assert linear(**bad) == _lib.LR_EINVAL, bad
     assert linear(m=0, s=None, sb=0) == _lib.LR_OK
     assert mxfp4_gemm._scratch(3, 64) == 768
+
+
+def test_quantize_transformer():
+    from test_host import _fake_transformer
+    t = _fake_transformer()
+    b1 = t.transformer_blocks[1]
+    q, k, v = b1.attn.to_q, b1.attn.to_k, b1.attn.to_v
+    report = mxfp4.quantize_transformer(t, protected_edges=1)
+    assert report["quantized_blocks"] == [1, 2] and report["quantized_linears"] == 8
+    for i, b in enumerate(t.transformer_blocks):
+        assert b.attn.to_q is None and b.attn.fused_projections
+        for layer in (b.attn.to_qkv, b.attn.to_out[0], b.ff.net[0].proj, b.ff.net[2]):
+            assert isinstance(layer, mxfp4.Mxfp4Linear) == (i in (1, 2))
+    codes, scale = mxfp4.quantize_weight(torch.cat([q.weight, k.weight, v.weight]))
+    assert torch.equal(b1.attn.to_qkv.weight_codes, codes)
+    assert torch.equal(b1.attn.to_qkv.weight_scale, mxfp4_gemm.tile_scales(scale))
+    with pytest.raises(ValueError, match="unconverted"):
+        mxfp4.quantize_transformer(t)
+    with pytest.raises(ValueError, match="protected"):
+        mxfp4.quantize_transformer(_fake_transformer(blocks=2), protected_edges=1)
+    again = mxfp4.Mxfp4Linear.from_packed(codes, scale, b1.attn.to_qkv.bias, in_features=q.in_features)
+    again.load_state_dict(b1.attn.to_qkv.state_dict())

@@ -4,8 +4,9 @@
 //   s = scale * q . k;  m' = max(m, s);  p = 2^(log2(e) (s - m'));
 //   l = l 2^(log2(e) (m - m')) + sum p;  o = o 2^(log2(e) (m - m')) + p V
 // and o / l at the end (0 where a row sees no key). Scores, m, l and o are fp32;
-// p is rounded to the inputs' type for the second product (l adds the unrounded
-// p), and o / l once at the end.
+// p is rounded to the inputs' type for the second product, and o / l once at the end.
+// l adds the rounded p (in fp32, by a dot product with ones): the weights p / l then
+// add up to one, and a rounding error of p counts with v - o instead of v.
 //
 // Both products run transposed on the 32x32x16 MFMA, S^T = K Q^T and O^T = V^T P^T:
 // lane l then holds keys of query l % 32 only, so maxima and sums are over a
@@ -79,6 +80,9 @@ template <> struct Mfma<__bf16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf2(a, b); }
+  static __device__ __forceinline__ float add2(uint32_t w, float l) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3f803f80u), l, false);
+  }
 };
 template <> struct Mfma<_Float16> {
   typedef v8h V;
@@ -90,6 +94,9 @@ template <> struct Mfma<_Float16> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const v2h h = {(_Float16)a, (_Float16)b};
     return __builtin_bit_cast(uint32_t, h);
+  }
+  static __device__ __forceinline__ float add2(uint32_t w, float l) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), l, false);
   }
 };
 
@@ -368,7 +375,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, const Item& it, con
 // are 62% busy: the chip's power is the bound, as for a large bf16 matrix product
 // (1505 TFLOP/s on the same card). 64 rows per wave and one wave per SIMD halves
 // the LDS reads and was slower (869 against 734 us on 8 heads), reading V by asm
-// blocks with their waits too (4.32 ms), sums by a dot product with ones level.
+// blocks with their waits too (4.32 ms).
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
   typedef typename Mfma<T>::V V8;
@@ -445,8 +452,8 @@ __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
     const int kc = j >> 2, w = j & 3, e = (kc & 1) * 8 + 2 * w;
     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kc >> 1][e], p.c, -off));
     const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kc >> 1][e + 1], p.c, -off));
-    l += p0 + p1;
     pk[kc][w] = Mfma<T>::pack(p0, p1);
+    l = Mfma<T>::add2(pk[kc][w], l);
     asm volatile("" : "+v"(pk[kc][w]), "+v"(l));
   };
   auto masked = [&](v16f (&nx)[2], int t) {
@@ -649,8 +656,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few(AttnArgs p) {
     for (int e = 0; e < 16; e += 2) {
       const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.c, -off));
       const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e + 1], p.c, -off));
-      l += p0 + p1;
       pk[e >> 1] = Mfma<T>::pack(p0, p1);
+      l = Mfma<T>::add2(pk[e >> 1], l);
     }
     // The wave's own writes are done before its reads: LDS operations of a wave
     // stay in order.

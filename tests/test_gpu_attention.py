@@ -1,8 +1,8 @@
 """GPU parity of the attention with the formula in 64 bits.
 
 Tolerance. With P the exact softmax row and eps = finfo(dtype).eps / 2 the half
-step of the inputs' type: rounding each weight to the type moves the output by at
-most eps * sum P |v|; the fp32 scores (D + 2 additions and products, each off by
+step of the inputs' type: rounding each weight to the type moves the sum over v by
+at most eps * sum P |v| and the sum of the weights, which divides it, by eps; the fp32 scores (D + 2 additions and products, each off by
 at most 2^-23 of sum |q k| * scale where the matrix unit truncates) and the
 exponential (an error of 2^-22 and, through its argument, the score's) move a
 weight by the factor 2 * ds + 2^-21 with ds = (D + 2) * 2^-23 * scale * sum |q k|;
@@ -39,7 +39,7 @@ def formula(q, k, v, scale, seen):
     ds = (q.shape[-1] + 2) * 2.0 ** -23 * torch.where(seen, size, 0.0).amax(-1, keepdim=True) if s.shape[-1] else 0.0
     o = p @ v
     pv = p @ v.abs()
-    bound = eps * o.abs() + (eps + 2 * ds + 2.0 ** -21 + 3 * 2.0 ** -24 * s.shape[-1]) * pv * 1.01
+    bound = 2 * eps * o.abs() + (eps + 2 * ds + 2.0 ** -21 + 3 * 2.0 ** -24 * s.shape[-1]) * pv * 1.01
     # fp16 weights far below the largest, and outputs below the normal numbers.
     bound = bound + 2.0 ** -32 * (seen.double() @ v.abs()) + torch.finfo(dtype).smallest_normal * eps
     return o.transpose(0, 1), bound.transpose(0, 1)

@@ -207,21 +207,24 @@ struct Item {
 // Everything fits 32 bits: workgroups are fewer than 2^24, rows than 2^31 (plan).
 template <int BM, int KEYS>
 __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
-  // Tiles of a head lie together, and each XCD (workgroups are dealt to them in
-  // turn) takes a contiguous run, so that its L2 serves a head's keys once. Splits
-  // share no keys: all heads of the same keys, which lie side by side, come first.
+  // Workgroups are dealt to the 8 XCDs in turn. Where all tiles cost the same, those of
+  // a head lie together and each XCD takes a contiguous run, so that its L2 serves a
+  // head's keys once. Where they do not (causal), the heads come first, so that
+  // the largest tiles of every head start before the small ones of any (with eight
+  // heads or a multiple an XCD then has heads of its own as well). Splits share no keys:
+  // all heads of the same ones, which lie side by side, come first.
   const uint32_t total = gridDim.x, pid = blockIdx.x;
   int tile;
-  if (p.splits > 1) {
+  if (p.splits > 1 || p.causal) {
     const uint32_t hds = (uint32_t)p.heads / (uint32_t)p.pack, item = pid / hds;
     tile = (int)(item / (uint32_t)p.splits);
-    it.hd = (int)(pid - item * hds);
+    it.hd = (int)(pid - item * hds);   // head, or key head where heads share rows
     it.split = (int)(item - tile * p.splits);
   } else {
     const uint32_t per = total >> 3, rest = total & 7, xcd = pid & 7;
     const uint32_t lid = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3);
     it.split = 0;
-    it.hd = (int)(lid / (uint32_t)p.tiles);   // head, or key head where heads share rows
+    it.hd = (int)(lid / (uint32_t)p.tiles);
     tile = (int)(lid - it.hd * p.tiles);
   }
   it.kv_head = p.pack > 1 ? it.hd : it.hd / p.group;
@@ -242,14 +245,17 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
     // Sequence i has the tile slots from first_row(i) * pack / BM + i on: at least
     // as many as its rows need, and its own.
     const int slot = tile;
-    auto start = [&](int64_t i) __attribute__((always_inline)) {
-      return (int)((uint32_t)(first_row(p, i) * p.pack) / BM) + (int)i;
+    auto start = [&](int i) __attribute__((always_inline)) {
+      return (int)((uint32_t)(first_row(p, i) * p.pack) / BM) + i;
     };
-    int64_t lo = 0, hi = p.n + 1;
+    // The last sequence whose first slot is not behind this one: the lanes probe 64
+    // places at once, so that a thousand sequences cost two loads in turn.
+    int lo = 0, hi = (int)p.n + 1;
     while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) >> 1;
-      if (start(mid) <= slot) lo = mid;
-      else hi = mid - 1;
+      const int step = (hi - lo + 64) >> 6, at = lo + (int)(threadIdx.x & 63) * step;
+      const uint64_t hit = __ballot(at <= hi && start(at) <= slot);
+      lo += (__builtin_popcountll(hit) - 1) * step;
+      hi = min(hi, lo + step - 1);
     }
     s.q0 = first_row(p, lo);
     s.qn = (int)clamp64(first_row(p, lo + 1) - s.q0, 0, p.q_rows);

@@ -127,7 +127,8 @@ def attention(query, key, value, *, causal=False, scale=None, key_lengths=None):
 def _first_rows(t, name):
     if t.dim() != 1 or t.numel() < 1 or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be int32 or int64 [sequences + 1]")
-    return t.to(torch.int32).contiguous()
+    # Clamped before the conversion, which would wrap what lies past 32 bits.
+    return (t.clamp(0, 2 ** 31 - 1).to(torch.int32) if t.dtype == torch.int64 else t).contiguous()
 
 
 def attention_packed(query, key, value, cu_query, cu_key=None, *, causal=False, scale=None):

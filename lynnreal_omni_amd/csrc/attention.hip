@@ -265,7 +265,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
       s.k0 = clamp64(p.cu_k[lo - 1], 0, p.k_rows);
       s.kn = (int)clamp64(clamp64(p.cu_k[lo], 0, p.k_rows) - s.k0, 0, p.k_rows);
     }
-    if (tile >= tiles) return false;
+    // (A list that is not in order can end the search at a sequence behind this slot.)
+    if (tile < 0 || tile >= tiles) return false;
   } else {
     tiles = p.seq_tiles;
     const int b = (int)((uint32_t)tile / (uint32_t)tiles);
@@ -684,39 +685,39 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few(AttnArgs p) {
   // Wave 2 into 0 and 3 into 1, then 1 into 0: a wave's o takes 128 * D bytes, two tiles.
   if (WAVES > 1 && it.t0 < it.t1) {
 #pragma unroll
-  for (int from = WAVES / 2; from >= 1; from /= 2) {
-    const int slot = from == 2 ? wave & 1 : 0;
-    float* const po = reinterpret_cast<float*>(smem_all + slot * 2 * TILE);
-    __syncthreads();   // the tiles, and what the round before left, have been read
-    if (wave >= from && wave < 2 * from) {
-      ml[slot][lane] = make_float2(m, l);
+    for (int from = WAVES / 2; from >= 1; from /= 2) {
+      const int slot = from == 2 ? wave & 1 : 0;
+      float* const po = reinterpret_cast<float*>(smem_all + slot * 2 * TILE);
+      __syncthreads();   // the tiles, and what the round before left, have been read
+      if (wave >= from && wave < 2 * from) {
+        ml[slot][lane] = make_float2(m, l);
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4*>(po + ((d * 4 + g) * 64 + lane) * 4) =
-              make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4*>(po + ((d * 4 + g) * 64 + lane) * 4) =
+                make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+      }
+      __syncthreads();
+      if (wave < from) {
+        const float2 other = ml[slot][lane];
+        const float mn = fmaxf(m, other.x);
+        const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c);
+        const float b = other.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((other.x - mn) * p.c);
+        m = mn;
+        l = l * a + other.y * b;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 x = *reinterpret_cast<const float4*>(po + ((d * 4 + g) * 64 + lane) * 4);
+            o[d][4 * g] = o[d][4 * g] * a + x.x * b;
+            o[d][4 * g + 1] = o[d][4 * g + 1] * a + x.y * b;
+            o[d][4 * g + 2] = o[d][4 * g + 2] * a + x.z * b;
+            o[d][4 * g + 3] = o[d][4 * g + 3] * a + x.w * b;
+          }
+      }
     }
-    __syncthreads();
-    if (wave < from) {
-      const float2 other = ml[slot][lane];
-      const float mn = fmaxf(m, other.x);
-      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c);
-      const float b = other.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((other.x - mn) * p.c);
-      m = mn;
-      l = l * a + other.y * b;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 x = *reinterpret_cast<const float4*>(po + ((d * 4 + g) * 64 + lane) * 4);
-          o[d][4 * g] = o[d][4 * g] * a + x.x * b;
-          o[d][4 * g + 1] = o[d][4 * g + 1] * a + x.y * b;
-          o[d][4 * g + 2] = o[d][4 * g + 2] * a + x.z * b;
-          o[d][4 * g + 3] = o[d][4 * g + 3] * a + x.w * b;
-        }
-    }
-  }
   }
   if (wave == 0) store_row<T, D>(p, it, qr, m, l, o, half);
 }
@@ -838,13 +839,14 @@ template <typename T, int D>
 int launch(AttnArgs p, const Plan& pl, hipStream_t s) {
   const int64_t grid = pl.tiles * (p.heads / pl.pack) * pl.splits;
   LR_REQUIRE(grid <= kMaxBlocks, "attention: %lld workgroups are not supported", (long long)grid);
+  const int64_t rows = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;   // of the output
+  LR_REQUIRE(pl.splits == 1 || rows <= kMaxBlocks, "attention: %lld rows are not supported with split keys",
+             (long long)rows);
   if (pl.rows == 32 && pl.waves == 1) attention_few<T, D, 1><<<(unsigned)grid, 64, 0, s>>>(p);
   else if (pl.rows == 32) attention_few<T, D, 4><<<(unsigned)grid, 256, 0, s>>>(p);
   else attention<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
   if (int rc = check_launch("attention")) return rc;
   if (pl.splits == 1) return LR_OK;
-  const int64_t rows = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;   // of the output
-  LR_REQUIRE(rows <= kMaxBlocks, "attention: %lld rows are not supported", (long long)rows);
   join_splits<T, D><<<(unsigned)rows, 256, 0, s>>>(p);
   return check_launch("attention");
 }

@@ -47,6 +47,8 @@ def test_lists():
         A.attention_packed(q, k, v, torch.zeros(2, 2, dtype=torch.int32))
     with pytest.raises(ValueError):
         A._first_rows(torch.zeros(3), "cu_query")
+    # What lies past 32 bits stays behind the last row instead of wrapping.
+    assert A._first_rows(torch.tensor([-2 ** 40, 5, 2 ** 40]), "cu_query").tolist() == [0, 5, 2 ** 31 - 1]
     with pytest.raises(ValueError):
         A._scale_bits(0.0)
     with pytest.raises(ValueError):

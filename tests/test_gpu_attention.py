@@ -189,6 +189,19 @@ def test_lists_that_lead_outside_are_clamped():
     assert torch.equal(A.attention_packed(q, k, v, torch.tensor([-7, 10, 4000], device="cuda")), want)
 
 
+@pytest.mark.parametrize("heads,kv_heads,rows", [(2, 2, 300), (8, 1, 40)])
+def test_lists_out_of_order_stay_inside(heads, kv_heads, rows):
+    """Lists that are not nondecreasing: any result, but nothing outside the output is written."""
+    q, k, v = tensors(rows, rows, heads, kv_heads, 64, torch.bfloat16, 7)
+    g = torch.Generator().manual_seed(rows)
+    size = q.numel()
+    for sequences in (1, 2, 70, 200):
+        cu = torch.randint(-9, rows + 9, (sequences + 1,), generator=g, dtype=torch.int32).cuda()
+        guarded = torch.full((3 * size,), 7.0, dtype=torch.bfloat16, device="cuda")
+        A._launch(q, k, v, guarded[size:2 * size].view(q.shape), sequences, rows, rows, cu, cu, None, False, None)
+        assert (guarded[:size] == 7).all() and (guarded[2 * size:] == 7).all()
+
+
 def test_long_rows_of_a_cache_past_32_bits():
     """Keys whose offsets pass 2^31 bytes, through the batch and the token stride."""
     size, heads, dim = 1 << 18, 8, 128

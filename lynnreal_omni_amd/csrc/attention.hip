@@ -48,8 +48,7 @@ struct AttnArgs {
   const int32_t* cu_k;
   const int32_t* lengths;  // valid keys per sequence of a dense batch, or null
   int64_t n, q_rows, k_rows;  // sequences; rows per sequence (dense) or in all (packed)
-  int heads, kv_heads, group;   // group = heads / kv_heads
-  int pack;              // query heads that share a tile's rows (group or 1)
+  int heads, kv_heads, group;   // group = heads / kv_heads: query heads that share a key head and a tile's rows
   int causal, splits;
   float c;               // scale * log2(e)
   int tiles, seq_tiles;  // row tiles per head in all (pieces: of a sequence), and of a dense batch's sequence
@@ -124,7 +123,8 @@ __device__ __forceinline__ V8 tr_pair(const char* a0, const char* a1) {
   return __builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-constexpr int kKeys = 64;        // keys per tile of a prompt
+constexpr int kRows = 128;       // rows per workgroup
+constexpr int kKeys = 64;        // keys per tile
 constexpr float kSlack = 8.0f;   // log2
 constexpr int kMaxSplits = 256;  // of a sequence
 
@@ -194,18 +194,21 @@ struct Pieces {
   }
 };
 
-// What a workgroup works on: its split, sequence, rows [r0, r0 + BM) of the
-// sequence's (row r: token r / pack, head hd * pack + r % pack), and key tiles.
+// What a workgroup works on: its split, sequence, rows [r0, r0 + kRows) of the
+// sequence's (row r: token r / group, head hd * group + r % group), and key tiles.
+// All heads that share a key head share its tiles, so that keys are read once for them,
+// a causal tile spans fewer tokens, and a few tokens leave less of it empty (eight packed
+// prompts of 40 heads over 8: 253 us with tiles of one head each, 236 so; one token of
+// them over 4096 keys: 27.0 and 13.0).
 struct Item {
   Seq s;
   int rows, r0;
-  int split, piece, hd, kv_head;   // piece: over all sequences (Pieces)
+  int split, piece, hd;   // piece: over all sequences (Pieces); hd: key head
   int sure;     // keys that every row of the workgroup sees
-  int t0, t1;   // its tiles of KEYS keys
+  int t0, t1;   // its tiles of kKeys keys
 };
 
-// Everything fits 32 bits: workgroups are fewer than 2^24, rows than 2^31 (plan).
-template <int BM, int KEYS>
+// Everything fits 32 bits: workgroups are fewer than 2^24, rows than 2^31 (lr_attention).
 __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
   // Workgroups are dealt to the 8 XCDs in turn. Where all tiles cost the same, those of
   // a head lie together and each XCD takes a contiguous run, so that its L2 serves a
@@ -216,9 +219,9 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
   const uint32_t total = gridDim.x, pid = blockIdx.x;
   int tile;
   if (p.splits > 1 || p.causal) {
-    const uint32_t hds = (uint32_t)p.heads / (uint32_t)p.pack, item = pid / hds;
+    const uint32_t hds = (uint32_t)p.kv_heads, item = pid / hds;
     tile = (int)(item / (uint32_t)p.splits);
-    it.hd = (int)(pid - item * hds);   // head, or key head where heads share rows
+    it.hd = (int)(pid - item * hds);
     it.split = (int)(item - tile * p.splits);
   } else {
     const uint32_t per = total >> 3, rest = total & 7, xcd = pid & 7;
@@ -227,7 +230,6 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
     it.hd = (int)(lid / (uint32_t)p.tiles);
     tile = (int)(lid - it.hd * p.tiles);
   }
-  it.kv_head = p.pack > 1 ? it.hd : it.hd / p.group;
   Seq s = {};
   int tiles;   // of the sequence
   Pieces pc = {};
@@ -242,11 +244,11 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
     s.qn = (int)p.q_rows;
     s.kn = pc.keys;
   } else if (p.cu_q) {
-    // Sequence i has the tile slots from first_row(i) * pack / BM + i on: at least
+    // Sequence i has the tile slots from first_row(i) * group / kRows + i on: at least
     // as many as its rows need, and its own.
     const int slot = tile;
     auto start = [&](int i) __attribute__((always_inline)) {
-      return (int)((uint32_t)(first_row(p, i) * p.pack) / BM) + i;
+      return (int)((uint32_t)(first_row(p, i) * p.group) / kRows) + i;
     };
     // The last sequence whose first slot is not behind this one: the lanes probe 64
     // places at once, so that a thousand sequences cost two loads in turn.
@@ -260,7 +262,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
     s.q0 = first_row(p, lo);
     s.qn = (int)clamp64(first_row(p, lo + 1) - s.q0, 0, p.q_rows);
     tile = slot - start(lo);
-    tiles = (int)((uint32_t)(s.qn * p.pack + BM - 1) / BM);
+    tiles = (int)((uint32_t)(s.qn * p.group + kRows - 1) / kRows);
     if (lo > 0 && lo <= p.n) {
       s.k0 = clamp64(p.cu_k[lo - 1], 0, p.k_rows);
       s.kn = (int)clamp64(clamp64(p.cu_k[lo], 0, p.k_rows) - s.k0, 0, p.k_rows);
@@ -278,19 +280,17 @@ __device__ __forceinline__ bool find_item(const AttnArgs& p, Item& it) {
   // Causal: the last tiles see the most keys and go first.
   if (p.causal) tile = tiles - 1 - tile;
   it.s = s;
-  it.rows = s.qn * p.pack;
-  it.r0 = tile * BM;
+  it.rows = s.qn * p.group;
+  it.r0 = tile * kRows;
   it.sure = s.kn;
   int seen = s.kn;
   if (p.causal) {
-    const int last = min(it.r0 + BM, it.rows) - 1;
-    const int last_tok = p.pack == 1 ? last : (int)((uint32_t)last / (uint32_t)p.pack);
-    const int first_tok = p.pack == 1 ? it.r0 : (int)((uint32_t)it.r0 / (uint32_t)p.pack);
-    seen = min(s.kn, max(0, s.kn - s.qn + last_tok + 1));
-    it.sure = min(s.kn, max(0, s.kn - s.qn + first_tok + 1));
+    const int last = min(it.r0 + kRows, it.rows) - 1;
+    seen = min(s.kn, max(0, s.kn - s.qn + (int)((uint32_t)last / (uint32_t)p.group) + 1));
+    it.sure = min(s.kn, max(0, s.kn - s.qn + (int)((uint32_t)it.r0 / (uint32_t)p.group) + 1));
   }
-  const int tiles_k = (seen + KEYS - 1) / KEYS;
-  const int chunk = ragged ? pc.chunk / KEYS : (tiles_k + p.splits - 1) / p.splits;
+  const int tiles_k = (seen + kKeys - 1) / kKeys;
+  const int chunk = ragged ? pc.chunk / kKeys : (tiles_k + p.splits - 1) / p.splits;
   it.t0 = min(tiles_k, it.split * chunk);
   it.t1 = min(tiles_k, it.t0 + chunk);
   return true;
@@ -302,8 +302,8 @@ struct QueryRow {
   int r, tok, head, limit;   // limit: keys that it sees
   __device__ __forceinline__ QueryRow(const AttnArgs& p, const Item& it, int row) : r(row) {
     const int rc = row < it.rows ? row : it.rows - 1;
-    tok = p.pack == 1 ? rc : (int)((uint32_t)rc / (uint32_t)p.pack);
-    head = p.pack == 1 ? it.hd : it.hd * p.pack + (rc - tok * p.pack);
+    tok = (int)((uint32_t)rc / (uint32_t)p.group);
+    head = it.hd * p.group + (rc - tok * p.group);
     off = it.s.b * p.qb + (it.s.q0 + tok) * p.qt + head * p.qh;
     limit = p.causal ? min(it.s.kn, max(0, it.s.kn - it.s.qn + tok + 1)) : it.s.kn;
   }
@@ -362,7 +362,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, const Item& it, con
                      Mfma<T>::pack(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
 }
 
-// ------------------------------------------------------------- prompts ----
+// -------------------------------------------------------------- kernel ----
 // Four waves of 32 rows; keys in tiles of 64 through two slots of LDS (K rows,
 // then V rows), by 16-byte DMA. A row's 16-byte chunk c lies in slot c ^ 2 * (row
 // / (256 / row bytes) % (row bytes / 32)): eight rows' equal 32-byte columns are
@@ -383,10 +383,14 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, const Item& it, con
 // (1505 TFLOP/s on the same card). 64 rows per wave and one wave per SIMD halves
 // the LDS reads and was slower (869 against 734 us on 8 heads), reading V by asm
 // blocks with their waits too (4.32 ms).
+// Few rows: what counts is the stream of keys, 64 KB in flight per workgroup; waves
+// without rows only load. One token of 56 heads over 131072 keys of 8 (537 MB): 106 us
+// with the join of 64 splits, 5.1 TB/s, as fast as a copy. Keys straight into
+// registers by waves that share nothing and meet no barrier: 129 us.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
   typedef typename Mfma<T>::V V8;
-  constexpr int BM = 128, WAVES = 4;
+  constexpr int WAVES = kRows / 32;
   constexpr int ROW = 2 * D;                     // bytes of a row
   constexpr int CH = ROW / 16;                   // chunks per row
   constexpr int RPB = 256 / ROW, PAIRS = ROW / 32;
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = lane >> 5, col = lane & 31;
   Item it;
-  if (!find_item<BM, kKeys>(p, it)) return;
+  if (!find_item(p, it)) return;
   const Seq s = it.s;
   const int t0 = it.t0, t1 = it.t1;
   const QueryRow qr(p, it, it.r0 + wave * 32 + col);
@@ -408,8 +412,8 @@ __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
 #pragma unroll
   for (int d = 0; d < KD; ++d) q[d] = *reinterpret_cast<const V8*>(p.q + qr.off + 16 * d + 8 * half);
 
-  const uint16_t* const kbase = p.k + s.b * p.kb + s.k0 * p.kt + it.kv_head * p.kh;
-  const uint16_t* const vbase = p.v + s.b * p.vb + s.k0 * p.vt + it.kv_head * p.vh;
+  const uint16_t* const kbase = p.k + s.b * p.kb + s.k0 * p.kt + it.hd * p.kh;
+  const uint16_t* const vbase = p.v + s.b * p.vb + s.k0 * p.vt + it.hd * p.vh;
   // DMA i of this wave: 1 KB of the tile's rows.
   uint32_t koff[DMAS], voff[DMAS];
 #pragma unroll
@@ -537,7 +541,20 @@ __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
   };
   auto advance = [&]() { off = move_max<DB>(max_with_partner(mx), m, l, o, p.c, kShift); };
 
-  if (t0 < t1) {
+  if (t0 < t1 && it.r0 + wave * 32 >= it.rows) {
+    // A wave without rows takes part in the loads and barriers alone.
+    issue(t0, 0);
+    publish();
+    issue(t0 + 1, 0);
+    issue(t0, 1);
+#pragma unroll 1
+    for (int t = t0; t + 1 < t1; ++t) {
+      publish();
+      issue(t + 2, 0);
+      issue(t + 1, 1);
+    }
+    publish();
+  } else if (t0 < t1) {
     // K(t + 1) and V(t) are used together; K(t0) alone first.
     issue(t0, 0);
     publish();
@@ -576,150 +593,6 @@ __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
     }
   }
   store_row<T, D>(p, it, qr, m, l, o, half);
-}
-
-// ---------------------------------------------------------- few queries ----
-// 32 rows (the heads that share a key head, times the new tokens) and a part of the
-// keys per workgroup. What counts is the stream of keys and values, so its four waves
-// share nothing and meet no barrier until their ends: each takes every fourth tile of
-// 32 keys straight into registers, K as the first product's fragments (lane: key l %
-// 32, 16 bytes), V row-major in 16-byte pieces that pass through the wave's own LDS
-// for the transposing read; the next tile's loads are in flight while this one is
-// worked on. Then the waves' o, m and l are joined in LDS, in a fixed order.
-// Measured, one token of 56 heads over 131072 keys of 8 heads (537 MB): key tiles
-// through LDS DMA by single waves 208 us, straight to registers 123 us and 16 us for
-// joining 256 splits.
-template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void attention_few(AttnArgs p) {
-  typedef typename Mfma<T>::V V8;
-  constexpr int BM = 32, KEYS = 32;
-  constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32;
-  constexpr int KD = D / 16, DB = D / 32;
-  constexpr int NVL = KEYS * ROW / 1024;   // 16-byte loads of V per lane and tile
-  constexpr int TILE = KEYS * ROW;         // a wave's V tile; two hold a wave's o
-  __shared__ __attribute__((aligned(1024))) char smem_all[WAVES * TILE];
-  __shared__ float2 ml[2][64];
-  constexpr float kShift = Mfma<T>::kShift;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int half = lane >> 5, col = lane & 31;
-  char* const smem = smem_all + wave * TILE;
-  Item it;
-  if (!find_item<BM, KEYS>(p, it)) return;
-  const Seq s = it.s;
-  const QueryRow qr(p, it, it.r0 + col);
-  V8 q[KD];
-#pragma unroll
-  for (int d = 0; d < KD; ++d) q[d] = *reinterpret_cast<const V8*>(p.q + qr.off + 16 * d + 8 * half);
-  const uint16_t* const kbase = p.k + s.b * p.kb + s.k0 * p.kt + it.kv_head * p.kh;
-  const uint16_t* const vbase = p.v + s.b * p.vb + s.k0 * p.vt + it.kv_head * p.vh;
-  const uint32_t koff = (uint32_t)(col * p.kt * 2 + 16 * half);
-  uint32_t voff[NVL];
-#pragma unroll
-  for (int i = 0; i < NVL; ++i) voff[i] = (uint32_t)((i * 64 + lane) / CH * p.vt * 2 + (i * 64 + lane) % CH * 16);
-  uint4 kr[KD], vr_[NVL];
-  auto load = [&](int t) {
-    const int left = min(KEYS, s.kn - t * KEYS);  // rows past the sequence's keys read as zero
-    const __amdgpu_buffer_rsrc_t rk =
-        row_rsrc(kbase + (int64_t)t * KEYS * p.kt, ((int64_t)(left - 1) * p.kt + D) * 2);
-    const __amdgpu_buffer_rsrc_t rv =
-        row_rsrc(vbase + (int64_t)t * KEYS * p.vt, ((int64_t)(left - 1) * p.vt + D) * 2);
-#pragma unroll
-    for (int d = 0; d < KD; ++d) kr[d] = buf_load16(rk, koff + 32 * d);
-#pragma unroll
-    for (int i = 0; i < NVL; ++i) vr_[i] = buf_load16(rv, voff[i]);
-  };
-  v16f o[DB];
-  float m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
-  const int i16 = lane & 15, vrow = 4 * half + (i16 >> 2);
-  if (it.t0 + wave < it.t1) load(it.t0 + wave);
-#pragma unroll 1
-  for (int t = it.t0 + wave; t < it.t1; t += WAVES) {
-    v16f sc;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < KD; ++d) sc = Mfma<T>::mul(__builtin_bit_cast(V8, kr[d]), q[d], sc);
-#pragma unroll
-    for (int i = 0; i < NVL; ++i) {
-      const int row = (i * 64 + lane) / CH, c = (i * 64 + lane) % CH ^ (row / RPB % PAIRS) * 2;
-      *reinterpret_cast<uint4*>(smem + row * ROW + c * 16) = vr_[i];
-    }
-    if (t + WAVES < it.t1) load(t + WAVES);
-    if ((t + 1) * KEYS > it.sure) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        sc[e] = t * KEYS + 8 * (e >> 2) + 4 * half + (e & 3) < qr.limit ? sc[e] : -INFINITY;
-    }
-    float mx = sc[0];
-#pragma unroll
-    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
-    const float off = move_max<DB>(max_with_partner(mx), m, l, o, p.c, kShift);
-    uint32_t pk[8];
-#pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.c, -off));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e + 1], p.c, -off));
-      pk[e >> 1] = Mfma<T>::pack(p0, p1);
-      l = Mfma<T>::add2(pk[e >> 1], l);
-    }
-    // The wave's own writes are done before its reads: LDS operations of a wave
-    // stay in order.
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int kc = 0; kc < 2; ++kc)
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const int c = 4 * d + 2 * ((lane >> 4) & 1) + (i16 >> 1 & 1);
-        const int row = 16 * kc + vrow, sub = (i16 & 1) * 8;
-        const V8 vf = tr_pair<V8>(smem + row * ROW + (c ^ (row / RPB % PAIRS) * 2) * 16 + sub,
-                                  smem + (row + 8) * ROW + (c ^ ((row + 8) / RPB % PAIRS) * 2) * 16 + sub);
-        const uint4 pw = make_uint4(pk[4 * kc], pk[4 * kc + 1], pk[4 * kc + 2], pk[4 * kc + 3]);
-        o[d] = Mfma<T>::mul(vf, __builtin_bit_cast(V8, pw), o[d]);
-      }
-    asm volatile("" ::: "memory");
-  }
-  // Wave 2 into 0 and 3 into 1, then 1 into 0: a wave's o takes 128 * D bytes, two tiles.
-  if (WAVES > 1 && it.t0 < it.t1) {
-#pragma unroll
-    for (int from = WAVES / 2; from >= 1; from /= 2) {
-      const int slot = from == 2 ? wave & 1 : 0;
-      float* const po = reinterpret_cast<float*>(smem_all + slot * 2 * TILE);
-      __syncthreads();   // the tiles, and what the round before left, have been read
-      if (wave >= from && wave < 2 * from) {
-        ml[slot][lane] = make_float2(m, l);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4*>(po + ((d * 4 + g) * 64 + lane) * 4) =
-                make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
-      }
-      __syncthreads();
-      if (wave < from) {
-        const float2 other = ml[slot][lane];
-        const float mn = fmaxf(m, other.x);
-        const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c);
-        const float b = other.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((other.x - mn) * p.c);
-        m = mn;
-        l = l * a + other.y * b;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float4 x = *reinterpret_cast<const float4*>(po + ((d * 4 + g) * 64 + lane) * 4);
-            o[d][4 * g] = o[d][4 * g] * a + x.x * b;
-            o[d][4 * g + 1] = o[d][4 * g + 1] * a + x.y * b;
-            o[d][4 * g + 2] = o[d][4 * g + 2] * a + x.z * b;
-            o[d][4 * g + 3] = o[d][4 * g + 3] * a + x.w * b;
-          }
-      }
-    }
-  }
-  if (wave == 0) store_row<T, D>(p, it, qr, m, l, o, half);
 }
 
 // Joins the splits of a row: weights 2^(c (m_s - max m)). A workgroup per row: D / 4
@@ -791,9 +664,9 @@ __global__ __launch_bounds__(256) void join_splits(AttnArgs p) {
 
 // How a call is laid over the GPU.
 struct Plan {
-  int pack, rows, waves, piece, splits;  // heads that share rows; a workgroup's rows, waves, least keys of a split
-  int64_t tiles, want;     // row tiles per head in all (pieces: of a sequence); workgroups to aim at
-  bool pieces = false;     // splits counts pieces of all sequences
+  int piece, splits;     // least keys of a piece; splits of the keys
+  int64_t tiles;         // row tiles per key head in all (pieces: of a sequence)
+  bool pieces = false;   // splits counts pieces of all sequences
 };
 
 Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int kind, int heads, int kv_heads) {
@@ -802,49 +675,53 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int kind, int heads, int kv
   const int64_t mean_q = packed ? (n > 0 ? q_rows / n : 0) : q_rows;   // rows per sequence
   const int64_t mean_k = packed ? (n > 0 ? k_rows / n : 0) : k_rows;
   Plan pl;
-  // Query heads share a tile's rows where their tokens leave most of it empty.
-  pl.pack = mean_q * group <= 128 && q_rows * group < (1LL << 31) ? group : 1;
-  pl.rows = mean_q * pl.pack <= 32 ? 32 : 128;
-  pl.tiles = packed ? q_rows * pl.pack / pl.rows + n + 2
-                    : n * ((q_rows * pl.pack + pl.rows - 1) / pl.rows);
-  const int64_t work = pl.tiles * (heads / pl.pack);
-  // The workgroups that are resident at once: two of four waves per CU, or eight of
-  // one. Single waves start and end faster, four joined leave fewer pieces to the
-  // second kernel: one token over eight caches of up to 5000 keys takes 23.3 us with
-  // single waves and 28.9 with four, over one of 131072 keys 123 us either way and
-  // then 16 or 5.8 us for the join. So four from 512 keys per wave up.
-  const int64_t cus = compute_units();
-  pl.waves = pl.rows == 32 && mean_k * work < 512 * 8 * cus ? 1 : 4;
-  pl.want = (pl.waves == 1 ? 8 : 2) * cus;
-  pl.piece = pl.waves == 1 ? 128 : 256;
-  int64_t s = work > 0 ? pl.want / work : 1;
-  const int64_t most = mean_k / pl.piece;
-  s = s < most ? s : most;
-  pl.splits = (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
+  pl.tiles = packed ? q_rows * group / kRows + n + 2 : n * ((q_rows * group + kRows - 1) / kRows);
+  const int64_t work = pl.tiles * kv_heads;
+  const int64_t tile_rows = mean_q * group < kRows ? mean_q * group : kRows;
+  // Workgroups to aim at. One wave's rows: two per CU, for the stream of keys (one token,
+  // 32768 keys, 8 heads of 64: 16.9 us, 19.8 with one). Several waves': one per CU, since
+  // two share its matrix units and leave twice the partial results (300 tokens, 4096
+  // keys, 8 heads: 20.0 us with 8 splits, 22.5 with 12).
+  const int64_t want = (tile_rows <= 32 ? 2 : 1) * compute_units();
+  // A split takes 1 us per tile of keys; joining s of them 2.8 us, and per row 0.6 ns and
+  // 0.15 ns per split (head_dim 128, from 12 shapes). So the best s is the root of
+  // tiles / (0.00015 rows), and one where joining costs more than it saves: 878 tokens,
+  // 8 heads, take 19.6 us as they are and 20.6 with 4 splits; 128 tokens, 40 heads, 4096
+  // keys 77.8 and 31.9 with 6. Two tiles per split at least (one token, 4096 keys, 8 heads:
+  // 11.2 us, 12.4 with one).
+  const double tiles_k = (double)((mean_k + kKeys - 1) / kKeys), rows = (double)((packed ? 1 : n) * q_rows * heads);
+  double s = sqrt(tiles_k / (0.00015 * rows));
+  s = fmin(fmin(s, tiles_k / 2), work > 0 ? (double)(want / work) : 1.0);
+  s = fmin(floor(s), kMaxSplits);
+  if (s > 1.0 && tiles_k / s + 2.8 + rows * (0.0006 + 0.00015 * s) > tiles_k) s = 1.0;
+  pl.splits = s > 1.0 ? (int)s : 1;
+  pl.piece = kKeys;
   if (kind == LR_ATTN_LENGTHS && pl.splits > 1) {
     // Places of a list of pieces over all sequences: as many as fill the GPU (one
-    // workgroup more would take a second round), n of them for the last pieces.
+    // workgroup more would take a second round), n of them for the last pieces. Pieces
+    // are at least as long as makes their partial results small beside their keys: 32
+    // rows over three caches of 4096, 16 heads: 31.3 us with 512 keys, 35.7 with 64; 5 rows
+    // over four of 512: 8.9 with 64, 9.7 with 128.
+    const int64_t keys = 16 * tile_rows / kKeys * kKeys;
+    pl.piece = (int)(keys < kKeys ? kKeys : (keys > 512 ? 512 : keys));
+    const int64_t most = mean_k / pl.piece;
     pl.pieces = true;
     pl.tiles /= n;
-    const int64_t places = pl.want / (pl.tiles * (heads / pl.pack));
+    const int64_t places = want / (pl.tiles * kv_heads);
     const int64_t all = n + n * (most < kMaxSplits ? most : kMaxSplits);
     pl.splits = (int)(places > all ? all : (places > n ? places : n + 1));
-    return pl;
   }
-  while (pl.splits > 1 && work * pl.splits > kMaxBlocks) --pl.splits;
   return pl;
 }
 
 template <typename T, int D>
 int launch(AttnArgs p, const Plan& pl, hipStream_t s) {
-  const int64_t grid = pl.tiles * (p.heads / pl.pack) * pl.splits;
+  const int64_t grid = pl.tiles * p.kv_heads * pl.splits;
   LR_REQUIRE(grid <= kMaxBlocks, "attention: %lld workgroups are not supported", (long long)grid);
   const int64_t rows = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;   // of the output
   LR_REQUIRE(pl.splits == 1 || rows <= kMaxBlocks, "attention: %lld rows are not supported with split keys",
              (long long)rows);
-  if (pl.rows == 32 && pl.waves == 1) attention_few<T, D, 1><<<(unsigned)grid, 64, 0, s>>>(p);
-  else if (pl.rows == 32) attention_few<T, D, 4><<<(unsigned)grid, 256, 0, s>>>(p);
-  else attention<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
+  attention<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
   if (int rc = check_launch("attention")) return rc;
   if (pl.splits == 1) return LR_OK;
   join_splits<T, D><<<(unsigned)rows, 256, 0, s>>>(p);
@@ -885,6 +762,8 @@ extern "C" int lr_attention(const void* q, const void* k, const void* v, void* o
   if (q_rows == 0 || (!packed && sequences == 0)) return LR_OK;
   LR_REQUIRE(q_rows < (1LL << 30) && k_rows < (1LL << 30) && sequences < (1LL << 30) && heads <= 65536,
              "attention: shapes past 2^30 rows or 65536 heads are not supported");
+  LR_REQUIRE(q_rows * (heads / kv_heads) < (1LL << 31) - kRows, "attention: %lld rows of a key head are not supported",
+             (long long)(q_rows * (heads / kv_heads)));
   LR_REQUIRE(q && out && (k_rows == 0 || (k && v)), "attention: null pointer");
   LR_REQUIRE(strides, "attention: null pointer");
   LR_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16),
@@ -929,7 +808,6 @@ extern "C" int lr_attention(const void* q, const void* k, const void* v, void* o
   else if (pl.pieces)   // one split: whole sequences
     pl.tiles *= sequences;
   pl.splits = splits;
-  p.pack = pl.pack;
   LR_REQUIRE(pl.tiles < (1LL << 31), "attention: %lld row tiles are not supported", (long long)pl.tiles);
   p.tiles = (int)pl.tiles;
   p.seq_tiles = packed || (key_lengths && splits > 1) ? 0 : (int)(pl.tiles / sequences);

@@ -6,7 +6,8 @@
 // and o / l at the end (0 where a row sees no key). Scores, m, l and o are fp32;
 // p is rounded to the inputs' type for the second product, and o / l once at the end.
 // l adds the rounded p (in fp32, by a dot product with ones): the weights p / l then
-// add up to one, and a rounding error of p counts with v - o instead of v.
+// add up to one, and a rounding error of p counts with v - o instead of v. Few rows
+// (FEW) leave the matrix units time to spare: there p is the sum of two such numbers.
 //
 // Both products run transposed on the 32x32x16 MFMA, S^T = K Q^T and O^T = V^T P^T:
 // lane l then holds keys of query l % 32 only, so maxima and sums are over a
@@ -79,6 +80,8 @@ template <> struct Mfma<__bf16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf2(a, b); }
+  static __device__ __forceinline__ float first(uint32_t w) { return bf_lo(w); }
+  static __device__ __forceinline__ float second(uint32_t w) { return bf_hi(w); }
   static __device__ __forceinline__ float add2(uint32_t w, float l) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3f803f80u), l, false);
   }
@@ -94,6 +97,8 @@ template <> struct Mfma<_Float16> {
     const v2h h = {(_Float16)a, (_Float16)b};
     return __builtin_bit_cast(uint32_t, h);
   }
+  static __device__ __forceinline__ float first(uint32_t w) { return (float)__builtin_bit_cast(v2h, w)[0]; }
+  static __device__ __forceinline__ float second(uint32_t w) { return (float)__builtin_bit_cast(v2h, w)[1]; }
   static __device__ __forceinline__ float add2(uint32_t w, float l) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), l, false);
   }
@@ -383,11 +388,15 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, const Item& it, con
 // (1505 TFLOP/s on the same card). 64 rows per wave and one wave per SIMD halves
 // the LDS reads and was slower (869 against 734 us on 8 heads), reading V by asm
 // blocks with their waits too (4.32 ms).
-// Few rows: what counts is the stream of keys, 64 KB in flight per workgroup; waves
-// without rows only load. One token of 56 heads over 131072 keys of 8 (537 MB): 106 us
-// with the join of 64 splits, 5.1 TB/s, as fast as a copy. Keys straight into
+// FEW, a wave's rows: what counts is the stream of keys, 32 KB in flight per workgroup;
+// waves without rows only load. No pipeline: the next tile is in flight while this one
+// is worked on, and the second product runs twice, for p rounded and for what the
+// rounding left, so that the output's rounding is all that remains (error against 64
+// bits 1.35 times smaller for long caches; 1 to 4% of the time, 4 to 13% with 64 to 128
+// rows, which do without). One token of 56 heads over 131072 keys of 8 (537 MB): 107-109
+// us with the join of 64 splits, 5.0 TB/s, as fast as a copy. Keys straight into
 // registers by waves that share nothing and meet no barrier: 129 us.
-template <typename T, int D>
+template <typename T, int D, bool FEW>
 __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
   typedef typename Mfma<T>::V V8;
   constexpr int WAVES = kRows / 32;
@@ -541,7 +550,49 @@ __global__ __launch_bounds__(256, 2) void attention(AttnArgs p) {
   };
   auto advance = [&]() { off = move_max<DB>(max_with_partner(mx), m, l, o, p.c, kShift); };
 
-  if (t0 < t1 && it.r0 + wave * 32 >= it.rows) {
+  if constexpr (FEW) {
+    uint32_t lo[4][4];
+    if (t0 < t1) {
+      issue(t0, 0);
+      issue(t0, 1);
+    }
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      publish();
+      issue(t + 1, 0);
+      issue(t + 1, 1);
+      if (it.r0 + wave * 32 >= it.rows) continue;   // without rows: loads and barriers alone
+      const char* const ks = smem + ((t - t0) & 1) * SLOT;
+      const char* const vs = ks + TILE;
+#pragma unroll
+      for (int g = 0; g < NQ; ++g) score(s0, kfrag(ks, g), g);
+      masked(s0, t);
+      mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s0[kb][e]);
+      advance();
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const int kc = j >> 2, w = j & 3, e = (kc & 1) * 8 + 2 * w;
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s0[kc >> 1][e], p.c, -off));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s0[kc >> 1][e + 1], p.c, -off));
+        pk[kc][w] = Mfma<T>::pack(p0, p1);
+        lo[kc][w] = Mfma<T>::pack(p0 - Mfma<T>::first(pk[kc][w]), p1 - Mfma<T>::second(pk[kc][w]));
+        l += p0 + p1;
+      }
+#pragma unroll
+      for (int g = 0; g < NV; ++g) {
+        const int kc = g / DB;
+        const V8 vf = vfrag(vs, g);
+        const uint4 hi4 = make_uint4(pk[kc][0], pk[kc][1], pk[kc][2], pk[kc][3]);
+        const uint4 lo4 = make_uint4(lo[kc][0], lo[kc][1], lo[kc][2], lo[kc][3]);
+        o[g % DB] = Mfma<T>::mul(vf, __builtin_bit_cast(V8, hi4), o[g % DB]);
+        o[g % DB] = Mfma<T>::mul(vf, __builtin_bit_cast(V8, lo4), o[g % DB]);
+      }
+    }
+  } else if (t0 < t1 && it.r0 + wave * 32 >= it.rows) {
     // A wave without rows takes part in the loads and barriers alone.
     issue(t0, 0);
     publish();
@@ -666,6 +717,7 @@ __global__ __launch_bounds__(256) void join_splits(AttnArgs p) {
 struct Plan {
   int piece, splits;     // least keys of a piece; splits of the keys
   int64_t tiles;         // row tiles per key head in all (pieces: of a sequence)
+  bool few;              // one wave's rows
   bool pieces = false;   // splits counts pieces of all sequences
 };
 
@@ -683,6 +735,8 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int kind, int heads, int kv
   // two share its matrix units and leave twice the partial results (300 tokens, 4096
   // keys, 8 heads: 20.0 us with 8 splits, 22.5 with 12).
   const int64_t want = (tile_rows <= 32 ? 2 : 1) * compute_units();
+  // (Packed rows have one kernel whatever lies around a sequence: the same bits.)
+  pl.few = tile_rows <= 32 && !packed;
   // A split takes 1 us per tile of keys; joining s of them 2.8 us, and per row 0.6 ns and
   // 0.15 ns per split (head_dim 128, from 12 shapes). So the best s is the root of
   // tiles / (0.00015 rows), and one where joining costs more than it saves: 878 tokens,
@@ -721,7 +775,8 @@ int launch(AttnArgs p, const Plan& pl, hipStream_t s) {
   const int64_t rows = (p.cu_q ? 1 : p.n) * p.q_rows * p.heads;   // of the output
   LR_REQUIRE(pl.splits == 1 || rows <= kMaxBlocks, "attention: %lld rows are not supported with split keys",
              (long long)rows);
-  attention<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
+  if (pl.few) attention<T, D, true><<<(unsigned)grid, 256, 0, s>>>(p);
+  else attention<T, D, false><<<(unsigned)grid, 256, 0, s>>>(p);
   if (int rc = check_launch("attention")) return rc;
   if (pl.splits == 1) return LR_OK;
   join_splits<T, D><<<(unsigned)rows, 256, 0, s>>>(p);

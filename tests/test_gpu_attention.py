@@ -22,8 +22,9 @@ from lynnreal_omni_amd import attention as A
 pytestmark = pytest.mark.gpu
 
 
-def formula(q, k, v, scale, seen):
-    """float64 [heads, rows, dim] outputs and their bounds; seen: bool [rows, keys]."""
+def formula(q, k, v, scale, seen, weights=None):
+    """float64 [heads, rows, dim] outputs and their bounds; seen: bool [rows, keys].
+    weights: the weights' relative rounding, the half step of the type if None."""
     dtype = q.dtype
     group = q.shape[1] // k.shape[1]
     q, k, v = (t.double().cpu().transpose(0, 1) for t in (q, k, v))
@@ -36,10 +37,11 @@ def formula(q, k, v, scale, seen):
     total = p.sum(-1, keepdim=True)
     p = torch.where(total > 0, p / total.clamp_min(1e-300), 0.0)
     eps = torch.finfo(dtype).eps / 2
+    weights = eps if weights is None else weights
     ds = (q.shape[-1] + 2) * 2.0 ** -23 * torch.where(seen, size, 0.0).amax(-1, keepdim=True) if s.shape[-1] else 0.0
     o = p @ v
     pv = p @ v.abs()
-    bound = 2 * eps * o.abs() + (eps + 2 * ds + 2.0 ** -21 + 3 * 2.0 ** -24 * s.shape[-1]) * pv * 1.01
+    bound = (eps + weights) * o.abs() + (weights + 2 * ds + 2.0 ** -21 + 3 * 2.0 ** -24 * s.shape[-1]) * pv * 1.01
     # fp16 weights far below the largest, and outputs below the normal numbers.
     bound = bound + 2.0 ** -32 * (seen.double() @ v.abs()) + torch.finfo(dtype).smallest_normal * eps
     return o.transpose(0, 1), bound.transpose(0, 1)
@@ -76,6 +78,19 @@ def test_one_sequence(rows, keys, heads, kv_heads, dim, causal, dtype):
     q, k, v = tensors(rows, keys, heads, kv_heads, dim, dtype, rows + keys)
     got = A.attention(q[None], k[None], v[None], causal=causal)
     check(got[0], *formula(q, k, v, dim ** -0.5, mask(rows, keys, causal)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,keys,heads,kv_heads,dim", [(1, 3000, 8, 8, 128), (1, 700, 14, 2, 64), (4, 300, 16, 2, 32),
+                                                          (32, 513, 2, 2, 128), (3, 64, 4, 1, 64)])
+def test_few_rows_round_the_output_alone(rows, keys, heads, kv_heads, dim, dtype):
+    """Up to 32 rows per key head keep the weights as a rounded number and the rounded
+    rest: off by the half step's square."""
+    q, k, v = tensors(rows, keys, heads, kv_heads, dim, dtype, 5 * rows + keys)
+    weights = (torch.finfo(dtype).eps / 2) ** 2
+    lengths = torch.tensor([keys], device="cuda", dtype=torch.int32)
+    for got in (A.attention(q[None], k[None], v[None]), A.attention(q[None], k[None], v[None], key_lengths=lengths)):
+        check(got[0], *formula(q, k, v, dim ** -0.5, mask(rows, keys, False), weights))
 
 
 @pytest.mark.parametrize("scale", [1e-3, 1.0, 20.0])

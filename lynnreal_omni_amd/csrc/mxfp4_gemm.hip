@@ -578,10 +578,9 @@ int launch_pingpong(Fp4Args p, int epilogue, hipStream_t s) {
 template <int FM, int FN, int WAVES, int S, int EPI>
 __global__ __launch_bounds__(64 * WAVES) void fp4_few(Fp4Args p) {
   constexpr int BK = 128;
-  constexpr int NA = FM == 4 ? 2 : 1, NB = FN == 4 ? 2 : 1;   // scale words per lane
-  constexpr int W_AT = FM * 2048, SA_AT = W_AT + FN * 2048, SB_AT = SA_AT + 256 * NA, SLOT = SB_AT + 256 * NB;
-  constexpr int LOADS = 2 * FM + 2 * FN + NA + NB;   // per k-step
-  static_assert((FM <= 2 || FM == 4) && (FN <= 2 || FN == 4) && (S - 2) * LOADS <= 63, "ring");
+  constexpr int W_AT = FM * 2048, SA_AT = W_AT + FN * 2048, SB_AT = SA_AT + 256, SLOT = SB_AT + 256;
+  constexpr int LOADS = 2 * FM + 2 * FN + 2;   // per k-step
+  static_assert(FM <= 2 && FN <= 2 && (S - 2) * LOADS <= 63, "one scale word per lane and operand; ring");
   static_assert(FM * FN * 1024 <= S * SLOT, "the sums fit the ring");
   __shared__ __attribute__((aligned(1024))) char smem[WAVES][S * SLOT];
   const int64_t n0 = (int64_t)blockIdx.x * (16 * FN), m0 = (int64_t)blockIdx.y * (16 * FM);
@@ -610,10 +609,8 @@ __global__ __launch_bounds__(64 * WAVES) void fp4_few(Fp4Args p) {
     for (int j = 0; j < 2 * FN; ++j) dma16(rb, slot + W_AT + j * 1024, (off0 + j * rows8) | past, soff);
 #pragma unroll
     for (int j = 0; j < 2 * FM; ++j) dma16(ra, slot + j * 1024, (off0 + j * rows8) | past, soff);
-#pragma unroll
-    for (int j = 0; j < NA; ++j) dma4(rsa, slot + SA_AT + 256 * j, sa_off + 4 * j, kt * 512);
-#pragma unroll
-    for (int j = 0; j < NB; ++j) dma4(rsb, slot + SB_AT + 256 * j, sb_off + 4 * j, kt * 512);
+    dma4(rsa, slot + SA_AT, sa_off, kt * 512);
+    dma4(rsb, slot + SB_AT, sb_off, kt * 512);
   };
   v4f acc[FM][FN];
 #pragma unroll
@@ -644,11 +641,8 @@ __global__ __launch_bounds__(64 * WAVES) void fp4_few(Fp4Args p) {
         w[0][f] = *reinterpret_cast<const v4i*>(slot + W_AT + f * 2048 + rd0);
         w[1][f] = *reinterpret_cast<const v4i*>(slot + W_AT + f * 2048 + rd1);
       }
-      uint32_t sa[NA], sb[NB];
-#pragma unroll
-      for (int f = 0; f < NA; ++f) sa[f] = *reinterpret_cast<const uint32_t*>(slot + SA_AT + 256 * f + lane * 4) >> sh_a;
-#pragma unroll
-      for (int f = 0; f < NB; ++f) sb[f] = *reinterpret_cast<const uint32_t*>(slot + SB_AT + 256 * f + lane * 4) >> sh_b;
+      const uint32_t sa = *reinterpret_cast<const uint32_t*>(slot + SA_AT + lane * 4) >> sh_a;
+      const uint32_t sb = *reinterpret_cast<const uint32_t*>(slot + SB_AT + lane * 4) >> sh_b;
       // The slot of k-step i - 1 is free: its reads were waited for by its products.
       issue(i + S - 1);
       each<2>([&](auto hh) __attribute__((always_inline)) {
@@ -657,7 +651,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp4_few(Fp4Args p) {
           constexpr int f = decltype(ii)::value;
           each<FN>([&](auto jj) __attribute__((always_inline)) {
             constexpr int j = decltype(jj)::value;
-            acc[f][j] = mfma_fp4<2 * (j & 1) + h, 2 * (f & 1) + h>(w[h][j], a[h][f], acc[f][j], sb[j >> 1], sa[f >> 1]);
+            acc[f][j] = mfma_fp4<2 * j + h, 2 * f + h>(w[h][j], a[h][f], acc[f][j], sb, sa);
           });
         });
       });

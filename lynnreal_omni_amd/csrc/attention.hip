@@ -688,14 +688,21 @@ __global__ __launch_bounds__(256) void join_splits(AttnArgs p) {
   l = wave_tree_sum(l);
   __syncthreads();
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = g; s < splits; s += G) {
-    const float w = weight[s];
-    if (w == 0.0f) continue;   // not written where the split had no keys
-    const float4 x = *reinterpret_cast<const float4*>(part + (at0 + s * rows) * D + 4 * at);
-    o.x += w * x.x;
-    o.y += w * x.y;
-    o.z += w * x.z;
-    o.w += w * x.w;
+  constexpr int BATCH = 4;   // loads in flight
+  for (int s0 = g; s0 < splits; s0 += BATCH * G) {
+    float4 x[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (s0 + i * G < splits) x[i] = *reinterpret_cast<const float4*>(part + (at0 + (s0 + i * G) * rows) * D + 4 * at);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float w = s0 + i * G < splits ? weight[s0 + i * G] : 0.0f;
+      if (w == 0.0f) continue;   // x was not written where the split had no keys
+      o.x += w * x[i].x;
+      o.y += w * x[i].y;
+      o.z += w * x[i].z;
+      o.w += w * x[i].w;
+    }
   }
   sums[g][at] = o;
   __syncthreads();

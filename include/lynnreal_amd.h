@@ -351,7 +351,8 @@ int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, const void*
                   int64_t table_rows, int64_t table_width, const int64_t* indices, int64_t sequence,
                   int gate_slot, void* stream);
 
-/* lr_quantize_rows_mxfp4 of x [m, k] into the scratch, then lr_mxfp4_gemm of it.
+/* lr_quantize_rows_mxfp4 of x [m, k] into the scratch, then lr_mxfp4_gemm of it; a
+ * single row may be quantized inside the product instead, to the same bits.
  * scratch: 16-byte aligned, the codes (m * 16 * ceil(k / 32) bytes, rounded up to
  * a multiple of 256) and behind them ceil(m / 64) * ceil(k / 256) * 512 bytes. */
 int lr_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t n, int64_t k, void* scratch,

@@ -21,6 +21,7 @@
 
 #include "lr_device.h"
 #include "lr_mxfp4.h"
+#include "lr_mxfp4_rows.h"
 #include "lr_runtime.h"
 
 namespace lr {
@@ -567,6 +568,47 @@ int launch_pingpong(Fp4Args p, int epilogue, hipStream_t s) {
 }
 
 // --------------------------------------------------------- few rows kernel ----
+// The waves' sums of (16 * FM) x (16 * FN) outputs, joined in wave order through LDS
+// (wave w's at sums + w * pitch), and the epilogue.
+template <int FM, int FN, int WAVES, int EPI>
+__device__ __forceinline__ void store_few(const Fp4Args& p, const v4f (&acc)[FM][FN], char* sums, int pitch,
+                                          int64_t m0, int64_t n0) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r16 = lane & 15, lg = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) *reinterpret_cast<v4f*>(sums + wave * pitch + (i * FN + j) * 1024 + lane * 16) = acc[i][j];
+  __syncthreads();
+  for (int t = threadIdx.x >> 6; t < FM * FN; t += WAVES) {
+    v4f v = *reinterpret_cast<const v4f*>(sums + t * 1024 + lane * 16);
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += *reinterpret_cast<const v4f*>(sums + w * pitch + t * 1024 + lane * 16);
+    const int64_t row = m0 + 16 * (t / FN) + r16, col = n0 + 16 * (t % FN) + 4 * lg;
+    if (row >= p.m) continue;
+    if (!p.staged) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < p.n) store_scalar<EPI>(p, row, col + e, v[e]);
+      continue;
+    }
+    if (col >= p.n) continue;
+    const int64_t o = row * p.n + col;
+    const uint2 b = p.bias ? *reinterpret_cast<const uint2*>(p.bias + col) : make_uint2(0u, 0u);
+    uint2 x = make_uint2(0u, 0u), g = x;
+    if (EPI == EPI_GATED) {
+      x = *reinterpret_cast<const uint2*>(p.resid + o);
+      g = *reinterpret_cast<const uint2*>(p.table + table_row(p, row) * p.table_width + (int64_t)p.gate_slot * p.n +
+                                          col);
+    }
+    const float y0 = finish<EPI>(round_bf(v[0] + bf_lo(b.x)), bf_lo(g.x), bf_lo(x.x));
+    const float y1 = finish<EPI>(round_bf(v[1] + bf_hi(b.x)), bf_hi(g.x), bf_hi(x.x));
+    const float y2 = finish<EPI>(round_bf(v[2] + bf_lo(b.y)), bf_lo(g.y), bf_lo(x.y));
+    const float y3 = finish<EPI>(round_bf(v[3] + bf_hi(b.y)), bf_hi(g.y), bf_hi(x.y));
+    *reinterpret_cast<uint2*>(p.c + o) = make_uint2(pack_bf2(y0, y1), pack_bf2(y2, y3));
+  }
+}
+
 // At most 16 * FM rows: what counts is the stream of weights. A workgroup has 16 * FN
 // columns; its WAVES waves take every WAVES-th k-step each and add their sums in wave
 // order at the end. A wave is on its own until then: it keeps the next S - 1 of its
@@ -659,38 +701,112 @@ __global__ __launch_bounds__(64 * WAVES) void fp4_few(Fp4Args p) {
     __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);  // vmcnt(0): the trailing DMAs have landed
     asm volatile("" ::: "memory");
   }
+  store_few<FM, FN, WAVES, EPI>(p, acc, smem[0], S * SLOT, m0, n0);
+}
+
+// One row, quantized by every workgroup for itself, which costs less than a kernel
+// before this one: fp4_few with the row's codes and scales in LDS, each wave those of
+// its own k-steps. The first weights are in flight meanwhile. Against the two kernels,
+// back to back: 1 x 21504 x 5376 14.1 us (15.4), 1 x 5120 x 5120 6.3 (7.3), 1 x 15360 x
+// 5120 9.9 (12.1); and the host launches one kernel, 13.7 us a layer for 16.7. The
+// quantizing takes every wave 50 instructions per 512 columns, so that from some 7000 on
+// it costs more than its kernel: 1 x 5120 x 20480 18.1 us (17.2), 1 x 5376 x 14336 11.6 (11.1).
+constexpr int kTokenPairs = 12, kTokenK = 512 * kTokenPairs;   // pairs of k-steps and columns per wave
+template <int DTYPE, int FN, int WAVES, int S, int EPI>
+__global__ __launch_bounds__(64 * WAVES) void fp4_token(Fp4Args p, const char* x, int64_t width) {
+  constexpr int BK = 128, SB_AT = FN * 2048, SLOT = SB_AT + 256, LOADS = 2 * FN + 1;
+  static_assert(FN <= 2 && (S - 2) * LOADS <= 63 && FN * 1024 <= S * SLOT, "ring");
+  // One object: between two the compiler would wait for all DMAs before every read.
+  constexpr int RINGS = WAVES * S * SLOT, CODES = WAVES * kTokenK / 2;
+  __shared__ __attribute__((aligned(1024))) char smem[RINGS + CODES + CODES / 16];
+  char* const codes = smem + RINGS;
+  char* const scales = codes + CODES;
+  typedef Row8<DTYPE> R;
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * FN);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  char* const ring = smem + wave * (S * SLOT);
+  const int r16 = lane & 15, lg = lane >> 4;
+  const int64_t K = p.kb;
+  const int KT = p.col_tiles;
+  const int mine = KT > wave ? (KT - wave + WAVES - 1) / WAVES : 0;   // this wave's k-steps
+  const int64_t rows_b = min((int64_t)(16 * FN), p.n - n0);
+  const __amdgpu_buffer_rsrc_t rb = row_rsrc(p.b + n0 * K, rows_b * K);
+  const __amdgpu_buffer_rsrc_t rsb = row_rsrc(p.bs + (n0 >> 6) * KT * 512, (int64_t)KT * 512);
+  const __amdgpu_buffer_rsrc_t rx = row_rsrc(x, width * R::kBytes);
+  const int drow = lane >> 3, dchunk = ((lane & 7) ^ drow) * 16;
+  const uint32_t off0 = (uint32_t)(drow * K + dchunk), rows8 = (uint32_t)(8 * K);
+  const int end = (int)K - dchunk;
+  const uint32_t sb_off = lane * 8 + ((uint32_t)n0 & 32) / 8;
+  auto issue = [&](int i) __attribute__((always_inline)) {
+    const int kt = wave + min(i, mine - 1) * WAVES;
+    char* const slot = ring + i % S * SLOT;
+    const uint32_t past = kt * BK < end ? 0u : 0x80000000u;   // a row's end: reads as zero
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+    for (int j = 0; j < 2 * FN; ++j) dma16(rb, slot + j * 1024, (off0 + j * rows8) | past, kt * BK);
+    dma4(rsb, slot + SB_AT, sb_off, kt * 512);
+  };
+  v4f acc[1][FN];
 #pragma unroll
-    for (int j = 0; j < FN; ++j) *reinterpret_cast<v4f*>(ring + (i * FN + j) * 1024 + lane * 16) = acc[i][j];
-  __syncthreads();
-  for (int t = threadIdx.x >> 6; t < FM * FN; t += WAVES) {
-    v4f v = *reinterpret_cast<const v4f*>(smem[0] + t * 1024 + lane * 16);
+  for (int j = 0; j < FN; ++j) acc[0][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  if (mine > 0) {
+    // Half a wave per k-step, eight values per lane.
+    const int chunk = lane & 31;
+    R v[kTokenPairs];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) v += *reinterpret_cast<const v4f*>(smem[w] + t * 1024 + lane * 16);
-    const int64_t row = m0 + 16 * (t / FN) + r16, col = n0 + 16 * (t % FN) + 4 * lg;
-    if (row >= p.m) continue;
-    if (!p.staged) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < p.n) store_scalar<EPI>(p, row, col + e, v[e]);
-      continue;
+    for (int u = 0; u < kTokenPairs; ++u) {
+      const int i = 2 * u + (lane >> 5);
+      // Past the row's end (width % 8 == 0) or the wave's k-steps: zeros.
+      v[u].load(rx, i < mine ? (uint32_t)((wave + i * WAVES) * 256 + chunk * 8) * R::kBytes : 0x80000000u);
     }
-    if (col >= p.n) continue;
-    const int64_t o = row * p.n + col;
-    const uint2 b = p.bias ? *reinterpret_cast<const uint2*>(p.bias + col) : make_uint2(0u, 0u);
-    uint2 x = make_uint2(0u, 0u), g = x;
-    if (EPI == EPI_GATED) {
-      x = *reinterpret_cast<const uint2*>(p.resid + o);
-      g = *reinterpret_cast<const uint2*>(p.table + table_row(p, row) * p.table_width + (int64_t)p.gate_slot * p.n +
-                                          col);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(i);
+#pragma unroll
+    for (int u = 0; u < kTokenPairs; ++u) {
+      const int i = 2 * u + (lane >> 5), kt = wave + i * WAVES;
+      const uint32_t byte = scale_byte(quad_max(v[u].magnitude()));
+      if (i >= mine) continue;
+      // 2^e as fp32 is the byte in the exponent field; e = -127 is a subnormal.
+      const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte << 23);
+      *reinterpret_cast<uint32_t*>(codes + kt * BK + chunk * 4) = byte == 255 ? 0u : v[u].codes(scale);
+      if ((lane & 3) == 0) scales[kt * 8 + (chunk >> 2)] = (char)byte;
     }
-    const float y0 = finish<EPI>(round_bf(v[0] + bf_lo(b.x)), bf_lo(g.x), bf_lo(x.x));
-    const float y1 = finish<EPI>(round_bf(v[1] + bf_hi(b.x)), bf_hi(g.x), bf_hi(x.x));
-    const float y2 = finish<EPI>(round_bf(v[2] + bf_lo(b.y)), bf_lo(g.y), bf_lo(x.y));
-    const float y3 = finish<EPI>(round_bf(v[3] + bf_hi(b.y)), bf_hi(g.y), bf_hi(x.y));
-    *reinterpret_cast<uint2*>(p.c + o) = make_uint2(pack_bf2(y0, y1), pack_bf2(y2, y3));
+    // The wave reads what it wrote itself: LDS operations of a wave stay in order.
+    asm volatile("" ::: "memory");
+    const int rd_row = (r16 >> 3) * 1024 + (r16 & 7) * 128;
+    const int rd0 = rd_row + (lg ^ (r16 & 7)) * 16, rd1 = rd_row + ((lg + 4) ^ (r16 & 7)) * 16;
+    const int sh_b = FN == 1 ? (int)(n0 & 16) : 0;
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      constexpr int kVm = (S - 2) * LOADS;
+      __builtin_amdgcn_s_waitcnt(0x70 | 0xf00 | vm(kVm));   // k-step i has landed
+      asm volatile("" ::: "memory");
+      const char* const slot = ring + i % S * SLOT;
+      const int kt = wave + i * WAVES;
+      // The row in all 16 of the fragment's: the others' outputs are not stored.
+      v4i a[2], w[2][FN];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) a[h] = *reinterpret_cast<const v4i*>(codes + kt * BK + 64 * h + 16 * lg);
+      const uint32_t sa = (uint8_t)scales[kt * 8 + lg] | (uint32_t)(uint8_t)scales[kt * 8 + 4 + lg] << 8;
+#pragma unroll
+      for (int f = 0; f < FN; ++f) {
+        w[0][f] = *reinterpret_cast<const v4i*>(slot + f * 2048 + rd0);
+        w[1][f] = *reinterpret_cast<const v4i*>(slot + f * 2048 + rd1);
+      }
+      const uint32_t sb = *reinterpret_cast<const uint32_t*>(slot + SB_AT + lane * 4) >> sh_b;
+      // The slot of k-step i - 1 is free: its reads were waited for by its products.
+      issue(i + S - 1);
+      each<2>([&](auto hh) __attribute__((always_inline)) {
+        constexpr int h = decltype(hh)::value;
+        each<FN>([&](auto jj) __attribute__((always_inline)) {
+          constexpr int j = decltype(jj)::value;
+          acc[0][j] = mfma_fp4<2 * j + h, h>(w[h][j], a[h], acc[0][j], sb, sa);
+        });
+      });
+    }
+    __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);  // vmcnt(0): the trailing DMAs have landed
+    asm volatile("" ::: "memory");
   }
+  store_few<1, FN, WAVES, EPI>(p, acc, smem, S * SLOT, 0, n0);
 }
 
 template <int FM, int FN, int WAVES, int S>
@@ -703,6 +819,22 @@ int launch_few(const Fp4Args& p, int epilogue, hipStream_t s) {
   else if (epilogue == EPI_GELU) fp4_few<FM, FN, WAVES, S, EPI_GELU><<<grid, 64 * WAVES, 0, s>>>(p);
   else fp4_few<FM, FN, WAVES, S, EPI_GATED><<<grid, 64 * WAVES, 0, s>>>(p);
   return check_launch("mxfp4_gemm");
+}
+
+template <int DTYPE, int WAVES>
+int launch_token_waves(const Fp4Args& p, const char* x, int64_t width, int epilogue, hipStream_t s) {
+  const dim3 grid((unsigned)((p.n + 31) / 32));
+  if (epilogue == EPI_BF16) fp4_token<DTYPE, 2, WAVES, 5, EPI_BF16><<<grid, 64 * WAVES, 0, s>>>(p, x, width);
+  else if (epilogue == EPI_GELU) fp4_token<DTYPE, 2, WAVES, 5, EPI_GELU><<<grid, 64 * WAVES, 0, s>>>(p, x, width);
+  else fp4_token<DTYPE, 2, WAVES, 5, EPI_GATED><<<grid, 64 * WAVES, 0, s>>>(p, x, width);
+  return check_launch("mxfp4_linear");
+}
+
+template <int DTYPE>
+int launch_token(const Fp4Args& p, const void* x, int64_t width, bool two, int epilogue, hipStream_t s) {
+  const char* const px = static_cast<const char*>(x);
+  return two ? launch_token_waves<DTYPE, 2>(p, px, width, epilogue, s)
+             : launch_token_waves<DTYPE, 1>(p, px, width, epilogue, s);
 }
 
 template <int BM, int BN, int WAVES_M, int WAVES_N, int S>
@@ -771,15 +903,10 @@ int launch(const Fp4Args& p, int epilogue, hipStream_t s) {
   return best->run(p, epilogue, s);
 }
 
-}  // namespace
-}  // namespace lr
-
-using namespace lr;
-
-extern "C" int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, const void* b_scale, int64_t m,
-                             int64_t n, int64_t k, const void* bias, void* out, int epilogue, const void* residual,
-                             const void* table, int64_t table_rows, int64_t table_width, const int64_t* indices,
-                             int64_t sequence, int gate_slot, void* stream) {
+// Checks a product's arguments and fills p with them; p.m stays 0 where there is nothing to do.
+int fill(Fp4Args& p, const void* a, const void* a_scale, const void* b, const void* b_scale, int64_t m, int64_t n,
+         int64_t k, const void* bias, void* out, int epilogue, const void* residual, const void* table,
+         int64_t table_rows, int64_t table_width, const int64_t* indices, int64_t sequence, int gate_slot) {
   LR_REQUIRE(epilogue == EPI_BF16 || epilogue == EPI_GELU || epilogue == EPI_GATED,
              "mxfp4_gemm: unknown epilogue %d", epilogue);
   LR_REQUIRE(m >= 0 && n >= 0 && k >= 0, "mxfp4_gemm: negative shape m=%lld n=%lld k=%lld", (long long)m,
@@ -798,7 +925,6 @@ extern "C" int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, 
                "mxfp4_gemm: gate slot %d of width %lld lies past a table row of %lld", gate_slot, (long long)n,
                (long long)table_width);
   }
-  Fp4Args p = {};
   p.a = static_cast<const uint8_t*>(a);
   p.as = static_cast<const uint8_t*>(a_scale);
   p.b = static_cast<const uint8_t*>(b);
@@ -818,7 +944,23 @@ extern "C" int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, 
   p.gate_slot = gate_slot;
   p.staged = n % 8 == 0 && aligned(out, 16) && (!bias || aligned(bias, 8)) &&
              (epilogue != EPI_GATED || (aligned(residual, 16) && aligned(table, 16) && table_width % 8 == 0));
-  return launch(p, epilogue, as_stream(stream));
+  return LR_OK;
+}
+
+}  // namespace
+}  // namespace lr
+
+using namespace lr;
+
+extern "C" int lr_mxfp4_gemm(const void* a, const void* a_scale, const void* b, const void* b_scale, int64_t m,
+                             int64_t n, int64_t k, const void* bias, void* out, int epilogue, const void* residual,
+                             const void* table, int64_t table_rows, int64_t table_width, const int64_t* indices,
+                             int64_t sequence, int gate_slot, void* stream) {
+  Fp4Args p = {};
+  if (int rc = fill(p, a, a_scale, b, b_scale, m, n, k, bias, out, epilogue, residual, table, table_rows, table_width,
+                    indices, sequence, gate_slot))
+    return rc;
+  return p.m ? launch(p, epilogue, as_stream(stream)) : LR_OK;
 }
 
 extern "C" int lr_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t n, int64_t k, void* scratch,
@@ -832,8 +974,22 @@ extern "C" int lr_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t n, i
   const int64_t need = codes + (m + 63) / 64 * mxfp4_scale_tiles(k) * 512;
   LR_REQUIRE(m == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= need),
              "mxfp4_linear: the scratch must be 16-byte aligned and hold %lld bytes", (long long)need);
+  LR_REQUIRE(dtype == LR_DTYPE_BF16 || dtype == LR_DTYPE_F16 || dtype == LR_DTYPE_F32,
+             "mxfp4_linear: unknown dtype %d", dtype);
   char* const scales = static_cast<char*>(scratch) + codes;
-  if (int rc = lr_quantize_rows_mxfp4(x, dtype, m, k, scratch, m ? scales : nullptr, stream)) return rc;
-  return lr_mxfp4_gemm(scratch, scales, b, b_scale, m, n, k, bias, out, epilogue, residual, table, table_rows,
-                       table_width, indices, sequence, gate_slot, stream);
+  Fp4Args p = {};
+  if (int rc = fill(p, scratch, scales, b, b_scale, m, n, k, bias, out, epilogue, residual, table, table_rows,
+                    table_width, indices, sequence, gate_slot))
+    return rc;
+  if (p.m == 0) return LR_OK;
+  hipStream_t s = as_stream(stream);
+  const int64_t few = (n + 31) / 32, cus = compute_units();
+  const bool two = few <= 2 * cus;   // waves, as in launch()
+  if (m == 1 && few <= 4 * cus && k <= (two ? 2 : 1) * kTokenK && k % 8 == 0 && x && aligned(x, 16)) {
+    if (dtype == LR_DTYPE_BF16) return launch_token<LR_DTYPE_BF16>(p, x, k, two, epilogue, s);
+    if (dtype == LR_DTYPE_F16) return launch_token<LR_DTYPE_F16>(p, x, k, two, epilogue, s);
+    return launch_token<LR_DTYPE_F32>(p, x, k, two, epilogue, s);
+  }
+  if (int rc = lr_quantize_rows_mxfp4(x, dtype, m, k, scratch, scales, stream)) return rc;
+  return launch(p, epilogue, s);
 }

@@ -120,6 +120,34 @@ def test_epilogues_are_the_separate_kernels(m, n, k):
     assert torch.equal(got, kernels._gated_residual(again, layer(two), table, indices, 0))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,k", [(64, 64), (33, 96), (520, 8), (5120, 264), (264, 5376), (17000, 2056), (48, 12288),
+                                 (40, 12296), (17000, 6144), (17000, 6152), (35000, 256), (100, 36)])
+def test_one_row_is_the_two_kernels(n, k, dtype):
+    """A layer's single row is quantized inside the product: the bits of the quantizer
+    and the product one after the other, for every epilogue."""
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    x = (torch.randn(1, k, device="cuda", generator=g) * 10 ** torch.linspace(-6, 4, k, device="cuda")).to(dtype)
+    w = torch.randn(n, k, device="cuda", generator=g)
+    layer = mxfp4.Mxfp4Linear.from_packed(*mxfp4.quantize_weight(w), torch.randn(n, device="cuda", generator=g).bfloat16(), k)
+    table = torch.randn(3, 2 * n, device="cuda", generator=g).bfloat16()
+    gated = dict(residual=torch.randn(1, 1, n, device="cuda", generator=g).bfloat16(), table=table,
+                 indices=torch.tensor([2], device="cuda"), gate_slot=1)
+    for epilogue in ({}, {"activation": "gelu_tanh"}, gated):
+        want = layer.forward_codes(*kernels.quantize_rows_mxfp4(x), (1,), **epilogue)
+        assert torch.equal(layer(x, **epilogue), want)
+    x[0, k // 2] = float("nan")
+    assert layer(x).isnan().all()
+    x[0, k // 2] = 0
+    x[0, :min(k, 40)] = 0
+    want = layer.forward_codes(*kernels.quantize_rows_mxfp4(x), (1,))
+    assert torch.equal(layer(x), want)
+    # A row of a wider tensor, and one that is not 16-byte aligned.
+    wide = torch.zeros(1, k + 1, device="cuda", dtype=dtype)
+    wide[:, 1:] = x
+    assert torch.equal(layer(wide[:, 1:]), want)
+
+
 def test_nan_blocks_reach_their_row_alone():
     x, w, b = operands(70, 136, 256, 4)
     layer = mxfp4.Mxfp4Linear.from_packed(*mxfp4.quantize_weight(w), b).cuda()

@@ -258,18 +258,18 @@ struct Scales {
 // ---------------------------------------------------------- tile kernel ----
 // BM x BN outputs per workgroup, a wave (BM / WAVES_M) x (BN / WAVES_N) of them.
 // Ring of S k-steps in LDS (1 KB blocks of 8 rows x 128 bytes, 16-byte chunk c of
-// row R in slot c ^ (R % 8)). k-step kt: wait for its DMAs, barrier (which also
-// says that every wave is done with k-step kt - 1), refill that slot with k-step
-// kt + S - 1, multiply. For what the ping-pong kernel does not take: 4096 x 4096 x 4128
-// 53 us (2.6 PFLOP/s) against 37.5 of it at K = 4096; with N = 4100, whose rows are
-// stored value by value, 70 us.
+// row R in slot c ^ (R % 8); behind them a KB per group of 64 rows, half of it its scale
+// tile). k-step kt: wait for its DMAs, barrier (which also says that every wave is
+// done with k-step kt - 1), refill that slot with k-step kt + S - 1, multiply.
 template <int BM, int BN, int WAVES_M, int WAVES_N, int S, int EPI>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void fp4_tile(Fp4Args p) {
   constexpr int BK = 128, NWAVES = WAVES_M * WAVES_N;
   constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
-  constexpr int A_BYTES = BM * BK, SLOT = (BM + BN) * BK;
+  constexpr int A_BYTES = BM * BK, SCALES = (BM + BN) * BK, GA = BM / 64, GB = BN / 64;
+  constexpr int SLOT = SCALES + (GA + GB) * 1024;
   constexpr int BLOCKS = (BM + BN) / 8, LOADS = BLOCKS / NWAVES;
   static_assert(BM % 64 == 0 && BN % 64 == 0 && BLOCKS % NWAVES == 0 && S >= 2, "tile shape");
+  static_assert((FM == 2 || FM == 4) && (FN == 2 || FN == 4) && GA + GB <= NWAVES, "scale words and DMAs");
   constexpr int STAGE = WM * (2 * WN + 16);
   __shared__ __attribute__((aligned(1024))) char smem[S * SLOT > NWAVES * STAGE ? S * SLOT : NWAVES * STAGE];
   int tm, tn;
@@ -281,9 +281,13 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void fp4_tile(Fp4Args p) {
   const int KT = p.col_tiles;
   const int64_t rows_a = min((int64_t)BM, p.m - m0), rows_b = min((int64_t)BN, p.n - n0);
   const __amdgpu_buffer_rsrc_t ra = row_rsrc(p.a + m0 * K, rows_a * K), rb = row_rsrc(p.b + n0 * K, rows_b * K);
-  const int groups_a = (int)((rows_a + 63) >> 6), groups_b = (int)((rows_b + 63) >> 6);
-  const __amdgpu_buffer_rsrc_t rsa = row_rsrc(p.as + (m0 >> 6) * KT * 512, (int64_t)groups_a * KT * 512);
-  const __amdgpu_buffer_rsrc_t rsb = row_rsrc(p.bs + (n0 >> 6) * KT * 512, (int64_t)groups_b * KT * 512);
+  // Wave g < GA + GB loads the scale tiles of group g (A's, then B's) with half its lanes;
+  // those of a group past the operand's rows lie past the buffer's end and read as zero.
+  const int group = wave < GA ? wave : wave - GA;
+  const int64_t groups = ((wave < GA ? rows_a : rows_b) + 63) >> 6;
+  const __amdgpu_buffer_rsrc_t rs = row_rsrc((wave < GA ? p.as + (m0 >> 6) * KT * 512 : p.bs + (n0 >> 6) * KT * 512),
+                                             groups * KT * 512);
+  const uint32_t soff = lane < 32 ? (uint32_t)(group * KT * 512 + lane * 16) : 0x80000000u;
 
   const int drow = lane >> 3;
   const int dchunk = ((lane & 7) ^ drow) * 16;
@@ -299,6 +303,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void fp4_tile(Fp4Args p) {
       const uint32_t off = in ? (uint32_t)(row * K + kt * BK + dchunk) : 0x80000000u;
       dma16(is_a ? ra : rb, slot + blk * 1024, off, 0);
     }
+    if (wave < GA + GB) dma16(rs, slot + SCALES + wave * 1024, soff, (kt < KT ? kt : KT - 1) * 512);
   };
   const int r16 = lane & 15;
   const int rd_row = (r16 >> 3) * 1024 + (r16 & 7) * 128;
@@ -311,30 +316,33 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void fp4_tile(Fp4Args p) {
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  Scales<FM, 64> sa, sa_next;
-  Scales<FN, 64> sb, sb_next;
-  sa.load(rsa, groups_a, wm * WM, KT, 0, lane);
-  sb.load(rsb, groups_b, wn * WN, KT, 0, lane);
 #pragma unroll
   for (int t = 0; t < S - 1; ++t) issue(t);
-  constexpr int kVm = (S - 2) * LOADS;
-  static_assert(kVm <= 63, "vmcnt range");
-  constexpr int kWait = 0x70 | 0xf00 | (kVm & 0xf) | ((kVm >> 4) << 14);  // vmcnt(kVm)
+  static_assert((S - 2) * (LOADS + 1) <= 63, "vmcnt range");
 #pragma unroll 1
   for (int kt = 0; kt < KT; ++kt) {
     // In flight: the DMAs of k-steps kt .. kt + S - 2, oldest first.
-    __builtin_amdgcn_s_waitcnt(kWait);
+    if (wave < GA + GB) __builtin_amdgcn_s_waitcnt(0x70 | 0xf00 | vm((S - 2) * (LOADS + 1)));
+    else __builtin_amdgcn_s_waitcnt(0x70 | 0xf00 | vm((S - 2) * LOADS));
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    const int next = kt + 1 < KT ? kt + 1 : kt;
-    sa_next.load(rsa, groups_a, wm * WM, KT, next, lane);
-    sb_next.load(rsb, groups_b, wn * WN, KT, next, lane);
-    __builtin_amdgcn_sched_barrier(0);  // the scale loads stay older than the DMAs (kWait counts those)
     issue(kt + S - 1);
     __builtin_amdgcn_sched_barrier(0);
     const char* const slot = smem + (kt % S) * SLOT;
+    // Byte 2 * (f % 2) + h of word f / 2 is fragment f's scale, half h.
+    uint32_t sa[FM / 2], sb[FN / 2];
+#pragma unroll
+    for (int f = 0; f < FM / 2; ++f) {
+      const int row = wm * WM + 32 * f;
+      sa[f] = *reinterpret_cast<const uint32_t*>(slot + SCALES + (row >> 6) * 1024 + lane * 8 + (row >> 3 & 4));
+    }
+#pragma unroll
+    for (int f = 0; f < FN / 2; ++f) {
+      const int row = wn * WN + 32 * f;
+      sb[f] = *reinterpret_cast<const uint32_t*>(slot + SCALES + (GA + (row >> 6)) * 1024 + lane * 8 + (row >> 3 & 4));
+    }
     each<2>([&](auto hh) __attribute__((always_inline)) {
       constexpr int h = decltype(hh)::value;
       v4i a[FM], w[FN];
@@ -346,14 +354,10 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void fp4_tile(Fp4Args p) {
         constexpr int i = decltype(ii)::value;
         each<FN>([&](auto jj) __attribute__((always_inline)) {
           constexpr int j = decltype(jj)::value;
-          typedef Scales<FM, 64> SA;
-          typedef Scales<FN, 64> SB;
-          acc[i][j] = mfma_fp4<SB::byte(j, h), SA::byte(i, h)>(w[j], a[i], acc[i][j], sb.w[j >> 1], sa.w[i >> 1]);
+          acc[i][j] = mfma_fp4<2 * (j & 1) + h, 2 * (i & 1) + h>(w[j], a[i], acc[i][j], sb[j >> 1], sa[i >> 1]);
         });
       });
     });
-    sa = sa_next;
-    sb = sb_next;
   }
   __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);  // vmcnt(0): the trailing DMAs have landed
   __syncthreads();
@@ -889,8 +893,14 @@ int launch(const Fp4Args& p, int epilogue, hipStream_t s) {
     if (rows == 16) return few <= 2 * cus ? launch_few<1, 2, 2, 5>(p, epilogue, s) : launch_few<1, 2, 1, 5>(p, epilogue, s);
     return few <= 2 * cus ? launch_few<2, 2, 2, 4>(p, epilogue, s) : launch_few<2, 2, 1, 4>(p, epilogue, s);
   }
+  // 64 x 128 tiles of one round: five k-steps in flight count more than matrix units that
+  // never pause (the ping-pong kernel has two): 256 x 5120 x 5120 12.3 us for 13.2, 64 x 21504 x
+  // 5376 14.5 for 16.2, 256 x 5120 x 20480 39 for 46; in two rounds 24.7 for 19.9 (128 x 20480 x
+  // 5120). And for 18.3, 22.0 and 77 of the 128 x 128 tiles.
+  const bool one_round = (p.m + 63) / 64 * ((p.n + 127) / 128) <= cus;
   // The ping-pong kernel takes whole k-steps and whole-line stores only.
-  if (p.kb % 128 || !p.staged) return launch_tile<128, 128, 2, 2, 2>(p, epilogue, s);
+  if (p.kb % 128 || !p.staged)
+    return one_round ? launch_tile<64, 128, 2, 4, 5>(p, epilogue, s) : launch_tile<128, 128, 2, 2, 2>(p, epilogue, s);
   const Tile* best = nullptr;
   double us = 0.0;
   for (const Tile& t : kTiles) {
@@ -900,6 +910,7 @@ int launch(const Fp4Args& p, int epilogue, hipStream_t s) {
       us = e;
     }
   }
+  if (best->rows == 64 && one_round) return launch_tile<64, 128, 2, 4, 5>(p, epilogue, s);
   return best->run(p, epilogue, s);
 }
 

@@ -97,6 +97,19 @@ def test_product(m, n, k, bias):
     check_product(layer(x.cuda()), y, size, k)
 
 
+# On 256 CUs: one round of 64 x 128 tiles (the last of an odd N), more than a round of
+# ragged ones, and the ping-pong kernel's tiles from 64 x 128 to 256 x 256, with odd and
+# even numbers of k-steps.
+TILES = [(100, 8200, 768), (200, 5128, 300), (65, 16001, 96), (256, 5120, 1280), (1000, 4104, 800), (700, 6001, 64),
+         (38, 37800, 256), (402, 22672, 768), (500, 4104, 768), (1000, 4104, 512), (2000, 4104, 768),
+         (2000, 5128, 256), (2000, 6152, 768)]
+
+
+@pytest.mark.parametrize("m,n,k", TILES)
+def test_product_of_every_tile(m, n, k):
+    test_product(m, n, k, True)
+
+
 def _table(n, rows_, seed):
     g = torch.Generator().manual_seed(seed)
     return torch.randn(rows_, 6 * n, generator=g).bfloat16().cuda()

@@ -96,9 +96,10 @@ class Mxfp4Linear(nn.Module):
         if value.shape[-1] != self.in_features:
             raise ValueError(f"the layer takes {self.in_features} features, got {value.shape[-1]}")
         buffers = self._buffers
-        y = mxfp4_gemm.linear_rows(value.reshape(-1, self.in_features), buffers["weight_codes"],
-                                   buffers["weight_scale"], buffers["bias"], **epilogue)
-        return y.view(*value.shape[:-1], self.out_features)
+        rows = value if value.dim() == 2 else value.reshape(-1, self.in_features)
+        y = mxfp4_gemm.linear_rows(rows, buffers["weight_codes"], buffers["weight_scale"], buffers["bias"],
+                                   **epilogue)
+        return y if rows is value else y.view(*value.shape[:-1], self.out_features)
 
 
 @torch.no_grad()

@@ -24,6 +24,7 @@ def code_bytes(width: int) -> int:
     return -(-width // BLOCK) * (BLOCK // 2)
 
 
+@functools.lru_cache(maxsize=4096)
 def scale_shape(rows: int, width: int) -> tuple[int, int, int]:
     """Shape of the tile-ordered scales of [rows, width] values."""
     return -(-rows // _TILE_ROWS), -(-width // (BLOCK * _TILE_BLOCKS)), _TILE_ROWS * _TILE_BLOCKS
@@ -54,13 +55,17 @@ def untile_scales(tiles: torch.Tensor, rows: int, blocks: int) -> torch.Tensor:
 
 
 def _operand(codes, scales, name):
+    shape = codes.shape
+    if (len(shape) == 2 and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and not shape[1] % 16
+            and scales.shape == scale_shape(shape[0], 2 * shape[1]) and codes.is_contiguous()
+            and scales.is_contiguous()):
+        return
     if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.shape[1] % 16:
         raise ValueError(f"{name} must be contiguous uint8 codes [rows, 16 * blocks]")
     if scales.dtype != torch.uint8 or tuple(scales.shape) != scale_shape(codes.shape[0], 2 * codes.shape[1]):
         raise ValueError(f"{name}_scale must be uint8 {scale_shape(codes.shape[0], 2 * codes.shape[1])}, "
                          f"got {scales.dtype} {tuple(scales.shape)}")
-    if not scales.is_contiguous():
-        raise ValueError(f"{name}_scale must be contiguous")
+    raise ValueError(f"{name}_scale must be contiguous")
 
 
 def _gated(m, n, residual, table, indices, gate_slot):

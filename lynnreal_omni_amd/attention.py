@@ -29,17 +29,32 @@ _HEAD_DIMS = (32, 64, 128)
 _DENSE, _PACKED, _LENGTHS = range(3)
 
 
+def _dense(stride, shape):
+    """Whether the kernel reads a tensor of these strides: a dense head dimension, rows
+    a multiple of 16 bytes apart."""
+    return stride[-1] == 1 and stride[-3] < 1 << 23 and all(not st % 8 or n == 1 for st, n in zip(stride[:-1], shape))
+
+
 def _rows(t):
-    """t with a dense head dimension and 16-byte aligned rows: t itself, or a copy."""
-    strides = t.stride()
-    if strides[-1] == 1 and t.data_ptr() % 16 == 0 and strides[-3] < 1 << 23:
-        for stride, size in zip(strides, t.shape[:-1]):
-            if stride % 8 and size > 1:
-                break
-        else:
-            return t
+    """t where the kernel can read it, or a copy."""
+    if not t.data_ptr() % 16 and _dense(t.stride(), t.shape):
+        return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+@functools.lru_cache(maxsize=4096)
+def _strides(q, k, v, q_shape, k_shape, copied):
+    """The nine strides that lr_attention takes, of tensors with the strides q, k, v;
+    None where one has to be copied first."""
+    nine = array("q")
+    for stride, shape in ((q, q_shape), (k, k_shape), (v, k_shape)):
+        if not copied and not _dense(stride, shape):
+            return None
+        # A dimension of one element may have any stride; it is not used.
+        s = [st if n > 1 else 0 for st, n in zip(stride, shape)]
+        nine.extend((s[-3], s[-2], s[0] if len(s) == 4 else 0))
+    return nine
 
 
 @functools.lru_cache(maxsize=4096)
@@ -72,7 +87,15 @@ def _check(query, key, value, dims):
     _lib.check_device(query)
 
 
-def _launch(query, key, value, out, sequences, q_rows, k_rows, cu_q, cu_k, lengths, causal, scale):
+def _launch(query, key, value, cu_q, cu_k, lengths, causal, scale, sequences, q_rows, k_rows, out=None):
+    strides = None
+    if not (query.data_ptr() | key.data_ptr() | value.data_ptr()) & 15:
+        strides = _strides(query.stride(), key.stride(), value.stride(), query.shape, key.shape, False)
+    if strides is None:
+        query, key, value = _rows(query), _rows(key), _rows(value)
+        strides = _strides(query.stride(), key.stride(), value.stride(), query.shape, key.shape, True)
+    if out is None:
+        out = query.new_empty(query.shape)
     heads, dim = query.shape[-2:]
     kv_heads = key.shape[-2]
     packed = cu_q is not None
@@ -82,11 +105,6 @@ def _launch(query, key, value, out, sequences, q_rows, k_rows, cu_q, cu_k, lengt
     if splits > 1:
         nbytes = splits * (sequences if kind == _DENSE else 1) * q_rows * heads * (dim + 2) * 4
         ws = _lib.workspace(query, nbytes)   # held until the launch
-    strides = array("q")
-    for t in (query, key, value):
-        # A dimension of one element may have any stride; it is not used.
-        s = [stride if size > 1 else 0 for stride, size in zip(t.stride(), t.shape)]
-        strides.extend((s[-3], s[-2], 0 if packed else s[0]))
     _lib.launch(query, "lr_attention", query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr(),
                 _DTYPES[query.dtype], sequences, q_rows, k_rows, heads, kv_heads, dim, strides.buffer_info()[0],
                 _lib.ptr(cu_q), _lib.ptr(cu_k), _lib.ptr(lengths), int(bool(causal)),
@@ -119,9 +137,7 @@ def attention(query, key, value, *, causal=False, scale=None, key_lengths=None):
         key_lengths = key_lengths.contiguous()
     else:
         _lib.same_device(query, key=key, value=value)
-    query, key, value = _rows(query), _rows(key), _rows(value)
-    out = torch.empty(query.shape, device=query.device, dtype=query.dtype)
-    return _launch(query, key, value, out, batch, tokens, keys, None, None, key_lengths, causal, scale)
+    return _launch(query, key, value, None, None, key_lengths, causal, scale, batch, tokens, keys)
 
 
 def _first_rows(t, name):
@@ -152,10 +168,8 @@ def attention_packed(query, key, value, cu_query, cu_key=None, *, causal=False, 
     same = cu_key is cu_query
     cu_query = _first_rows(cu_query, "cu_query")
     cu_key = cu_query if same else _first_rows(cu_key, "cu_key")
-    query, key, value = _rows(query), _rows(key), _rows(value)
-    out = torch.empty(query.shape, device=query.device, dtype=query.dtype)
-    return _launch(query, key, value, out, cu_query.numel() - 1, query.shape[0], key.shape[0], cu_query, cu_key, None,
-                   causal, scale)
+    return _launch(query, key, value, cu_query, cu_key, None, causal, scale, cu_query.numel() - 1, query.shape[0],
+                   key.shape[0])
 
 
 def block_attention(query, key, value, attention_mask, processor=None):

@@ -213,7 +213,7 @@ def test_lists_out_of_order_stay_inside(heads, kv_heads, rows):
     for sequences in (1, 2, 70, 200):
         cu = torch.randint(-9, rows + 9, (sequences + 1,), generator=g, dtype=torch.int32).cuda()
         guarded = torch.full((3 * size,), 7.0, dtype=torch.bfloat16, device="cuda")
-        A._launch(q, k, v, guarded[size:2 * size].view(q.shape), sequences, rows, rows, cu, cu, None, False, None)
+        A._launch(q, k, v, cu, cu, None, False, None, sequences, rows, rows, guarded[size:2 * size].view(q.shape))
         assert (guarded[:size] == 7).all() and (guarded[2 * size:] == 7).all()
 
 

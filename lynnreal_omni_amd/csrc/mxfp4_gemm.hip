@@ -712,7 +712,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp4_few(Fp4Args p) {
 // before this one: fp4_few with the row's codes and scales in LDS, each wave those of
 // its own k-steps. The first weights are in flight meanwhile. Against the two kernels,
 // back to back: 1 x 21504 x 5376 14.1 us (15.4), 1 x 5120 x 5120 6.3 (7.3), 1 x 15360 x
-// 5120 9.9 (12.1); and the host launches one kernel, 13.7 us a layer for 16.7. The
+// 5120 9.9 (12.1); and the host launches one kernel, 10 us a call for 13. The
 // quantizing takes every wave 50 instructions per 512 columns, so that from some 7000 on
 // it costs more than its kernel: 1 x 5120 x 20480 18.1 us (17.2), 1 x 5376 x 14336 11.6 (11.1).
 constexpr int kTokenPairs = 12, kTokenK = 512 * kTokenPairs;   // pairs of k-steps and columns per wave

@@ -155,8 +155,8 @@ def linear_rows(rows, b, b_scale, bias=None, *, activation=None, residual=None, 
                 gate_slot=None):
     """mxfp4_matmul of kernels.quantize_rows_mxfp4(rows) and the weight, with one
     allocation for codes and scales and one call for both kernels. At a few rows the
-    host bounds a layer: 16.5 us (13.7 at one row, which one kernel quantizes and
-    multiplies), 21.7 for the two functions one after the other."""
+    host bounds a layer: 13 us (10 at one row, which one kernel quantizes and
+    multiplies), 20 for the two functions one after the other."""
     m, k = rows.shape
     n = b.shape[0]
     dtype = _ROW_DTYPES.get(rows.dtype)

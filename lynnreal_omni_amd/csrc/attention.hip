@@ -759,13 +759,17 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int kind, int heads, int kv
   pl.piece = kKeys;
   if (kind == LR_ATTN_LENGTHS && pl.splits > 1) {
     // Places of a list of pieces over all sequences: as many as fill the GPU (one
-    // workgroup more would take a second round), n of them for the last pieces. Pieces
-    // are at least as long as makes their partial results small beside their keys: 32
-    // rows over three caches of 4096, 16 heads: 31.3 us with 512 keys, 35.7 with 64; 5 rows
-    // over four of 512: 8.9 with 64, 9.7 with 128.
-    const int64_t keys = 16 * tile_rows / kKeys * kKeys;
-    pl.piece = (int)(keys < kKeys ? kKeys : (keys > 512 ? 512 : keys));
+    // workgroup more would take a second round), n of them for the last pieces. Least
+    // keys of a piece by the same cost, halved since the caches are rarely all full: 32
+    // rows over three caches of 4096, 16 heads, take 31.3 us with 512 keys and 35.7 with
+    // 64; 5 rows over four of 512 8.9 with 64 and 9.7 with 128.
+    const double each = fmin(sqrt(tiles_k / (0.0003 * rows)), tiles_k);
+    pl.piece = (int)ceil((double)mean_k / fmax(each, 1.0) / kKeys) * kKeys;
     const int64_t most = mean_k / pl.piece;
+    if (most < 2) {
+      pl.splits = 1;
+      return pl;
+    }
     pl.pieces = true;
     pl.tiles /= n;
     const int64_t places = want / (pl.tiles * kv_heads);

@@ -87,4 +87,7 @@ def test_entry_point_refusals_without_a_gpu():
         assert call(**bad) == _lib.LR_EINVAL, bad
     assert lib.lr_attention_splits(0, 1, 1, 0, 4, 2) == 1
     assert lib.lr_attention_splits(1, 1, 131072, 0, 56, 8) > 1
+    # Padded caches: pieces of all sequences, none where there is a single tile of keys.
+    assert lib.lr_attention_splits(8, 1, 8192, 2, 40, 8) > 8
+    assert lib.lr_attention_splits(2, 32, 64, 2, 8, 8) == 1
     assert lib.lr_attention_splits(1, 12605, 12605, 0, 56, 56) == 1

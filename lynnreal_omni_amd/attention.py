@@ -174,8 +174,11 @@ def attention_packed(query, key, value, cu_query, cu_key=None, *, causal=False, 
 
 def block_attention(query, key, value, attention_mask, processor=None):
     """The attention of fusion.FusedAttention on this kernel: all tokens of
-    [batch, tokens, heads, head_dim] see all keys. Masks are not supported, and
-    that error is one a guarded block falls back from."""
+    [batch, tokens, heads, head_dim] see all keys. Masks are not supported, nor
+    tokens that a processor's _parallel_config spreads over ranks (each would see its
+    own alone); those errors are ones a guarded block falls back from."""
     if attention_mask is not None:
         raise RuntimeError("an attention mask is not supported by the HIP attention")
+    if getattr(processor, "_parallel_config", None) is not None:
+        raise RuntimeError("a parallel configuration is not supported by the HIP attention")
     return attention(query, key, value)

@@ -16,7 +16,6 @@ require a gradient are refused.
 from __future__ import annotations
 
 import functools
-import math
 import struct
 from array import array
 
@@ -26,6 +25,7 @@ from . import _lib
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _HEAD_DIMS = (32, 64, 128)
+_MAX_SCALE = torch.finfo(torch.float32).max
 _DENSE, _PACKED, _LENGTHS = range(3)
 
 
@@ -64,8 +64,8 @@ def _splits(sequences, q_rows, k_rows, kind, heads, kv_heads):
 
 @functools.lru_cache(maxsize=64)
 def _scale_bits(scale):
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 0 < scale <= _MAX_SCALE:
+        raise ValueError(f"scale must be positive and finite in fp32, got {scale}")
     return struct.unpack("i", struct.pack("f", scale))[0]
 
 

@@ -4,7 +4,8 @@ Weights and activations are E2M1 codes with an E8M0 scale for each 32 values
 along K (the OCP microscaling format MXFP4, scale exponent floor(log2(absmax))
 - 2). Against W8A8 a weight takes 0.53 bytes instead of one and the products
 run at twice the rate; the price is 4-bit precision in weights and activations.
-Inference only, as the rest of the package.
+Inference only, as the rest of the package: inputs that require a gradient are
+refused.
 """
 from __future__ import annotations
 

@@ -4,7 +4,8 @@ gfx950's scaled MFMA: the 4-bit counterpart of int8_gemm.
 Operands are what kernels.quantize_rows_mxfp4 returns for [rows, K] values:
 codes uint8 [rows, 16 * ceil(K / 32)] and scales uint8 in tile order. The
 weight is [N, K] like nn.Linear's, so mxfp4_matmul(a, w, ...) is a @ w.T.
-Inference only: the outputs carry no gradient.
+Inference only: the outputs carry no gradient, and inputs that require one are
+refused.
 """
 from __future__ import annotations
 
@@ -105,6 +106,11 @@ _PLAIN = (_lib.EPI_BF16, None, None, 0, 0, None, 0, 0)
 _GELU = (_lib.EPI_GELU_TANH, None, None, 0, 0, None, 0, 0)
 
 
+def _no_gradient(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("gradients are not supported by the MXFP4 product: call it under torch.no_grad()")
+
+
 def _bias(bias, n):
     if bias is None:
         return None
@@ -129,6 +135,7 @@ def mxfp4_matmul(a, b, a_scale, b_scale, bias=None, *, activation=None, residual
         raise ValueError(f"a has {a.shape[1]} bytes of codes per row, b {b.shape[1]}")
     if a.shape[1] == 0:
         raise ValueError("a and b have no columns")
+    _no_gradient(bias, residual, table)
     _lib.check_device(a)
     _lib.same_device(a, b=b, a_scale=a_scale, b_scale=b_scale, bias=bias, residual=residual, table=table,
                      indices=indices)
@@ -165,6 +172,7 @@ def linear_rows(rows, b, b_scale, bias=None, *, activation=None, residual=None, 
     _operand(b, b_scale, "b")
     if b.shape[1] != code_bytes(k) or k == 0:
         raise ValueError(f"rows of {k} columns do not fit a weight of {2 * b.shape[1]}")
+    _no_gradient(rows, bias, residual, table)
     _lib.check_device(rows)
     epilogue = _PLAIN
     if activation is None and residual is None and table is None and indices is None and gate_slot is None:

@@ -376,7 +376,8 @@ int lr_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t n, int64_t k, v
  *   keys cu_k[i] .. of the k_rows; the sequence strides are not used. Rows of no
  *   sequence become 0. Values are clamped to the rows.
  * causal: a token sees the keys up to its own place counted from the end, that
- *   is the last token all keys. A token that sees no key gives 0.
+ *   is the last token all keys. A token that sees no key gives 0, one whose keys
+ *   all score -inf NaN.
  * scale_bits: the fp32 bits of the scale, positive and finite.
  * splits > 1 cuts a sequence's keys for as many workgroups, joined in order by a
  *   second kernel; needs a workspace of splits * rows * (head_dim + 2) * 4 bytes,

@@ -121,7 +121,8 @@ def attention(query, key, value, *, causal=False, scale=None, key_lengths=None):
     token sees all keys, each one before it one key fewer. scale defaults to
     head_dim ** -0.5. key_lengths (int32 or int64 [batch], on the GPU): sequence i
     has its first key_lengths[i] keys; what lies behind them, the unused part of a
-    cache, is not read. A token that sees no key gives zeros.
+    cache, is not read. A token that sees no key gives zeros, one whose keys all
+    score -inf NaN (the formula's 0 / 0).
     """
     _check(query, key, value, 4)
     if key.shape[0] != query.shape[0]:

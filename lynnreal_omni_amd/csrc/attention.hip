@@ -3,8 +3,9 @@
 // One pass over the keys with a running maximum m and sum l per query row:
 //   s = scale * q . k;  m' = max(m, s);  p = 2^(log2(e) (s - m'));
 //   l = l 2^(log2(e) (m - m')) + sum p;  o = o 2^(log2(e) (m - m')) + p V
-// and o / l at the end (0 where a row sees no key). Scores, m, l and o are fp32;
-// p is rounded to the inputs' type for the second product, and o / l once at the end.
+// and o / l at the end: 0 where a row sees no key, NaN where all that it sees score -inf
+// (l is 0 in both). Scores, m, l and o are fp32; p is rounded to the inputs' type for
+// the second product, and o / l once at the end.
 // l adds the rounded p (in fp32, by a dot product with ones): the weights p / l then
 // add up to one, and a rounding error of p counts with v - o instead of v. Few rows
 // (FEW) leave the matrix units time to spare: there p is the sum of two such numbers.
@@ -344,10 +345,11 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, const Item& it, con
     float* const po = p.part + at * D;
     float* const ml = p.part + (int64_t)p.splits * all * D + at * 2;
     if (half == 0) {
-      ml[0] = m;
+      // Without a sum: whether the row has keys here (m is -inf either way).
+      ml[0] = sum == 0.0f && qr.limit > it.t0 * kKeys ? INFINITY : m;
       ml[1] = sum;
     }
-    if (sum == 0.0f) return;   // without keys of this row: left out of the join by its l
+    if (sum == 0.0f) return;   // left out of the join by its l
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -356,7 +358,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, const Item& it, con
             make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
     return;
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inv = sum == 0.0f ? (qr.limit > 0 ? NAN : 0.0f) : 1.0f / sum;
   uint16_t* const po = p.out + row * D;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
@@ -671,11 +673,13 @@ __global__ __launch_bounds__(256) void join_splits(AttnArgs p) {
   // Every wave finds the maximum and the sum by itself (at most 256 splits).
   float2 v[4];
   float m = -INFINITY;
+  bool keys = false;   // whether a split without a sum has some of the row (store_row)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = 64 * i + (t & 63);
     v[i] = s < splits ? ml[at0 + s * rows] : make_float2(0.0f, 0.0f);
     if (v[i].y != 0.0f) m = fmaxf(m, v[i].x);
+    else keys |= v[i].x == INFINITY;
   }
   m = wave_max(m);
   float l = 0.0f;
@@ -686,6 +690,7 @@ __global__ __launch_bounds__(256) void join_splits(AttnArgs p) {
     l += w * v[i].y;
   }
   l = wave_tree_sum(l);
+  const bool sees = __any(keys);
   __syncthreads();
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   constexpr int BATCH = 4;   // loads in flight
@@ -715,7 +720,7 @@ __global__ __launch_bounds__(256) void join_splits(AttnArgs p) {
     o.z += x.z;
     o.w += x.w;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = l == 0.0f ? (sees ? NAN : 0.0f) : 1.0f / l;
   *reinterpret_cast<uint2*>(p.out + row * D + 4 * at) =
       make_uint2(Mfma<T>::pack(o.x * inv, o.y * inv), Mfma<T>::pack(o.z * inv, o.w * inv));
 }

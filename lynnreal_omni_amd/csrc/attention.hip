@@ -148,8 +148,8 @@ __device__ __forceinline__ int wave_prefix_sum(int v) {
 
 // Few queries over sequences of different numbers of keys: all are cut into pieces of
 // one size, so that the longest is not what everybody waits for, in a list over the
-// sequences that every wave works out from the lengths by itself. With n sequences and
-// p.splits > n places, pieces of (keys in all) / (p.splits - n) keys fit the list.
+// sequences that every wave works out from the lengths by itself. It has p.splits >= 2 n
+// places for n sequences (lr_attention).
 struct Pieces {
   int chunk = 0;              // keys of a piece, a multiple of 64
   int seq = -1, keys = 0;     // the sequence asked for (-1: the list ends before)
@@ -161,9 +161,9 @@ struct Pieces {
     auto length = [&](int64_t i) __attribute__((always_inline)) {
       return i < p.n ? (int)clamp64(p.lengths[i], 0, p.k_rows) : 0;
     };
-    // The smallest pieces that the list holds: from an even share up in steps, at the
-    // latest where n of the places are left for sequences' last pieces. Sums in fp32,
-    // in units of 64 keys: they may pass 32 bits (sequences of an expanded tensor
+    // The smallest pieces that the list holds: from an even share up in steps, which end
+    // at the latest where n of the places are left for sequences' last pieces. Sums in
+    // fp32, in units of 64 keys: they may pass 32 bits (sequences of an expanded tensor
     // share their keys); the counts that have to be exact are below 2^24.
     auto units_of = [&](int size) __attribute__((always_inline)) {
       float sum = 0.0f;
@@ -172,13 +172,10 @@ struct Pieces {
       // The same in every lane; said so, since what depends on it addresses memory.
       return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_tree_sum(sum))));
     };
-    const float all = units_of(1) * 1.001f;
     const int least = (int)((p.k_rows + 64 * kMaxSplits - 1) / (64 * kMaxSplits));   // of one sequence
-    const bool tight = p.splits < 2 * p.n;
-    const float share = all / (float)(tight ? p.splits - (int)p.n : p.splits);
-    int size = max(max(p.piece >> 6, least), share < 1.6e7f ? (int)share + (tight ? 1 : 0) : 1 << 24);
-    if (!tight)
-      while (units_of(size) > (float)p.splits) size += max(1, size >> 4);
+    const float share = units_of(1) / (float)p.splits;
+    int size = max(max(p.piece >> 6, least), share < 1.6e7f ? (int)share : 1 << 24);
+    while (units_of(size) > (float)p.splits) size += max(1, size >> 4);
     chunk = __builtin_amdgcn_readfirstlane(size) * 64;
     int before = 0;   // pieces of the sequences before this group of 64
     for (int64_t base = 0; base < p.n; base += 64) {
@@ -764,10 +761,12 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int kind, int heads, int kv
   pl.piece = kKeys;
   if (kind == LR_ATTN_LENGTHS && pl.splits > 1) {
     // Places of a list of pieces over all sequences: as many as fill the GPU (one
-    // workgroup more would take a second round), n of them for the last pieces. Least
-    // keys of a piece by the same cost, halved since the caches are rarely all full: 32
-    // rows over three caches of 4096, 16 heads, take 31.3 us with 512 keys and 35.7 with
-    // 64; 5 rows over four of 512 8.9 with 64 and 9.7 with 128.
+    // workgroup more would take a second round), at least 2 n, since want / work is 2 or
+    // more here; past that (257 pairs of a sequence and a key head with few rows on 256
+    // CUs) every sequence is walked whole. Least keys of a piece by the same cost, halved
+    // since the caches are rarely all full: 32 rows over three caches of 4096, 16 heads,
+    // take 31.3 us with 512 keys and 35.7 with 64; 5 rows over four of 512 8.9 with 64 and
+    // 9.7 with 128.
     const double each = fmin(sqrt(tiles_k / (0.0003 * rows)), tiles_k);
     pl.piece = (int)ceil((double)mean_k / fmax(each, 1.0) / kKeys) * kKeys;
     const int64_t most = mean_k / pl.piece;
@@ -779,7 +778,7 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int kind, int heads, int kv
     pl.tiles /= n;
     const int64_t places = want / (pl.tiles * kv_heads);
     const int64_t all = n + n * (most < kMaxSplits ? most : kMaxSplits);
-    pl.splits = (int)(places > all ? all : (places > n ? places : n + 1));
+    pl.splits = (int)(places > all ? all : places);
   }
   return pl;
 }
@@ -874,8 +873,8 @@ extern "C" int lr_attention(const void* q, const void* k, const void* v, void* o
   LR_REQUIRE(splits >= 1 && (splits == 1 || splits <= (pl.splits > kMaxSplits ? pl.splits : kMaxSplits)),
              "attention: %d splits", splits);
   if (key_lengths && splits > 1)
-    LR_REQUIRE(pl.pieces && splits == pl.splits, "attention: with key lengths, 1 or the %d splits of lr_attention_splits",
-               pl.splits);
+    LR_REQUIRE(pl.pieces && splits == pl.splits && splits >= 2 * sequences,
+               "attention: with key lengths, 1 or the %d splits of lr_attention_splits", pl.splits);
   else if (pl.pieces)   // one split: whole sequences
     pl.tiles *= sequences;
   pl.splits = splits;

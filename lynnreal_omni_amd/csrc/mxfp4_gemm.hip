@@ -366,7 +366,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void fp4_tile(Fp4Args p) {
 }
 
 // ------------------------------------------------------ ping-pong kernel ----
-// K % 256 == 0. Eight waves, 2 x 4; those of the upper half of the rows (one per
+// K % 256 == 0, staged outputs. Eight waves, 2 x 4; those of the upper half of the rows (one per
 // SIMD) and of the lower half (the SIMD's other wave) take turns: while one group
 // issues nothing but the matrix instructions of its k-step, from registers, the
 // other reads its next fragments from LDS and issues DMAs and scale loads, with a
@@ -553,14 +553,13 @@ __global__ __launch_bounds__(512) void fp4_pingpong(Fp4Args p) {
   }
   __builtin_amdgcn_s_waitcnt(kPro);  // the trailing DMAs have landed
   __syncthreads();
-  const int64_t mw = m0 + grp * WM, nw = n0 + q * WN;
-  if (p.staged) store_staged<FM, FN, EPI>(p, acc, smem + wave * STAGE, mw, nw, lane);
-  else store_direct<FM, FN, EPI>(p, acc, mw, nw, lane);
+  store_staged<FM, FN, EPI>(p, acc, smem + wave * STAGE, m0 + grp * WM, n0 + q * WN, lane);
 }
 
 template <int BM, int BN>
 int launch_pingpong(Fp4Args p, int epilogue, hipStream_t s) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
+  LR_REQUIRE(p.kb % 128 == 0 && p.staged, "mxfp4_gemm: not a shape of the ping-pong kernel");
   LR_REQUIRE(tm * tn <= kMaxBlocks / 2, "mxfp4_gemm: %lld output tiles are not supported", (long long)(tm * tn));
   p.tiles_m = (int)tm;
   p.tiles_n = (int)tn;

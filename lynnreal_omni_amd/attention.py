@@ -8,7 +8,17 @@ RoPE (kernels.qk_norm_rope) and the output projection.
                     fusion.enable_fusion(..., attention=block_attention)
 
 bf16 or fp16; head_dim 32, 64 or 128; query heads may share key heads. Scores,
-maxima, sums and accumulators are fp32. Keys that a token may not see are left
+maxima, sums and accumulators are fp32. The softmax weights are rounded to the
+inputs' type for the product with v; where `attention` has at most 32 rows (tokens
+x query heads of a key head) they keep the rest of that rounding as a second number,
+so that the output's own rounding is all that remains. attention_packed rounds them
+once whatever its number of tokens, so that a sequence gives the same bits whatever
+lies around it: the same token may differ by the weights' rounding between the two.
+
+Tensors whose last dimension is dense, whose other strides are multiples of 8 elements
+(those between tokens below 2^23) and whose memory is 16-byte aligned are read as
+they are: slices of a fused projection, caches with the heads outside, expanded
+batches. Any other is copied as a whole in every call: lay a cache out so. Keys that a token may not see are left
 out whatever their scores; the values of a sequence have to be finite (a weight
 of zero times an infinity is NaN, as in the formula). Inference only: inputs that
 require a gradient are refused.
@@ -114,8 +124,7 @@ def _launch(query, key, value, cu_q, cu_k, lengths, causal, scale, sequences, q_
 
 def attention(query, key, value, *, causal=False, scale=None, key_lengths=None):
     """softmax(scale * q k^T) v for query [batch, tokens, heads, head_dim] and key,
-    value [batch, keys, kv_heads, head_dim] (views with dense heads are taken as
-    they are); returns a contiguous tensor like query.
+    value [batch, keys, kv_heads, head_dim]; returns a contiguous tensor like query.
 
     heads / kv_heads query heads in a row share a key head. causal: the last
     token sees all keys, each one before it one key fewer. scale defaults to

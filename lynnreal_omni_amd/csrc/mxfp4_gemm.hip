@@ -386,8 +386,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void fp4_tile(Fp4Args p) {
 // Measured: 5.0 PFLOP/s in the loop (4096 x 4096 x 65536: 450-461 us). Matrix
 // instructions on random codes from registers alone reach 6.9 to 7.4 (9.6 on zeros:
 // the chip's power bounds them); without its scale loads the loop takes 430 us, without
-// DMAs 383, without LDS reads 413. With starts and ends of tiles 4.4 PFLOP/s (12605 x
-// 28672 x 5376: 877-890 us, of which storing 723 MB costs 100: a tile's registers are
+// DMAs 383, without LDS reads 413. With starts and ends of tiles 4.3 to 4.4 PFLOP/s (12605 x
+// 28672 x 5376: 877-902 us, of which storing 723 MB costs 100: a tile's registers are
 // all in use, so that the next tile cannot start under its end; starting the CUs at
 // different times, 904 us, does not spread that). One workgroup looping over tiles
 // with the next one's loads in flight spilled and was slower.
@@ -618,8 +618,8 @@ __device__ __forceinline__ void store_few(const Fp4Args& p, const v4f (&acc)[FM]
 // k-steps in flight into a ring of LDS that no other wave touches, so that it meets
 // no barrier, with whole 128-byte lines of both operands and their scales (fragments
 // straight into registers read half lines, and their waits, which count in issue
-// order, would hold up the ring). 1 x 21504 x 5376: 12.0 us, 5.1 TB/s of weights; 16 x
-// 5376 x 14336: 9.1 us, 4.5 TB/s.
+// order, would hold up the ring). 1 x 21504 x 5376: 12.0 us, 5.1 TB/s of weights that partly
+// come out of the caches, 13.2 us, 4.6 TB/s, where none do; 16 x 5376 x 14336: 9.1 us, 4.5.
 template <int FM, int FN, int WAVES, int S, int EPI>
 __global__ __launch_bounds__(64 * WAVES) void fp4_few(Fp4Args p) {
   constexpr int BK = 128;
@@ -710,7 +710,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp4_few(Fp4Args p) {
 // One row, quantized by every workgroup for itself, which costs less than a kernel
 // before this one: fp4_few with the row's codes and scales in LDS, each wave those of
 // its own k-steps. The first weights are in flight meanwhile. Against the two kernels,
-// back to back: 1 x 21504 x 5376 14.1 us (15.4), 1 x 5120 x 5120 6.3 (7.3), 1 x 15360 x
+// back to back: 1 x 21504 x 5376 14.1-14.6 us (15.4), 4.2 TB/s of weights, 1 x 5120 x 5120 6.3 (7.3), 1 x 15360 x
 // 5120 9.9 (12.1); and the host launches one kernel, 10 us a call for 13. The
 // quantizing takes every wave 50 instructions per 512 columns, so that from some 7000 on
 // it costs more than its kernel: 1 x 5120 x 20480 18.1 us (17.2), 1 x 5376 x 14336 11.6 (11.1).
@@ -855,9 +855,10 @@ int launch_tile(Fp4Args p, int epilogue, hipStream_t s) {
 
 // -------------------------------------------------------------- schedule ----
 // The ping-pong kernel's tiles, and what one costs: us of a k-step and of a tile's
-// start and end, for the 256 CUs' tiles together, from 1320 timings (M 72 to 12605, N
-// 2048 to 28672, K 1024 to 20480; mean error 5%). The choice that it makes is on
-// average 0.1% and at most 7% slower than the fastest tile of those shapes.
+// start and end, for the 256 CUs' tiles together, from 990 timings (six tiles, 165
+// shapes, M 72 to 12605, N 2048 to 28672, K 1024 to 20480; mean error 5% beside 3 us per
+// call). The choice that it makes is on average 0.1% and at most 7% slower than the
+// fastest tile of those shapes.
 struct Tile {
   int rows, cols;
   double factor;

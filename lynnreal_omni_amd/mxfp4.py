@@ -2,8 +2,9 @@
 
 Weights and activations are E2M1 codes with an E8M0 scale for each 32 values
 along K (the OCP microscaling format MXFP4, scale exponent floor(log2(absmax))
-- 2). Against W8A8 a weight takes 0.53 bytes instead of one and the products
-run at twice the rate; the price is 4-bit precision in weights and activations.
+- 2). Against W8A8 a weight takes 0.53 bytes instead of one and a large product
+1.5 times less time (12605 x 28672 x 5376: 0.90 ms for 1.37); the price is 4-bit
+precision in weights and activations.
 Inference only, as the rest of the package: inputs that require a gradient are
 refused.
 """

@@ -393,6 +393,24 @@ int lr_attention(const void* q, const void* k, const void* v, void* out, int dty
                  const int32_t* cu_q, const int32_t* cu_k, const int32_t* key_lengths, int causal,
                  int scale_bits, void* workspace, int64_t workspace_bytes, int splits, void* stream);
 
+/* lr_attention of `sequences` sequences that all see prefix_rows keys in common before
+ * their own: out = softmax(scale * q [prefix_k; k]^T) [prefix_v; v], and where lse is not
+ * NULL the logarithm of each softmax's sum, fp32 [sequences, q_rows, heads] (-inf for
+ * a token that sees no key, or whose keys all score -inf).
+ *   q, k, v, out, key_lengths, causal, scale_bits as in lr_attention, for dense batches
+ *   (causal counts the own keys; every token sees the whole prefix). prefix_k and
+ *   prefix_v [prefix_rows, kv_heads, head_dim]. strides, thirteen: q (token, head,
+ *   sequence), prefix_k (token, head), prefix_v (token, head), k and v like q.
+ * workspace: 16-byte aligned, of the bytes that lr_attention_prefix_workspace gives for
+ *   the same shape on the same device (0: it may be NULL). */
+int lr_attention_prefix_workspace(int64_t sequences, int64_t q_rows, int64_t k_rows, int64_t prefix_rows, int heads,
+                                  int kv_heads, int head_dim, int64_t* bytes);
+int lr_attention_prefix(const void* q, const void* prefix_k, const void* prefix_v, const void* k, const void* v,
+                        void* out, float* lse, int dtype, int64_t sequences, int64_t q_rows, int64_t k_rows,
+                        int64_t prefix_rows, int heads, int kv_heads, int head_dim, const int64_t* strides,
+                        const int32_t* key_lengths, int causal, int scale_bits, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -71,6 +71,9 @@ SIGNATURES = {
     "lr_attention_splits": [_I64, _I64, _I64, _I32, _I32, _I32],
     "lr_attention": [_P, _P, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _I32, _P, _I64,
                      _I32, _P],
+    "lr_attention_prefix_workspace": [_I64, _I64, _I64, _I64, _I32, _I32, _I32, _P],
+    "lr_attention_prefix": [_P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32,
+                            _I32, _P, _I64, _P],
     "lr_device_supported": [_I32],
     "lr_abi_version": [],
 }

@@ -4,6 +4,8 @@ RoPE (kernels.qk_norm_rope) and the output projection.
   attention         a batch of sequences of one length, or a few new tokens over
                     padded caches with their own numbers of valid keys
   attention_packed  sequences of different lengths behind each other
+  attention_shared_prefix  a batch whose sequences all see a common prefix of keys
+                    before their own caches, which is read for all of them at once
   block_attention   the same as fusion.FusedAttention calls it, for
                     fusion.enable_fusion(..., attention=block_attention)
 
@@ -122,6 +124,16 @@ def _launch(query, key, value, cu_q, cu_k, lengths, causal, scale, sequences, q_
     return out
 
 
+def _lengths(key_lengths, batch, keys):
+    """key_lengths as the kernels read them."""
+    if key_lengths.shape != (batch,) or key_lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError("key_lengths must be int32 or int64 [batch]")
+    # Clamped before the conversion, which would wrap what lies past 32 bits.
+    if key_lengths.dtype == torch.int64:
+        key_lengths = key_lengths.clamp(0, keys).to(torch.int32)
+    return key_lengths.contiguous()
+
+
 def attention(query, key, value, *, causal=False, scale=None, key_lengths=None):
     """softmax(scale * q k^T) v for query [batch, tokens, heads, head_dim] and key,
     value [batch, keys, kv_heads, head_dim]; returns a contiguous tensor like query.
@@ -138,15 +150,8 @@ def attention(query, key, value, *, causal=False, scale=None, key_lengths=None):
         raise ValueError(f"query has a batch of {query.shape[0]}, key of {key.shape[0]}")
     batch, tokens, keys = query.shape[0], query.shape[1], key.shape[1]
     if key_lengths is not None:
-        if key_lengths.shape != (batch,) or key_lengths.dtype not in (torch.int32, torch.int64):
-            raise ValueError("key_lengths must be int32 or int64 [batch]")
-        _lib.same_device(query, key=key, value=value, key_lengths=key_lengths)
-        # Clamped before the conversion, which would wrap what lies past 32 bits.
-        if key_lengths.dtype == torch.int64:
-            key_lengths = key_lengths.clamp(0, keys).to(torch.int32)
-        key_lengths = key_lengths.contiguous()
-    else:
-        _lib.same_device(query, key=key, value=value)
+        key_lengths = _lengths(key_lengths, batch, keys)
+    _lib.same_device(query, key=key, value=value, key_lengths=key_lengths)
     return _launch(query, key, value, None, None, key_lengths, causal, scale, batch, tokens, keys)
 
 
@@ -180,6 +185,68 @@ def attention_packed(query, key, value, cu_query, cu_key=None, *, causal=False, 
     cu_key = cu_query if same else _first_rows(cu_key, "cu_key")
     return _launch(query, key, value, cu_query, cu_key, None, causal, scale, cu_query.numel() - 1, query.shape[0],
                    key.shape[0])
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_strides(query, prefix_key, prefix_value, key, value):
+    """The thirteen strides that lr_attention_prefix takes, of tensors given as (stride,
+    shape): token, head and, of batches, sequence."""
+    thirteen = array("q")
+    for stride, shape in (query, prefix_key, prefix_value, key, value):
+        s = [st if n > 1 else 0 for st, n in zip(stride, shape)]
+        thirteen.extend((s[-3], s[-2]) if len(s) == 3 else (s[1], s[2], s[0]))
+    return thirteen
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_workspace(device, batch, tokens, keys, prefix, heads, kv_heads, dim):
+    nbytes = array("q", [0])
+    with torch.cuda.device(device):
+        _lib.call("lr_attention_prefix_workspace", batch, tokens, keys, prefix, heads, kv_heads, dim,
+                  nbytes.buffer_info()[0])
+    return nbytes[0]
+
+
+def attention_shared_prefix(query, prefix_key, prefix_value, key, value, *, causal=False, scale=None, key_lengths=None,
+                            return_lse=False):
+    """attention of a batch whose sequences share their first keys: query [batch, tokens,
+    heads, head_dim], prefix_key and prefix_value [prefix, kv_heads, head_dim], key and
+    value [batch, keys, kv_heads, head_dim]; returns a contiguous tensor like query.
+
+    A token sees the whole prefix and the keys of its own sequence that it sees in
+    attention(query, key, value, causal=.., key_lengths=..): causal counts the own
+    keys alone. The prefix is read once for all sequences where they have few tokens
+    each. Prefix, keys or both may be empty. return_lse: returns (output, lse), lse
+    fp32 [batch, tokens, heads] the logarithm of the sum of exp(scale * q k) over the
+    keys that a token sees, -inf where it sees none or all score -inf.
+    """
+    _check(query, key, value, 4)
+    if prefix_key.dim() != 3 or prefix_value.shape != prefix_key.shape or prefix_key.shape[1:] != key.shape[2:]:
+        raise ValueError("prefix_key and prefix_value must be [prefix, kv_heads, head_dim], with key's heads")
+    if prefix_key.dtype != query.dtype or prefix_value.dtype != query.dtype:
+        raise ValueError(f"the prefix must have the query's dtype, got {prefix_key.dtype}, {prefix_value.dtype}")
+    if torch.is_grad_enabled() and (prefix_key.requires_grad or prefix_value.requires_grad):
+        raise RuntimeError("gradients are not supported by the HIP attention: call it under torch.no_grad()")
+    if key.shape[0] != query.shape[0]:
+        raise ValueError(f"query has a batch of {query.shape[0]}, key of {key.shape[0]}")
+    batch, tokens, heads, dim = query.shape
+    keys, kv_heads = key.shape[1:3]
+    if key_lengths is not None:
+        key_lengths = _lengths(key_lengths, batch, keys)
+    _lib.same_device(query, prefix_key=prefix_key, prefix_value=prefix_value, key=key, value=value,
+                     key_lengths=key_lengths)
+    scale = _scale_bits(float(dim ** -0.5 if scale is None else scale))
+    given = (query, prefix_key, prefix_value, key, value)
+    given = tuple(t if not t.data_ptr() & 15 and _dense(t.stride(), t.shape) else _rows(t) for t in given)
+    strides = _prefix_strides(*((t.stride(), t.shape) for t in given))
+    out = query.new_empty(query.shape)
+    lse = query.new_empty((batch, tokens, heads), dtype=torch.float32) if return_lse else None
+    nbytes = _prefix_workspace(query.get_device(), batch, tokens, keys, prefix_key.shape[0], heads, kv_heads, dim)
+    ws = _lib.workspace(query, nbytes)   # held until the launch
+    _lib.launch(query, "lr_attention_prefix", *(t.data_ptr() for t in given), out.data_ptr(), _lib.ptr(lse),
+                _DTYPES[query.dtype], batch, tokens, keys, prefix_key.shape[0], heads, kv_heads, dim,
+                strides.buffer_info()[0], _lib.ptr(key_lengths), int(bool(causal)), scale, _lib.ptr(ws), nbytes)
+    return (out, lse) if return_lse else out
 
 
 def block_attention(query, key, value, attention_mask, processor=None):

@@ -1,0 +1,507 @@
+// attention_prefix.hip - attention of a batch whose sequences share a prefix of keys:
+//
+//   out = softmax(scale q [Kp; Ki]^T) [Vp; Vi],  lse = log sum exp(scale q [Kp; Ki]^T)
+//
+// for tokens q of sequence i, the prefix Kp, Vp and the sequence's own padded cache Ki,
+// Vi. Every token sees the whole prefix. Running maximum, sum and output of a row over
+// any set of keys join with those over any other (attention.hip), so there are two ways:
+//
+// Few rows per sequence (single tokens): the prefix is read once for the rows of all
+// sequences, 128 of them per workgroup, cut into pieces over the GPU; so are the own
+// caches, each for its own rows; a second kernel joins a row's pieces in order.
+// What that reads is the floor: the prefix once, not once per sequence.
+//
+// Many rows per sequence: a workgroup's 128 rows walk the prefix and then the own cache
+// in one pass. Nothing is joined, and the prefix comes out of the caches, since the
+// matrix units, not the keys, are what bounds it.
+#include "lr_attention.h"
+#include "lr_runtime.h"
+
+namespace lr {
+namespace {
+
+constexpr int kMaxPieces = 256;   // of a cache, and of the prefix
+constexpr int kListed = 512;      // sequences of a list of pieces: eight lengths per lane
+
+struct PrefixArgs {
+  const uint16_t *q, *pk, *pv, *k, *v;
+  uint16_t* out;
+  float* lse;            // or null
+  float* part;           // o [parts][dim], then (exponent, l, exact l, sees keys) [parts]
+  int64_t qt, qh, qb;    // strides of a token, a head, a sequence, in elements
+  int64_t pkt, pkh, pvt, pvh;
+  int64_t kt, kh, kb;
+  int64_t vt, vh, vb;
+  const int32_t* lengths;   // valid keys of the own caches, or null
+  int n, q_rows, k_rows, prefix;
+  int heads, kv_heads, group;
+  int causal;
+  float c;               // scale * log2(e)
+  int seq_tiles;         // tiles of 128 rows of a sequence
+  int all_tiles;         // and of all sequences' rows together
+  int places;            // workgroups per key head (pieces); 0: more sequences than a list holds
+  int shares;            // most pieces of the prefix
+  int own;               // most pieces of the own caches
+  int piece;             // least tiles of 64 keys of a piece
+};
+
+__device__ __forceinline__ int own_keys(const PrefixArgs& p, int i) {
+  return p.lengths ? (int)clamp64(p.lengths[i], 0, p.k_rows) : p.k_rows;
+}
+__device__ __forceinline__ int key_tiles(int keys) { return (int)((uint32_t)(keys + kKeys - 1) / kKeys); }
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)((uint32_t)(a + b - 1) / (uint32_t)b); }
+
+// How prefix and caches are cut: pieces of `size` tiles of 64 keys, the smallest for
+// which all of them have a place. Every wave works it out from the lengths by itself.
+struct Cut {
+  int size, prefix;     // tiles of a piece; pieces of the prefix
+  int mine[kListed / 64];   // key tiles of sequences lane, lane + 64, ..
+  int groups;
+  __device__ __forceinline__ explicit Cut(const PrefixArgs& p) {
+    const int lane = threadIdx.x & 63, tiles = key_tiles(p.prefix);
+    size = max(p.piece, ceil_div(tiles, p.shares));
+    groups = 0;
+    if (p.places) {
+      groups = (p.n + 63) >> 6;
+#pragma unroll
+      for (int g = 0; g < kListed / 64; ++g) {
+        const int i = 64 * g + lane;
+        mine[g] = i < p.n ? key_tiles(own_keys(p, i)) : 0;
+      }
+      // Places that pieces of `size` take. Sums in fp32: what has to be exact is below 2^24.
+      auto taken = [&](int size) __attribute__((always_inline)) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int g = 0; g < kListed / 64; ++g)
+          if (g < groups) sum += (float)ceil_div(mine[g], size);
+        sum = wave_tree_sum(sum) * (float)p.seq_tiles + (float)(ceil_div(tiles, size) * p.all_tiles);
+        // The same in every lane; said so, since what depends on it addresses memory.
+        return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sum)));
+      };
+      // From an even share up in steps, which end at the latest where every cache is one piece
+      // (lr_attention_prefix gives as many places).
+      size = max(max(size, ceil_div(key_tiles(p.k_rows), kMaxPieces)), (int)(taken(1) / (float)p.places));
+      while (taken(size) > (float)p.places) size += max(1, size >> 4);
+    }
+    size = __builtin_amdgcn_readfirstlane(size);
+    prefix = ceil_div(tiles, size);
+  }
+  // Of sequence `want`, or where that is -1 the one that has piece `place` of the caches
+  // (-1: there is none): its number, its first piece and how many there are.
+  __device__ __forceinline__ void find(const PrefixArgs& p, int want, int place, int& seq, int& first, int& count) const {
+    const int lane = threadIdx.x & 63;
+    seq = -1;
+    if (!p.places) {   // a piece each
+      seq = want >= 0 ? want : (place < p.n ? place : -1);
+      first = seq;
+      count = seq >= 0 && own_keys(p, seq) > 0;
+      return;
+    }
+    int before = 0;
+#pragma unroll
+    for (int g = 0; g < kListed / 64; ++g) {
+      if (g >= groups || seq >= 0) continue;
+      const int n = ceil_div(mine[g], size);
+      const int upto = wave_prefix_sum(n);
+      const bool here = want >= 0 ? 64 * g + lane == want : (before + upto > place && 64 * g + lane < p.n);
+      const uint64_t hit = __ballot(here);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        seq = 64 * g + l;
+        count = __builtin_amdgcn_readlane(n, l);
+        first = before + __builtin_amdgcn_readlane(upto, l) - count;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+};
+
+// The rows of a part of the prefix, of all sequences, come before those of the own pieces.
+__device__ __forceinline__ int64_t own_part(const PrefixArgs& p, int piece) {
+  const int64_t each = (int64_t)p.q_rows * p.heads;
+  return ((int64_t)p.shares * p.n + piece) * each;
+}
+__device__ __forceinline__ int64_t all_parts(const PrefixArgs& p) { return own_part(p, p.own); }
+
+// A sequence's rows 128 * tile .. and the own keys that they see.
+struct OwnRows {
+  int kn, rows, r0, sure, tiles;   // tiles: of the keys that any of them sees
+  __device__ __forceinline__ OwnRows(const PrefixArgs& p, int seq, int tile) {
+    kn = own_keys(p, seq);
+    rows = p.q_rows * p.group;
+    r0 = tile * kRows;
+    sure = kn;
+    int any = kn;
+    if (p.causal) {
+      const int last = min(r0 + kRows, rows) - 1;
+      any = min(kn, max(0, kn - p.q_rows + (int)((uint32_t)last / (uint32_t)p.group) + 1));
+      sure = min(kn, max(0, kn - p.q_rows + (int)((uint32_t)r0 / (uint32_t)p.group) + 1));
+    }
+    tiles = key_tiles(any);
+  }
+};
+
+struct Row {
+  int tok, head, seen;   // token (of the sequence or of all), head, own keys that it sees
+  __device__ __forceinline__ Row(const PrefixArgs& p, int r, int rows, int hd, int kn) {
+    const int rc = min(r, rows - 1);
+    tok = (int)((uint32_t)rc / (uint32_t)p.group);
+    head = hd * p.group + (rc - tok * p.group);
+    seen = p.causal ? min(kn, max(0, kn - p.q_rows + tok + 1)) : kn;
+  }
+};
+
+__device__ __forceinline__ OneCache own_cache(const PrefixArgs& p, int seq, int hd, const OwnRows& w, int seen) {
+  return {p.k + seq * p.kb + hd * p.kh, p.v + seq * p.vb + hd * p.vh, p.kt, p.vt, w.kn, w.sure, seen};
+}
+__device__ __forceinline__ OneCache prefix_cache(const PrefixArgs& p, int hd) {
+  return {p.pk + hd * p.pkh, p.pv + hd * p.pvh, p.pkt, p.pvt, p.prefix, p.prefix, p.prefix};
+}
+
+// One piece of the prefix or of a cache for at most 128 rows.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[kTileBytes<D>];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, col = lane & 31;
+  // All key heads of the same keys, which lie side by side, come first.
+  const int hds = p.kv_heads, item = (int)(blockIdx.x / (uint32_t)hds), hd = (int)(blockIdx.x - item * hds);
+  const Cut cut(p);
+  OneCache keys;
+  int t0, t1, rows, r0;
+  int64_t part, qoff;
+  bool sees;
+  if (item < cut.prefix * p.all_tiles) {
+    // The row tiles of a piece lie side by side, so that they share its keys in a cache.
+    const int piece = (int)((uint32_t)item / (uint32_t)p.all_tiles);
+    rows = p.n * p.q_rows * p.group;
+    r0 = (item - piece * p.all_tiles) * kRows;
+    const Row row(p, r0 + wave * 32 + col, rows, hd, 0);
+    const int seq = (int)((uint32_t)row.tok / (uint32_t)p.q_rows);
+    qoff = seq * p.qb + (row.tok - seq * p.q_rows) * p.qt + row.head * p.qh;
+    keys = prefix_cache(p, hd);
+    t0 = piece * cut.size;
+    t1 = min(key_tiles(p.prefix), t0 + cut.size);
+    part = ((int64_t)piece * p.n * p.q_rows + row.tok) * p.heads + row.head;
+    sees = true;
+  } else {
+    const int place = item - cut.prefix * p.all_tiles, piece = (int)((uint32_t)place / (uint32_t)p.seq_tiles);
+    int seq, first, count;
+    cut.find(p, -1, piece, seq, first, count);
+    if (seq < 0) return;
+    const OwnRows w(p, seq, place - piece * p.seq_tiles);
+    rows = w.rows;
+    r0 = w.r0;
+    const Row row(p, r0 + wave * 32 + col, rows, hd, w.kn);
+    qoff = seq * p.qb + row.tok * p.qt + row.head * p.qh;
+    keys = own_cache(p, seq, hd, w, row.seen);
+    const int size = p.places ? cut.size : w.tiles;
+    t0 = min(w.tiles, (piece - first) * size);
+    t1 = min(w.tiles, t0 + size);
+    part = own_part(p, piece) + (int64_t)row.tok * p.heads + row.head;
+    sees = row.seen > t0 * kKeys;
+  }
+  v16f o[D / 32];
+  float m, l, exact, off;
+  const bool idle = r0 + wave * 32 >= rows;
+  if (rows - r0 <= 32) attend<T, D, true, true>(smem, keys, p.q + qoff, p.c, t0, t1, idle, m, l, exact, off, o);
+  else attend<T, D, false, true>(smem, keys, p.q + qoff, p.c, t0, t1, idle, m, l, exact, off, o);
+  l = add_partner(l);
+  exact = add_partner(exact);
+  if (r0 + wave * 32 + col >= rows) return;
+  float* const po = p.part + part * D;
+  if (half == 0) reinterpret_cast<float4*>(p.part + all_parts(p) * D)[part] = make_float4(off, l, exact, sees);
+  if (l == 0.0f) return;   // left out of the join by its l
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(po + 32 * d + 8 * g + 4 * half) =
+          make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+}
+
+constexpr float kLn2 = 0.69314718055994531f;
+
+// Joins the pieces of a row: weights 2^(exponent - the largest). A workgroup per row: D / 4
+// threads hold a piece's columns, and the groups of them take every G-th piece, then are
+// added in order, so that the result does not depend on timing.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_join(PrefixArgs p) {
+  constexpr int LANES = D / 4, G = 256 / LANES, NV = 2 * kMaxPieces / 64;
+  __shared__ float weight[2 * kMaxPieces];
+  __shared__ float4 sums[G][LANES];
+  const int64_t row = blockIdx.x;
+  const int each = p.q_rows * p.heads, seq = (int)(blockIdx.x / (uint32_t)each);
+  const Cut cut(p);
+  int found, first, count;
+  cut.find(p, seq, 0, found, first, count);
+  const int parts = cut.prefix + count;
+  const int64_t own = own_part(p, first) + (row - (int64_t)seq * each);
+  auto at = [&](int i) __attribute__((always_inline)) {
+    return i < cut.prefix ? row + (int64_t)i * p.n * each : own + (int64_t)(i - cut.prefix) * each;
+  };
+  const float4* const stats = reinterpret_cast<const float4*>(p.part + all_parts(p) * D);
+  const int t = threadIdx.x, lane = t & 63, x = t % LANES, g = t / LANES;
+  // Every wave finds the maximum and the sums by itself.
+  float4 v[NV];
+  float top = -INFINITY, seen = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    v[i] = 64 * i + lane < parts ? stats[at(64 * i + lane)] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (v[i].y != 0.0f) top = fmaxf(top, v[i].x);
+    seen = fmaxf(seen, v[i].w);
+  }
+  top = wave_max(top);
+  float l = 0.0f, exact = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const float w = v[i].y != 0.0f ? __builtin_amdgcn_exp2f(v[i].x - top) : 0.0f;
+    weight[64 * i + lane] = w;   // the same value from each wave
+    l += w * v[i].y;
+    exact += w * v[i].z;
+  }
+  l = wave_tree_sum(l);
+  exact = wave_tree_sum(exact);
+  seen = wave_max(seen);
+  __syncthreads();
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  constexpr int BATCH = 4;   // loads in flight
+  for (int s0 = g; s0 < parts; s0 += BATCH * G) {
+    float4 y[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (s0 + i * G < parts) y[i] = *reinterpret_cast<const float4*>(p.part + at(s0 + i * G) * D + 4 * x);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float w = s0 + i * G < parts ? weight[s0 + i * G] : 0.0f;
+      if (w == 0.0f) continue;   // y was not written where the piece had no keys
+      o.x += w * y[i].x;
+      o.y += w * y[i].y;
+      o.z += w * y[i].z;
+      o.w += w * y[i].w;
+    }
+  }
+  sums[g][x] = o;
+  __syncthreads();
+  if (g != 0) return;
+#pragma unroll
+  for (int i = 1; i < G; ++i) {
+    const float4 y = sums[i][x];
+    o.x += y.x;
+    o.y += y.y;
+    o.z += y.z;
+    o.w += y.w;
+  }
+  const float inv = l == 0.0f ? (seen != 0.0f ? NAN : 0.0f) : 1.0f / l;
+  *reinterpret_cast<uint2*>(p.out + row * D + 4 * x) =
+      make_uint2(Mfma<T>::pack(o.x * inv, o.y * inv), Mfma<T>::pack(o.z * inv, o.w * inv));
+  if (p.lse && x == 0) p.lse[row] = l == 0.0f ? -INFINITY : kLn2 * (top + __builtin_amdgcn_logf(exact));
+}
+
+// The prefix, then the own cache. (Both sides of a choice are values: chosen between by
+// address, the two would have to lie in memory.)
+__device__ __forceinline__ int64_t either(bool first, int64_t a, int64_t b) { return first ? a : b; }
+struct TwoCaches {
+  OneCache a, b;
+  int tiles;   // of a
+  __device__ __forceinline__ int64_t stride(int t, int is_v) const {
+    return is_v ? either(t < tiles, a.vt, b.vt) : either(t < tiles, a.kt, b.kt);
+  }
+  __device__ __forceinline__ const uint16_t* at(int t, int is_v) const {
+    const int64_t base = is_v ? either(t < tiles, (int64_t)a.v, (int64_t)b.v) : either(t < tiles, (int64_t)a.k, (int64_t)b.k);
+    return reinterpret_cast<const uint16_t*>(base) + (int64_t)first(t) * stride(t, is_v);
+  }
+  __device__ __forceinline__ int left(int t) const { return (int)either(t < tiles, a.kn, b.kn) - first(t); }
+  __device__ __forceinline__ bool whole(int t) const { return first(t) + kKeys <= (int)either(t < tiles, a.sure, b.sure); }
+  __device__ __forceinline__ int first(int t) const { return (t < tiles ? t : t - tiles) * kKeys; }
+  __device__ __forceinline__ int limit(int t) const { return (int)either(t < tiles, a.seen, b.seen); }
+  __device__ __forceinline__ bool turns(int t) const { return t == tiles; }
+};
+
+template <typename T, int D, bool LSE>
+__global__ __launch_bounds__(256, 2) void prefix_walk(PrefixArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[kTileBytes<D>];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, col = lane & 31;
+  // Each XCD takes a contiguous run of the heads' tiles, so that its L2 serves a head's
+  // prefix to them all.
+  const uint32_t total = gridDim.x, pid = blockIdx.x, per = total >> 3, rest = total & 7, xcd = pid & 7;
+  const uint32_t id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3);
+  const uint32_t tiles = (uint32_t)(p.n * p.seq_tiles);
+  const int hd = (int)(id / tiles), at = (int)(id - hd * tiles);
+  const int seq = (int)((uint32_t)at / (uint32_t)p.seq_tiles);
+  const OwnRows w(p, seq, at - seq * p.seq_tiles);
+  const int r = w.r0 + wave * 32 + col;
+  const Row row(p, r, w.rows, hd, w.kn);
+  const TwoCaches keys = {prefix_cache(p, hd), own_cache(p, seq, hd, w, row.seen), key_tiles(p.prefix)};
+  const uint16_t* const q = p.q + seq * p.qb + row.tok * p.qt + row.head * p.qh;
+  v16f o[D / 32];
+  float m, l, exact, off;
+  const bool idle = w.r0 + wave * 32 >= w.rows;
+  const int t1 = keys.tiles + w.tiles;
+  attend<T, D, false, LSE>(smem, keys, q, p.c, 0, t1, idle, m, l, exact, off, o);
+  l = add_partner(l);
+  if (LSE) exact = add_partner(exact);
+  if (r >= w.rows) return;
+  const int64_t to = ((int64_t)seq * p.q_rows + row.tok) * p.heads + row.head;
+  if (LSE && half == 0) p.lse[to] = l == 0.0f ? -INFINITY : kLn2 * (off + __builtin_amdgcn_logf(exact));
+  const float inv = l == 0.0f ? (p.prefix + row.seen > 0 ? NAN : 0.0f) : 1.0f / l;
+  uint16_t* const po = p.out + to * D;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<uint2*>(po + 32 * d + 8 * g + 4 * half) =
+          make_uint2(Mfma<T>::pack(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
+                     Mfma<T>::pack(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+}
+
+// How a call is laid over the GPU.
+struct Plan {
+  bool walk;
+  int64_t seq_tiles, all_tiles;
+  int places, shares, own, piece;
+  int64_t parts;   // rows of partial results
+};
+
+Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, int kv_heads) {
+  const int group = heads / kv_heads;
+  const int64_t cus = compute_units(), rows = n * q_rows * heads;   // of the output
+  Plan pl = {};
+  pl.seq_tiles = (q_rows * group + kRows - 1) / kRows;
+  pl.all_tiles = (n * q_rows * group + kRows - 1) / kRows;
+  const double tiles_p = (double)((prefix + kKeys - 1) / kKeys), tiles_k = (double)((k_rows + kKeys - 1) / kKeys);
+  // Two workgroups per CU, for the stream of keys.
+  int64_t places = 2 * cus / kv_heads;
+  const int64_t least = 2 * (pl.all_tiles + pl.seq_tiles * n);
+  if (places < least) places = least;
+  // The most pieces of the prefix, and the least tiles of one, by the cost of joining: 1 us per
+  // tile of keys against 0.15 ns per row and piece, as in attention.hip.
+  const double s = fmin(fmin(sqrt(tiles_p / (0.00015 * (double)rows)), (double)(places / pl.all_tiles)), kMaxPieces);
+  pl.shares = s > 1.0 ? (int)s : 1;
+  const double each = fmax(1.0, fmin(sqrt(tiles_k / (0.0003 * (double)rows)), tiles_k));
+  pl.piece = (int)ceil(tiles_k / each);
+  if (pl.piece < 1) pl.piece = 1;
+  pl.places = n > kListed ? 0 : (int)places;
+  pl.own = (int)(n > kListed ? n : places / pl.seq_tiles);
+  pl.parts = (pl.shares * n + pl.own) * q_rows * heads;
+  const double walk = fmax(1.0, (double)(n * pl.seq_tiles * kv_heads) / (double)cus) * (tiles_p + tiles_k);
+  const double pieces = ((double)pl.all_tiles * tiles_p + (double)(n * pl.seq_tiles) * tiles_k) * kv_heads / (double)cus +
+                        2.8 + (double)rows * (0.0006 + 0.00015 * pl.shares);
+  pl.walk = walk <= pieces || rows > kMaxBlocks;
+  return pl;
+}
+
+template <typename T, int D>
+int launch(const PrefixArgs& p, const Plan& pl, hipStream_t s) {
+  if (pl.walk) {
+    const int64_t grid = p.n * pl.seq_tiles * p.kv_heads;
+    LR_REQUIRE(grid <= kMaxBlocks, "attention_prefix: %lld workgroups are not supported", (long long)grid);
+    if (p.lse) prefix_walk<T, D, true><<<(unsigned)grid, 256, 0, s>>>(p);
+    else prefix_walk<T, D, false><<<(unsigned)grid, 256, 0, s>>>(p);
+    return check_launch("attention_prefix");
+  }
+  const int64_t grid = (p.places ? p.places : pl.shares * pl.all_tiles + p.n * pl.seq_tiles) * p.kv_heads;
+  LR_REQUIRE(grid <= kMaxBlocks, "attention_prefix: %lld workgroups are not supported", (long long)grid);
+  prefix_pieces<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
+  if (int rc = check_launch("attention_prefix")) return rc;
+  prefix_join<T, D><<<(unsigned)((int64_t)p.n * p.q_rows * p.heads), 256, 0, s>>>(p);
+  return check_launch("attention_prefix");
+}
+
+template <typename T>
+int by_dim(const PrefixArgs& p, int dim, const Plan& pl, hipStream_t s) {
+  if (dim == 32) return launch<T, 32>(p, pl, s);
+  if (dim == 64) return launch<T, 64>(p, pl, s);
+  return launch<T, 128>(p, pl, s);
+}
+
+int check_shape(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, int kv_heads, int head_dim) {
+  LR_REQUIRE(n >= 0 && q_rows >= 0 && k_rows >= 0 && prefix >= 0, "attention_prefix: negative shape");
+  LR_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
+             "attention_prefix: %d heads do not share %d key heads evenly", heads, kv_heads);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(LR_EUNSUPPORTED, "attention_prefix: head_dim %d is not supported (32, 64 or 128)", head_dim);
+  LR_REQUIRE(n < (1LL << 24) && q_rows < (1LL << 30) && k_rows < (1LL << 30) && prefix < (1LL << 30) && heads <= 65536,
+             "attention_prefix: shapes past 2^24 sequences, 2^30 rows or 65536 heads are not supported");
+  LR_REQUIRE(q_rows == 0 || n < (1LL << 30) / q_rows / heads, "attention_prefix: %lld x %lld tokens of %d heads are not supported",
+             (long long)n, (long long)q_rows, heads);
+  return LR_OK;
+}
+
+}  // namespace
+}  // namespace lr
+
+using namespace lr;
+
+extern "C" int lr_attention_prefix_workspace(int64_t sequences, int64_t q_rows, int64_t k_rows, int64_t prefix_rows,
+                                             int heads, int kv_heads, int head_dim, int64_t* bytes) {
+  if (int rc = check_shape(sequences, q_rows, k_rows, prefix_rows, heads, kv_heads, head_dim)) return rc;
+  LR_REQUIRE(bytes, "attention_prefix: null pointer");
+  *bytes = 0;
+  if (sequences == 0 || q_rows == 0) return LR_OK;
+  const Plan pl = plan(sequences, q_rows, k_rows, prefix_rows, heads, kv_heads);
+  if (!pl.walk) *bytes = pl.parts * (head_dim + 4) * 4;
+  return LR_OK;
+}
+
+extern "C" int lr_attention_prefix(const void* q, const void* prefix_k, const void* prefix_v, const void* k, const void* v,
+                                   void* out, float* lse, int dtype, int64_t sequences, int64_t q_rows, int64_t k_rows,
+                                   int64_t prefix_rows, int heads, int kv_heads, int head_dim, const int64_t* strides,
+                                   const int32_t* key_lengths, int causal, int scale_bits, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+  LR_REQUIRE(dtype == LR_DTYPE_BF16 || dtype == LR_DTYPE_F16, "attention_prefix: unknown dtype %d", dtype);
+  if (int rc = check_shape(sequences, q_rows, k_rows, prefix_rows, heads, kv_heads, head_dim)) return rc;
+  if (sequences == 0 || q_rows == 0) return LR_OK;
+  LR_REQUIRE(q && out && strides && (k_rows == 0 || (k && v)) && (prefix_rows == 0 || (prefix_k && prefix_v)),
+             "attention_prefix: null pointer");
+  LR_REQUIRE(aligned(q, 16) && aligned(prefix_k, 16) && aligned(prefix_v, 16) && aligned(k, 16) && aligned(v, 16) &&
+                 aligned(out, 16) && aligned(lse, 4),
+             "attention_prefix: pointers must be 16-byte aligned");
+  for (int i = 0; i < 13; ++i)
+    LR_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0,
+               "attention_prefix: stride %d is %lld, not a multiple of 8 from 0 on", i, (long long)strides[i]);
+  // A tile's keys are addressed by 32-bit byte offsets from its first one.
+  for (int i : {3, 5, 7, 10})
+    LR_REQUIRE(strides[i] < (1LL << 23),
+               "attention_prefix: strides of 2^23 and more between keys or values are not supported");
+  PrefixArgs p = {};
+  p.q = static_cast<const uint16_t*>(q);
+  p.pk = static_cast<const uint16_t*>(prefix_k);
+  p.pv = static_cast<const uint16_t*>(prefix_v);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.out = static_cast<uint16_t*>(out);
+  p.lse = lse;
+  p.part = static_cast<float*>(workspace);
+  p.qt = strides[0]; p.qh = strides[1]; p.qb = strides[2];
+  p.pkt = strides[3]; p.pkh = strides[4]; p.pvt = strides[5]; p.pvh = strides[6];
+  p.kt = strides[7]; p.kh = strides[8]; p.kb = strides[9];
+  p.vt = strides[10]; p.vh = strides[11]; p.vb = strides[12];
+  p.lengths = key_lengths;
+  p.n = (int)sequences;
+  p.q_rows = (int)q_rows;
+  p.k_rows = (int)k_rows;
+  p.prefix = (int)prefix_rows;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.group = heads / kv_heads;
+  p.causal = causal != 0;
+  float scale;
+  static_assert(sizeof scale == sizeof scale_bits, "fp32");
+  __builtin_memcpy(&scale, &scale_bits, sizeof scale);
+  p.c = scale * 1.4426950408889634f;
+  LR_REQUIRE(p.c > 0.0f && isfinite(p.c), "attention_prefix: the scale must be positive and finite");
+  const Plan pl = plan(sequences, q_rows, k_rows, prefix_rows, heads, kv_heads);
+  p.seq_tiles = (int)pl.seq_tiles;
+  p.all_tiles = (int)pl.all_tiles;
+  p.places = pl.places;
+  p.shares = pl.shares;
+  p.own = pl.own;
+  p.piece = pl.piece;
+  if (!pl.walk)
+    LR_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= pl.parts * (head_dim + 4) * 4,
+               "attention_prefix: needs a workspace of %lld bytes", (long long)(pl.parts * (head_dim + 4) * 4));
+  hipStream_t s = as_stream(stream);
+  return dtype == LR_DTYPE_BF16 ? by_dim<__bf16>(p, head_dim, pl, s) : by_dim<_Float16>(p, head_dim, pl, s);
+}

@@ -1,0 +1,213 @@
+"""GPU parity of attention over a shared prefix with the formula in 64 bits: the prefix
+and a sequence's own keys behind each other. Tolerances of the outputs as in
+test_gpu_attention, one key more for each join.
+
+The logarithm of the sum: the scores move it by at most ds = (D + 2) * 2^-23 * scale *
+sum |q k| (the largest of a row), scale * log2(e) is rounded to fp32 (2^-24 relative to
+the score), as are the exponent's subtrahend and the two steps back from the binary
+logarithm (2^-23 of their size together); the weights and their sum have 2^-21 and
+2^-24 per key relative, which is as much in the logarithm.
+"""
+import math
+
+import pytest
+import torch
+
+from lynnreal_omni_amd import attention as A
+from test_gpu_attention import check, formula, mask
+
+pytestmark = pytest.mark.gpu
+
+
+def make(batch, new, prefix, size, heads, kv_heads, dim, dtype, seed, scale=1.5):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(batch, new, heads, dim, generator=g) * scale
+    pk, pv = (torch.randn(prefix, kv_heads, dim, generator=g) for _ in range(2))
+    k, v = (torch.randn(batch, size, kv_heads, dim, generator=g) for _ in range(2))
+    return tuple(t.to(dtype).cuda() for t in (q, pk, pv, k, v))
+
+
+def check_lse(got, q, k, scale, seen):
+    group = q.shape[1] // k.shape[1]
+    q, k = (t.double().cpu().transpose(0, 1) for t in (q, k))
+    k = k.repeat_interleave(group, 0)
+    s = (q @ k.transpose(1, 2) * scale).masked_fill(~seen, -math.inf)
+    want = torch.logsumexp(s, -1).transpose(0, 1) if k.shape[1] else torch.full(got.shape, -math.inf)
+    size = torch.where(seen, q.abs() @ k.abs().transpose(1, 2) * scale, 0.0)
+    size = size.amax(-1).transpose(0, 1) if k.shape[1] else torch.zeros(got.shape)
+    bound = (q.shape[-1] + 2) * 2.0 ** -23 * size + 2.0 ** -22 * (size + 16) + 2.0 ** -24 * k.shape[1]
+    got = got.double().cpu()
+    assert torch.equal(got == -math.inf, want == -math.inf)
+    off = torch.where(want == -math.inf, 0.0, (got - want).abs() - bound)
+    assert not off.isnan().any() and off.max() <= 0
+
+
+def check_all(args, lengths, causal, scale=None):
+    q, pk, pv, k, v = args
+    new, dim = q.shape[1], q.shape[-1]
+    scale = dim ** -0.5 if scale is None else scale
+    given = None if lengths is None else torch.tensor(lengths, device="cuda", dtype=torch.int32)
+    got, lse = A.attention_shared_prefix(*args, causal=causal, scale=scale, key_lengths=given, return_lse=True)
+    assert got.shape == q.shape and lse.shape == q.shape[:3] and got.is_contiguous()
+    for i in range(q.shape[0]):
+        n = k.shape[1] if lengths is None else lengths[i]
+        keys, values = (torch.cat([a, b[i, :n]]) for a, b in ((pk, k), (pv, v)))
+        seen = torch.cat([torch.ones(new, pk.shape[0], dtype=torch.bool), mask(new, n, causal)], 1)
+        check(got[i], *formula(q[i], keys, values, scale, seen))
+        check_lse(lse[i], q[i], keys, scale, seen)
+    alone = A.attention_shared_prefix(*args, causal=causal, scale=scale, key_lengths=given)
+    assert torch.equal(alone, got)
+    return got, lse
+
+
+CASES = [
+    # batch, new, prefix, size, heads, kv_heads, dim, lengths
+    (1, 1, 1, 1, 1, 1, 32, None), (1, 1, 0, 5, 2, 1, 64, None), (2, 1, 64, 0, 4, 2, 128, None),
+    (3, 1, 0, 0, 2, 2, 64, None), (4, 1, 878, 128, 40, 8, 128, [17, 0, 96, 128]), (3, 2, 65, 9, 6, 2, 64, [9, 0, 1]),
+    (32, 1, 1000, 40, 8, 8, 32, [i for i in range(32)]), (70, 1, 130, 70, 4, 2, 64, [i % 71 for i in range(70)]),
+    (2, 4, 4097, 300, 16, 2, 128, [300, 4]), (5, 1, 20000, 1000, 5, 1, 128, [1000, 1, 0, 64, 65]),
+    (2, 33, 129, 100, 2, 2, 64, [33, 100]), (2, 130, 300, 257, 3, 1, 32, [257, 140]), (3, 200, 63, 200, 4, 4, 128, None),
+    (1, 300, 64, 700, 2, 1, 64, None), (8, 40, 500, 64, 14, 2, 128, [40 + i for i in range(8)]),
+    (2, 513, 1025, 513, 2, 2, 128, None), (1, 5, 70000, 10, 4, 4, 64, None),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("batch,new,prefix,size,heads,kv_heads,dim,lengths", CASES)
+def test_cases(batch, new, prefix, size, heads, kv_heads, dim, lengths, causal, dtype):
+    check_all(make(batch, new, prefix, size, heads, kv_heads, dim, dtype, batch + prefix), lengths, causal)
+
+
+@pytest.mark.parametrize("batch", [512, 513, 700])
+def test_many_sequences(batch):
+    """On both sides of the most sequences that a list of pieces holds."""
+    lengths = [(i * 37) % 90 for i in range(batch)]
+    lengths[3] = 400
+    check_all(make(batch, 1, 300, 400, 4, 2, 32, torch.bfloat16, batch), lengths, True)
+
+
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 20.0])
+def test_scales(scale, new):
+    check_all(make(2, new, 200, 150, 4, 2, 64, torch.bfloat16, 3), [150, 150], True, scale)
+
+
+@pytest.mark.parametrize("new", [1, 3, 140])
+def test_nothing_shared_is_plain_attention(new):
+    args = make(3, new, 0, 300, 6, 2, 64, torch.bfloat16, new)
+    lengths = torch.tensor([300, 7, 150], device="cuda")
+    got = A.attention_shared_prefix(*args, causal=True, key_lengths=lengths)
+    plain = A.attention(args[0], *args[3:], causal=True, key_lengths=lengths)
+    # Two roundings of the same sums apart.
+    assert (got.float() - plain.float()).abs().max() <= 2 * 2.0 ** -7 * plain.float().abs().max()
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_unused_places_are_not_read(new):
+    """NaN and infinities behind a cache's keys and in keys that causality hides."""
+    lengths = [new, new + 70, new + 1]
+    q, pk, pv, k, v = make(3, new, 100, new + 200, 4, 2, 64, torch.float16, 9)
+    want = A.attention_shared_prefix(q, pk, pv, k, v, causal=True, key_lengths=torch.tensor(lengths, device="cuda"))
+    for i, n in enumerate(lengths):
+        k[i, n:], v[i, n:] = float("nan"), float("inf")
+    got, lse = A.attention_shared_prefix(q, pk, pv, k, v, causal=True, key_lengths=torch.tensor(lengths, device="cuda"),
+                                         return_lse=True)
+    assert torch.equal(got, want) and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_scores_of_minus_infinity(new):
+    """A row that sees only such scores is NaN (0 / 0), one that also sees others leaves them out;
+    the logarithm of the sum is -inf and finite."""
+    q, pk, pv, k, v = make(2, new, 70, 40, 2, 2, 64, torch.bfloat16, 5)
+    q[..., 0] = 1.0
+    pk[..., 0] = -math.inf
+    got, lse = A.attention_shared_prefix(q, pk, pv, k, v, return_lse=True)
+    assert torch.isfinite(got).all() and torch.isfinite(lse).all()
+    for i in range(2):
+        check(got[i], *formula(q[i], k[i], v[i], 64 ** -0.5, mask(new, 40, False)))
+        check_lse(lse[i], q[i], k[i], 64 ** -0.5, mask(new, 40, False))
+    k[..., 0] = -math.inf
+    got, lse = A.attention_shared_prefix(q, pk, pv, k, v, return_lse=True)
+    assert got.isnan().all() and (lse == -math.inf).all()
+    empty = torch.zeros(2, device="cuda", dtype=torch.int32)
+    got, lse = A.attention_shared_prefix(q, pk[:0], pv[:0], k, v, key_lengths=empty, return_lse=True)
+    assert (got == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("new", [1, 140])
+def test_layouts(new):
+    """Slices of a fused projection, heads outside, an expanded batch, a prefix inside a
+    larger buffer whose rows are further apart than the caches': read as they are. Odd ones
+    are copied."""
+    dim, lengths = 64, torch.tensor([new, new + 9, 150], device="cuda")
+    g = torch.Generator().manual_seed(new)
+    fused = torch.randn(3, new, 8 * dim, generator=g).bfloat16().cuda()
+    q = fused[..., :4 * dim].unflatten(-1, (4, dim))
+    k = torch.randn(3, 2, 200, dim, generator=g).bfloat16().cuda().transpose(1, 2)
+    v = torch.randn(1, 200, 2, dim, generator=g).bfloat16().cuda().expand(3, -1, -1, -1)
+    pk = torch.randn(300, 5, dim, generator=g).bfloat16().cuda()[10:190, 1:3]
+    pv = torch.randn(2, 180, dim, generator=g).bfloat16().cuda().transpose(0, 1)
+    views = (q, pk, pv, k, v)
+    kwargs = dict(causal=True, key_lengths=lengths, return_lse=True)
+    got = A.attention_shared_prefix(*views, **kwargs)
+    want = A.attention_shared_prefix(*(t.contiguous() for t in views), **kwargs)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    odd = [torch.zeros(*t.shape[:-1], dim + 1, dtype=t.dtype, device="cuda")[..., 1:].copy_(t) for t in views]
+    got = A.attention_shared_prefix(*odd, **kwargs)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_lengths_are_clamped():
+    args = make(3, 2, 50, 80, 4, 2, 64, torch.bfloat16, 2)
+    for dtype in (torch.int64, torch.int32):
+        far = torch.tensor([-5, 2 ** 31 - 1, 80], device="cuda").to(dtype)
+        got = A.attention_shared_prefix(*args, key_lengths=far)
+        want = A.attention_shared_prefix(*args, key_lengths=torch.tensor([0, 80, 80], device="cuda"))
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("new", [1, 150])
+def test_graph_whose_lengths_change(new):
+    q, pk, pv, k, v = make(4, new, 3000, 400, 8, 2, 64, torch.bfloat16, 7)
+    lengths = torch.full((4,), 400, device="cuda", dtype=torch.int32)
+    call = lambda: A.attention_shared_prefix(q, pk, pv, k, v, causal=True, key_lengths=lengths, return_lse=True)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for step in range(4):
+        lengths.copy_(torch.tensor([new, 400 - step, new + 7 * step, 399], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, call()))
+
+
+def test_other_stream():
+    args = make(4, 1, 3000, 400, 8, 2, 64, torch.bfloat16, 8)
+    want = A.attention_shared_prefix(*args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = A.attention_shared_prefix(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_prefix_past_2_31_elements():
+    """A prefix of which the last keys lie past 2^31 elements from the first."""
+    rows = 2 ** 31 // (4096 * 64) + 40
+    big = torch.zeros(rows * 64, 4096, dtype=torch.bfloat16, device="cuda")
+    pk = big.view(rows * 64, 32, 128)[:, :2]
+    assert (pk.shape[0] - 1) * pk.stride(0) > 2 ** 31
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(2, 1, 2, 128, generator=g).bfloat16().cuda()
+    k = torch.randn(2, 3, 2, 128, generator=g).bfloat16().cuda()
+    pk[-1] = q[0, 0] * 4
+    pv = big.view(rows * 64, 32, 128)[:, 2:4]
+    pv[-1] = 1.0
+    got = A.attention_shared_prefix(q, pk, pv, k, k)
+    keys, values = (torch.cat([t, k[0]]) for t in (pk, pv))
+    check(got[0], *formula(q[0], keys, values, 128 ** -0.5, mask(1, keys.shape[0], False)))

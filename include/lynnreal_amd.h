@@ -411,6 +411,38 @@ int lr_attention_prefix(const void* q, const void* prefix_k, const void* prefix_
                         const int32_t* key_lengths, int causal, int scale_bits, void* workspace,
                         int64_t workspace_bytes, void* stream);
 
+/* The attention weight that each key gets, added to what it had:
+ *   out[i, h, j] = weights[i, h, j] + sum of exp(scale * q . k_j - lse)
+ * over the tokens and the query heads of key head h that see key j of sequence i, in fp32
+ * and in a fixed order; places behind a sequence's keys keep their weight. lse fp32
+ * [sequences, q_rows, heads] (lr_attention_prefix); weights and out fp32 [sequences,
+ * kv_heads, k_rows], which may be one. q, k, key_lengths, causal, scale_bits as in
+ * lr_attention, for dense batches; strides, six: of q (token, head, sequence), then k.
+ * workspace of the bytes that lr_attention_weights_workspace gives (0: it may be NULL). */
+int lr_attention_weights_workspace(int64_t sequences, int64_t q_rows, int64_t k_rows, int heads, int kv_heads,
+                                   int head_dim, int64_t* bytes);
+int lr_attention_weights(const void* q, const void* k, const float* lse, const float* weights, float* out, int dtype,
+                         int64_t sequences, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int head_dim,
+                         const int64_t* strides, const int32_t* key_lengths, int causal, int scale_bits,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Caches cut down to `budget` keys per head. Of sequence i's key_lengths[i] keys (size
+ * where NULL; values are clamped to it) head h keeps the last `recent` and, of those before them,
+ * the ones of most weight; of equal weights the first; NaN counts least; all where there are
+ * no more than the budget. They keep their order:
+ *   kept int32 [sequences, kv_heads, budget]: their places, -1 behind the last
+ *   lengths_out int32 [sequences]: how many
+ *   weights_out fp32 [sequences, kv_heads, capacity]: theirs, 0 behind
+ *   k_out, v_out: their rows; those behind become 0 up to the budget where `clear`, and
+ *   stay as they were where not.
+ * weights fp32 [sequences, kv_heads, size]. strides, twelve, in bytes, multiples of 16: from
+ * one key, head and sequence of k to the next, then of v, k_out and v_out; a row has
+ * row_bytes, a multiple of 16. The outputs must not overlap the inputs. */
+int lr_cache_evict(const void* k, const void* v, const float* weights, const int32_t* key_lengths, void* k_out,
+                   void* v_out, float* weights_out, int32_t* lengths_out, int32_t* kept, int64_t sequences, int64_t size,
+                   int kv_heads, int64_t row_bytes, int64_t budget, int64_t recent, int64_t capacity,
+                   const int64_t* strides, int clear, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -81,7 +81,7 @@ def _scale_bits(scale):
     return struct.unpack("i", struct.pack("f", scale))[0]
 
 
-def _check(query, key, value, dims):
+def _check_tensors(query, key, value, dims):
     names = "[batch, tokens, heads, head_dim]" if dims == 4 else "[tokens, heads, head_dim]"
     if query.dim() != dims or key.dim() != dims or value.shape != key.shape:
         raise ValueError(f"query, key and value must be {names}, key and value of one shape")
@@ -96,6 +96,10 @@ def _check(query, key, value, dims):
         raise RuntimeError(f"head_dim {dim} is not supported by the HIP attention (32, 64 or 128)")
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         raise RuntimeError("gradients are not supported by the HIP attention: call it under torch.no_grad()")
+
+
+def _check(query, key, value, dims):
+    _check_tensors(query, key, value, dims)
     _lib.check_device(query)
 
 
@@ -220,7 +224,7 @@ def attention_shared_prefix(query, prefix_key, prefix_value, key, value, *, caus
     fp32 [batch, tokens, heads] the logarithm of the sum of exp(scale * q k) over the
     keys that a token sees, -inf where it sees none or all score -inf.
     """
-    _check(query, key, value, 4)
+    _check_tensors(query, key, value, 4)
     if prefix_key.dim() != 3 or prefix_value.shape != prefix_key.shape or prefix_key.shape[1:] != key.shape[2:]:
         raise ValueError("prefix_key and prefix_value must be [prefix, kv_heads, head_dim], with key's heads")
     if prefix_key.dtype != query.dtype or prefix_value.dtype != query.dtype:
@@ -233,6 +237,7 @@ def attention_shared_prefix(query, prefix_key, prefix_value, key, value, *, caus
     keys, kv_heads = key.shape[1:3]
     if key_lengths is not None:
         key_lengths = _lengths(key_lengths, batch, keys)
+    _lib.check_device(query)
     _lib.same_device(query, prefix_key=prefix_key, prefix_value=prefix_value, key=key, value=value,
                      key_lengths=key_lengths)
     scale = _scale_bits(float(dim ** -0.5 if scale is None else scale))

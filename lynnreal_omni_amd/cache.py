@@ -1,0 +1,215 @@
+"""Padded key/value caches of bounded size, on gfx950: which keys the attention needs,
+and caches cut down to those.
+
+  accumulate_weights  adds to each key's weight what new tokens' softmax gives it
+  evict               the latest keys and those of most weight, moved to a smaller cache
+
+A step of a request whose cache has a budget:
+
+  out, lse = attention_shared_prefix(q, prefix_k, prefix_v, k, v, causal=True,
+                                     key_lengths=lengths, return_lse=True)
+  weights = accumulate_weights(weights, q, k, lse, causal=True, key_lengths=lengths, out=weights)
+  ..      # and when the caches have outgrown the budget
+  k, v, weights, lengths, kept = evict(k, v, weights, lengths, budget, recent=64)
+
+(without a shared prefix: attention_shared_prefix with an empty one). Keys are
+[batch, keys, kv_heads, head_dim], bf16 or fp16, read as attention reads them;
+each head keeps its own keys, so that after an eviction a place holds other keys in
+other heads, with the same number of them in all. Weights are fp32 [batch, kv_heads,
+keys]. Lengths are never copied to the host. Inference only: inputs that require a
+gradient are refused.
+"""
+from __future__ import annotations
+
+import functools
+from array import array
+
+import torch
+
+from . import _lib
+from . import attention as _attention
+
+
+def _check_weights(weights, key, name="weights"):
+    batch, keys, kv_heads = key.shape[:3]
+    if weights.shape != (batch, kv_heads, keys) or weights.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32 [batch, kv_heads, keys] = {(batch, kv_heads, keys)}, "
+                         f"got {weights.dtype} {tuple(weights.shape)}")
+
+
+def _no_gradients(*tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("gradients are not supported by the HIP caches: call it under torch.no_grad()")
+
+
+@functools.lru_cache(maxsize=4096)
+def _weights_workspace(device, batch, tokens, keys, heads, kv_heads, dim):
+    nbytes = array("q", [0])
+    with torch.cuda.device(device):
+        _lib.call("lr_attention_weights_workspace", batch, tokens, keys, heads, kv_heads, dim, nbytes.buffer_info()[0])
+    return nbytes[0]
+
+
+@functools.lru_cache(maxsize=4096)
+def _six_strides(query, key):
+    """Token, head and sequence strides of two batches given as (stride, shape)."""
+    six = array("q")
+    for stride, shape in (query, key):
+        s = [st if n > 1 else 0 for st, n in zip(stride, shape)]
+        six.extend((s[1], s[2], s[0]))
+    return six
+
+
+def accumulate_weights(weights, query, key, lse, *, causal=False, scale=None, key_lengths=None, out=None):
+    """weights plus the attention weight that each key gets from query's tokens: exp(scale *
+    q . k - lse), summed over the tokens and query heads that see the key, for query
+    [batch, tokens, heads, head_dim], key [batch, keys, kv_heads, head_dim] and lse
+    float32 [batch, tokens, heads], the logarithm of each softmax's sum.
+
+    weights: float32 [batch, kv_heads, keys]; returned as a new tensor, or in `out`,
+    which may be weights itself. causal, scale and key_lengths as in attention: what a
+    token does not see gets nothing from it, and places behind key_lengths keep their
+    weight. Sums are fp32 in a fixed order.
+    """
+    _attention._check_tensors(query, key, key, 4)
+    if key.shape[0] != query.shape[0]:
+        raise ValueError(f"query has a batch of {query.shape[0]}, key of {key.shape[0]}")
+    _check_weights(weights, key)
+    if lse.shape != query.shape[:3] or lse.dtype != torch.float32:
+        raise ValueError(f"lse must be float32 [batch, tokens, heads] = {tuple(query.shape[:3])}")
+    _no_gradients(weights, lse)
+    batch, tokens, heads, dim = query.shape
+    keys, kv_heads = key.shape[1:3]
+    if key_lengths is not None:
+        key_lengths = _attention._lengths(key_lengths, batch, keys)
+    if out is not None:
+        _check_weights(out, key, "out")
+        _no_gradients(out)
+        same = out.data_ptr() == weights.data_ptr() and weights.is_contiguous()
+        if not out.is_contiguous() or _overlap(out, lse) or (not same and _overlap(out, weights)):
+            raise ValueError("out must be contiguous, and weights themselves or memory of its own")
+    scale = _attention._scale_bits(float(dim ** -0.5 if scale is None else scale))
+    _lib.check_device(query)
+    _lib.same_device(query, key=key, weights=weights, lse=lse, key_lengths=key_lengths, out=out)
+    if out is None:
+        out = torch.empty_like(weights, memory_format=torch.contiguous_format)
+    weights, lse = weights.contiguous(), lse.contiguous()
+    if query.data_ptr() & 15 or not _attention._dense(query.stride(), query.shape) or not _near(query):
+        query = _attention._rows(query.contiguous())
+    if key.data_ptr() & 15 or not _attention._dense(key.stride(), key.shape):
+        key = _attention._rows(key)
+    nbytes = _weights_workspace(query.get_device(), batch, tokens, keys, heads, kv_heads, dim)
+    ws = _lib.workspace(query, nbytes)   # held until the launch
+    strides = _six_strides((query.stride(), query.shape), (key.stride(), key.shape))
+    _lib.launch(query, "lr_attention_weights", query.data_ptr(), key.data_ptr(), lse.data_ptr(), weights.data_ptr(),
+                out.data_ptr(), _attention._DTYPES[query.dtype], batch, tokens, keys, heads, kv_heads, dim,
+                strides.buffer_info()[0], _lib.ptr(key_lengths), int(bool(causal)), scale, _lib.ptr(ws), nbytes)
+    return out
+
+
+def _near(query):
+    """Whether the kernel's 32-bit offsets reach the heads of a key head and 64 tokens."""
+    return query.stride(1) < 1 << 23 and (query.shape[2] == 1 or query.stride(2) * query.shape[2] < 1 << 30)
+
+
+def _span(t):
+    """First and last byte (exclusive) of what a tensor's elements lie in."""
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _overlap(a, b):
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _distinct(t):
+    """Whether no two elements of t are the same memory, for strides that nest (as those
+    of slices and transposes do)."""
+    at = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < at:
+            return False
+        at = st * (n - 1) + at
+    return True
+
+
+def _byte_strides(t):
+    s = [st * t.element_size() if n > 1 else 0 for st, n in zip(t.stride(), t.shape)]
+    return s[1], s[2], s[0]
+
+
+def evict(key, value, weights, key_lengths, budget, *, recent=0, out=None):
+    """Caches cut down to `budget` keys per head: of each cache's first key_lengths[i] keys
+    (all where None) the last `recent` and, of those before them, the ones of most weight; of
+    equal weights the first ones, NaN counting least; all of them where there are no more than
+    the budget. They keep their order.
+
+    key, value [batch, keys, kv_heads, head_dim], weights float32 [batch, kv_heads, keys],
+    budget >= 1, 0 <= recent <= budget. Returns (key, value, weights, lengths, kept):
+    new caches [batch, budget, kv_heads, head_dim], zeros behind their last keys; their
+    weights [batch, kv_heads, budget], 0 behind; lengths int32 [batch]; and kept int32
+    [batch, kv_heads, budget], the places that the keys had, -1 behind the last.
+
+    out = (key, value, weights): caches of any number of places from `budget` on, on
+    whose memory the inputs do not lie, written instead of new ones; rows of theirs
+    behind the last key stay as they were, weights there become 0.
+    """
+    if key.dim() != 4 or value.shape != key.shape or value.dtype != key.dtype:
+        raise ValueError("key and value must be [batch, keys, kv_heads, head_dim], of one shape and dtype")
+    if key.dtype not in _attention._DTYPES:
+        raise RuntimeError(f"dtype {key.dtype} is not supported by the HIP caches (bfloat16 or float16)")
+    batch, keys, kv_heads, dim = key.shape
+    if kv_heads == 0 or dim == 0:
+        raise ValueError("key and value have no heads or no columns")
+    if dim % 8:
+        raise RuntimeError(f"head_dim {dim} is not supported by the HIP caches (a multiple of 8)")
+    _check_weights(weights, key)
+    budget, recent = int(budget), int(recent)
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"budget must be at least 1 and recent from 0 to budget, got {budget} and {recent}")
+    _no_gradients(key, value, weights)
+    if key_lengths is not None:
+        key_lengths = _attention._lengths(key_lengths, batch, keys)
+    if out is not None:
+        key_out, value_out, weights_out = out
+        _check_out(key, value, weights, key_out, value_out, weights_out, budget)
+    _lib.check_device(key)
+    _lib.same_device(key, value=value, weights=weights, key_lengths=key_lengths)
+    if out is None:
+        shape = (batch, budget, kv_heads, dim)
+        key_out, value_out = key.new_empty(shape), key.new_empty(shape)
+        weights_out = weights.new_empty((batch, kv_heads, budget))
+    lengths = torch.empty(batch, dtype=torch.int32, device=key.device)
+    kept = torch.empty((batch, kv_heads, budget), dtype=torch.int32, device=key.device)
+    key, value = (t if not t.data_ptr() & 15 and _attention._dense(t.stride(), t.shape) else _attention._rows(t)
+                  for t in (key, value))
+    weights = weights.contiguous()
+    strides = array("q")
+    for t in (key, value, key_out, value_out):
+        strides.extend(_byte_strides(t))
+    _lib.launch(key, "lr_cache_evict", key.data_ptr(), value.data_ptr(), weights.data_ptr(), _lib.ptr(key_lengths),
+                key_out.data_ptr(), value_out.data_ptr(), weights_out.data_ptr(), lengths.data_ptr(), kept.data_ptr(),
+                batch, keys, kv_heads, 2 * dim, budget, recent, key_out.shape[1], strides.buffer_info()[0],
+                int(out is None))
+    return key_out, value_out, weights_out, lengths, kept
+
+
+def _check_out(key, value, weights, key_out, value_out, weights_out, budget):
+    batch, _, kv_heads, dim = key.shape
+    if (key_out.dim() != 4 or key_out.shape[1] < budget or key_out.shape != (batch, key_out.shape[1], kv_heads, dim)
+            or value_out.shape != key_out.shape or key_out.dtype != key.dtype or value_out.dtype != key.dtype):
+        raise ValueError(f"out must hold {key.dtype} caches [{batch}, at least {budget}, {kv_heads}, {dim}]")
+    _check_weights(weights_out, key_out, "out's weights")
+    _lib.same_device(key, key_out=key_out, value_out=value_out, weights_out=weights_out)
+    _no_gradients(key_out, value_out, weights_out)
+    if not weights_out.is_contiguous() or any(
+            t.data_ptr() & 15 or not _attention._dense(t.stride(), t.shape) or not _distinct(t)
+            for t in (key_out, value_out)):
+        raise ValueError("out must be caches whose rows are dense, 16-byte aligned and distinct, and contiguous weights")
+    if any(_overlap(a, b) for a in (key_out, value_out, weights_out) for b in (key, value, weights)):
+        raise ValueError("out must not overlap the caches that are cut down")
+    if key_out.numel() and key_out.data_ptr() == value_out.data_ptr():
+        raise ValueError("out's keys and values must be different memory")

@@ -1,0 +1,513 @@
+// cache.hip - caches of bounded size: the attention weight that each key gets, and the
+// choice of the keys that stay.
+//
+// Weights. With the logarithm of each row's softmax sum given, a key j of key head h gets
+//   w[j] += sum over rows r of h that see j of exp(scale q_r . k_j - lse_r),
+// rows being tokens x the query heads that share h. A sum over rows per key is the
+// transpose of what attention does, so a workgroup keeps keys, in registers, and the
+// queries go by: S^T = K Q^T on the 32x32x16 MFMA leaves a lane with 16 keys of one query,
+// each added to its own fp32 sum; the sums over the 32 lanes come once at the end. Every
+// key is read once, and the order of additions does not depend on timing.
+//
+// Eviction reads the weights, finds for every cache and head the keys that stay, and moves
+// their rows to another cache, in their order.
+#include "lr_attention.h"
+#include "lr_runtime.h"
+
+namespace lr {
+namespace {
+
+// x / d for x below 2^31 by a multiplication: with 2^(l - 1) < d <= 2^l and m = ceil(2^(31 + l) / d),
+// m d exceeds 2^(31 + l) by less than d <= 2^l, which x < 2^31 cannot bring to the next quotient.
+struct Divisor {
+  uint32_t m;
+  int shift;
+  explicit Divisor(uint32_t d) {
+    int l = 0;
+    while ((1u << l) < d) ++l;
+    shift = 31 + l;
+    m = (uint32_t)(((1ULL << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ int of(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
+};
+
+struct WeighArgs {
+  const uint16_t *q, *k;
+  const float *lse, *w;   // lse [n][q_rows][heads]; w, out [n][kv_heads][k_rows]
+  float* out;
+  float* part;            // sums of splits of the rows [splits][n][kv_heads][k_rows]
+  int64_t qt, qh, qb, kt, kh, kb;
+  const int32_t* lengths;
+  int n, q_rows, k_rows, heads, kv_heads, group;
+  int causal, splits;
+  float c;                // scale * log2(e)
+  Divisor by_group;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Sum over the 32 lanes of a half of the wave.
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  v += xor_partner<8>(v);
+  v += xor_partner<4>(v);
+  v += xor_partner<2>(v);
+  return v + xor_partner<1>(v);
+}
+
+// Four waves with KB blocks of 32 keys each; queries in tiles of 64 rows through two slots
+// of LDS, which first hold the keys on their way to the registers. Swizzle as in lr_attention.h.
+template <typename T, int D, int KB>
+__global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
+  typedef typename Mfma<T>::V V8;
+  constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32, KD = D / 16;
+  constexpr int WAVES = 4, TILE = kKeys * ROW, DMAS = TILE / 1024 / WAVES, KEYS = 32 * WAVES * KB;
+  static_assert(KEYS * ROW >= 2 * TILE, "the keys' LDS holds two tiles of queries");
+  __shared__ __attribute__((aligned(1024))) char smem[KEYS * ROW];
+  __shared__ float sums[KEYS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, col = lane & 31;
+  // Heads, which lie side by side, first; then sequences, so that the first keys, which
+  // the most rows see where causal, come first.
+  uint32_t id = blockIdx.x;
+  const int hd = (int)(id % (uint32_t)p.kv_heads);
+  id /= (uint32_t)p.kv_heads;
+  const int seq = (int)(id % (uint32_t)p.n);
+  id /= (uint32_t)p.n;
+  const int split = (int)(id % (uint32_t)p.splits), key0 = (int)(id / (uint32_t)p.splits) * KEYS;
+  const int kn = p.lengths ? (int)clamp64(p.lengths[seq], 0, p.k_rows) : p.k_rows;
+  const int hidden = kn - p.q_rows;   // causal: token t sees keys up to hidden + t
+  const int rows = p.q_rows * p.group;
+  const int first = p.causal ? (int)min((int64_t)rows, max(0, key0 - hidden) * (int64_t)p.group) : 0;
+  const int tiles = key0 < kn ? (rows - first + kKeys - 1) / kKeys : 0;
+  const int chunk = (tiles + p.splits - 1) / p.splits;
+  const int t0 = min(tiles, split * chunk), t1 = min(tiles, t0 + chunk);
+  float acc[KB][16];
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[b][e] = 0.0f;
+  if (t0 < t1) {
+    auto publish = [&]() {
+      __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);  // vmcnt(0)
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // The 16-byte slots of a tile that this lane fetches: row and chunk.
+    auto slot_row = [&](int i) __attribute__((always_inline)) { return ((wave * DMAS + i) * 64 + lane) / CH; };
+    auto slot_chunk = [&](int i) __attribute__((always_inline)) {
+      return ((wave * DMAS + i) * 64 + lane) % CH ^ (slot_row(i) / RPB % PAIRS) * 2;
+    };
+    const uint16_t* const kbase = p.k + seq * p.kb + hd * p.kh;
+#pragma unroll
+    for (int g = 0; g < KEYS / kKeys; ++g) {
+      const int left = min(kKeys, kn - key0 - g * kKeys);   // keys past the last read as zero
+      const __amdgpu_buffer_rsrc_t r = row_rsrc(kbase + (key0 + (int64_t)g * kKeys) * p.kt,
+                                                left > 0 ? ((int64_t)(left - 1) * p.kt + D) * 2 : 0);
+#pragma unroll
+      for (int i = 0; i < DMAS; ++i)
+        dma16(r, smem + g * TILE + (wave * DMAS + i) * 1024, (uint32_t)(slot_row(i) * p.kt * 2 + slot_chunk(i) * 16));
+    }
+    publish();
+    V8 kf[KB][KD];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      const int row = (wave * KB + b) * 32 + col;
+#pragma unroll
+      for (int d = 0; d < KD; ++d)
+        kf[b][d] = *reinterpret_cast<const V8*>(smem + row * ROW + ((2 * d + half) ^ (row / RPB % PAIRS) * 2) * 16);
+    }
+    __syncthreads();   // the keys are in registers: the queries may take their place
+    const uint16_t* const qbase = p.q + seq * p.qb + (int64_t)hd * p.group * p.qh;
+    const float* const lbase = p.lse + (int64_t)seq * p.q_rows * p.heads + hd * p.group;
+    // Rows past the last one repeat it and are masked.
+    auto issue = [&](int t) {
+      if (t >= t1) return;
+      const int r0 = first + t * kKeys, tok0 = p.by_group.of(r0);
+      char* const slot = smem + ((t - t0) & 1) * TILE;
+      const int toks = min(kKeys, p.q_rows - tok0);   // that 64 rows from r0 on can have
+      const __amdgpu_buffer_rsrc_t rs =
+          row_rsrc(qbase + (int64_t)tok0 * p.qt, ((toks - 1) * p.qt + (p.group - 1) * p.qh + D) * 2);
+#pragma unroll
+      for (int i = 0; i < DMAS; ++i) {
+        const int r = min(r0 + slot_row(i), rows - 1), tok = p.by_group.of(r);
+        dma16(rs, slot + (wave * DMAS + i) * 1024,
+              (uint32_t)((tok - tok0) * p.qt * 2 + (r - tok * p.group) * p.qh * 2 + slot_chunk(i) * 16));
+      }
+    };
+    // Of the lane's row in block b of tile t: lse * log2(e), and the keys that it sees.
+    float sum[2];
+    int seen[2];
+    auto rows_of = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int r = first + t * kKeys + 32 * b + col, tok = p.by_group.of(min(r, rows - 1));
+        sum[b] = lbase[(int64_t)tok * p.heads + (min(r, rows - 1) - tok * p.group)];
+        seen[b] = r >= rows ? 0 : (p.causal ? hidden + tok + 1 : kn);
+      }
+    };
+    issue(t0);
+    rows_of(t0);
+    for (int t = t0; t < t1; ++t) {
+      const float l2[2] = {sum[0] * kLog2e, sum[1] * kLog2e};
+      const int lim[2] = {seen[0], seen[1]};
+      publish();
+      issue(t + 1);
+      if (t + 1 < t1) rows_of(t + 1);
+      const char* const qs = smem + ((t - t0) & 1) * TILE;
+      // Whether every row of the tile sees all of the workgroup's keys.
+      const int r0 = first + t * kKeys;
+      const bool whole = r0 + kKeys <= rows && (!p.causal || hidden + p.by_group.of(r0) + 1 >= key0 + KEYS);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        v16f s[KB];
+#pragma unroll
+        for (int x = 0; x < KB; ++x)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[x][e] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < KD; ++d) {
+          const V8 qf = *reinterpret_cast<const V8*>(qs + (32 * b + col) * ROW + ((2 * d + half) ^ (col / RPB % PAIRS) * 2) * 16);
+#pragma unroll
+          for (int x = 0; x < KB; ++x) s[x] = Mfma<T>::mul(kf[x][d], qf, s[x]);
+        }
+        if (whole) {
+#pragma unroll
+          for (int x = 0; x < KB; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[x][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], p.c, -l2[b]));
+        } else {
+#pragma unroll
+          for (int x = 0; x < KB; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int key = key0 + (wave * KB + x) * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+              const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], p.c, -l2[b]));
+              acc[x][e] += key < lim[b] ? w : 0.0f;
+            }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < KB; ++x)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float v = half_sum(acc[x][e]);
+      if (col == 0) sums[(wave * KB + x) * 32 + 8 * (e >> 2) + 4 * half + (e & 3)] = v;
+    }
+  __syncthreads();
+  const int64_t at = ((int64_t)seq * p.kv_heads + hd) * p.k_rows + key0;
+  for (int i = threadIdx.x; i < KEYS; i += 256) {
+    if (key0 + i >= p.k_rows) return;
+    // Places behind the cache's keys stay as they were.
+    if (p.splits > 1) p.part[(int64_t)split * p.n * p.kv_heads * p.k_rows + at + i] = key0 + i < kn ? sums[i] : 0.0f;
+    else p.out[at + i] = key0 + i < kn ? p.w[at + i] + sums[i] : p.w[at + i];
+  }
+}
+
+// out = w + the splits' sums, in order.
+__global__ __launch_bounds__(256) void add_splits(const float* part, const float* w, float* out, int64_t n, int splits) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float v = part[i];
+  for (int s = 1; s < splits; ++s) v += part[s * n + i];
+  out[i] = w[i] + v;
+}
+
+// ------------------------------------------------------------- eviction ----
+// Of a cache's n > budget keys stay the last `recent` and, of the others, the
+// budget - recent of most weight; of equal weights the first ones. They keep their order.
+struct EvictArgs {
+  const float* w;          // [n][heads][size]
+  const int32_t* lengths;  // or null
+  float* w_out;            // [n][heads][capacity]
+  int32_t* lengths_out;    // [n]
+  int32_t* kept;           // [n][heads][budget]: places in the cache, -1 behind the last
+  const char *k, *v;
+  char *k_out, *v_out;
+  int64_t kt, kh, kb, vt, vh, vb;        // strides of a key, a head, a cache, in bytes
+  int64_t kot, koh, kob, vot, voh, vob;
+  int n, heads, size, budget, recent, capacity;
+  int chunks;              // 16-byte pieces of a row
+  int clear;               // whether rows behind a cache's last are set to zero
+};
+
+// A weight's place in an order of 32-bit numbers: NaN below all others, -0 like 0.
+__device__ __forceinline__ uint32_t order_of(float w) {
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return w != w ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
+}
+
+constexpr int kSelect = 1024;   // threads
+
+// The places that stay, by a workgroup per cache and head: the border between staying and
+// leaving is found from the most significant digit on (11, 11 and 10 bits, counted in
+// LDS), then every wave goes through its stretch of the cache in order.
+__global__ __launch_bounds__(kSelect) void choose_keys(EvictArgs p) {
+  constexpr int WAVES = kSelect / 64, BINS = 2048;
+  __shared__ uint32_t bins[BINS];
+  __shared__ uint32_t found[2];            // digit, keys above it
+  __shared__ uint32_t counts[WAVES][2];    // keys above the border, and on it
+  __shared__ uint32_t part[WAVES];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int head = blockIdx.x % (uint32_t)p.heads, seq = blockIdx.x / (uint32_t)p.heads;
+  const int n = p.lengths ? (int)clamp64(p.lengths[seq], 0, p.size) : p.size;
+  const int stay = min(n, p.budget);
+  const int64_t row = (int64_t)seq * p.heads + head;
+  const float* const w = p.w + row * p.size;
+  float* const w_out = p.w_out + row * p.capacity;
+  int32_t* const kept = p.kept + row * p.budget;
+  if (head == 0 && t == 0) p.lengths_out[seq] = stay;
+  for (int i = stay + t; i < p.capacity; i += kSelect) w_out[i] = 0.0f;
+  for (int i = stay + t; i < p.budget; i += kSelect) kept[i] = -1;
+  if (n <= p.budget) {
+    for (int i = t; i < n; i += kSelect) {
+      kept[i] = i;
+      w_out[i] = w[i];
+    }
+    return;
+  }
+  const int recent = min(p.recent, n), old = n - recent, need = p.budget - recent;   // old > need
+  // The border: the need-th largest of the old weights, and how many of its equals stay.
+  uint32_t border = 0, equals = need;
+  if (need > 0) {
+    int shift = 32;
+    for (int digit = 0; digit < 3; ++digit) {
+      const int bits = digit < 2 ? 11 : 10;
+      shift -= bits;
+      for (int i = t; i < BINS; i += kSelect) bins[i] = 0;
+      __syncthreads();
+      for (int i = t; i < old; i += kSelect) {
+        const uint32_t o = order_of(w[i]);
+        if (digit == 0 || o >> (shift + bits) == border >> (shift + bits)) atomicAdd(&bins[o >> shift & ((1u << bits) - 1)], 1u);
+      }
+      __syncthreads();
+      // Bins from the top: thread t has the two that 2 t and 2 t + 1 others lie above.
+      const int b0 = BINS - 1 - 2 * t;
+      const uint32_t c0 = bins[b0], c1 = bins[b0 - 1];
+      const uint32_t upto = (uint32_t)wave_prefix_sum((int)(c0 + c1));
+      if (lane == 63) part[wave] = upto;
+      __syncthreads();
+      uint32_t above = upto - c0 - c1;
+      for (int i = 0; i < wave; ++i) above += part[i];
+      if (above < equals && above + c0 >= equals) {
+        found[0] = (uint32_t)b0;
+        found[1] = above;
+      } else if (above + c0 < equals && above + c0 + c1 >= equals) {
+        found[0] = (uint32_t)b0 - 1;
+        found[1] = above + c0;
+      }
+      __syncthreads();
+      border |= found[0] << shift;
+      equals -= found[1];
+      __syncthreads();
+    }
+  } else {
+    border = 0xffffffffu;   // none
+    equals = 0;
+  }
+  // What stays of each wave's stretch, and with it where the stretch's own go to.
+  const int stretch = ((n + WAVES - 1) / WAVES + 63) & ~63;
+  const int i0 = min(n, wave * stretch), i1 = min(n, i0 + stretch);
+  uint32_t larger = 0, on = 0;
+  for (int i = i0 + lane; i < i1; i += 64) {
+    const uint32_t o = i < old ? order_of(w[i]) : 0;
+    larger += i >= old || o > border;
+    on += i < old && o == border;
+  }
+  larger = (uint32_t)wave_prefix_sum((int)larger);
+  on = (uint32_t)wave_prefix_sum((int)on);
+  if (lane == 63) {
+    counts[wave][0] = larger;
+    counts[wave][1] = on;
+  }
+  __syncthreads();
+  larger = on = 0;
+  for (int i = 0; i < wave; ++i) {
+    larger += counts[i][0];
+    on += counts[i][1];
+  }
+  const uint64_t below = (1ULL << lane) - 1;
+  for (int i = i0; i < i1; i += 64) {
+    const int at = i + lane;
+    const float x = at < i1 ? w[at] : 0.0f;
+    const uint32_t o = order_of(x);
+    const bool is_larger = at < i1 && (at >= old || o > border), is_on = at < i1 && at < old && o == border;
+    const uint64_t ml = __ballot(is_larger), mo = __ballot(is_on);
+    const uint32_t rank = on + (uint32_t)__builtin_popcountll(mo & below);
+    if (is_larger || (is_on && rank < equals)) {
+      const uint32_t to = larger + (uint32_t)__builtin_popcountll(ml & below) + min(rank, equals);
+      kept[to] = at;
+      w_out[to] = x;
+    }
+    larger += (uint32_t)__builtin_popcountll(ml);
+    on += (uint32_t)__builtin_popcountll(mo);
+  }
+}
+
+// Rows of keys and values that stay: a thread moves 16 bytes of each.
+__global__ __launch_bounds__(256) void move_rows(EvictArgs p) {
+  const uint32_t per_place = (uint32_t)(p.heads * p.chunks), total = (uint32_t)p.budget * per_place;
+  const uint32_t blocks = (total + 255) / 256;
+  const int seq = (int)(blockIdx.x / blocks);
+  const uint32_t i = (blockIdx.x - seq * blocks) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int place = (int)(i / per_place), rest = (int)(i - place * per_place);
+  const int head = rest / p.chunks, at = (rest - head * p.chunks) * 16;
+  const int from = p.kept[((int64_t)seq * p.heads + head) * p.budget + place];
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
+  if (from >= 0) {
+    k = load_nt(reinterpret_cast<const uint4*>(p.k + seq * p.kb + from * p.kt + head * p.kh + at));
+    v = load_nt(reinterpret_cast<const uint4*>(p.v + seq * p.vb + from * p.vt + head * p.vh + at));
+  } else if (!p.clear) {
+    return;
+  }
+  store_nt(reinterpret_cast<uint4*>(p.k_out + seq * p.kob + place * p.kot + head * p.koh + at), k);
+  store_nt(reinterpret_cast<uint4*>(p.v_out + seq * p.vob + place * p.vot + head * p.voh + at), v);
+}
+
+struct WeighPlan {
+  int blocks, splits;   // of 32 keys per wave; of the rows
+  int64_t grid;
+};
+
+WeighPlan weigh_plan(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int kv_heads) {
+  WeighPlan pl;
+  const int64_t rows = q_rows * (heads / kv_heads), tiles = (rows + kKeys - 1) / kKeys;
+  // 64 keys per wave halve what the queries' fragments take of the LDS; with a tile or two
+  // of them the keys' stream counts, and smaller workgroups.
+  pl.blocks = tiles > 2 ? 2 : 1;
+  const int64_t groups = n * kv_heads * ((k_rows + 128 * pl.blocks - 1) / (128 * pl.blocks));
+  // Rows are split while that leaves two tiles and more to each of two workgroups per CU.
+  int64_t s = groups > 0 ? 2 * compute_units() / groups : 1;
+  if (s > tiles / 2) s = tiles / 2;
+  pl.splits = s < 1 ? 1 : (s > 64 ? 64 : (int)s);
+  pl.grid = groups * pl.splits;
+  return pl;
+}
+
+template <typename T, int D>
+void weigh(const WeighArgs& p, const WeighPlan& pl, hipStream_t s) {
+  if (pl.blocks == 1) weigh_keys<T, D, 1><<<(unsigned)pl.grid, 256, 0, s>>>(p);
+  else weigh_keys<T, D, 2><<<(unsigned)pl.grid, 256, 0, s>>>(p);
+}
+
+template <typename T>
+void weigh_by_dim(const WeighArgs& p, int dim, const WeighPlan& pl, hipStream_t s) {
+  if (dim == 32) weigh<T, 32>(p, pl, s);
+  else if (dim == 64) weigh<T, 64>(p, pl, s);
+  else weigh<T, 128>(p, pl, s);
+}
+
+int check_weigh(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int head_dim) {
+  LR_REQUIRE(n >= 0 && q_rows >= 0 && k_rows >= 0, "attention_weights: negative shape");
+  LR_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
+             "attention_weights: %d heads do not share %d key heads evenly", heads, kv_heads);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(LR_EUNSUPPORTED, "attention_weights: head_dim %d is not supported (32, 64 or 128)", head_dim);
+  LR_REQUIRE(n < (1LL << 24) && q_rows < (1LL << 30) && k_rows < (1LL << 30) && heads <= 65536,
+             "attention_weights: shapes past 2^24 sequences, 2^30 rows or 65536 heads are not supported");
+  LR_REQUIRE(q_rows * (heads / kv_heads) < (1LL << 30), "attention_weights: %lld rows of a key head are not supported",
+             (long long)(q_rows * (heads / kv_heads)));
+  LR_REQUIRE(k_rows == 0 || n < (1LL << 40) / k_rows / kv_heads, "attention_weights: %lld caches of %lld keys are not supported",
+             (long long)n, (long long)k_rows);
+  return LR_OK;
+}
+
+}  // namespace
+}  // namespace lr
+
+using namespace lr;
+
+extern "C" int lr_attention_weights_workspace(int64_t sequences, int64_t q_rows, int64_t k_rows, int heads, int kv_heads,
+                                              int head_dim, int64_t* bytes) {
+  if (int rc = check_weigh(sequences, q_rows, k_rows, heads, kv_heads, head_dim)) return rc;
+  LR_REQUIRE(bytes, "attention_weights: null pointer");
+  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads);
+  *bytes = pl.splits > 1 ? pl.splits * sequences * kv_heads * k_rows * 4 : 0;
+  return LR_OK;
+}
+
+extern "C" int lr_attention_weights(const void* q, const void* k, const float* lse, const float* weights, float* out,
+                                    int dtype, int64_t sequences, int64_t q_rows, int64_t k_rows, int heads,
+                                    int kv_heads, int head_dim, const int64_t* strides, const int32_t* key_lengths,
+                                    int causal, int scale_bits, void* workspace, int64_t workspace_bytes, void* stream) {
+  LR_REQUIRE(dtype == LR_DTYPE_BF16 || dtype == LR_DTYPE_F16, "attention_weights: unknown dtype %d", dtype);
+  if (int rc = check_weigh(sequences, q_rows, k_rows, heads, kv_heads, head_dim)) return rc;
+  if (sequences == 0 || k_rows == 0) return LR_OK;
+  LR_REQUIRE(k && weights && out && strides && (q_rows == 0 || (q && lse)), "attention_weights: null pointer");
+  LR_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(lse, 4) && aligned(weights, 4) && aligned(out, 4),
+             "attention_weights: queries and keys must be 16-byte aligned, sums and weights 4-byte");
+  for (int i = 0; i < 6; ++i)
+    LR_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0,
+               "attention_weights: stride %d is %lld, not a multiple of 8 from 0 on", i, (long long)strides[i]);
+  const int group = heads / kv_heads;
+  // A tile's keys and queries are addressed by 32-bit byte offsets from its first one.
+  LR_REQUIRE(strides[3] < (1LL << 23), "attention_weights: strides of 2^23 and more between keys are not supported");
+  LR_REQUIRE((group == 1 || strides[1] < (1LL << 30) / group) && strides[0] < (1LL << 29) / kKeys,
+             "attention_weights: queries of a key head and tile more than 2^31 bytes apart are not supported");
+  float scale;
+  static_assert(sizeof scale == sizeof scale_bits, "fp32");
+  __builtin_memcpy(&scale, &scale_bits, sizeof scale);
+  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads);
+  const WeighArgs p = {static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), lse, weights, out,
+                       static_cast<float*>(workspace), strides[0], strides[1], strides[2], strides[3], strides[4],
+                       strides[5], key_lengths, (int)sequences, (int)q_rows, (int)k_rows, heads, kv_heads, group,
+                       causal != 0, pl.splits, scale * 1.4426950408889634f, Divisor((uint32_t)group)};
+  LR_REQUIRE(p.c > 0.0f && isfinite(p.c), "attention_weights: the scale must be positive and finite");
+  const int64_t all = sequences * kv_heads * k_rows;
+  LR_REQUIRE(pl.grid <= kMaxBlocks && (pl.splits == 1 || all <= kMaxBlocks * 256),
+             "attention_weights: %lld workgroups are not supported", (long long)pl.grid);
+  if (pl.splits > 1)
+    LR_REQUIRE(workspace && aligned(workspace, 4) && workspace_bytes >= pl.splits * all * 4,
+               "attention_weights: needs a workspace of %lld bytes", (long long)(pl.splits * all * 4));
+  hipStream_t s = as_stream(stream);
+  if (dtype == LR_DTYPE_BF16) weigh_by_dim<__bf16>(p, head_dim, pl, s);
+  else weigh_by_dim<_Float16>(p, head_dim, pl, s);
+  if (int rc = check_launch("attention_weights")) return rc;
+  if (pl.splits == 1) return LR_OK;
+  add_splits<<<(unsigned)((all + 255) / 256), 256, 0, s>>>(p.part, weights, out, all, pl.splits);
+  return check_launch("attention_weights");
+}
+
+extern "C" int lr_cache_evict(const void* k, const void* v, const float* weights, const int32_t* key_lengths, void* k_out,
+                              void* v_out, float* weights_out, int32_t* lengths_out, int32_t* kept, int64_t sequences,
+                              int64_t size, int kv_heads, int64_t row_bytes, int64_t budget, int64_t recent,
+                              int64_t capacity, const int64_t* strides, int clear, void* stream) {
+  LR_REQUIRE(sequences >= 0 && size >= 0 && kv_heads > 0 && row_bytes > 0, "cache_evict: negative shape");
+  LR_REQUIRE(budget > 0 && recent >= 0 && recent <= budget && capacity >= budget,
+             "cache_evict: a budget of %lld, %lld of them the latest, in caches of %lld", (long long)budget,
+             (long long)recent, (long long)capacity);
+  if (sequences == 0) return LR_OK;
+  LR_REQUIRE(row_bytes % 16 == 0 && row_bytes <= (1 << 20), "cache_evict: rows of %lld bytes, not a multiple of 16",
+             (long long)row_bytes);
+  LR_REQUIRE(sequences < (1LL << 24) && size < (1LL << 30) && capacity < (1LL << 30) && kv_heads <= 65536,
+             "cache_evict: shapes past 2^24 caches, 2^30 keys or 65536 heads are not supported");
+  LR_REQUIRE((k && v && weights) || size == 0, "cache_evict: null pointer");
+  LR_REQUIRE(k_out && v_out && weights_out && lengths_out && kept && strides, "cache_evict: null pointer");
+  LR_REQUIRE(aligned(k, 16) && aligned(v, 16) && aligned(k_out, 16) && aligned(v_out, 16) && aligned(weights, 4) &&
+                 aligned(weights_out, 4) && aligned(lengths_out, 4) && aligned(kept, 4),
+             "cache_evict: keys and values must be 16-byte aligned");
+  for (int i = 0; i < 12; ++i)
+    LR_REQUIRE(strides[i] >= 0 && strides[i] % 16 == 0,
+               "cache_evict: stride %d is %lld bytes, not a multiple of 16 from 0 on", i, (long long)strides[i]);
+  const int64_t chunks = row_bytes / 16, moved = budget * kv_heads * chunks;
+  const int64_t blocks = (moved + 255) / 256 * sequences;
+  LR_REQUIRE(moved < (1LL << 31) && blocks <= kMaxBlocks && sequences * kv_heads <= kMaxBlocks / 4,
+             "cache_evict: %lld rows of %lld caches are not supported", (long long)(budget * kv_heads),
+             (long long)sequences);
+  const EvictArgs p = {weights, key_lengths, weights_out, lengths_out, kept, static_cast<const char*>(k),
+                       static_cast<const char*>(v), static_cast<char*>(k_out), static_cast<char*>(v_out), strides[0],
+                       strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8],
+                       strides[9], strides[10], strides[11], (int)sequences, kv_heads, (int)size, (int)budget,
+                       (int)recent, (int)capacity, (int)chunks, clear != 0};
+  hipStream_t s = as_stream(stream);
+  choose_keys<<<(unsigned)(sequences * kv_heads), kSelect, 0, s>>>(p);
+  if (int rc = check_launch("cache_evict")) return rc;
+  move_rows<<<(unsigned)blocks, 256, 0, s>>>(p);
+  return check_launch("cache_evict");
+}

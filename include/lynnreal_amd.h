@@ -443,6 +443,26 @@ int lr_cache_evict(const void* k, const void* v, const float* weights, const int
                    int kv_heads, int64_t row_bytes, int64_t budget, int64_t recent, int64_t capacity,
                    const int64_t* strides, int clear, void* stream);
 
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[t] = base[t] + scale[a] * (x[t] down[a]^T) up[a]^T, a = index[t],
+ *   out[t] = base[t] where index[t] is not in [0, adapters).
+ * lr_adapter_plan sorts the tokens by adapter, once for all products of a batch: order
+ * int32 [tokens], tiles int32 [lr_adapter_tiles(tokens, adapters)][4] (adapter, first
+ * place in order, tokens, 0), 16-byte aligned. At most 1000 adapters, 2^24 - 1 tokens.
+ * lr_adapter_add: x [tokens, k], base and out [tokens, n] (rows x_stride, .. elements
+ * apart; out may be base, and may not overlap x or base otherwise), down [adapters, rank, k8] and up [adapters, n,
+ * rank8], all of one 16-bit type, k8 and rank8 being k and rank rounded up to multiples of 8; what
+ * lies behind k in the rows of x (x_stride >= k8) and of down, and behind rank in those of up,
+ * must be 0. scale fp32 [adapters]. rank at most 128. Sums are fp32 in a fixed order, rounded
+ * once. workspace: 16-byte aligned, of the bytes that lr_adapter_workspace gives. */
+int lr_adapter_tiles(int64_t tokens, int adapters);
+int lr_adapter_plan(const int32_t* index, int64_t tokens, int adapters, int32_t* order, int32_t* tiles, void* stream);
+int lr_adapter_workspace(int64_t tokens, int64_t n, int64_t k, int rank, int adapters, int64_t* bytes);
+int lr_adapter_add(const void* x, int64_t x_stride, const void* down, const void* up, const float* scale,
+                   const void* base, int64_t base_stride, void* out, int64_t out_stride, int dtype, int64_t tokens,
+                   int64_t n, int64_t k, int rank, int adapters, const int32_t* order, const int32_t* tiles,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,152 @@
+"""What the adapters of many requests refuse, and how they hold their weights, on the CPU."""
+from array import array
+
+import pytest
+import torch
+from torch import nn
+
+from lynnreal_omni_amd import _lib, adapters as L
+
+BF16 = torch.bfloat16
+
+
+def some(count=3, rank=4, k=24, n=40, dtype=BF16, scale=1.0):
+    return L.LowRankAdapters(torch.ones(count, rank, k, dtype=dtype), torch.ones(count, n, rank, dtype=dtype), scale)
+
+
+class Plan:
+    def __init__(self, tokens=5, adapters=3):
+        self.tokens, self.adapters, self.order = tokens, adapters, torch.zeros(tokens, dtype=torch.int32)
+
+
+def test_weights_are_filled_up_with_zeros():
+    a = some(rank=5, k=13, n=7, scale=torch.tensor([1.0, 2.0, 3.0], dtype=torch.float64))
+    assert a.down.shape == (3, 5, 16) and a.up.shape == (3, 7, 8) and len(a) == 3
+    assert (a.down[..., :13] == 1).all() and (a.down[..., 13:] == 0).all() and (a.up[..., 5:] == 0).all()
+    assert a.scale.tolist() == [1.0, 2.0, 3.0] and a.scale.dtype == torch.float32
+    assert some(scale=0.5).scale.tolist() == [0.5] * 3
+    assert set(dict(a.named_buffers())) == {"down", "up", "scale"}
+
+
+@pytest.mark.parametrize("down,up", [
+    (torch.zeros(2, 4, 8), torch.zeros(3, 8, 4)), (torch.zeros(2, 4, 8), torch.zeros(2, 4, 8)),
+    (torch.zeros(4, 8), torch.zeros(8, 4)), (torch.zeros(2, 4, 8), torch.zeros(2, 8, 4, dtype=BF16)),
+    (torch.zeros(2, 4, 0, dtype=BF16), torch.zeros(2, 8, 4, dtype=BF16)),
+    (torch.zeros(0, 4, 8, dtype=BF16), torch.zeros(0, 8, 4, dtype=BF16))])
+def test_wrong_adapters(down, up):
+    with pytest.raises(ValueError):
+        L.LowRankAdapters(down, up)
+
+
+def test_wrong_scales():
+    for scale in (torch.ones(2), torch.ones(1, 3)):
+        with pytest.raises(ValueError, match="scale"):
+            some(scale=scale)
+
+
+def test_not_supported():
+    for kwargs in (dict(dtype=torch.float32), dict(rank=129), dict(count=1001, rank=1, k=8, n=8)):
+        with pytest.raises(RuntimeError, match="not supported"):
+            some(**kwargs)
+
+
+@pytest.mark.parametrize("indices,count", [(torch.zeros(5), 3), (torch.zeros(5, dtype=torch.int32), 0),
+                                           (torch.zeros(5, dtype=torch.int32), 1001), (torch.zeros(5, dtype=torch.int16), 3),
+                                           (torch.zeros(5, dtype=torch.int32), 3)])
+def test_plans(indices, count):
+    with pytest.raises(ValueError):     # the last: right, but not on a GPU
+        L.AdapterPlan(indices, count)
+
+
+@pytest.mark.parametrize("x,base,plan,match", [
+    ((5, 23), (5, 40), Plan(), "expected x"), ((5, 24), (5, 41), Plan(), "expected x"), ((5, 24), (1, 5, 40), Plan(), "expected"),
+    ((5, 24), (5, 40), Plan(6), "plan"), ((5, 24), (5, 40), Plan(5, 2), "plan"), ((5, 24), (5, 40), Plan(), "GPU"),
+    ((5, 1, 24), (5, 1, 40), Plan(), "GPU")])
+def test_wrong_calls(x, base, plan, match):
+    with pytest.raises(ValueError, match=match):
+        some()(torch.zeros(x, dtype=BF16), torch.zeros(base, dtype=BF16), plan)
+
+
+def test_dtypes_and_gradients():
+    x, base = torch.zeros(5, 24, dtype=BF16), torch.zeros(5, 40, dtype=BF16)
+    for bad in ((x.float(), base), (x, base.half())):
+        with pytest.raises(ValueError, match="dtype"):
+            some()(*bad, Plan())
+    for bad in ((x.clone().requires_grad_(), base), (x, base.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="gradients are not supported"):
+            some()(*bad, Plan())
+    # A module moved to other types.
+    with pytest.raises(RuntimeError, match="not supported"):
+        some().float()(x.float(), base.float(), Plan())
+    with pytest.raises(ValueError, match="scale float32"):
+        some().bfloat16()(x, base, Plan())
+
+
+def test_out_is_base_or_other_memory():
+    memory = torch.zeros(400, dtype=BF16)
+    x, base = torch.zeros(5, 24, dtype=BF16), memory[:200].view(5, 40)
+    for out in (memory[8:208].view(5, 40), torch.zeros(5, 41, dtype=BF16)[:, :40], torch.zeros(5, 40), memory[:160].view(4, 40)):
+        with pytest.raises(ValueError, match="out must"):
+            some()(x, base, Plan(), out=out)
+    with pytest.raises(ValueError, match="out must"):
+        some()(memory[100:220].view(5, 24), torch.zeros(5, 40, dtype=BF16), Plan(), out=base)
+    for out in (base, memory[200:].view(5, 40)):
+        with pytest.raises(ValueError, match="GPU"):
+            some()(x, base, Plan(), out=out)
+
+
+def test_rows_are_read_as_they_are_where_they_can():
+    wide = torch.zeros(9, 64, dtype=BF16)
+    assert L._readable(wide) and L._readable(wide[:, 8:32]) and L._readable(wide[:1].expand(9, -1)) and L._readable(wide[::2])
+    assert not L._readable(wide[:, 1:25]) and not L._readable(wide.t())
+    assert not L._readable(torch.zeros(9, 65, dtype=BF16)[:, :64])
+    assert not L._readable(torch.zeros(100, dtype=BF16).as_strided((5, 64), (8, 1)))
+
+
+def test_adapted_transformer():
+    """Names are checked before any layer is changed; without a plan a layer is the layer."""
+    model = nn.Sequential(nn.Linear(24, 40, dtype=BF16), nn.ModuleDict({"out": nn.Linear(40, 24, dtype=BF16)}))
+    x = torch.randn(5, 24, dtype=BF16)
+    want = model[0](x)
+    with pytest.raises(ValueError, match="maps"):
+        L.adapt_transformer(model, {"0": some(), "1.out": some()})
+    with pytest.raises(AttributeError):
+        L.adapt_transformer(model, {"0": some(), "2": some()})
+    assert type(model[0]) is nn.Linear
+    requests = L.adapt_transformer(model, {"0": some(), "1.out": some(k=40, n=24)})
+    assert isinstance(model[0], L.AdaptedLinear) and isinstance(model[1]["out"], L.AdaptedLinear)
+    assert model[0].requests is requests and model[1]["out"].requests is requests
+    assert torch.equal(model[0](x), want)
+    assert model[0].weight is model[0].layer.weight and model[0].bias is model[0].layer.bias
+    requests.plan = Plan()
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+        model[0](x)
+    with pytest.raises(ValueError, match="already"):
+        L.adapt_transformer(model, {"0": some()})
+
+
+def test_entry_point_refusals_without_a_gpu():
+    lib, p = _lib.load(), 4096
+    assert lib.lr_adapter_tiles(0, 3) == 0 and lib.lr_adapter_tiles(5, 1001) == 0 and lib.lr_adapter_tiles(-1, 3) == 0
+    assert lib.lr_adapter_tiles(1, 8) == 1 and lib.lr_adapter_tiles(64, 8) == 10 and lib.lr_adapter_tiles(5, 8) == 5
+    good = dict(index=p, tokens=5, adapters=3, order=p, tiles=p, stream=None)
+    call = lambda **kw: lib.lr_adapter_plan(*{**good, **kw}.values())  # noqa: E731
+    assert call(tokens=0) == _lib.LR_OK and call(adapters=1001) == _lib.LR_EUNSUPPORTED
+    for bad in [dict(index=None), dict(order=None), dict(tiles=None), dict(tiles=p + 4), dict(index=p + 2), dict(tokens=-1),
+                dict(tokens=1 << 24), dict(adapters=0)]:
+        assert call(**bad) == _lib.LR_EINVAL, bad
+    out = array("q", [0])
+    size = lambda *shape: lib.lr_adapter_workspace(*shape, out.buffer_info()[0])  # noqa: E731
+    assert size(5, 40, 24, 4, 3) == _lib.LR_OK and out[0] > 0
+    assert size(0, 40, 24, 4, 3) == _lib.LR_OK and out[0] == 0
+    assert size(5, 40, 24, 129, 3) == _lib.LR_EUNSUPPORTED and size(5, 0, 24, 4, 3) == _lib.LR_EINVAL
+    good = dict(x=p, xs=24, down=p, up=p, scale=p, base=p, bs=40, out=p, os=40, dtype=0, tokens=5, n=40, k=24, rank=4,
+                adapters=3, order=p, tiles=p, ws=p, wsb=1 << 30, stream=None)
+    call = lambda **kw: lib.lr_adapter_add(*{**good, **kw}.values())  # noqa: E731
+    assert call(tokens=0) == _lib.LR_OK
+    assert call(rank=129) == _lib.LR_EUNSUPPORTED and call(adapters=1001) == _lib.LR_EUNSUPPORTED
+    for bad in [dict(x=None), dict(down=None), dict(up=None), dict(scale=None), dict(base=None), dict(out=None), dict(order=None),
+                dict(tiles=None), dict(ws=None), dict(wsb=8), dict(x=p + 8), dict(up=p + 2), dict(base=p + 1), dict(tiles=p + 4),
+                dict(xs=16), dict(xs=25), dict(xs=1 << 30), dict(os=39), dict(bs=-8), dict(dtype=2), dict(tokens=-1),
+                dict(tokens=1 << 24), dict(n=0), dict(n=1 << 24), dict(k=(1 << 23) + 8), dict(rank=0)]:
+        assert call(**bad) == _lib.LR_EINVAL, bad

@@ -21,6 +21,7 @@ constexpr int kMaxAdapters = 1000;  // a plan counts each wave's tokens of them 
 constexpr int kMaxRank = 128;
 constexpr int kStep = 64;           // columns of x per step of shrink
 constexpr int kColumns = 128;       // columns of out per step of expand
+constexpr int kFewTokens = 256;     // up to which expand_few runs
 // An offset past every buffer here: such a lane reads zeros.
 constexpr uint32_t kOutside = 0xfff80000u;
 constexpr int64_t kMaxWindow = 0xfff00000ll;
@@ -120,7 +121,6 @@ struct AdapterArgs {
   int k8, rank8;         // rows of down and up, in elements
   int splits;            // of k
   int columns;           // of a workgroup of expand
-  int vector;            // whether base and out are read and written 16 bytes at a time
 };
 
 template <int COUNT>
@@ -129,16 +129,24 @@ __device__ __forceinline__ void wait_loads() {   // all but the last COUNT
   __builtin_amdgcn_s_waitcnt((COUNT & 15) | (COUNT >> 4) << 14 | 0x70 | 0xf00);
 }
 
+// Slots of the ring: what three, two and one workgroups per CU can have of its LDS, so that 105
+// to 125 KB are on their way to each CU (at rank 128, 12605 x 14336, four slots took 131 us).
+template <int RP>
+constexpr int kRing = kStep == 64 ? (RP == 32 ? 4 : (RP == 64 ? 5 : 6)) : (RP == 32 ? 3 : (RP == 64 ? 2 : 3));
+
 // Four waves; steps of 64 columns through a ring of LDS slots that hold 64 rows of x and RP of
 // down, 128 bytes each (16-byte chunk c of row r in place c ^ r % 8). Wave w takes the columns
 // 16 w .. of a step for all rows, so that each element leaves the LDS once; the waves' sums are
 // added at the end. The product is transposed, down x^T: a lane holds four ranks of a token
 // next to each other.
+// (One array holds all of a kernel's LDS: between two the compiler cannot tell which a DMA
+// writes, and waits for all of them before any read. With a second one 12605 x 14336 at
+// rank 128 took 285 us.)
 template <typename T, int RP>
 __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
   typedef typename Mfma<T>::V V8;
-  constexpr int RB = RP / 32, TB = kTokens / 32, ROW = 2 * kStep, RING = 4;
-  constexpr int SLOT = (kTokens + RP) * ROW, XD = kTokens / 8 / 4, DD = RP / 8 / 4;   // DMAs of a wave
+  constexpr int RB = RP / 32, TB = kTokens / 32, ROW = 2 * kStep, RING = kRing<RP>, CH = ROW / 16, PER = 1024 / ROW;
+  constexpr int SLOT = (kTokens + RP) * ROW, XD = kTokens / PER / 4, DD = RP / PER / 4;   // DMAs of a wave
   constexpr int GROUP = 4 < TB * RB ? 4 : TB * RB;   // blocks that are added at a time
   static_assert(RING * SLOT >= 4 * GROUP * 4096, "the sums take the ring's place");
   __shared__ __attribute__((aligned(1024))) char smem[RING * SLOT];
@@ -152,35 +160,34 @@ __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
   const int s0 = min(steps, split * chunk), s1 = min(steps, s0 + chunk);
   const __amdgpu_buffer_rsrc_t xr = row_rsrc(p.x + p.first * p.xs, ((int64_t)(p.window - 1) * p.xs + p.k8) * 2);
   const __amdgpu_buffer_rsrc_t dr = row_rsrc(p.down + (int64_t)a * p.rank * p.k8, (int64_t)p.rank * p.k8 * 2);
-  // This lane's rows and chunk of each DMA (8 rows of 128 bytes).
+  // This lane's rows and chunk of each DMA: chunk c of row r lies in place c ^ turn(r).
   uint32_t xo[XD], dof[DD];
-  int mine = 0;   // rows of this window
-  const int at = (lane & 7) ^ (lane >> 3);   // chunk of a step (rows of a DMA start at multiples of 8)
+  auto turn = [](int r) __attribute__((always_inline)) { return r * ROW / 256 % CH; };
 #pragma unroll
   for (int i = 0; i < XD; ++i) {
-    const int r = (wave * XD + i) * 8 + (lane >> 3);
+    const int r = (wave * XD + i) * PER + lane / CH;
     const int64_t tok = r < count ? p.order[info.y + r] - p.first : -1;
     const bool in = tok >= 0 && tok < p.window;
-    xo[i] = in ? (uint32_t)(tok * p.xs * 2 + at * 16) : kOutside;
-    mine += in;
+    xo[i] = in ? (uint32_t)(tok * p.xs * 2) : kOutside;
   }
-  if (__syncthreads_count(mine) == 0) return;
 #pragma unroll
   for (int i = 0; i < DD; ++i) {
-    const int r = (wave * DD + i) * 8 + (lane >> 3);
-    dof[i] = r < p.rank ? (uint32_t)((int64_t)r * p.k8 * 2 + at * 16) : kOutside;
+    const int r = (wave * DD + i) * PER + lane / CH;
+    dof[i] = r < p.rank ? (uint32_t)((int64_t)r * p.k8 * 2) : kOutside;
   }
   auto issue = [&](int s) {
     char* const slot = smem + (s - s0) % RING * SLOT;
     // Chunks past the last column read as zero on both sides.
-    const bool in = s < s1 && s * kStep + at * 8 < p.k8;
-    const uint32_t off = (uint32_t)s * (kStep * 2);
+    auto at = [&](uint32_t row, int r) __attribute__((always_inline)) {
+      const int k = s * kStep + (lane % CH ^ turn(r)) * 8;
+      return s < s1 && k < p.k8 && row != kOutside ? row + k * 2 : kOutside;
+    };
 #pragma unroll
     for (int i = 0; i < XD; ++i)
-      dma16(xr, slot + (wave * XD + i) * 1024, in && xo[i] != kOutside ? xo[i] + off : kOutside);
+      dma16(xr, slot + (wave * XD + i) * 1024, at(xo[i], (wave * XD + i) * PER + lane / CH));
 #pragma unroll
     for (int i = 0; i < DD; ++i)
-      dma16(dr, slot + kTokens * ROW + (wave * DD + i) * 1024, in && dof[i] != kOutside ? dof[i] + off : kOutside);
+      dma16(dr, slot + kTokens * ROW + (wave * DD + i) * 1024, at(dof[i], (wave * DD + i) * PER + lane / CH));
   };
   v16f acc[TB][RB];
 #pragma unroll
@@ -189,29 +196,36 @@ __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
     for (int c = 0; c < RB; ++c)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[b][c][e] = 0.0f;
-  const int place = ((2 * wave + half) ^ (col & 7)) * 16;
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i) issue(s0 + i);
+  auto steps_of = [&](auto blocks) {   // of 32 tokens
 #pragma unroll 1
-  for (int s = s0; s < s1; ++s) {
-    wait_loads<(RING - 2) * (XD + DD)>();
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();   // step s is there, and every wave is done with step s - 1
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    issue(s + RING - 1);
-    const char* const slot = smem + (s - s0) % RING * SLOT;
-    V8 df[RB];
+    for (int s = s0; s < s1; ++s) {
+      wait_loads<(RING - 2) * (XD + DD)>();
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();   // step s is there, and every wave is done with step s - 1
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      issue(s + RING - 1);
+      const char* const slot = smem + (s - s0) % RING * SLOT;
 #pragma unroll
-    for (int c = 0; c < RB; ++c) df[c] = *reinterpret_cast<const V8*>(slot + (kTokens + 32 * c + col) * ROW + place);
+      for (int d = 0; d < kStep / 64; ++d) {
+        // (All rows of a block have the turn of the first: 32 rows are whole turns.)
+        const int place = ((8 * d + 2 * wave + half) ^ turn(col)) * 16;
+        V8 df[RB];
 #pragma unroll
-    for (int b = 0; b < TB; ++b) {
-      if (32 * b >= count) continue;
-      const V8 xf = *reinterpret_cast<const V8*>(slot + (32 * b + col) * ROW + place);
+        for (int c = 0; c < RB; ++c) df[c] = *reinterpret_cast<const V8*>(slot + (kTokens + 32 * c + col) * ROW + place);
 #pragma unroll
-      for (int c = 0; c < RB; ++c) acc[b][c] = Mfma<T>::mul(df[c], xf, acc[b][c]);
+        for (int b = 0; b < decltype(blocks)::value; ++b) {
+          const V8 xf = *reinterpret_cast<const V8*>(slot + (32 * b + col) * ROW + place);
+#pragma unroll
+          for (int c = 0; c < RB; ++c) acc[b][c] = Mfma<T>::mul(df[c], xf, acc[b][c]);
+        }
+      }
     }
-  }
+  };
+  if (count <= 32) steps_of(std::integral_constant<int, 1>{});
+  else steps_of(std::integral_constant<int, TB>{});
   float4* const sums = reinterpret_cast<float4*>(smem);
   float* const part = p.part + ((int64_t)split * p.max_tiles + tile) * kTokens * RP;
 #pragma unroll
@@ -250,25 +264,214 @@ __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
 }
 
 // ------------------------------------------------------------------ expand ----
-template <typename T> __device__ __forceinline__ float to_float(uint16_t v) {
-  return (float)__builtin_bit_cast(T, v);
+// inner: the shares of k added up in order, in place of the first one. A thread per four ranks.
+template <int RP>
+__global__ __launch_bounds__(256) void add_shares(AdapterArgs p) {
+  const int at = (int)(blockIdx.x * 256 + threadIdx.x), tile = at / (kTokens * RP / 4), tok = at / (RP / 4) % kTokens;
+  if (tile >= p.max_tiles || p.tiles[tile].x < 0 || tok >= p.tiles[tile].z) return;
+  float4* const to = reinterpret_cast<float4*>(p.part) + at;
+  const int64_t share = (int64_t)p.max_tiles * kTokens * RP / 4;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  constexpr int COUNT = 8;   // on their way at a time
+  for (int s = 0; s < p.splits; s += COUNT) {
+    float4 y[COUNT];
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) y[i] = s + i < p.splits ? to[(s + i) * share] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      v.x += y[i].x;
+      v.y += y[i].y;
+      v.z += y[i].z;
+      v.w += y[i].w;
+    }
+  }
+  *to = v;
+}
+
+// The power of two that takes a row's largest to [1, 2); 0 for one that is zero or infinite.
+__device__ __forceinline__ int exponent_of(float top) {
+  return top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+}
+
+// v * 2^-ex as numbers of the type and what their rounding leaves. An infinity has no rest.
+template <typename T>
+__device__ __forceinline__ void split8(const float* v, int ex, uint4& hi, uint4& lo) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float y0 = __builtin_amdgcn_ldexpf(v[2 * j], -ex), y1 = __builtin_amdgcn_ldexpf(v[2 * j + 1], -ex);
+    const uint32_t w = Mfma<T>::pack(y0, y1);
+    const float d0 = y0 - Mfma<T>::first(w), d1 = y1 - Mfma<T>::second(w);
+    set_word(hi, j, w);
+    set_word(lo, j, Mfma<T>::pack(__builtin_fabsf(y0) < INFINITY ? d0 : 0.0f, __builtin_fabsf(y1) < INFINITY ? d1 : 0.0f));
+  }
+}
+
+// Few tokens, most tiles with one or some: what counts is the stream of up's rows. Every wave has
+// its quarter of the columns, 32 at a time, straight in registers; a lane adds four columns of its
+// token at a time. The waves add up inner's shares together, a quarter of them each. Tiles of
+// more than 32 tokens take two turns. (All of a workgroup's rows sent to LDS at once instead: 22.7
+// against 20.4 us with shrink, 64 tokens of 32 adapters, 5120 to 15360 columns at rank 32.)
+template <typename T, int RP, bool VECTOR>
+__global__ __launch_bounds__(256, VECTOR && RP < 128 ? (RP == 32 ? 3 : 2) : 1) void expand_few(AdapterArgs p) {
+  typedef typename Mfma<T>::V V8;
+  constexpr int KR = RP / 16, BLOCKS = 2;   // of 32 columns on their way
+  __shared__ float4 sums[4][32][RP / 4 + 1];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, col = lane & 31;
+  const int tile = (int)(blockIdx.x % (uint32_t)p.max_tiles), run = (int)(blockIdx.x / (uint32_t)p.max_tiles);
+  const int4 info = p.tiles[tile];
+  const int a = info.x, count = info.z, quarter = p.columns / 4;
+  const int first = run * p.columns + wave * quarter, last = min(p.n, first + quarter);
+  if (count == 0 || (a < 0 && p.out == p.base)) return;
+  const uint16_t* const up = p.up + (int64_t)(a < 0 ? 0 : a) * p.n * p.rank8;
+  const float scale = p.scale[a < 0 ? 0 : a];
+  for (int t0 = 0; t0 < count; t0 += 32) {
+    const bool mine = t0 + col < count;
+    const int row = min(t0 + col, count - 1);
+    const int64_t tok = p.order[info.y + row];
+    const uint16_t* const base = p.base + tok * p.bs;
+    uint16_t* const out = p.out + tok * p.os;
+    V8 uf[BLOCKS][KR];
+    auto load = [&](int n) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const uint16_t* const from = up + (int64_t)min(n + 32 * b + col, p.n - 1) * p.rank8;
+#pragma unroll
+        for (int d = 0; d < KR; ++d) {
+          const int r = 16 * d + 8 * half;
+          uf[b][d] = *reinterpret_cast<const V8*>(from + (r < p.rank8 ? r : 0));   // (inner is 0 there)
+        }
+      }
+    };
+    // The lane's token, ranks 16 d + 8 half + 0 .. 7.
+    V8 hi[KR], lo[KR];
+    float back = 1.0f;
+    if (a >= 0) {
+      load(min(first, p.n - 1));
+      float v[KR][8], top = 0.0f;
+      const float* const from = p.part + ((int64_t)tile * kTokens + row) * RP + 8 * half;
+      const int64_t share = (int64_t)p.max_tiles * kTokens * RP;
+#pragma unroll
+      for (int d = 0; d < KR; ++d)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[d][e] = 0.0f;
+      for (int s = wave; s < p.splits; s += 4)
+#pragma unroll
+        for (int d = 0; d < KR; ++d)
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(from + s * share + 16 * d + e);
+            v[d][e] += y.x;
+            v[d][e + 1] += y.y;
+            v[d][e + 2] += y.z;
+            v[d][e + 3] += y.w;
+          }
+      if (t0) __syncthreads();   // the tokens before have been read
+#pragma unroll
+      for (int d = 0; d < KR; ++d)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          sums[wave][col][4 * d + 2 * half + e / 4] = make_float4(v[d][e], v[d][e + 1], v[d][e + 2], v[d][e + 3]);
+      __syncthreads();
+#pragma unroll
+      for (int d = 0; d < KR; ++d)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          float4 y = sums[0][col][4 * d + 2 * half + e / 4];
+#pragma unroll
+          for (int w = 1; w < 4; ++w) {
+            const float4 z = sums[w][col][4 * d + 2 * half + e / 4];
+            y.x += z.x;
+            y.y += z.y;
+            y.z += z.z;
+            y.w += z.w;
+          }
+          *reinterpret_cast<float4*>(&v[d][e]) = y;
+        }
+#pragma unroll
+      for (int d = 0; d < KR; ++d)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[d][e] = 16 * d + 8 * half + e < p.rank ? v[d][e] * scale : 0.0f;   // (a row past the rank may hold 0 * infinity)
+          top = fmaxf(top, __builtin_fabsf(v[d][e]));
+        }
+      const int ex = exponent_of(max_with_partner(top));
+      back = __builtin_amdgcn_ldexpf(1.0f, ex);
+#pragma unroll
+      for (int d = 0; d < KR; ++d) {
+        uint4 h, l;
+        split8<T>(v[d], ex, h, l);
+        hi[d] = __builtin_bit_cast(V8, h);
+        lo[d] = __builtin_bit_cast(V8, l);
+      }
+    }
+    for (int n = first; n < last; n += 32 * BLOCKS) {
+      uint2 kept[BLOCKS][4];
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int at = n + 32 * b + 8 * g + 4 * half;
+          if constexpr (VECTOR) {
+            kept[b][g] = *reinterpret_cast<const uint2*>(base + min(at, last - 4));
+          } else {
+            kept[b][g].x = base[min(at, last - 1)] | (uint32_t)base[min(at + 1, last - 1)] << 16;
+            kept[b][g].y = base[min(at + 2, last - 1)] | (uint32_t)base[min(at + 3, last - 1)] << 16;
+          }
+        }
+      v16f s[BLOCKS];
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+        if (a < 0) continue;
+#pragma unroll
+        for (int d = 0; d < KR; ++d) {
+          s[b] = Mfma<T>::mul(uf[b][d], lo[d], s[b]);
+          s[b] = Mfma<T>::mul(uf[b][d], hi[d], s[b]);
+        }
+      }
+      if (a >= 0 && n + 32 * BLOCKS < last) load(n + 32 * BLOCKS);
+      if (!mine) continue;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int at = n + 32 * b + 8 * g + 4 * half;
+          if (at >= last) continue;
+          uint2 w = kept[b][g];
+          if (a >= 0) {
+            w.x = Mfma<T>::pack(Mfma<T>::first(w.x) + s[b][4 * g] * back, Mfma<T>::second(w.x) + s[b][4 * g + 1] * back);
+            w.y = Mfma<T>::pack(Mfma<T>::first(w.y) + s[b][4 * g + 2] * back, Mfma<T>::second(w.y) + s[b][4 * g + 3] * back);
+          }
+          if constexpr (VECTOR) {
+            *reinterpret_cast<uint2*>(out + at) = w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (at + e < last) out[at + e] = (uint16_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
+          }
+        }
+    }
+  }
 }
 
 // Four waves: 32 tokens x 64 columns each of a step of 128 columns. up's rows come through
 // LDS like the keys of lr_attention.h (a row holds RP numbers); the sums leave through LDS
-// too, so that base and out are read and written in whole lines.
-template <typename T, int RP>
+// too, so that base and out are read and written in whole lines. VECTOR: 16 bytes at a time.
+template <typename T, int RP, bool VECTOR>
 __global__ __launch_bounds__(256) void expand(AdapterArgs p) {
   typedef typename Mfma<T>::V V8;
   constexpr int ROW = 2 * RP, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32, KR = RP / 16;
   constexpr int UP = kColumns * ROW, DMAS = UP / 1024 / 4, PITCH = kColumns + 4;
   constexpr int INNER = 2 * kTokens * ROW;   // rounded and rest
   constexpr int OUT = kTokens * PITCH * 4;
-  __shared__ __attribute__((aligned(1024))) char smem[UP + (OUT > INNER ? OUT : INNER)];
-  __shared__ float exponents[kTokens];
-  __shared__ int tokens[kTokens];
+  constexpr int RESULT = OUT > INNER ? OUT : INNER;
+  __shared__ __attribute__((aligned(1024))) char smem[UP + RESULT + kTokens * 8];
   char* const inner = smem + UP;
   float* const result = reinterpret_cast<float*>(smem + UP);
+  float* const exponents = reinterpret_cast<float*>(smem + UP + RESULT);
+  int* const tokens = reinterpret_cast<int*>(exponents + kTokens);
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int half = lane >> 5, col = lane & 31;
   const int tile = (int)(blockIdx.x % (uint32_t)p.max_tiles), run = (int)(blockIdx.x / (uint32_t)p.max_tiles);
@@ -276,41 +479,41 @@ __global__ __launch_bounds__(256) void expand(AdapterArgs p) {
   const int a = info.x, count = info.z;
   if (count == 0 || (a < 0 && p.out == p.base)) return;
   const int n0 = run * p.columns, n1 = min(p.n, n0 + p.columns);
-  if (t < kTokens) tokens[t] = t < count ? p.order[info.y + t] : 0;
+  if (t < kTokens) tokens[t] = p.order[info.y + min(t, count - 1)];
   // Step c: this thread's row (16 threads of 8 columns each, 16 rows at a time) of base.
   const int c8 = (t & 15) * 8, row0 = t >> 4;
   uint4 kept[kTokens / 16];
   auto load_base = [&](int c) {
 #pragma unroll
     for (int i = 0; i < kTokens / 16; ++i) {
-      const int r = 16 * i + row0, n = c + c8;
-      if (r >= count || n >= n1) continue;
-      const uint16_t* const from = p.base + tokens[r] * p.bs + n;
-      if (p.vector) kept[i] = load_nt(reinterpret_cast<const uint4*>(from));
+      // What lies outside repeats the last row and columns: a load that is left out would
+      // cost copies, and with them a wait, where the loop closes.
+      const uint16_t* const row = p.base + tokens[16 * i + row0] * p.bs;
+      if constexpr (VECTOR) kept[i] = load_nt(reinterpret_cast<const uint4*>(row + min(c + c8, n1 - 8)));
       else
 #pragma unroll
         for (int e = 0; e < 8; e += 2)
-          set_word(kept[i], e / 2, (n + e < n1 ? from[e] : 0u) | (n + e + 1 < n1 ? (uint32_t)from[e + 1] << 16 : 0u));
+          set_word(kept[i], e / 2, row[min(c + c8 + e, n1 - 1)] | (uint32_t)row[min(c + c8 + e + 1, n1 - 1)] << 16);
     }
   };
-  auto store_out = [&](int c) {
+  auto store_out = [&](int c, const uint4 (&from)[kTokens / 16]) {
 #pragma unroll
     for (int i = 0; i < kTokens / 16; ++i) {
       const int r = 16 * i + row0, n = c + c8;
       if (r >= count || n >= n1) continue;
       uint16_t* const to = p.out + tokens[r] * p.os + n;
-      if (p.vector) store_nt(reinterpret_cast<uint4*>(to), kept[i]);
+      if constexpr (VECTOR) store_nt(reinterpret_cast<uint4*>(to), from[i]);
       else
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (n + e < n1) to[e] = (uint16_t)(word(kept[i], e / 2) >> (16 * (e & 1)));
+          if (n + e < n1) to[e] = (uint16_t)(word(from[i], e / 2) >> (16 * (e & 1)));
     }
   };
   __syncthreads();
   if (a < 0) {
     for (int c = n0; c < n1; c += kColumns) {
       load_base(c);
-      store_out(c);
+      store_out(c, kept);
     }
     return;
   }
@@ -331,19 +534,10 @@ __global__ __launch_bounds__(256) void expand(AdapterArgs p) {
     const int tok = t >> 2, r0 = (t & 3) * EACH;
     float v[EACH];
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) v[e] = 0.0f;
-    if (tok < count) {
-      const float* from = p.part + ((int64_t)tile * kTokens + tok) * RP + r0;
-      for (int s = 0; s < p.splits; ++s, from += (int64_t)p.max_tiles * kTokens * RP)
-#pragma unroll
-        for (int e = 0; e < EACH; e += 4) {
-          const float4 y = *reinterpret_cast<const float4*>(from + e);
-          v[e] += y.x;
-          v[e + 1] += y.y;
-          v[e + 2] += y.z;
-          v[e + 3] += y.w;
-        }
-    }
+    for (int e = 0; e < EACH; e += 4)
+      *reinterpret_cast<float4*>(v + e) =
+          tok < count ? *reinterpret_cast<const float4*>(p.part + ((int64_t)tile * kTokens + tok) * RP + r0 + e)
+                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const float scale = p.scale[a];
     float top = 0.0f;
 #pragma unroll
@@ -353,22 +547,12 @@ __global__ __launch_bounds__(256) void expand(AdapterArgs p) {
     }
     top = fmaxf(top, xor_partner<1>(top));
     top = fmaxf(top, xor_partner<2>(top));
-    // The largest of the row to [1, 2); what is infinite or zero stays.
-    const int ex = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+    const int ex = exponent_of(top);
     if ((t & 3) == 0) exponents[tok] = __builtin_amdgcn_ldexpf(1.0f, ex);
-    __syncthreads();
 #pragma unroll
     for (int e = 0; e < EACH; e += 8) {
       uint4 hi, lo;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float y0 = __builtin_amdgcn_ldexpf(v[e + 2 * j], -ex), y1 = __builtin_amdgcn_ldexpf(v[e + 2 * j + 1], -ex);
-        const uint32_t w = Mfma<T>::pack(y0, y1);
-        const float d0 = y0 - Mfma<T>::first(w), d1 = y1 - Mfma<T>::second(w);
-        set_word(hi, j, w);
-        // An infinity has no rest.
-        set_word(lo, j, Mfma<T>::pack(__builtin_fabsf(y0) < INFINITY ? d0 : 0.0f, __builtin_fabsf(y1) < INFINITY ? d1 : 0.0f));
-      }
+      split8<T>(v + e, ex, hi, lo);
       const int ch = (r0 + e) / 8 ^ (tok / RPB % PAIRS) * 2;
       *reinterpret_cast<uint4*>(inner + tok * ROW + ch * 16) = hi;
       *reinterpret_cast<uint4*>(inner + kTokens * ROW + tok * ROW + ch * 16) = lo;
@@ -386,8 +570,15 @@ __global__ __launch_bounds__(256) void expand(AdapterArgs p) {
   }
   const float back = exponents[row];
   for (int c = n0; c < n1; c += kColumns) {
-    wait_loads<0>();
-    __syncthreads();   // up's rows are there; inner, or the step before, has been read
+    // Up's rows and base are there; the stores of the step before, which come behind them
+    // (four per thread of a full tile), may be on their way.
+    if (VECTOR && count == kTokens && c > n0) wait_loads<kTokens / 16>();
+    else wait_loads<0>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): inner, or the step before, has been read
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
     if (!idle) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -407,29 +598,39 @@ __global__ __launch_bounds__(256) void expand(AdapterArgs p) {
               make_float4(s[4 * g] * back, s[4 * g + 1] * back, s[4 * g + 2] * back, s[4 * g + 3] * back);
       }
     }
-    __syncthreads();
-    if (c + kColumns < n1) issue(c + kColumns);
+    __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the sums are written, up's rows read
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // The sums leave the LDS before the next DMA, for which the compiler would wait otherwise.
+    uint4 sum[kTokens / 16];
 #pragma unroll
     for (int i = 0; i < kTokens / 16; ++i) {
       const int r = 16 * i + row0;
-      if (r >= count) continue;
       const float4 y0 = *reinterpret_cast<const float4*>(result + r * PITCH + c8);
       const float4 y1 = *reinterpret_cast<const float4*>(result + r * PITCH + c8 + 4);
       const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t w = word(kept[i], e);
-        set_word(kept[i], e, Mfma<T>::pack(Mfma<T>::first(w) + y[2 * e], Mfma<T>::second(w) + y[2 * e + 1]));
+        set_word(sum[i], e, Mfma<T>::pack(Mfma<T>::first(w) + y[2 * e], Mfma<T>::second(w) + y[2 * e + 1]));
       }
     }
-    store_out(c);
-    if (c + kColumns < n1) load_base(c + kColumns);
+    __builtin_amdgcn_sched_barrier(0);
+    if (c + kColumns < n1) {
+      issue(c + kColumns);
+      load_base(c + kColumns);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    store_out(c, sum);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 struct AddPlan {
   int rank;      // padded
   int splits, columns;
+  bool few;
   int64_t tiles, bytes;
 };
 
@@ -437,21 +638,35 @@ AddPlan add_plan(int64_t tokens, int64_t n, int64_t k, int rank, int64_t adapter
   AddPlan pl;
   pl.rank = rank <= 32 ? 32 : (rank <= 64 ? 64 : 128);
   pl.tiles = plan_tiles(tokens, adapters);
-  const int64_t want = 2 * compute_units(), steps = (k + kStep - 1) / kStep;
-  // Shares of k of at least four steps, at most 16 of them, to two workgroups per CU.
-  int64_t s = (want + pl.tiles - 1) / pl.tiles;
-  if (s > steps / 4) s = steps / 4;
-  pl.splits = s < 1 ? 1 : (s > 16 ? 16 : (int)s);
-  // Columns of an expanding workgroup: up to 1024, less where that leaves CUs idle.
+  const int64_t cus = compute_units(), steps = (k + kStep - 1) / kStep;
+  // Columns of an expanding workgroup: up to 1024, less where that leaves fewer than two
+  // workgroups per CU; one for few tokens, where each of them adds up the shares (64 tokens of
+  // 32 adapters, 15360 columns at rank 32: 19.4 us so, 21.8 with two; 16 tokens 12.0 and 14.3).
+  pl.few = tokens <= kFewTokens;
   int64_t c = 1024;
-  while (c > kColumns && pl.tiles * ((n + c - 1) / c) < want) c /= 2;
+  while (c > kColumns && pl.tiles * ((n + c - 1) / c) < (pl.few ? cus : 2 * cus)) c /= 2;
   pl.columns = (int)c;
+  // Shares of k, of four steps and more: what the rounds of workgroups take, their steps at
+  // 45 KB/us for each CU and six of them to fill the ring, against a launch to add the shares
+  // and their way through memory.
+  const int per_cu = pl.rank == 32 ? 3 : (pl.rank == 64 ? 2 : 1);
+  const double step = per_cu * (kTokens + pl.rank) * 2.0 * kStep / 45e3;
+  const double share = (double)pl.tiles * kTokens * pl.rank * 4 * 2.0 / 5e6;
+  double least = 0.0;
+  for (int s = 1; s <= 16 && (s == 1 || s <= steps / 4); ++s) {
+    const double rounds = ceil((double)(pl.tiles * s) / (double)(cus * per_cu));
+    const double us = rounds * ((double)((steps + s - 1) / s) + 6.0) * step + (s > 1 ? 2.5 + s * share : 0.0);
+    if (s == 1 || us < least) {
+      least = us;
+      pl.splits = s;
+    }
+  }
   pl.bytes = pl.splits * pl.tiles * kTokens * pl.rank * 4;
   return pl;
 }
 
 template <typename T, int RP>
-int add(AdapterArgs p, const AddPlan& pl, hipStream_t s) {
+int add(AdapterArgs p, const AddPlan& pl, bool vector, hipStream_t s) {
   const int64_t rows = kMaxWindow / (p.xs * 2 > 2 * p.k8 ? p.xs * 2 : 2 * p.k8);
   for (int64_t first = 0; first < p.tokens; first += rows) {
     p.first = first;
@@ -459,15 +674,23 @@ int add(AdapterArgs p, const AddPlan& pl, hipStream_t s) {
     shrink<T, RP><<<(unsigned)(pl.tiles * pl.splits), 256, 0, s>>>(p);
     if (int rc = check_launch("adapter_add")) return rc;
   }
-  expand<T, RP><<<(unsigned)(pl.tiles * ((p.n + pl.columns - 1) / pl.columns)), 256, 0, s>>>(p);
+  const unsigned grid = (unsigned)(pl.tiles * ((p.n + pl.columns - 1) / pl.columns));
+  if (pl.splits > 1 && !pl.few) {
+    add_shares<RP><<<(unsigned)((pl.tiles * (kTokens * RP / 4) + 255) / 256), 256, 0, s>>>(p);
+    if (int rc = check_launch("adapter_add")) return rc;
+  }
+  if (pl.few && vector) expand_few<T, RP, true><<<grid, 256, 0, s>>>(p);
+  else if (pl.few) expand_few<T, RP, false><<<grid, 256, 0, s>>>(p);
+  else if (vector) expand<T, RP, true><<<grid, 256, 0, s>>>(p);
+  else expand<T, RP, false><<<grid, 256, 0, s>>>(p);
   return check_launch("adapter_add");
 }
 
 template <typename T>
-int add_by_rank(const AdapterArgs& p, const AddPlan& pl, hipStream_t s) {
-  if (pl.rank == 32) return add<T, 32>(p, pl, s);
-  if (pl.rank == 64) return add<T, 64>(p, pl, s);
-  return add<T, 128>(p, pl, s);
+int add_by_rank(const AdapterArgs& p, const AddPlan& pl, bool vector, hipStream_t s) {
+  if (pl.rank == 32) return add<T, 32>(p, pl, vector, s);
+  if (pl.rank == 64) return add<T, 64>(p, pl, vector, s);
+  return add<T, 128>(p, pl, vector, s);
 }
 
 int check_add(int64_t tokens, int64_t n, int64_t k, int rank, int64_t adapters) {
@@ -552,7 +775,7 @@ extern "C" int lr_adapter_add(const void* x, int64_t x_stride, const void* down,
   p.rank8 = (rank + 7) & ~7;
   p.splits = pl.splits;
   p.columns = pl.columns;
-  p.vector = n % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned(base, 16) && aligned(out, 16);
+  const bool vector = n % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned(base, 16) && aligned(out, 16);
   hipStream_t s = as_stream(stream);
-  return dtype == LR_DTYPE_BF16 ? add_by_rank<__bf16>(p, pl, s) : add_by_rank<_Float16>(p, pl, s);
+  return dtype == LR_DTYPE_BF16 ? add_by_rank<__bf16>(p, pl, vector, s) : add_by_rank<_Float16>(p, pl, vector, s);
 }

@@ -64,8 +64,9 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
   constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32, KD = D / 16;
   constexpr int WAVES = 4, TILE = kKeys * ROW, DMAS = TILE / 1024 / WAVES, KEYS = 32 * WAVES * KB;
   static_assert(KEYS * ROW >= 2 * TILE, "the keys' LDS holds two tiles of queries");
-  __shared__ __attribute__((aligned(1024))) char smem[KEYS * ROW];
-  __shared__ float sums[KEYS];
+  // (One array for all of it: between two the compiler waits for every DMA before any read.)
+  __shared__ __attribute__((aligned(1024))) char smem[KEYS * (ROW + 4)];
+  float* const sums = reinterpret_cast<float*>(smem + KEYS * ROW);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = lane >> 5, col = lane & 31;
   // Heads, which lie side by side, first; then sequences, so that the first keys, which

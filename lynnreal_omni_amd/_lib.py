@@ -77,7 +77,9 @@ SIGNATURES = {
     "lr_attention_weights_workspace": [_I64, _I64, _I64, _I32, _I32, _I32, _P],
     "lr_attention_weights": [_P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32, _I32, _P, _I64,
                              _P],
-    "lr_cache_evict": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _P, _I32, _P],
+    "lr_cache_evict_workspace": [_I64, _I64, _I32, _P],
+    "lr_cache_evict": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _P, _I32, _P, _I64,
+                       _P],
     "lr_adapter_tiles": [_I64, _I32],
     "lr_adapter_plan": [_P, _I64, _I32, _P, _P, _P],
     "lr_adapter_workspace": [_I64, _I64, _I64, _I32, _I32, _P],

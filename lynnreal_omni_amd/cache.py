@@ -190,11 +190,20 @@ def evict(key, value, weights, key_lengths, budget, *, recent=0, out=None):
     strides = array("q")
     for t in (key, value, key_out, value_out):
         strides.extend(_byte_strides(t))
+    nbytes = _evict_workspace(batch, keys, kv_heads)
+    ws = _lib.workspace(key, nbytes)   # held until the launch
     _lib.launch(key, "lr_cache_evict", key.data_ptr(), value.data_ptr(), weights.data_ptr(), _lib.ptr(key_lengths),
                 key_out.data_ptr(), value_out.data_ptr(), weights_out.data_ptr(), lengths.data_ptr(), kept.data_ptr(),
                 batch, keys, kv_heads, 2 * dim, budget, recent, key_out.shape[1], strides.buffer_info()[0],
-                int(out is None))
+                int(out is None), _lib.ptr(ws), nbytes)
     return key_out, value_out, weights_out, lengths, kept
+
+
+@functools.lru_cache(maxsize=4096)
+def _evict_workspace(batch, keys, kv_heads):
+    nbytes = array("q", [0])
+    _lib.call("lr_cache_evict_workspace", batch, keys, kv_heads, nbytes.buffer_info()[0])
+    return nbytes[0]
 
 
 def _check_out(key, value, weights, key_out, value_out, weights_out, budget):

@@ -235,6 +235,8 @@ struct EvictArgs {
   int n, heads, size, budget, recent, capacity;
   int chunks;              // 16-byte pieces of a row
   int clear;               // whether rows behind a cache's last are set to zero
+  uint32_t* hist;          // counts of three digits [3][n][heads][parts][2048], where parts > 1
+  int parts;               // of kPart keys
 };
 
 // A weight's place in an order of 32-bit numbers: NaN below all others, -0 like 0.
@@ -243,107 +245,192 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return w != w ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
 }
 
-constexpr int kSelect = 1024;   // threads
+constexpr uint32_t kZeroOrder = 0x80000000u;
+constexpr int kSelect = 1024;           // threads
+constexpr int kEach = 16;               // weights of a thread
+constexpr int kPart = kSelect * kEach;  // and of a workgroup
+constexpr int kBins = 2048;
+constexpr int kDigitShift[3] = {21, 10, 0}, kDigitBits[3] = {11, 11, 10};
 
-// The places that stay, by a workgroup per cache and head: the border between staying and
-// leaving is found from the most significant digit on (11, 11 and 10 bits, counted in
-// LDS), then every wave goes through its stretch of the cache in order.
+// The places that stay, for each cache and head. The border between staying and leaving is found
+// digit by digit from the most significant one on, by counting how many weights have each
+// value of it; then every weight's place among those that stay is a count of the ones before
+// it. A workgroup has 16384 weights, in registers; a wave's are next to each other.
+//   WHOLE   a cache of one workgroup: all of it in one kernel
+//   0, 1, 2 counts of that digit, for each workgroup's part, into p.hist
+//   PLACE   the border and the parts before this one from those counts, then the places
+// (Four caches of 40000 to 131072 keys, 8 heads: a workgroup for each, that went through its weights
+// five times, took 159 us.)
+constexpr int kPlace = 3, kWhole = 4;
+
+// Sum of the waves' numbers v[0], v[2], .. before wave `end`.
+__device__ __forceinline__ uint32_t sum_before(const uint32_t* v, int end) {
+  const int lane = threadIdx.x & 63;
+  return (uint32_t)__builtin_amdgcn_readlane(wave_prefix_sum(lane < end ? (int)v[2 * lane] : 0), 63);
+}
+
+template <int STEP>
 __global__ __launch_bounds__(kSelect) void choose_keys(EvictArgs p) {
-  constexpr int WAVES = kSelect / 64, BINS = 2048;
-  __shared__ uint32_t bins[BINS];
+  constexpr int WAVES = kSelect / 64;
+  __shared__ uint32_t bins[kBins];
   __shared__ uint32_t found[2];            // digit, keys above it
-  __shared__ uint32_t counts[WAVES][2];    // keys above the border, and on it
-  __shared__ uint32_t part[WAVES];
+  __shared__ uint32_t counts[WAVES][2];    // of a wave: keys above the border, and on it
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int head = blockIdx.x % (uint32_t)p.heads, seq = blockIdx.x / (uint32_t)p.heads;
+  const int part = blockIdx.x % (uint32_t)p.parts, row = blockIdx.x / (uint32_t)p.parts;
+  const int head = row % (uint32_t)p.heads, seq = row / (uint32_t)p.heads;
   const int n = p.lengths ? (int)clamp64(p.lengths[seq], 0, p.size) : p.size;
   const int stay = min(n, p.budget);
-  const int64_t row = (int64_t)seq * p.heads + head;
-  const float* const w = p.w + row * p.size;
-  float* const w_out = p.w_out + row * p.capacity;
-  int32_t* const kept = p.kept + row * p.budget;
-  if (head == 0 && t == 0) p.lengths_out[seq] = stay;
-  for (int i = stay + t; i < p.capacity; i += kSelect) w_out[i] = 0.0f;
-  for (int i = stay + t; i < p.budget; i += kSelect) kept[i] = -1;
+  const float* const w = p.w + (int64_t)row * p.size;
+  float* const w_out = p.w_out + (int64_t)row * p.capacity;
+  int32_t* const kept = p.kept + (int64_t)row * p.budget;
+  // The thread's weights: `each`, this one and every 64th on. (Small caches are spread over all waves.)
+  const int each = p.parts > 1 ? kEach : (p.size + kSelect - 1) / kSelect;
+  const int first = part * kPart + wave * (64 * each) + lane;
+  if (STEP >= kPlace && part == 0) {
+    if (head == 0 && t == 0) p.lengths_out[seq] = stay;
+    for (int i = stay + t; i < p.capacity; i += kSelect) w_out[i] = 0.0f;
+    for (int i = stay + t; i < p.budget; i += kSelect) kept[i] = -1;
+  }
+  if (STEP < kPlace && n <= p.budget) return;
+  float x[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) x[j] = j < each && first + 64 * j < n ? w[first + 64 * j] : 0.0f;
   if (n <= p.budget) {
-    for (int i = t; i < n; i += kSelect) {
-      kept[i] = i;
-      w_out[i] = w[i];
-    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (j < each && first + 64 * j < n) {
+        kept[first + 64 * j] = first + 64 * j;
+        w_out[first + 64 * j] = x[j];
+      }
     return;
   }
   const int recent = min(p.recent, n), old = n - recent, need = p.budget - recent;   // old > need
-  // The border: the need-th largest of the old weights, and how many of its equals stay.
+  // Weights of this part by digit d, those with the border's digits before it.
   uint32_t border = 0, equals = need;
-  if (need > 0) {
-    int shift = 32;
-    for (int digit = 0; digit < 3; ++digit) {
-      const int bits = digit < 2 ? 11 : 10;
-      shift -= bits;
-      for (int i = t; i < BINS; i += kSelect) bins[i] = 0;
-      __syncthreads();
-      for (int i = t; i < old; i += kSelect) {
-        const uint32_t o = order_of(w[i]);
-        if (digit == 0 || o >> (shift + bits) == border >> (shift + bits)) atomicAdd(&bins[o >> shift & ((1u << bits) - 1)], 1u);
-      }
-      __syncthreads();
-      // Bins from the top: thread t has the two that 2 t and 2 t + 1 others lie above.
-      const int b0 = BINS - 1 - 2 * t;
-      const uint32_t c0 = bins[b0], c1 = bins[b0 - 1];
-      const uint32_t upto = (uint32_t)wave_prefix_sum((int)(c0 + c1));
-      if (lane == 63) part[wave] = upto;
-      __syncthreads();
-      uint32_t above = upto - c0 - c1;
-      for (int i = 0; i < wave; ++i) above += part[i];
-      if (above < equals && above + c0 >= equals) {
-        found[0] = (uint32_t)b0;
-        found[1] = above;
-      } else if (above + c0 < equals && above + c0 + c1 >= equals) {
-        found[0] = (uint32_t)b0 - 1;
-        found[1] = above + c0;
-      }
-      __syncthreads();
-      border |= found[0] << shift;
-      equals -= found[1];
-      __syncthreads();
+  auto count = [&](int d) {
+    const int shift = kDigitShift[d], bits = kDigitBits[d];
+    for (int i = t; i < kBins; i += kSelect) bins[i] = 0;
+    __syncthreads();
+    int zeros = 0;   // a common weight, which would queue at its bin
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if (j >= each) break;
+      const uint32_t o = order_of(x[j]);
+      const bool in = first + 64 * j < old && (d == 0 || o >> (shift + bits) == border >> (shift + bits));
+      zeros += in && o == kZeroOrder;
+      if (in && o != kZeroOrder) atomicAdd(&bins[o >> shift & ((1u << bits) - 1)], 1u);
+    }
+    zeros = wave_prefix_sum(zeros);
+    if (lane == 63 && zeros) atomicAdd(&bins[kZeroOrder >> shift & ((1u << bits) - 1)], (uint32_t)zeros);
+    __syncthreads();
+  };
+  // The digit at which the counts from the top on reach what is left to stay. Thread t has bins
+  // 2047 - 2 t and 2046 - 2 t.
+  auto settle = [&](int d, uint32_t c0, uint32_t c1) {
+    const uint32_t upto = (uint32_t)wave_prefix_sum((int)(c0 + c1));
+    __syncthreads();
+    if (lane == 63) counts[wave][0] = upto;
+    __syncthreads();
+    const uint32_t above = upto - c0 - c1 + sum_before(&counts[0][0], wave);
+    if (above < equals && above + c0 >= equals) {
+      found[0] = (uint32_t)(kBins - 1 - 2 * t);
+      found[1] = above;
+    } else if (above + c0 < equals && above + c0 + c1 >= equals) {
+      found[0] = (uint32_t)(kBins - 2 - 2 * t);
+      found[1] = above + c0;
+    }
+    __syncthreads();
+    border |= found[0] << kDigitShift[d];
+    equals -= found[1];
+  };
+  // The counts of a digit, of part q, at this thread's bins (the upper one in y).
+  auto counted = [&](int d, int q) {
+    return *reinterpret_cast<const uint2*>(p.hist + (((int64_t)d * p.n * p.heads + row) * p.parts + q) * kBins + kBins - 2 - 2 * t);
+  };
+  uint32_t before[2] = {0, 0};   // this part: keys above the border, and on it
+  if (need == 0) {
+    if (STEP < kPlace) return;
+    border = 0xffffffffu;   // none
+  } else if (STEP == kWhole) {
+    for (int d = 0; d < 3; ++d) {
+      count(d);
+      settle(d, bins[kBins - 1 - 2 * t], bins[kBins - 2 - 2 * t]);
     }
   } else {
-    border = 0xffffffffu;   // none
-    equals = 0;
+    // All digits' counts first: their loads wait for none of them.
+    constexpr int DIGITS = STEP < kPlace ? STEP : 3, COUNT = 8;   // parts on their way at a time
+    uint32_t c0[DIGITS + 1] = {}, c1[DIGITS + 1] = {}, mine0[DIGITS + 1] = {}, mine1[DIGITS + 1] = {};
+    for (int q = 0; q < p.parts; q += COUNT) {
+      uint2 c[DIGITS + 1][COUNT];
+#pragma unroll
+      for (int d = 0; d < DIGITS; ++d)
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) c[d][i] = q + i < p.parts ? counted(d, q + i) : make_uint2(0, 0);
+#pragma unroll
+      for (int d = 0; d < DIGITS; ++d)
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+          c0[d] += c[d][i].y;
+          c1[d] += c[d][i].x;
+          mine0[d] += q + i < part ? c[d][i].y : 0;
+          mine1[d] += q + i < part ? c[d][i].x : 0;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DIGITS; ++d) {
+      settle(d, c0[d], c1[d]);
+      const int digit = (int)found[0], mine = kBins - 1 - 2 * t;
+      before[0] += (mine > digit ? mine0[d] : 0) + (mine - 1 > digit ? mine1[d] : 0);
+      if (d == 2) before[1] = (mine == digit ? mine0[d] : 0) + (mine - 1 == digit ? mine1[d] : 0);
+    }
+    if (STEP < kPlace) {
+      count(STEP);
+      uint32_t* const to = p.hist + (((int64_t)STEP * p.n * p.heads + row) * p.parts + part) * kBins;
+      for (int i = t; i < kBins; i += kSelect) to[i] = bins[i];
+      return;
+    }
+    // The sums over the threads' bins.
+    const uint32_t a = (uint32_t)wave_prefix_sum((int)before[0]), b = (uint32_t)wave_prefix_sum((int)before[1]);
+    __syncthreads();
+    if (lane == 63) {
+      counts[wave][0] = a;
+      counts[wave][1] = b;
+    }
+    __syncthreads();
+    before[0] = sum_before(&counts[0][0], WAVES);
+    before[1] = sum_before(&counts[0][1], WAVES);
   }
-  // What stays of each wave's stretch, and with it where the stretch's own go to.
-  const int stretch = ((n + WAVES - 1) / WAVES + 63) & ~63;
-  const int i0 = min(n, wave * stretch), i1 = min(n, i0 + stretch);
   uint32_t larger = 0, on = 0;
-  for (int i = i0 + lane; i < i1; i += 64) {
-    const uint32_t o = i < old ? order_of(w[i]) : 0;
-    larger += i >= old || o > border;
-    on += i < old && o == border;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (j >= each) break;
+    const uint32_t o = order_of(x[j]);
+    const bool in = first + 64 * j < old;
+    larger += (uint32_t)__builtin_popcountll(__ballot(in && o > border));
+    on += (uint32_t)__builtin_popcountll(__ballot(in && o == border));
   }
-  larger = (uint32_t)wave_prefix_sum((int)larger);
-  on = (uint32_t)wave_prefix_sum((int)on);
-  if (lane == 63) {
+  __syncthreads();
+  if (lane == 0) {
     counts[wave][0] = larger;
     counts[wave][1] = on;
   }
   __syncthreads();
-  larger = on = 0;
-  for (int i = 0; i < wave; ++i) {
-    larger += counts[i][0];
-    on += counts[i][1];
-  }
+  larger = before[0] + sum_before(&counts[0][0], wave);
+  on = before[1] + sum_before(&counts[0][1], wave);
   const uint64_t below = (1ULL << lane) - 1;
-  for (int i = i0; i < i1; i += 64) {
-    const int at = i + lane;
-    const float x = at < i1 ? w[at] : 0.0f;
-    const uint32_t o = order_of(x);
-    const bool is_larger = at < i1 && (at >= old || o > border), is_on = at < i1 && at < old && o == border;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (j >= each) break;
+    const int at = first + 64 * j;
+    const uint32_t o = order_of(x[j]);
+    const bool is_larger = at < old && o > border, is_on = at < old && o == border;
     const uint64_t ml = __ballot(is_larger), mo = __ballot(is_on);
     const uint32_t rank = on + (uint32_t)__builtin_popcountll(mo & below);
-    if (is_larger || (is_on && rank < equals)) {
-      const uint32_t to = larger + (uint32_t)__builtin_popcountll(ml & below) + min(rank, equals);
+    uint32_t to = larger + (uint32_t)__builtin_popcountll(ml & below) + min(rank, equals);
+    if (at >= old) to = (uint32_t)(need + at - old);   // the latest come last
+    if (is_larger || (is_on && rank < equals) || (at >= old && at < n)) {
       kept[to] = at;
-      w_out[to] = x;
+      w_out[to] = x[j];
     }
     larger += (uint32_t)__builtin_popcountll(ml);
     on += (uint32_t)__builtin_popcountll(mo);
@@ -475,10 +562,24 @@ extern "C" int lr_attention_weights(const void* q, const void* k, const float* l
   return check_launch("attention_weights");
 }
 
+static int64_t evict_bytes(int64_t sequences, int64_t size, int kv_heads) {
+  return size > kPart ? 3 * sequences * kv_heads * ((size + kPart - 1) / kPart) * kBins * 4 : 0;
+}
+
+extern "C" int lr_cache_evict_workspace(int64_t sequences, int64_t size, int kv_heads, int64_t* bytes) {
+  LR_REQUIRE(sequences >= 0 && sequences < (1LL << 24) && size >= 0 && size < (1LL << 30) && kv_heads > 0 &&
+                 kv_heads <= 65536,
+             "cache_evict: %lld caches of %lld keys are not supported", (long long)sequences, (long long)size);
+  LR_REQUIRE(bytes, "cache_evict: null pointer");
+  *bytes = evict_bytes(sequences, size, kv_heads);
+  return LR_OK;
+}
+
 extern "C" int lr_cache_evict(const void* k, const void* v, const float* weights, const int32_t* key_lengths, void* k_out,
                               void* v_out, float* weights_out, int32_t* lengths_out, int32_t* kept, int64_t sequences,
                               int64_t size, int kv_heads, int64_t row_bytes, int64_t budget, int64_t recent,
-                              int64_t capacity, const int64_t* strides, int clear, void* stream) {
+                              int64_t capacity, const int64_t* strides, int clear, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
   LR_REQUIRE(sequences >= 0 && size >= 0 && kv_heads > 0 && row_bytes > 0, "cache_evict: negative shape");
   LR_REQUIRE(budget > 0 && recent >= 0 && recent <= budget && capacity >= budget,
              "cache_evict: a budget of %lld, %lld of them the latest, in caches of %lld", (long long)budget,
@@ -498,16 +599,32 @@ extern "C" int lr_cache_evict(const void* k, const void* v, const float* weights
                "cache_evict: stride %d is %lld bytes, not a multiple of 16 from 0 on", i, (long long)strides[i]);
   const int64_t chunks = row_bytes / 16, moved = budget * kv_heads * chunks;
   const int64_t blocks = (moved + 255) / 256 * sequences;
-  LR_REQUIRE(moved < (1LL << 31) && blocks <= kMaxBlocks && sequences * kv_heads <= kMaxBlocks / 4,
+  const int64_t parts = size > kPart ? (size + kPart - 1) / kPart : 1;
+  LR_REQUIRE(moved < (1LL << 31) && blocks <= kMaxBlocks && sequences * kv_heads * parts <= kMaxBlocks / 4,
              "cache_evict: %lld rows of %lld caches are not supported", (long long)(budget * kv_heads),
              (long long)sequences);
+  const int64_t needs = evict_bytes(sequences, size, kv_heads);
+  LR_REQUIRE(needs == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= needs),
+             "cache_evict: needs a workspace of %lld bytes", (long long)needs);
   const EvictArgs p = {weights, key_lengths, weights_out, lengths_out, kept, static_cast<const char*>(k),
                        static_cast<const char*>(v), static_cast<char*>(k_out), static_cast<char*>(v_out), strides[0],
                        strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8],
                        strides[9], strides[10], strides[11], (int)sequences, kv_heads, (int)size, (int)budget,
-                       (int)recent, (int)capacity, (int)chunks, clear != 0};
+                       (int)recent, (int)capacity, (int)chunks, clear != 0, static_cast<uint32_t*>(workspace),
+                       (int)parts};
   hipStream_t s = as_stream(stream);
-  choose_keys<<<(unsigned)(sequences * kv_heads), kSelect, 0, s>>>(p);
+  const unsigned grid = (unsigned)(sequences * kv_heads * parts);
+  if (parts == 1) {
+    choose_keys<kWhole><<<grid, kSelect, 0, s>>>(p);
+  } else {
+    choose_keys<0><<<grid, kSelect, 0, s>>>(p);
+    if (int rc = check_launch("cache_evict")) return rc;
+    choose_keys<1><<<grid, kSelect, 0, s>>>(p);
+    if (int rc = check_launch("cache_evict")) return rc;
+    choose_keys<2><<<grid, kSelect, 0, s>>>(p);
+    if (int rc = check_launch("cache_evict")) return rc;
+    choose_keys<kPlace><<<grid, kSelect, 0, s>>>(p);
+  }
   if (int rc = check_launch("cache_evict")) return rc;
   move_rows<<<(unsigned)blocks, 256, 0, s>>>(p);
   return check_launch("cache_evict");

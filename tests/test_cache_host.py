@@ -136,13 +136,19 @@ def test_entry_point_refusals_without_a_gpu():
     assert size(64, 1, 8192, 40, 8, 128) == _lib.LR_OK and out[0] == 0
     assert size(1, 1, 1, 3, 2, 64) == _lib.LR_EINVAL
 
+    size = lambda *shape: lib.lr_cache_evict_workspace(*shape, out.buffer_info()[0])  # noqa: E731
+    assert size(4, 16384, 8) == _lib.LR_OK and out[0] == 0
+    assert size(4, 16385, 8) == _lib.LR_OK and out[0] == 3 * 4 * 8 * 2 * 2048 * 4
+    assert size(1 << 24, 1, 8) == _lib.LR_EINVAL and size(1, 1, 0) == _lib.LR_EINVAL
+
     twelve = (256, 128, 1280) * 4
     good = dict(k=p, v=p, w=p, lens=None, ko=p, vo=p, wo=p, lo=p, kept=p, n=1, size=5, heads=2, row=128, budget=3, recent=1,
-                capacity=3, st=numbers(twelve), clear=1, stream=None)
+                capacity=3, st=numbers(twelve), clear=1, ws=None, wsb=0, stream=None)
     call = lambda **kw: lib.lr_cache_evict(*{**good, **kw}.values())  # noqa: E731
     assert call(n=0) == _lib.LR_OK
     for bad in [dict(k=None), dict(w=None), dict(ko=None), dict(kept=None), dict(lo=None), dict(k=p + 8), dict(vo=p + 2),
                 dict(w=p + 1), dict(row=120), dict(row=0), dict(heads=0), dict(budget=0), dict(recent=4), dict(recent=-1),
                 dict(capacity=2), dict(n=-1), dict(n=1 << 24), dict(size=1 << 30), dict(budget=1 << 29, capacity=1 << 29),
-                dict(st=None), dict(st=numbers(twelve, 3, 136)), dict(st=numbers(twelve, 11, -16))]:
+                dict(st=None), dict(st=numbers(twelve, 3, 136)), dict(st=numbers(twelve, 11, -16)), dict(size=16385),
+                dict(size=16385, ws=p, wsb=8)]:
         assert call(**bad) == _lib.LR_EINVAL, bad

@@ -43,10 +43,11 @@ def _no_gradients(*tensors):
 
 
 @functools.lru_cache(maxsize=4096)
-def _weights_workspace(device, batch, tokens, keys, heads, kv_heads, dim):
+def _weights_workspace(device, batch, tokens, keys, heads, kv_heads, dim, causal):
     nbytes = array("q", [0])
     with torch.cuda.device(device):
-        _lib.call("lr_attention_weights_workspace", batch, tokens, keys, heads, kv_heads, dim, nbytes.buffer_info()[0])
+        _lib.call("lr_attention_weights_workspace", batch, tokens, keys, heads, kv_heads, dim, causal,
+                  nbytes.buffer_info()[0])
     return nbytes[0]
 
 
@@ -98,7 +99,7 @@ def accumulate_weights(weights, query, key, lse, *, causal=False, scale=None, ke
         query = _attention._rows(query.contiguous())
     if key.data_ptr() & 15 or not _attention._dense(key.stride(), key.shape):
         key = _attention._rows(key)
-    nbytes = _weights_workspace(query.get_device(), batch, tokens, keys, heads, kv_heads, dim)
+    nbytes = _weights_workspace(query.get_device(), batch, tokens, keys, heads, kv_heads, dim, int(bool(causal)))
     ws = _lib.workspace(query, nbytes)   # held until the launch
     strides = _six_strides((query.stride(), query.shape), (key.stride(), key.shape))
     _lib.launch(query, "lr_attention_weights", query.data_ptr(), key.data_ptr(), lse.data_ptr(), weights.data_ptr(),

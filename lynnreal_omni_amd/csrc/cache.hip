@@ -39,12 +39,17 @@ struct WeighArgs {
   int64_t qt, qh, qb, kt, kh, kb;
   const int32_t* lengths;
   int n, q_rows, k_rows, heads, kv_heads, group;
-  int causal, splits;
+  int causal, splits;     // splits: of the rows, `chunk` tiles of 64 each
+  int chunk;
   float c;                // scale * log2(e)
   Divisor by_group;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rsrc, void* lds, uint32_t voffset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)lds, 4, voffset, 0, 0, 0);
+}
 
 // Sum over the 32 lanes of a half of the wave.
 __device__ __forceinline__ float half_sum(float v) {
@@ -56,17 +61,19 @@ __device__ __forceinline__ float half_sum(float v) {
   return v + xor_partner<1>(v);
 }
 
-// Four waves with KB blocks of 32 keys each; queries in tiles of 64 rows through two slots
-// of LDS, which first hold the keys on their way to the registers. Swizzle as in lr_attention.h.
+// Four waves with KB blocks of 32 keys each; queries in tiles of 64 rows, with their sums,
+// through a ring in the LDS that first holds the keys on their way to the registers. Swizzle as
+// in lr_attention.h.
 template <typename T, int D, int KB>
 __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
   typedef typename Mfma<T>::V V8;
   constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32, KD = D / 16;
   constexpr int WAVES = 4, TILE = kKeys * ROW, DMAS = TILE / 1024 / WAVES, KEYS = 32 * WAVES * KB;
-  static_assert(KEYS * ROW >= 2 * TILE, "the keys' LDS holds two tiles of queries");
+  constexpr int RING = KEYS / kKeys, LOADS = DMAS + 1;   // slots that fit into the keys' LDS; DMAs per wave and tile
   // (One array for all of it: between two the compiler waits for every DMA before any read.)
-  __shared__ __attribute__((aligned(1024))) char smem[KEYS * (ROW + 4)];
+  __shared__ __attribute__((aligned(1024))) char smem[KEYS * (ROW + 4) + RING * WAVES * kKeys * 4];
   float* const sums = reinterpret_cast<float*>(smem + KEYS * ROW);
+  char* const lses = smem + KEYS * (ROW + 4);   // [RING][WAVES][64], each wave's own
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = lane >> 5, col = lane & 31;
   // Heads, which lie side by side, first; then sequences, so that the first keys, which
@@ -82,16 +89,17 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
   const int rows = p.q_rows * p.group;
   const int first = p.causal ? (int)min((int64_t)rows, max(0, key0 - hidden) * (int64_t)p.group) : 0;
   const int tiles = key0 < kn ? (rows - first + kKeys - 1) / kKeys : 0;
-  const int chunk = (tiles + p.splits - 1) / p.splits;
-  const int t0 = min(tiles, split * chunk), t1 = min(tiles, t0 + chunk);
+  // Splits of one size, whatever the keys' own number of rows: causal ones are then as long.
+  const int t0 = min(tiles, split * p.chunk), t1 = min(tiles, t0 + p.chunk);
   float acc[KB][16];
 #pragma unroll
   for (int b = 0; b < KB; ++b)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[b][e] = 0.0f;
   if (t0 < t1) {
-    auto publish = [&]() {
-      __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);  // vmcnt(0)
+    auto publish = [&](auto left) __attribute__((always_inline)) {   // loads that may still be on their way
+      constexpr int N = decltype(left)::value;
+      __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x70 | 0xf00);
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
@@ -112,7 +120,7 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
       for (int i = 0; i < DMAS; ++i)
         dma16(r, smem + g * TILE + (wave * DMAS + i) * 1024, (uint32_t)(slot_row(i) * p.kt * 2 + slot_chunk(i) * 16));
     }
-    publish();
+    publish(std::integral_constant<int, 0>{});
     V8 kf[KB][KD];
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
@@ -124,75 +132,109 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
     __syncthreads();   // the keys are in registers: the queries may take their place
     const uint16_t* const qbase = p.q + seq * p.qb + (int64_t)hd * p.group * p.qh;
     const float* const lbase = p.lse + (int64_t)seq * p.q_rows * p.heads + hd * p.group;
-    // Rows past the last one repeat it and are masked.
+    // Rows past the last one repeat it and are masked; tiles past the last one, which keep
+    // the count of loads the same, repeat that.
     auto issue = [&](int t) {
-      if (t >= t1) return;
-      const int r0 = first + t * kKeys, tok0 = p.by_group.of(r0);
-      char* const slot = smem + ((t - t0) & 1) * TILE;
+      const int slot = (t - t0) % RING, r0 = first + min(t, t1 - 1) * kKeys, tok0 = p.by_group.of(r0);
       const int toks = min(kKeys, p.q_rows - tok0);   // that 64 rows from r0 on can have
       const __amdgpu_buffer_rsrc_t rs =
           row_rsrc(qbase + (int64_t)tok0 * p.qt, ((toks - 1) * p.qt + (p.group - 1) * p.qh + D) * 2);
 #pragma unroll
       for (int i = 0; i < DMAS; ++i) {
         const int r = min(r0 + slot_row(i), rows - 1), tok = p.by_group.of(r);
-        dma16(rs, slot + (wave * DMAS + i) * 1024,
+        dma16(rs, smem + slot * TILE + (wave * DMAS + i) * 1024,
               (uint32_t)((tok - tok0) * p.qt * 2 + (r - tok * p.group) * p.qh * 2 + slot_chunk(i) * 16));
       }
+      const __amdgpu_buffer_rsrc_t ls =
+          row_rsrc(lbase + (int64_t)tok0 * p.heads, ((int64_t)(toks - 1) * p.heads + p.group) * 4);
+      const int r = min(r0 + lane, rows - 1), tok = p.by_group.of(r);
+      dma4(ls, lses + (slot * WAVES + wave) * kKeys * 4, (uint32_t)(((tok - tok0) * p.heads + r - tok * p.group) * 4));
     };
-    // Of the lane's row in block b of tile t: lse * log2(e), and the keys that it sees.
-    float sum[2];
-    int seen[2];
-    auto rows_of = [&](int t) __attribute__((always_inline)) {
+    // Adds a block's shares, which are those of keys past `lim` too where WHOLE. lim counts from
+    // the lane's first key on.
+    const int own = key0 + wave * KB * 32 + 4 * half;
+    auto add = [&](const v16f (&s)[KB], float l2, int lim, int x, int e, auto whole) __attribute__((always_inline)) {
+      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], p.c, -l2));
+      acc[x][e] += decltype(whole)::value || 32 * x + 8 * (e >> 2) + (e & 3) < lim ? w : 0.0f;
+    };
+    // The scores of block b of a tile, while the exponentials of the block before, which every
+    // row sees whole, run between the matrix instructions.
+    auto product = [&](v16f (&s)[KB], const char* qs, int b, const v16f (&before)[KB], float l2) __attribute__((always_inline)) {
+      constexpr int AHEAD = KD < 3 ? KD : 3;
+      V8 qf[4];
+      // (2 d + half) ^ turn, hidden so that its values for every d do not stay in registers.
+      int turn = (half ^ (col / RPB % PAIRS) * 2) * 16;
+      asm volatile("" : "+v"(turn));
+      auto read = [&](int d) __attribute__((always_inline)) {
+        return *reinterpret_cast<const V8*>(qs + (32 * b + col) * ROW + (turn ^ 32 * d));
+      };
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int r = first + t * kKeys + 32 * b + col, tok = p.by_group.of(min(r, rows - 1));
-        sum[b] = lbase[(int64_t)tok * p.heads + (min(r, rows - 1) - tok * p.group)];
-        seen[b] = r >= rows ? 0 : (p.causal ? hidden + tok + 1 : kn);
+      for (int d = 0; d < AHEAD; ++d) qf[d] = read(d);
+      const v16f zero = {};
+#pragma unroll
+      for (int d = 0; d < KD; ++d) {
+        if (d + AHEAD < KD) qf[(d + AHEAD) & 3] = read(d + AHEAD);
+#pragma unroll
+        for (int x = 0; x < KB; ++x) s[x] = Mfma<T>::mul(kf[x][d], qf[d & 3], d ? s[x] : zero);
+#pragma unroll
+        for (int i = 16 * KB * d / KD; i < 16 * KB * (d + 1) / KD; ++i) add(before, l2, 0, i / 16, i % 16, std::true_type{});
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
-    issue(t0);
-    rows_of(t0);
+    // A block without shares, for the start and behind one that was not whole.
+    v16f s0[KB] = {}, s1[KB] = {};
+    float l2 = INFINITY;   // of the block before
+    auto block = [&](v16f (&s)[KB], v16f (&before)[KB], const char* qs, int t, int b, float sum2, int lim) __attribute__((always_inline)) {
+      product(s, qs, b, before, l2);
+      l2 = sum2;
+      const int r0 = first + t * kKeys + 32 * b;
+      if (r0 + 32 <= rows && (!p.causal || hidden + p.by_group.of(r0) + 1 >= key0 + KEYS)) return;
+#pragma unroll
+      for (int x = 0; x < KB; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          add(s, l2, lim, x, e, std::false_type{});
+          s[x][e] = 0.0f;
+        }
+      l2 = INFINITY;
+    };
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) issue(t0 + i);
+#pragma unroll 1
     for (int t = t0; t < t1; ++t) {
-      const float l2[2] = {sum[0] * kLog2e, sum[1] * kLog2e};
-      const int lim[2] = {seen[0], seen[1]};
-      publish();
-      issue(t + 1);
-      if (t + 1 < t1) rows_of(t + 1);
-      const char* const qs = smem + ((t - t0) & 1) * TILE;
-      // Whether every row of the tile sees all of the workgroup's keys.
-      const int r0 = first + t * kKeys;
-      const bool whole = r0 + kKeys <= rows && (!p.causal || hidden + p.by_group.of(r0) + 1 >= key0 + KEYS);
+      publish(std::integral_constant<int, (RING - 2) * LOADS>{});   // tile t; every wave is done with tile t - 1
+      issue(t + RING - 1);
+      const int slot = (t - t0) % RING;
+      const char* const qs = smem + slot * TILE;
+      // Of the lane's row in each block: lse * log2(e), and the keys that it sees.
+      float now[2];
+      int lim[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        v16f s[KB];
+        now[b] = reinterpret_cast<const float*>(lses)[(slot * WAVES + wave) * kKeys + 32 * b + col] * kLog2e;
+        const int r = first + t * kKeys + 32 * b + col;
+        lim[b] = r >= rows ? 0 : (p.causal ? hidden + p.by_group.of(r) + 1 : kn) - own;
+      }
+      block(s0, s1, qs, t, 0, now[0], lim[0]);
+      if (first + t * kKeys + 32 >= rows) {   // the last tile, without a second block
 #pragma unroll
         for (int x = 0; x < KB; ++x)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[x][e] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < KD; ++d) {
-          const V8 qf = *reinterpret_cast<const V8*>(qs + (32 * b + col) * ROW + ((2 * d + half) ^ (col / RPB % PAIRS) * 2) * 16);
-#pragma unroll
-          for (int x = 0; x < KB; ++x) s[x] = Mfma<T>::mul(kf[x][d], qf, s[x]);
-        }
-        if (whole) {
-#pragma unroll
-          for (int x = 0; x < KB; ++x)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[x][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], p.c, -l2[b]));
-        } else {
-#pragma unroll
-          for (int x = 0; x < KB; ++x)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int key = key0 + (wave * KB + x) * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-              const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], p.c, -l2[b]));
-              acc[x][e] += key < lim[b] ? w : 0.0f;
-            }
-        }
+          for (int e = 0; e < 16; ++e) {
+            add(s0, l2, 0, x, e, std::true_type{});
+            s1[x][e] = 0.0f;
+          }
+        l2 = INFINITY;
+        break;
       }
+      block(s1, s0, qs, t, 1, now[1], lim[1]);
     }
+#pragma unroll
+    for (int x = 0; x < KB; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) add(s1, l2, 0, x, e, std::true_type{});
   }
+  __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);   // the last DMAs have landed before the LDS goes to another
 #pragma unroll
   for (int x = 0; x < KB; ++x)
 #pragma unroll
@@ -459,21 +501,28 @@ __global__ __launch_bounds__(256) void move_rows(EvictArgs p) {
 }
 
 struct WeighPlan {
-  int blocks, splits;   // of 32 keys per wave; of the rows
+  int blocks, splits, chunk;   // of 32 keys per wave; of the rows, and their tiles
   int64_t grid;
 };
 
-WeighPlan weigh_plan(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int kv_heads) {
+WeighPlan weigh_plan(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, bool causal) {
   WeighPlan pl;
-  const int64_t rows = q_rows * (heads / kv_heads), tiles = (rows + kKeys - 1) / kKeys;
-  // 64 keys per wave halve what the queries' fragments take of the LDS; with a tile or two
-  // of them the keys' stream counts, and smaller workgroups.
-  pl.blocks = tiles > 2 ? 2 : 1;
-  const int64_t groups = n * kv_heads * ((k_rows + 128 * pl.blocks - 1) / (128 * pl.blocks));
-  // Rows are split while that leaves two tiles and more to each of two workgroups per CU.
-  int64_t s = groups > 0 ? 2 * compute_units() / groups : 1;
-  if (s > tiles / 2) s = tiles / 2;
-  pl.splits = s < 1 ? 1 : (s > 64 ? 64 : (int)s);
+  const int64_t rows = q_rows * (heads / kv_heads), tiles = (rows + kKeys - 1) / kKeys, cus = compute_units();
+  auto groups_of = [&](int blocks) { return n * kv_heads * ((k_rows + 128 * blocks - 1) / (128 * blocks)); };
+  // 64 keys per wave halve what the queries' fragments take of the LDS. With a tile or two of
+  // queries the keys' stream counts, and smaller workgroups; so with too few to fill the GPU.
+  pl.blocks = tiles > 2 && groups_of(2) * ((tiles + 3) / 4) >= cus ? 2 : 1;
+  const int64_t groups = groups_of(pl.blocks);
+  // Rows are split, in runs of four tiles and more, for four workgroups per CU, of which two
+  // are resident; where causal, half of the runs have no rows and the others differ, for twelve
+  // (3683 tokens, 40 heads over 8: 153 us with twelve, 183 with four; all keys 179 with
+  // four, 200 with twelve).
+  int64_t s = groups > 0 ? (causal ? 12 : 4) * cus / groups : 1;
+  if (s > tiles / 4) s = tiles / 4;
+  if (s < 1) s = 1;
+  if (s > 64) s = 64;
+  pl.chunk = (int)((tiles + s - 1) / s);
+  pl.splits = pl.chunk > 0 ? (int)((tiles + pl.chunk - 1) / pl.chunk) : 1;
   pl.grid = groups * pl.splits;
   return pl;
 }
@@ -512,10 +561,10 @@ int check_weigh(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int kv_hea
 using namespace lr;
 
 extern "C" int lr_attention_weights_workspace(int64_t sequences, int64_t q_rows, int64_t k_rows, int heads, int kv_heads,
-                                              int head_dim, int64_t* bytes) {
+                                              int head_dim, int causal, int64_t* bytes) {
   if (int rc = check_weigh(sequences, q_rows, k_rows, heads, kv_heads, head_dim)) return rc;
   LR_REQUIRE(bytes, "attention_weights: null pointer");
-  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads);
+  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads, causal != 0);
   *bytes = pl.splits > 1 ? pl.splits * sequences * kv_heads * k_rows * 4 : 0;
   return LR_OK;
 }
@@ -541,11 +590,11 @@ extern "C" int lr_attention_weights(const void* q, const void* k, const float* l
   float scale;
   static_assert(sizeof scale == sizeof scale_bits, "fp32");
   __builtin_memcpy(&scale, &scale_bits, sizeof scale);
-  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads);
+  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads, causal != 0);
   const WeighArgs p = {static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), lse, weights, out,
                        static_cast<float*>(workspace), strides[0], strides[1], strides[2], strides[3], strides[4],
                        strides[5], key_lengths, (int)sequences, (int)q_rows, (int)k_rows, heads, kv_heads, group,
-                       causal != 0, pl.splits, scale * 1.4426950408889634f, Divisor((uint32_t)group)};
+                       causal != 0, pl.splits, pl.chunk, scale * 1.4426950408889634f, Divisor((uint32_t)group)};
   LR_REQUIRE(p.c > 0.0f && isfinite(p.c), "attention_weights: the scale must be positive and finite");
   const int64_t all = sequences * kv_heads * k_rows;
   LR_REQUIRE(pl.grid <= kMaxBlocks && (pl.splits == 1 || all <= kMaxBlocks * 256),

@@ -43,6 +43,7 @@ struct PrefixArgs {
   int shares;            // most pieces of the prefix
   int own;               // most pieces of the own caches
   int piece;             // least tiles of 64 keys of a piece
+  int whole, left, cuts; // walk: workgroups for all keys of their rows; those cut into `cuts`
 };
 
 __device__ __forceinline__ int own_keys(const PrefixArgs& p, int i) {
@@ -54,12 +55,13 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (int)((uint32_t)(
 // How prefix and caches are cut: pieces of `size` tiles of 64 keys, the smallest for
 // which all of them have a place. Every wave works it out from the lengths by itself.
 struct Cut {
-  int size, prefix;     // tiles of a piece; pieces of the prefix
+  int size, shared, prefix;   // tiles of a piece of a cache, and of the prefix; pieces of that one
   int mine[kListed / 64];   // key tiles of sequences lane, lane + 64, ..
   int groups;
   __device__ __forceinline__ explicit Cut(const PrefixArgs& p) {
     const int lane = threadIdx.x & 63, tiles = key_tiles(p.prefix);
-    size = max(p.piece, ceil_div(tiles, p.shares));
+    auto shared_of = [&](int size) __attribute__((always_inline)) { return max(size, ceil_div(tiles, p.shares)); };
+    size = p.piece;
     groups = 0;
     if (p.places) {
       groups = (p.n + 63) >> 6;
@@ -74,7 +76,7 @@ struct Cut {
 #pragma unroll
         for (int g = 0; g < kListed / 64; ++g)
           if (g < groups) sum += (float)ceil_div(mine[g], size);
-        sum = wave_tree_sum(sum) * (float)p.seq_tiles + (float)(ceil_div(tiles, size) * p.all_tiles);
+        sum = wave_tree_sum(sum) * (float)p.seq_tiles + (float)(ceil_div(tiles, shared_of(size)) * p.all_tiles);
         // The same in every lane; said so, since what depends on it addresses memory.
         return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sum)));
       };
@@ -84,17 +86,16 @@ struct Cut {
       while (taken(size) > (float)p.places) size += max(1, size >> 4);
     }
     size = __builtin_amdgcn_readfirstlane(size);
-    prefix = ceil_div(tiles, size);
+    shared = max(1, __builtin_amdgcn_readfirstlane(shared_of(size)));
+    prefix = ceil_div(tiles, shared);
   }
-  // Of sequence `want`, or where that is -1 the one that has piece `place` of the caches
-  // (-1: there is none): its number, its first piece and how many there are.
-  __device__ __forceinline__ void find(const PrefixArgs& p, int want, int place, int& seq, int& first, int& count) const {
+  // What has piece `place` of the caches: the sequence (-1: none) and its first piece.
+  __device__ __forceinline__ void find(const PrefixArgs& p, int place, int& seq, int& first) const {
     const int lane = threadIdx.x & 63;
     seq = -1;
     if (!p.places) {   // a piece each
-      seq = want >= 0 ? want : (place < p.n ? place : -1);
+      seq = place < p.n ? place : -1;
       first = seq;
-      count = seq >= 0 && own_keys(p, seq) > 0;
       return;
     }
     int before = 0;
@@ -103,16 +104,32 @@ struct Cut {
       if (g >= groups || seq >= 0) continue;
       const int n = ceil_div(mine[g], size);
       const int upto = wave_prefix_sum(n);
-      const bool here = want >= 0 ? 64 * g + lane == want : (before + upto > place && 64 * g + lane < p.n);
-      const uint64_t hit = __ballot(here);
+      const uint64_t hit = __ballot(before + upto > place && 64 * g + lane < p.n);
       if (hit) {
         const int l = __builtin_ctzll(hit);
         seq = 64 * g + l;
-        count = __builtin_amdgcn_readlane(n, l);
-        first = before + __builtin_amdgcn_readlane(upto, l) - count;
+        first = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
       }
       before += __builtin_amdgcn_readlane(upto, 63);
     }
+  }
+  // Each sequence's first piece and how many there are, and behind them the pieces of the prefix,
+  // by one wave for the kernel that joins them.
+  __device__ __forceinline__ void publish(const PrefixArgs& p, int2* table) const {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    if (p.places) {
+#pragma unroll
+      for (int g = 0; g < kListed / 64; ++g) {
+        if (g >= groups) continue;
+        const int n = ceil_div(mine[g], size), upto = wave_prefix_sum(n);
+        if (64 * g + lane < p.n) table[64 * g + lane] = make_int2(before + upto - n, n);
+        before += __builtin_amdgcn_readlane(upto, 63);
+      }
+    } else {
+      for (int i = lane; i < p.n; i += 64) table[i] = make_int2(i, own_keys(p, i) > 0);
+    }
+    if (lane == 0) table[p.n] = make_int2(prefix, 0);
   }
 };
 
@@ -122,6 +139,11 @@ __device__ __forceinline__ int64_t own_part(const PrefixArgs& p, int piece) {
   return ((int64_t)p.shares * p.n + piece) * each;
 }
 __device__ __forceinline__ int64_t all_parts(const PrefixArgs& p) { return own_part(p, p.own); }
+// Behind the parts: which pieces a sequence has (Cut::publish).
+template <int D>
+__device__ __forceinline__ int2* pieces_of(const PrefixArgs& p) {
+  return reinterpret_cast<int2*>(p.part + all_parts(p) * (D + 4));
+}
 
 // A sequence's rows 128 * tile .. and the own keys that they see.
 struct OwnRows {
@@ -167,6 +189,7 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
   // All key heads of the same keys, which lie side by side, come first.
   const int hds = p.kv_heads, item = (int)(blockIdx.x / (uint32_t)hds), hd = (int)(blockIdx.x - item * hds);
   const Cut cut(p);
+  if (blockIdx.x == 0 && wave == 0) cut.publish(p, pieces_of<D>(p));
   OneCache keys;
   int t0, t1, rows, r0;
   int64_t part, qoff;
@@ -180,14 +203,14 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
     const int seq = (int)((uint32_t)row.tok / (uint32_t)p.q_rows);
     qoff = seq * p.qb + (row.tok - seq * p.q_rows) * p.qt + row.head * p.qh;
     keys = prefix_cache(p, hd);
-    t0 = piece * cut.size;
-    t1 = min(key_tiles(p.prefix), t0 + cut.size);
+    t0 = piece * cut.shared;
+    t1 = min(key_tiles(p.prefix), t0 + cut.shared);
     part = ((int64_t)piece * p.n * p.q_rows + row.tok) * p.heads + row.head;
     sees = true;
   } else {
     const int place = item - cut.prefix * p.all_tiles, piece = (int)((uint32_t)place / (uint32_t)p.seq_tiles);
-    int seq, first, count;
-    cut.find(p, -1, piece, seq, first, count);
+    int seq, first;
+    cut.find(p, piece, seq, first);
     if (seq < 0) return;
     const OwnRows w(p, seq, place - piece * p.seq_tiles);
     rows = w.rows;
@@ -221,33 +244,23 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
 }
 
 constexpr float kLn2 = 0.69314718055994531f;
+constexpr int kMaxParts = 2 * kMaxPieces;
 
-// Joins the pieces of a row: weights 2^(exponent - the largest). A workgroup per row: D / 4
-// threads hold a piece's columns, and the groups of them take every G-th piece, then are
-// added in order, so that the result does not depend on timing.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void prefix_join(PrefixArgs p) {
-  constexpr int LANES = D / 4, G = 256 / LANES, NV = 2 * kMaxPieces / 64;
-  __shared__ float weight[2 * kMaxPieces];
+// Joins the parts of a row, at(0) .. at(n - 1): weights 2^(exponent - the largest). A workgroup
+// per row: D / 4 threads hold a part's columns, and the groups of them take every G-th part,
+// then are added in order, so that the result does not depend on timing.
+template <typename T, int D, class At>
+__device__ __forceinline__ void join_row(const float* part, const float4* stats, int n, const At& at, uint16_t* out, float* lse) {
+  constexpr int LANES = D / 4, G = 256 / LANES, NV = kMaxParts / 64;
+  __shared__ float weight[kMaxParts];
   __shared__ float4 sums[G][LANES];
-  const int64_t row = blockIdx.x;
-  const int each = p.q_rows * p.heads, seq = (int)(blockIdx.x / (uint32_t)each);
-  const Cut cut(p);
-  int found, first, count;
-  cut.find(p, seq, 0, found, first, count);
-  const int parts = cut.prefix + count;
-  const int64_t own = own_part(p, first) + (row - (int64_t)seq * each);
-  auto at = [&](int i) __attribute__((always_inline)) {
-    return i < cut.prefix ? row + (int64_t)i * p.n * each : own + (int64_t)(i - cut.prefix) * each;
-  };
-  const float4* const stats = reinterpret_cast<const float4*>(p.part + all_parts(p) * D);
   const int t = threadIdx.x, lane = t & 63, x = t % LANES, g = t / LANES;
   // Every wave finds the maximum and the sums by itself.
   float4 v[NV];
   float top = -INFINITY, seen = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    v[i] = 64 * i + lane < parts ? stats[at(64 * i + lane)] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    v[i] = 64 * i + lane < n ? stats[at(64 * i + lane)] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (v[i].y != 0.0f) top = fmaxf(top, v[i].x);
     seen = fmaxf(seen, v[i].w);
   }
@@ -266,15 +279,15 @@ __global__ __launch_bounds__(256) void prefix_join(PrefixArgs p) {
   __syncthreads();
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   constexpr int BATCH = 4;   // loads in flight
-  for (int s0 = g; s0 < parts; s0 += BATCH * G) {
+  for (int s0 = g; s0 < n; s0 += BATCH * G) {
     float4 y[BATCH];
 #pragma unroll
     for (int i = 0; i < BATCH; ++i)
-      if (s0 + i * G < parts) y[i] = *reinterpret_cast<const float4*>(p.part + at(s0 + i * G) * D + 4 * x);
+      if (s0 + i * G < n) y[i] = *reinterpret_cast<const float4*>(part + at(s0 + i * G) * D + 4 * x);
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
-      const float w = s0 + i * G < parts ? weight[s0 + i * G] : 0.0f;
-      if (w == 0.0f) continue;   // y was not written where the piece had no keys
+      const float w = s0 + i * G < n ? weight[s0 + i * G] : 0.0f;
+      if (w == 0.0f) continue;   // y was not written where the part had no keys
       o.x += w * y[i].x;
       o.y += w * y[i].y;
       o.z += w * y[i].z;
@@ -293,9 +306,24 @@ __global__ __launch_bounds__(256) void prefix_join(PrefixArgs p) {
     o.w += y.w;
   }
   const float inv = l == 0.0f ? (seen != 0.0f ? NAN : 0.0f) : 1.0f / l;
-  *reinterpret_cast<uint2*>(p.out + row * D + 4 * x) =
+  *reinterpret_cast<uint2*>(out + 4 * x) =
       make_uint2(Mfma<T>::pack(o.x * inv, o.y * inv), Mfma<T>::pack(o.z * inv, o.w * inv));
-  if (p.lse && x == 0) p.lse[row] = l == 0.0f ? -INFINITY : kLn2 * (top + __builtin_amdgcn_logf(exact));
+  if (lse && x == 0) *lse = l == 0.0f ? -INFINITY : kLn2 * (top + __builtin_amdgcn_logf(exact));
+}
+
+// A row's pieces of the prefix and of its cache.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_join(PrefixArgs p) {
+  const int64_t row = blockIdx.x;
+  const int each = p.q_rows * p.heads, seq = (int)(blockIdx.x / (uint32_t)each);
+  const int2 mine = pieces_of<D>(p)[seq];
+  const int shared = pieces_of<D>(p)[p.n].x;
+  const int64_t own = own_part(p, mine.x) + (row - (int64_t)seq * each);
+  auto at = [&](int i) __attribute__((always_inline)) {
+    return i < shared ? row + (int64_t)i * p.n * each : own + (int64_t)(i - shared) * each;
+  };
+  join_row<T, D>(p.part, reinterpret_cast<const float4*>(p.part + all_parts(p) * D), shared + mine.y, at, p.out + row * D,
+                 p.lse ? p.lse + row : nullptr);
 }
 
 // The prefix, then the own cache. (Both sides of a choice are values: chosen between by
@@ -315,9 +343,23 @@ struct TwoCaches {
   __device__ __forceinline__ bool whole(int t) const { return first(t) + kKeys <= (int)either(t < tiles, a.sure, b.sure); }
   __device__ __forceinline__ int first(int t) const { return (t < tiles ? t : t - tiles) * kKeys; }
   __device__ __forceinline__ int limit(int t) const { return (int)either(t < tiles, a.seen, b.seen); }
-  __device__ __forceinline__ bool turns(int t) const { return t == tiles; }
+  static constexpr bool kOneStride = false;
 };
 
+// What a workgroup of the walk has: a head's rows, of a sequence.
+struct WalkItem {
+  int hd, seq, tile;
+  __device__ __forceinline__ WalkItem(const PrefixArgs& p, uint32_t id) {
+    const uint32_t tiles = (uint32_t)(p.n * p.seq_tiles);
+    hd = (int)(id / tiles);
+    const int at = (int)(id - hd * tiles);
+    seq = (int)((uint32_t)at / (uint32_t)p.seq_tiles);
+    tile = at - seq * p.seq_tiles;
+  }
+};
+
+// The first `whole` workgroups walk all keys of their rows. Those that would be left for a round
+// of their own are cut into `cuts` runs of keys instead, joined by a second kernel.
 template <typename T, int D, bool LSE>
 __global__ __launch_bounds__(256, 2) void prefix_walk(PrefixArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[kTileBytes<D>];
@@ -325,27 +367,43 @@ __global__ __launch_bounds__(256, 2) void prefix_walk(PrefixArgs p) {
   const int half = lane >> 5, col = lane & 31;
   // Each XCD takes a contiguous run of the heads' tiles, so that its L2 serves a head's
   // prefix to them all.
-  const uint32_t total = gridDim.x, pid = blockIdx.x, per = total >> 3, rest = total & 7, xcd = pid & 7;
-  const uint32_t id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3);
-  const uint32_t tiles = (uint32_t)(p.n * p.seq_tiles);
-  const int hd = (int)(id / tiles), at = (int)(id - hd * tiles);
-  const int seq = (int)((uint32_t)at / (uint32_t)p.seq_tiles);
-  const OwnRows w(p, seq, at - seq * p.seq_tiles);
+  const uint32_t whole = (uint32_t)p.whole, pid = blockIdx.x, per = whole >> 3, rest = whole & 7, xcd = pid & 7;
+  const bool cut = pid >= whole;
+  const uint32_t run = cut ? (pid - whole) / (uint32_t)p.cuts : 0, piece = cut ? pid - whole - run * p.cuts : 0;
+  const WalkItem it(p, cut ? whole + run
+                           : (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (pid >> 3));
+  const OwnRows w(p, it.seq, it.tile);
   const int r = w.r0 + wave * 32 + col;
-  const Row row(p, r, w.rows, hd, w.kn);
-  const TwoCaches keys = {prefix_cache(p, hd), own_cache(p, seq, hd, w, row.seen), key_tiles(p.prefix)};
-  const uint16_t* const q = p.q + seq * p.qb + row.tok * p.qt + row.head * p.qh;
+  const Row row(p, r, w.rows, it.hd, w.kn);
+  const TwoCaches keys = {prefix_cache(p, it.hd), own_cache(p, it.seq, it.hd, w, row.seen), key_tiles(p.prefix)};
+  const uint16_t* const q = p.q + it.seq * p.qb + row.tok * p.qt + row.head * p.qh;
   v16f o[D / 32];
   float m, l, exact, off;
   const bool idle = w.r0 + wave * 32 >= w.rows;
-  const int t1 = keys.tiles + w.tiles;
-  attend<T, D, false, LSE>(smem, keys, q, p.c, 0, t1, idle, m, l, exact, off, o);
+  const int tiles = keys.tiles + w.tiles, size = cut ? ceil_div(tiles, p.cuts) : tiles;
+  const int t0 = min(tiles, (int)piece * size), t1 = min(tiles, t0 + size);
+  attend<T, D, false, LSE>(smem, keys, q, p.c, t0, t1, idle, m, l, exact, off, o);
   l = add_partner(l);
   if (LSE) exact = add_partner(exact);
   if (r >= w.rows) return;
-  const int64_t to = ((int64_t)seq * p.q_rows + row.tok) * p.heads + row.head;
+  const bool sees = p.prefix + row.seen > 0;
+  if (cut) {
+    const int64_t part = ((int64_t)run * p.cuts + piece) * kRows + wave * 32 + col;
+    const int64_t parts = (int64_t)p.left * p.cuts * kRows;
+    if (half == 0) reinterpret_cast<float4*>(p.part + parts * D)[part] = make_float4(off, l, LSE ? exact : l, sees);
+    if (l == 0.0f) return;   // left out of the join by its l
+    float* const po = p.part + part * D;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(po + 32 * d + 8 * g + 4 * half) =
+            make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    return;
+  }
+  const int64_t to = ((int64_t)it.seq * p.q_rows + row.tok) * p.heads + row.head;
   if (LSE && half == 0) p.lse[to] = l == 0.0f ? -INFINITY : kLn2 * (off + __builtin_amdgcn_logf(exact));
-  const float inv = l == 0.0f ? (p.prefix + row.seen > 0 ? NAN : 0.0f) : 1.0f / l;
+  const float inv = l == 0.0f ? (sees ? NAN : 0.0f) : 1.0f / l;
   uint16_t* const po = p.out + to * D;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
@@ -356,12 +414,31 @@ __global__ __launch_bounds__(256, 2) void prefix_walk(PrefixArgs p) {
                      Mfma<T>::pack(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
 }
 
+// The cut workgroups' rows.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void walk_join(PrefixArgs p) {
+  const int run = (int)(blockIdx.x / kRows), at0 = (int)(blockIdx.x % kRows);
+  const WalkItem it(p, (uint32_t)(p.whole + run));
+  const int rows = p.q_rows * p.group, r = it.tile * kRows + at0;
+  if (r >= rows) return;
+  const Row row(p, r, rows, it.hd, 0);
+  const int64_t to = ((int64_t)it.seq * p.q_rows + row.tok) * p.heads + row.head;
+  const int64_t parts = (int64_t)p.left * p.cuts * kRows;
+  auto at = [&](int i) __attribute__((always_inline)) { return ((int64_t)run * p.cuts + i) * kRows + at0; };
+  join_row<T, D>(p.part, reinterpret_cast<const float4*>(p.part + parts * D), p.cuts, at, p.out + to * D,
+                 p.lse ? p.lse + to : nullptr);
+}
+
 // How a call is laid over the GPU.
 struct Plan {
   bool walk;
   int64_t seq_tiles, all_tiles;
   int places, shares, own, piece;
+  int64_t whole, left;
+  int cuts;
   int64_t parts;   // rows of partial results
+  int64_t table;   // sequences that have a line behind them
+  int64_t bytes(int dim) const { return parts * (dim + 4) * 4 + table * 8; }
 };
 
 Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, int kv_heads) {
@@ -371,10 +448,12 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, 
   pl.seq_tiles = (q_rows * group + kRows - 1) / kRows;
   pl.all_tiles = (n * q_rows * group + kRows - 1) / kRows;
   const double tiles_p = (double)((prefix + kKeys - 1) / kKeys), tiles_k = (double)((k_rows + kKeys - 1) / kKeys);
-  // Two workgroups per CU, for the stream of keys.
-  int64_t places = 2 * cus / kv_heads;
-  const int64_t least = 2 * (pl.all_tiles + pl.seq_tiles * n);
-  if (places < least) places = least;
+  // Two workgroups per CU are resident: as many full rounds of them as leave pieces to choose
+  // beside the one that each cache and each of the prefix's row tiles takes (one token of 64
+  // sequences, 4096 shared keys, 512 own at most, 40 heads over 8: 42 us in two rounds, 94 in
+  // one; of 16 over 131072 shared ones 145 in one, 159 in two).
+  const int64_t least = pl.all_tiles + pl.seq_tiles * n, round = 2 * cus / kv_heads > 0 ? 2 * cus / kv_heads : 1;
+  const int64_t places = (least * 7 / 5 + round - 1) / round * round;
   // The most pieces of the prefix, and the least tiles of one, by the cost of joining: 1 us per
   // tile of keys against 0.15 ns per row and piece, as in attention.hip.
   const double s = fmin(fmin(sqrt(tiles_p / (0.00015 * (double)rows)), (double)(places / pl.all_tiles)), kMaxPieces);
@@ -385,20 +464,35 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, 
   pl.places = n > kListed ? 0 : (int)places;
   pl.own = (int)(n > kListed ? n : places / pl.seq_tiles);
   pl.parts = (pl.shares * n + pl.own) * q_rows * heads;
+  pl.table = n + 1;
   const double walk = fmax(1.0, (double)(n * pl.seq_tiles * kv_heads) / (double)cus) * (tiles_p + tiles_k);
   const double pieces = ((double)pl.all_tiles * tiles_p + (double)(n * pl.seq_tiles) * tiles_k) * kv_heads / (double)cus +
                         2.8 + (double)rows * (0.0006 + 0.00015 * pl.shares);
   pl.walk = walk <= pieces || rows > kMaxBlocks;
+  if (pl.walk) {
+    // Two workgroups per CU are resident. What is left behind full rounds is cut so that it fills
+    // the GPU once more, for a part of a round (8 at most, for what is written and read again).
+    const int64_t items = n * pl.seq_tiles * kv_heads, slots = 2 * cus, left = items % slots;
+    const int64_t cuts = left > 0 ? slots / left : 1;
+    pl.cuts = cuts > 8 ? 8 : (int)cuts;
+    pl.left = pl.cuts > 1 ? left : 0;
+    pl.whole = items - pl.left;
+    pl.parts = pl.left * pl.cuts * kRows;
+    pl.table = 0;
+  }
   return pl;
 }
 
 template <typename T, int D>
 int launch(const PrefixArgs& p, const Plan& pl, hipStream_t s) {
   if (pl.walk) {
-    const int64_t grid = p.n * pl.seq_tiles * p.kv_heads;
+    const int64_t grid = pl.whole + pl.left * pl.cuts;
     LR_REQUIRE(grid <= kMaxBlocks, "attention_prefix: %lld workgroups are not supported", (long long)grid);
     if (p.lse) prefix_walk<T, D, true><<<(unsigned)grid, 256, 0, s>>>(p);
     else prefix_walk<T, D, false><<<(unsigned)grid, 256, 0, s>>>(p);
+    if (int rc = check_launch("attention_prefix")) return rc;
+    if (pl.left == 0) return LR_OK;
+    walk_join<T, D><<<(unsigned)(pl.left * kRows), 256, 0, s>>>(p);
     return check_launch("attention_prefix");
   }
   const int64_t grid = (p.places ? p.places : pl.shares * pl.all_tiles + p.n * pl.seq_tiles) * p.kv_heads;
@@ -441,7 +535,7 @@ extern "C" int lr_attention_prefix_workspace(int64_t sequences, int64_t q_rows, 
   *bytes = 0;
   if (sequences == 0 || q_rows == 0) return LR_OK;
   const Plan pl = plan(sequences, q_rows, k_rows, prefix_rows, heads, kv_heads);
-  if (!pl.walk) *bytes = pl.parts * (head_dim + 4) * 4;
+  *bytes = pl.bytes(head_dim);
   return LR_OK;
 }
 
@@ -499,9 +593,12 @@ extern "C" int lr_attention_prefix(const void* q, const void* prefix_k, const vo
   p.shares = pl.shares;
   p.own = pl.own;
   p.piece = pl.piece;
-  if (!pl.walk)
-    LR_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= pl.parts * (head_dim + 4) * 4,
-               "attention_prefix: needs a workspace of %lld bytes", (long long)(pl.parts * (head_dim + 4) * 4));
+  p.whole = (int)pl.whole;
+  p.left = (int)pl.left;
+  p.cuts = pl.cuts;
+  if (pl.bytes(head_dim))
+    LR_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= pl.bytes(head_dim),
+               "attention_prefix: needs a workspace of %lld bytes", (long long)pl.bytes(head_dim));
   hipStream_t s = as_stream(stream);
   return dtype == LR_DTYPE_BF16 ? by_dim<__bf16>(p, head_dim, pl, s) : by_dim<_Float16>(p, head_dim, pl, s);
 }

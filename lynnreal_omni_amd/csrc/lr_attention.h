@@ -123,7 +123,7 @@ struct OneCache {
   __device__ __forceinline__ bool whole(int t) const { return (t + 1) * kKeys <= sure; }
   __device__ __forceinline__ int first(int t) const { return t * kKeys; }   // key of tile t
   __device__ __forceinline__ int limit(int) const { return seen; }          // keys that the row sees, counted as first() does
-  __device__ __forceinline__ bool turns(int) const { return false; }                   // whether strides change at tile t
+  static constexpr bool kOneStride = true;   // whether all tiles have the strides of the first
 };
 
 template <int D>
@@ -187,25 +187,28 @@ __device__ __forceinline__ void attend(char* smem, const Keys& keys, const uint1
 
   // DMA i of this wave: 1 KB of the tile's rows.
   uint32_t koff[DMAS], voff[DMAS];
-  auto place = [&](uint32_t (&to)[DMAS], int64_t stride) __attribute__((always_inline)) {
+  auto offset = [&](int i, uint32_t stride) __attribute__((always_inline)) {
+    const int at = (wave * DMAS + i) * 64 + lane;  // 16-byte slot of the tile
+    const int row = at / CH, ch = at % CH ^ (row / RPB % PAIRS) * 2;
+    return (uint32_t)row * stride * 2 + ch * 16;
+  };
+  if constexpr (Keys::kOneStride) {
 #pragma unroll
     for (int i = 0; i < DMAS; ++i) {
-      const int at = (wave * DMAS + i) * 64 + lane;  // 16-byte slot of the tile
-      const int row = at / CH, ch = at % CH ^ (row / RPB % PAIRS) * 2;
-      to[i] = (uint32_t)(row * stride * 2 + ch * 16);
+      koff[i] = offset(i, (uint32_t)keys.stride(t0, 0));
+      voff[i] = offset(i, (uint32_t)keys.stride(t0, 1));
     }
-  };
-  place(koff, keys.stride(t0, 0));
-  place(voff, keys.stride(t0, 1));
+  }
   auto issue = [&](int t, int v) {
     if (t >= t1) return;
     char* const slot = smem + ((t - t0) & 1) * SLOT + v * TILE;
     const int left = min(kKeys, keys.left(t));  // rows past the last key read as zero
     const int64_t stride = keys.stride(t, v);
-    if (keys.turns(t)) place(v ? voff : koff, stride);
     const __amdgpu_buffer_rsrc_t r = row_rsrc(keys.at(t, v), ((int64_t)(left - 1) * stride + D) * 2);
 #pragma unroll
-    for (int i = 0; i < DMAS; ++i) dma16(r, slot + (wave * DMAS + i) * 1024, v ? voff[i] : koff[i]);
+    for (int i = 0; i < DMAS; ++i)
+      dma16(r, slot + (wave * DMAS + i) * 1024,
+            Keys::kOneStride ? (v ? voff[i] : koff[i]) : offset(i, (uint32_t)stride));
   };
 
   v16f s0[2], s1[2];

@@ -68,7 +68,7 @@ CASES = [
     (2, 4, 4097, 300, 16, 2, 128, [300, 4]), (5, 1, 20000, 1000, 5, 1, 128, [1000, 1, 0, 64, 65]),
     (2, 33, 129, 100, 2, 2, 64, [33, 100]), (2, 130, 300, 257, 3, 1, 32, [257, 140]), (3, 200, 63, 200, 4, 4, 128, None),
     (1, 300, 64, 700, 2, 1, 64, None), (8, 40, 500, 64, 14, 2, 128, [40 + i for i in range(8)]),
-    (2, 513, 1025, 513, 2, 2, 128, None), (1, 5, 70000, 10, 4, 4, 64, None),
+    (2, 513, 1025, 513, 2, 2, 128, None), (8, 1100, 70, 1100, 8, 8, 32, [1100 - i for i in range(8)]), (1, 5, 70000, 10, 4, 4, 64, None),
 ]
 
 

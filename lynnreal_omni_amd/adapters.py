@@ -75,16 +75,13 @@ def _workspace(device, tokens, n, k, rank, adapters):
     return nbytes[0]
 
 
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _readable(rows):
-    """Whether the kernel reads rows as they are: dense ones, 16-byte aligned, that are one or
-    do not overlap."""
-    step = _row_stride(rows)
-    return (not rows.data_ptr() & 15 and (rows.stride(1) == 1 or rows.shape[1] == 1) and not step % 8
-            and step < 1 << 30 and (step >= rows.shape[1] or step == 0))
+@functools.lru_cache(maxsize=4096)
+def _row_step(stride, rows, width):
+    """Elements from one row of x to the next as the kernel reads them: dense rows, 16 bytes
+    apart or a multiple, that are one or do not overlap; None where they are not so."""
+    step = stride[0] if rows > 1 else width
+    dense = stride[1] == 1 or width == 1
+    return step if dense and not step % 8 and step < 1 << 30 and (step >= width or step == 0) else None
 
 
 class LowRankAdapters(nn.Module):
@@ -129,9 +126,10 @@ class LowRankAdapters(nn.Module):
     def forward(self, x, base, plan, *, out=None):
         """base [.., out_features] plus the adapters' products with x [.., in_features], a new
         tensor like base, or `out`, contiguous, which may be base."""
-        if x.shape[-1] != self.in_features or base.shape != (*x.shape[:-1], self.out_features):
+        x_shape, base_shape = x.shape, base.shape
+        if x_shape[-1] != self.in_features or base_shape[-1] != self.out_features or x_shape[:-1] != base_shape[:-1]:
             raise ValueError(f"expected x [.., {self.in_features}] and base [.., {self.out_features}], "
-                             f"got {tuple(x.shape)} and {tuple(base.shape)}")
+                             f"got {tuple(x_shape)} and {tuple(base_shape)}")
         buffers = self._buffers
         down, up, scale = buffers["down"], buffers["up"], buffers["scale"]
         if x.dtype != down.dtype or base.dtype != down.dtype or up.dtype != down.dtype or scale.dtype != torch.float32:
@@ -153,20 +151,24 @@ class LowRankAdapters(nn.Module):
                 raise ValueError("out must be base itself or memory of its own")
         _lib.check_device(x)
         _lib.same_device(x, base=base, down=down, plan=plan.order, out=out)
-        rows = x if x.dim() == 2 else x.reshape(tokens, self.in_features)
-        onto = base if base.dim() == 2 else base.reshape(tokens, self.out_features)
+        rows = x if len(x_shape) == 2 else x.reshape(tokens, self.in_features)
+        onto = base if len(base_shape) == 2 else base.reshape(tokens, self.out_features)
         if self.in_features % 8:
             rows = nn.functional.pad(rows, (0, -self.in_features % 8))
-        if tokens and not _readable(rows):
+        x_step = _row_step(rows.stride(), tokens, rows.shape[1])
+        if x_step is None or rows.data_ptr() & 15:
             rows = rows.clone(memory_format=torch.contiguous_format)
-        if onto.stride(1) != 1 and onto.shape[1] > 1:
+            x_step = rows.shape[1]
+        base_step, column = onto.stride()
+        if column != 1 and self.out_features > 1:
             onto = onto.contiguous()
+            base_step = self.out_features
         if out is None:
-            out = base.new_empty(base.shape)
+            out = base.new_empty(base_shape)
         nbytes = _workspace(x.get_device(), tokens, self.out_features, self.in_features, self.rank, self.adapters)
-        ws = _lib.workspace(x, nbytes)   # held until the launch
-        _lib.launch(x, "lr_adapter_add", rows.data_ptr(), _row_stride(rows), down.data_ptr(), up.data_ptr(),
-                    scale.data_ptr(), onto.data_ptr(), _row_stride(onto), out.data_ptr(), self.out_features,
+        ws = _lib.workspace(x, nbytes) if nbytes else None   # held until the launch
+        _lib.launch(x, "lr_adapter_add", rows.data_ptr(), x_step, down.data_ptr(), up.data_ptr(),
+                    scale.data_ptr(), onto.data_ptr(), base_step, out.data_ptr(), self.out_features,
                     _DTYPES[down.dtype], tokens, self.out_features, self.in_features, self.rank, self.adapters,
                     plan.order.data_ptr(), plan.tiles.data_ptr(), _lib.ptr(ws), nbytes)
         return out

@@ -192,21 +192,32 @@ def attention_packed(query, key, value, cu_query, cu_key=None, *, causal=False, 
 
 
 @functools.lru_cache(maxsize=4096)
-def _prefix_strides(query, prefix_key, prefix_value, key, value):
-    """The thirteen strides that lr_attention_prefix takes, of tensors given as (stride,
-    shape): token, head and, of batches, sequence."""
+def _prefix_strides(query, prefix_key, prefix_value, key, value, copied, q_shape, p_shape, k_shape):
+    """The thirteen strides that lr_attention_prefix takes, of tensors with these strides:
+    token, head and, of batches, sequence; None where one has to be copied first."""
     thirteen = array("q")
-    for stride, shape in (query, prefix_key, prefix_value, key, value):
+    for stride, shape in ((query, q_shape), (prefix_key, p_shape), (prefix_value, p_shape), (key, k_shape),
+                          (value, k_shape)):
+        if not copied and not _dense(stride, shape):
+            return None
         s = [st if n > 1 else 0 for st, n in zip(stride, shape)]
         thirteen.extend((s[-3], s[-2]) if len(s) == 3 else (s[1], s[2], s[0]))
     return thirteen
 
 
 @functools.lru_cache(maxsize=4096)
-def _prefix_workspace(device, batch, tokens, keys, prefix, heads, kv_heads, dim):
+def _prefix_workspace(device, q_shape, p_shape, k_shape):
+    """The bytes of its workspace, for shapes that fit together (checked here, once for each)."""
+    batch, tokens, heads, dim = q_shape
+    if p_shape[1:] != k_shape[2:]:
+        raise ValueError("prefix_key and prefix_value must be [prefix, kv_heads, head_dim], with key's heads")
+    if k_shape[0] != batch:
+        raise ValueError(f"query has a batch of {batch}, key of {k_shape[0]}")
+    if device < 0:
+        return 0
     nbytes = array("q", [0])
     with torch.cuda.device(device):
-        _lib.call("lr_attention_prefix_workspace", batch, tokens, keys, prefix, heads, kv_heads, dim,
+        _lib.call("lr_attention_prefix_workspace", batch, tokens, k_shape[1], p_shape[0], heads, k_shape[2], dim,
                   nbytes.buffer_info()[0])
     return nbytes[0]
 
@@ -225,16 +236,17 @@ def attention_shared_prefix(query, prefix_key, prefix_value, key, value, *, caus
     keys that a token sees, -inf where it sees none or all score -inf.
     """
     _check_tensors(query, key, value, 4)
-    if prefix_key.dim() != 3 or prefix_value.shape != prefix_key.shape or prefix_key.shape[1:] != key.shape[2:]:
+    q_shape, p_shape, k_shape = query.shape, prefix_key.shape, key.shape
+    if len(p_shape) != 3 or prefix_value.shape != p_shape:
         raise ValueError("prefix_key and prefix_value must be [prefix, kv_heads, head_dim], with key's heads")
-    if prefix_key.dtype != query.dtype or prefix_value.dtype != query.dtype:
+    dtype = query.dtype
+    if prefix_key.dtype != dtype or prefix_value.dtype != dtype:
         raise ValueError(f"the prefix must have the query's dtype, got {prefix_key.dtype}, {prefix_value.dtype}")
     if torch.is_grad_enabled() and (prefix_key.requires_grad or prefix_value.requires_grad):
         raise RuntimeError("gradients are not supported by the HIP attention: call it under torch.no_grad()")
-    if key.shape[0] != query.shape[0]:
-        raise ValueError(f"query has a batch of {query.shape[0]}, key of {key.shape[0]}")
-    batch, tokens, heads, dim = query.shape
-    keys, kv_heads = key.shape[1:3]
+    batch, tokens, heads, dim = q_shape
+    keys, kv_heads = k_shape[1:3]
+    nbytes = _prefix_workspace(query.get_device(), q_shape, p_shape, k_shape)
     if key_lengths is not None:
         key_lengths = _lengths(key_lengths, batch, keys)
     _lib.check_device(query)
@@ -242,15 +254,20 @@ def attention_shared_prefix(query, prefix_key, prefix_value, key, value, *, caus
                      key_lengths=key_lengths)
     scale = _scale_bits(float(dim ** -0.5 if scale is None else scale))
     given = (query, prefix_key, prefix_value, key, value)
-    given = tuple(t if not t.data_ptr() & 15 and _dense(t.stride(), t.shape) else _rows(t) for t in given)
-    strides = _prefix_strides(*((t.stride(), t.shape) for t in given))
-    out = query.new_empty(query.shape)
-    lse = query.new_empty((batch, tokens, heads), dtype=torch.float32) if return_lse else None
-    nbytes = _prefix_workspace(query.get_device(), batch, tokens, keys, prefix_key.shape[0], heads, kv_heads, dim)
-    ws = _lib.workspace(query, nbytes)   # held until the launch
-    _lib.launch(query, "lr_attention_prefix", *(t.data_ptr() for t in given), out.data_ptr(), _lib.ptr(lse),
-                _DTYPES[query.dtype], batch, tokens, keys, prefix_key.shape[0], heads, kv_heads, dim,
-                strides.buffer_info()[0], _lib.ptr(key_lengths), int(bool(causal)), scale, _lib.ptr(ws), nbytes)
+    pointers = [t.data_ptr() for t in given]
+    strides = None
+    if not (pointers[0] | pointers[1] | pointers[2] | pointers[3] | pointers[4]) & 15:
+        strides = _prefix_strides(*[t.stride() for t in given], False, q_shape, p_shape, k_shape)
+    if strides is None:
+        given = [_rows(t) for t in given]
+        pointers = [t.data_ptr() for t in given]
+        strides = _prefix_strides(*[t.stride() for t in given], True, q_shape, p_shape, k_shape)
+    out = query.new_empty(q_shape)
+    lse = torch.empty((batch, tokens, heads), dtype=torch.float32, device=query.device) if return_lse else None
+    ws = _lib.workspace(query, nbytes) if nbytes else None   # held until the launch
+    _lib.launch(query, "lr_attention_prefix", *pointers, out.data_ptr(), _lib.ptr(lse), _DTYPES[dtype], batch, tokens,
+                keys, p_shape[0], heads, kv_heads, dim, strides.buffer_info()[0], _lib.ptr(key_lengths),
+                int(bool(causal)), scale, _lib.ptr(ws), nbytes)
     return (out, lse) if return_lse else out
 
 

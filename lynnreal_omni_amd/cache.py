@@ -52,13 +52,17 @@ def _weights_workspace(device, batch, tokens, keys, heads, kv_heads, dim, causal
 
 
 @functools.lru_cache(maxsize=4096)
-def _six_strides(query, key):
-    """Token, head and sequence strides of two batches given as (stride, shape)."""
+def _six_strides(query, key, copied, q_shape, k_shape):
+    """The six strides that lr_attention_weights takes, of batches with these strides: token,
+    head and sequence; None where one has to be copied first."""
     six = array("q")
-    for stride, shape in (query, key):
+    for stride, shape in ((query, q_shape), (key, k_shape)):
+        if not copied and not _attention._dense(stride, shape):
+            return None
         s = [st if n > 1 else 0 for st, n in zip(stride, shape)]
         six.extend((s[1], s[2], s[0]))
-    return six
+    # The kernel's 32-bit offsets have to reach the heads of a key head and 64 tokens.
+    return six if copied or q_shape[2] * six[1] < 1 << 30 else None
 
 
 def accumulate_weights(weights, query, key, lse, *, causal=False, scale=None, key_lengths=None, out=None):
@@ -95,22 +99,18 @@ def accumulate_weights(weights, query, key, lse, *, causal=False, scale=None, ke
     if out is None:
         out = torch.empty_like(weights, memory_format=torch.contiguous_format)
     weights, lse = weights.contiguous(), lse.contiguous()
-    if query.data_ptr() & 15 or not _attention._dense(query.stride(), query.shape) or not _near(query):
-        query = _attention._rows(query.contiguous())
-    if key.data_ptr() & 15 or not _attention._dense(key.stride(), key.shape):
-        key = _attention._rows(key)
+    strides = None
+    if not (query.data_ptr() | key.data_ptr()) & 15:
+        strides = _six_strides(query.stride(), key.stride(), False, query.shape, key.shape)
+    if strides is None:
+        query, key = query.clone(memory_format=torch.contiguous_format), _attention._rows(key)
+        strides = _six_strides(query.stride(), key.stride(), True, query.shape, key.shape)
     nbytes = _weights_workspace(query.get_device(), batch, tokens, keys, heads, kv_heads, dim, int(bool(causal)))
-    ws = _lib.workspace(query, nbytes)   # held until the launch
-    strides = _six_strides((query.stride(), query.shape), (key.stride(), key.shape))
+    ws = _lib.workspace(query, nbytes) if nbytes else None   # held until the launch
     _lib.launch(query, "lr_attention_weights", query.data_ptr(), key.data_ptr(), lse.data_ptr(), weights.data_ptr(),
                 out.data_ptr(), _attention._DTYPES[query.dtype], batch, tokens, keys, heads, kv_heads, dim,
                 strides.buffer_info()[0], _lib.ptr(key_lengths), int(bool(causal)), scale, _lib.ptr(ws), nbytes)
     return out
-
-
-def _near(query):
-    """Whether the kernel's 32-bit offsets reach the heads of a key head and 64 tokens."""
-    return query.stride(1) < 1 << 23 and (query.shape[2] == 1 or query.stride(2) * query.shape[2] < 1 << 30)
 
 
 def _span(t):
@@ -137,9 +137,17 @@ def _distinct(t):
     return True
 
 
-def _byte_strides(t):
-    s = [st * t.element_size() if n > 1 else 0 for st, n in zip(t.stride(), t.shape)]
-    return s[1], s[2], s[0]
+@functools.lru_cache(maxsize=4096)
+def _byte_strides(copied, *tensors):
+    """The twelve strides in bytes that lr_cache_evict takes, of 16-bit tensors given as
+    (stride, shape); None where one of the first two has to be copied first."""
+    twelve = array("q")
+    for i, (stride, shape) in enumerate(tensors):
+        if i < 2 and not copied and not _attention._dense(stride, shape):
+            return None
+        s = [2 * st if n > 1 else 0 for st, n in zip(stride, shape)]
+        twelve.extend((s[1], s[2], s[0]))
+    return twelve
 
 
 def evict(key, value, weights, key_lengths, budget, *, recent=0, out=None):
@@ -185,17 +193,21 @@ def evict(key, value, weights, key_lengths, budget, *, recent=0, out=None):
         weights_out = weights.new_empty((batch, kv_heads, budget))
     lengths = torch.empty(batch, dtype=torch.int32, device=key.device)
     kept = torch.empty((batch, kv_heads, budget), dtype=torch.int32, device=key.device)
-    key, value = (t if not t.data_ptr() & 15 and _attention._dense(t.stride(), t.shape) else _attention._rows(t)
-                  for t in (key, value))
-    weights = weights.contiguous()
-    strides = array("q")
-    for t in (key, value, key_out, value_out):
-        strides.extend(_byte_strides(t))
+    if not weights.is_contiguous():
+        weights = weights.contiguous()
+    shape, new = key.shape, key_out.shape
+    outs = (key_out.stride(), new), (value_out.stride(), new)
+    strides = None
+    if not (key.data_ptr() | value.data_ptr()) & 15:
+        strides = _byte_strides(False, (key.stride(), shape), (value.stride(), shape), *outs)
+    if strides is None:
+        key, value = _attention._rows(key), _attention._rows(value)
+        strides = _byte_strides(True, (key.stride(), shape), (value.stride(), shape), *outs)
     nbytes = _evict_workspace(batch, keys, kv_heads)
-    ws = _lib.workspace(key, nbytes)   # held until the launch
+    ws = _lib.workspace(key, nbytes) if nbytes else None   # held until the launch
     _lib.launch(key, "lr_cache_evict", key.data_ptr(), value.data_ptr(), weights.data_ptr(), _lib.ptr(key_lengths),
                 key_out.data_ptr(), value_out.data_ptr(), weights_out.data_ptr(), lengths.data_ptr(), kept.data_ptr(),
-                batch, keys, kv_heads, 2 * dim, budget, recent, key_out.shape[1], strides.buffer_info()[0],
+                batch, keys, kv_heads, 2 * dim, budget, recent, new[1], strides.buffer_info()[0],
                 int(out is None), _lib.ptr(ws), nbytes)
     return key_out, value_out, weights_out, lengths, kept
 

@@ -86,9 +86,11 @@ struct Cut {
       while (taken(size) > (float)p.places) size += max(1, size >> 4);
     }
     size = __builtin_amdgcn_readfirstlane(size);
-    shared = max(1, __builtin_amdgcn_readfirstlane(shared_of(size)));
-    prefix = ceil_div(tiles, shared);
+    prefix = ceil_div(tiles, max(1, __builtin_amdgcn_readfirstlane(shared_of(size))));
+    shared = even(tiles, prefix);
   }
+  // Tiles of a piece where `all` are cut into `count`: even ones, the last at most smaller.
+  static __device__ __forceinline__ int even(int all, int count) { return count > 1 ? ceil_div(all, count) : all; }
   // What has piece `place` of the caches: the sequence (-1: none) and its first piece.
   __device__ __forceinline__ void find(const PrefixArgs& p, int place, int& seq, int& first) const {
     const int lane = threadIdx.x & 63;
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
     const Row row(p, r0 + wave * 32 + col, rows, hd, w.kn);
     qoff = seq * p.qb + row.tok * p.qt + row.head * p.qh;
     keys = own_cache(p, seq, hd, w, row.seen);
-    const int size = p.places ? cut.size : w.tiles;
+    const int all = key_tiles(w.kn), size = p.places ? Cut::even(all, ceil_div(all, cut.size)) : all;
     t0 = min(w.tiles, (piece - first) * size);
     t1 = min(w.tiles, t0 + size);
     part = own_part(p, piece) + (int64_t)row.tok * p.heads + row.head;

@@ -97,10 +97,11 @@ def test_out_is_base_or_other_memory():
 
 def test_rows_are_read_as_they_are_where_they_can():
     wide = torch.zeros(9, 64, dtype=BF16)
-    assert L._readable(wide) and L._readable(wide[:, 8:32]) and L._readable(wide[:1].expand(9, -1)) and L._readable(wide[::2])
-    assert not L._readable(wide[:, 1:25]) and not L._readable(wide.t())
-    assert not L._readable(torch.zeros(9, 65, dtype=BF16)[:, :64])
-    assert not L._readable(torch.zeros(100, dtype=BF16).as_strided((5, 64), (8, 1)))
+    step = lambda t: L._row_step(t.stride(), *t.shape)  # noqa: E731
+    assert step(wide) == 64 and step(wide[:, 8:32]) == 64 and step(wide[::2]) == 128 and step(wide[3:4, :24]) == 24
+    assert step(wide[:1].expand(9, -1)) == 0
+    assert step(wide.t()) is None and step(torch.zeros(9, 65, dtype=BF16)[:, :64]) is None
+    assert step(torch.zeros(100, dtype=BF16).as_strided((5, 64), (8, 1))) is None
 
 
 def test_adapted_transformer():

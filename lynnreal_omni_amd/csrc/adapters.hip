@@ -123,19 +123,32 @@ struct AdapterArgs {
   int columns;           // of a workgroup of expand
 };
 
+__device__ __forceinline__ void dma16s(__amdgpu_buffer_rsrc_t rsrc, void* lds, uint32_t voffset, uint32_t soffset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)lds, 16, voffset, soffset, 0, 0);
+}
+
+// Workgroups are dealt to the 8 XCDs in turn; here each XCD takes a contiguous run of tiles, so
+// that its L2 serves an adapter to the tiles that share it (3683 tokens, 5376 columns, rank 64:
+// 14.6 us without, 13.2 so).
+__device__ __forceinline__ uint32_t run_of_xcd() {
+  const uint32_t per = gridDim.x >> 3, rest = gridDim.x & 7, xcd = blockIdx.x & 7;
+  return (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (blockIdx.x >> 3);
+}
+
 template <int COUNT>
 __device__ __forceinline__ void wait_loads() {   // all but the last COUNT
   static_assert(COUNT < 64, "vmcnt");
   __builtin_amdgcn_s_waitcnt((COUNT & 15) | (COUNT >> 4) << 14 | 0x70 | 0xf00);
 }
 
-// Slots of the ring: what three, two and one workgroups per CU can have of its LDS, so that 105
-// to 125 KB are on their way to each CU (at rank 128, 12605 x 14336, four slots took 131 us).
+// Slots of the rings: three, two and one workgroups per CU.
 template <int RP>
-constexpr int kRing = kStep == 64 ? (RP == 32 ? 4 : (RP == 64 ? 5 : 6)) : (RP == 32 ? 3 : (RP == 64 ? 2 : 3));
+constexpr int kRingX = RP == 32 ? 5 : (RP == 64 ? 6 : 8);
+template <int RP>
+constexpr int kRingD = RP == 32 ? 3 : 4;
 
-// Four waves; steps of 64 columns through a ring of LDS slots that hold 64 rows of x and RP of
-// down, 128 bytes each (16-byte chunk c of row r in place c ^ r % 8). Wave w takes the columns
+// Four waves; steps of 64 columns through rings of LDS slots that hold 64 rows of x or RP of
+// down, 128 bytes each (16-byte chunk c of row r in place c ^ r / 2 % 8). Wave w takes the columns
 // 16 w .. of a step for all rows, so that each element leaves the LDS once; the waves' sums are
 // added at the end. The product is transposed, down x^T: a lane holds four ranks of a token
 // next to each other.
@@ -145,14 +158,15 @@ constexpr int kRing = kStep == 64 ? (RP == 32 ? 4 : (RP == 64 ? 5 : 6)) : (RP ==
 template <typename T, int RP>
 __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
   typedef typename Mfma<T>::V V8;
-  constexpr int RB = RP / 32, TB = kTokens / 32, ROW = 2 * kStep, RING = kRing<RP>, CH = ROW / 16, PER = 1024 / ROW;
-  constexpr int SLOT = (kTokens + RP) * ROW, XD = kTokens / PER / 4, DD = RP / PER / 4;   // DMAs of a wave
+  constexpr int RB = RP / 32, TB = kTokens / 32, ROW = 2 * kStep, RX = kRingX<RP>, RD = kRingD<RP>, CH = ROW / 16, PER = 1024 / ROW;
+  constexpr int SX = kTokens * ROW, SD = RP * ROW, LDS = RX * SX + RD * SD, XD = kTokens / PER / 4, DD = RP / PER / 4;   // DMAs of a wave
   constexpr int GROUP = 4 < TB * RB ? 4 : TB * RB;   // blocks that are added at a time
-  static_assert(RING * SLOT >= 4 * GROUP * 4096, "the sums take the ring's place");
-  __shared__ __attribute__((aligned(1024))) char smem[RING * SLOT];
+  static_assert(LDS >= 4 * GROUP * 4096, "the sums take the rings' place");
+  __shared__ __attribute__((aligned(1024))) char smem[LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = lane >> 5, col = lane & 31;
-  const int tile = (int)(blockIdx.x % (uint32_t)p.max_tiles), split = (int)(blockIdx.x / (uint32_t)p.max_tiles);
+  const uint32_t id = run_of_xcd();
+  const int tile = (int)(id % (uint32_t)p.max_tiles), split = (int)(id / (uint32_t)p.max_tiles);
   const int4 info = p.tiles[tile];
   const int a = info.x, count = info.z;
   if (a < 0 || count == 0) return;
@@ -175,19 +189,25 @@ __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
     const int r = (wave * DD + i) * PER + lane / CH;
     dof[i] = r < p.rank ? (uint32_t)((int64_t)r * p.k8 * 2) : kOutside;
   }
-  auto issue = [&](int s) {
-    char* const slot = smem + (s - s0) % RING * SLOT;
-    // Chunks past the last column read as zero on both sides.
-    auto at = [&](uint32_t row, int r) __attribute__((always_inline)) {
-      const int k = s * kStep + (lane % CH ^ turn(r)) * 8;
-      return s < s1 && k < p.k8 && row != kOutside ? row + k * 2 : kOutside;
-    };
+  // Steps of whole chunks take a scalar offset; in others those past the last column, or all of
+  // them past the last step, read as zero on both sides.
+  const int full = min(s1, p.k8 / kStep);
+  auto load = [&](__amdgpu_buffer_rsrc_t from, char* lds, uint32_t row, int r, int s) __attribute__((always_inline)) {
+    const int c = (lane % CH ^ turn(r)) * 8;
+    if (s < full) dma16s(from, lds, row == kOutside ? kOutside : row + c * 2, (uint32_t)s * (kStep * 2));
+    else dma16(from, lds, s < s1 && s * kStep + c < p.k8 && row != kOutside ? row + (s * kStep + c) * 2 : kOutside);
+  };
+  int slot_x = 0, slot_d = 0;   // that the next step goes to
+  auto issue_x = [&](int s) {
 #pragma unroll
-    for (int i = 0; i < XD; ++i)
-      dma16(xr, slot + (wave * XD + i) * 1024, at(xo[i], (wave * XD + i) * PER + lane / CH));
+    for (int i = 0; i < XD; ++i) load(xr, smem + slot_x * SX + (wave * XD + i) * 1024, xo[i], (wave * XD + i) * PER + lane / CH, s);
+    slot_x = slot_x + 1 == RX ? 0 : slot_x + 1;
+  };
+  auto issue_d = [&](int s) {
 #pragma unroll
     for (int i = 0; i < DD; ++i)
-      dma16(dr, slot + kTokens * ROW + (wave * DD + i) * 1024, at(dof[i], (wave * DD + i) * PER + lane / CH));
+      load(dr, smem + RX * SX + slot_d * SD + (wave * DD + i) * 1024, dof[i], (wave * DD + i) * PER + lane / CH, s);
+    slot_d = slot_d + 1 == RD ? 0 : slot_d + 1;
   };
   v16f acc[TB][RB];
 #pragma unroll
@@ -196,33 +216,66 @@ __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
     for (int c = 0; c < RB; ++c)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[b][c][e] = 0.0f;
+  // Step s issues x(s + RX - 1) and then down(s + RD - 1); before the first one:
 #pragma unroll
-  for (int i = 0; i < RING - 1; ++i) issue(s0 + i);
+  for (int i = 0; i < RX - RD; ++i) issue_x(s0 + i);
+#pragma unroll
+  for (int i = 0; i < RD - 1; ++i) {
+    issue_x(s0 + RX - RD + i);
+    issue_d(s0 + i);
+  }
+  // A step's fragments are read while the one before is multiplied.
   auto steps_of = [&](auto blocks) {   // of 32 tokens
-#pragma unroll 1
-    for (int s = s0; s < s1; ++s) {
-      wait_loads<(RING - 2) * (XD + DD)>();
+    constexpr int B = decltype(blocks)::value, PARTS = kStep / 64;
+    V8 df[2][PARTS][RB], xf[2][PARTS][B];
+    int read_x = 0, read_d = 0;
+    auto fetch = [&](V8 (&d)[PARTS][RB], V8 (&x)[PARTS][B]) __attribute__((always_inline)) {
+      const char* const xs = smem + read_x * SX;
+      const char* const ds = smem + RX * SX + read_d * SD;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        // (All rows of a block have the turn of the first: 32 rows are whole turns.)
+        const int place = ((8 * i + 2 * wave + half) ^ turn(col)) * 16;
+#pragma unroll
+        for (int c = 0; c < RB; ++c) d[i][c] = *reinterpret_cast<const V8*>(ds + (32 * c + col) * ROW + place);
+#pragma unroll
+        for (int b = 0; b < B; ++b) x[i][b] = *reinterpret_cast<const V8*>(xs + (32 * b + col) * ROW + place);
+      }
+      read_x = read_x + 1 == RX ? 0 : read_x + 1;
+      read_d = read_d + 1 == RD ? 0 : read_d + 1;
+    };
+    auto arrive = [&](auto left) __attribute__((always_inline)) {
+      wait_loads<decltype(left)::value>();
       __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_barrier();   // step s is there, and every wave is done with step s - 1
+      __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      issue(s + RING - 1);
-      const char* const slot = smem + (s - s0) % RING * SLOT;
+    };
+    auto step = [&](V8 (&d)[PARTS][RB], V8 (&x)[PARTS][B], V8 (&nd)[PARTS][RB], V8 (&nx)[PARTS][B], int s)
+        __attribute__((always_inline)) {
+      // Step s + 1 is there, and every wave is done with step s - 1, whose slots are next.
+      arrive(std::integral_constant<int, (RD - 3) * (XD + DD)>{});
+      issue_x(s + RX - 1);
+      issue_d(s + RD - 1);
+      fetch(nd, nx);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < kStep / 64; ++d) {
-        // (All rows of a block have the turn of the first: 32 rows are whole turns.)
-        const int place = ((8 * d + 2 * wave + half) ^ turn(col)) * 16;
-        V8 df[RB];
+      for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-        for (int c = 0; c < RB; ++c) df[c] = *reinterpret_cast<const V8*>(slot + (kTokens + 32 * c + col) * ROW + place);
+        for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int b = 0; b < decltype(blocks)::value; ++b) {
-          const V8 xf = *reinterpret_cast<const V8*>(slot + (32 * b + col) * ROW + place);
-#pragma unroll
-          for (int c = 0; c < RB; ++c) acc[b][c] = Mfma<T>::mul(df[c], xf, acc[b][c]);
-        }
-      }
+          for (int c = 0; c < RB; ++c) acc[b][c] = Mfma<T>::mul(d[i][c], x[i][b], acc[b][c]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    arrive(std::integral_constant<int, (RD - 2) * (XD + DD)>{});
+    fetch(df[0], xf[0]);
+    int s = s0;
+#pragma unroll 1
+    for (; s + 1 < s1; s += 2) {
+      step(df[0], xf[0], df[1], xf[1], s);
+      step(df[1], xf[1], df[0], xf[0], s + 1);
     }
+    if (s < s1) step(df[0], xf[0], df[1], xf[1], s);
   };
   if (count <= 32) steps_of(std::integral_constant<int, 1>{});
   else steps_of(std::integral_constant<int, TB>{});

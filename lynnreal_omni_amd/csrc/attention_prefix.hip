@@ -15,13 +15,13 @@
 // in one pass. Nothing is joined, and the prefix comes out of the caches, since the
 // matrix units, not the keys, are what bounds it.
 #include "lr_attention.h"
+#include "lr_pieces.h"
 #include "lr_runtime.h"
 
 namespace lr {
 namespace {
 
 constexpr int kMaxPieces = 256;   // of a cache, and of the prefix
-constexpr int kListed = 512;      // sequences of a list of pieces: eight lengths per lane
 
 struct PrefixArgs {
   const uint16_t *q, *pk, *pv, *k, *v;
@@ -46,39 +46,22 @@ struct PrefixArgs {
   int whole, left, cuts; // walk: workgroups for all keys of their rows; those cut into `cuts`
 };
 
-__device__ __forceinline__ int own_keys(const PrefixArgs& p, int i) {
-  return p.lengths ? (int)clamp64(p.lengths[i], 0, p.k_rows) : p.k_rows;
-}
+__device__ __forceinline__ int own_keys(const PrefixArgs& p, int i) { return keys_of(p.lengths, i, p.k_rows); }
 __device__ __forceinline__ int key_tiles(int keys) { return (int)((uint32_t)(keys + kKeys - 1) / kKeys); }
-__device__ __forceinline__ int ceil_div(int a, int b) { return (int)((uint32_t)(a + b - 1) / (uint32_t)b); }
 
 // How prefix and caches are cut: pieces of `size` tiles of 64 keys, the smallest for
 // which all of them have a place. Every wave works it out from the lengths by itself.
 struct Cut {
   int size, shared, prefix;   // tiles of a piece of a cache, and of the prefix; pieces of that one
-  int mine[kListed / 64];   // key tiles of sequences lane, lane + 64, ..
-  int groups;
+  Pieces own;
   __device__ __forceinline__ explicit Cut(const PrefixArgs& p) {
-    const int lane = threadIdx.x & 63, tiles = key_tiles(p.prefix);
+    const int tiles = key_tiles(p.prefix);
     auto shared_of = [&](int size) __attribute__((always_inline)) { return max(size, ceil_div(tiles, p.shares)); };
     size = p.piece;
-    groups = 0;
     if (p.places) {
-      groups = (p.n + 63) >> 6;
-#pragma unroll
-      for (int g = 0; g < kListed / 64; ++g) {
-        const int i = 64 * g + lane;
-        mine[g] = i < p.n ? key_tiles(own_keys(p, i)) : 0;
-      }
-      // Places that pieces of `size` take. Sums in fp32: what has to be exact is below 2^24.
+      own.load(p.lengths, p.n, p.k_rows, kKeys);
       auto taken = [&](int size) __attribute__((always_inline)) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int g = 0; g < kListed / 64; ++g)
-          if (g < groups) sum += (float)ceil_div(mine[g], size);
-        sum = wave_tree_sum(sum) * (float)p.seq_tiles + (float)(ceil_div(tiles, shared_of(size)) * p.all_tiles);
-        // The same in every lane; said so, since what depends on it addresses memory.
-        return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sum)));
+        return own.count(size) * (float)p.seq_tiles + (float)(ceil_div(tiles, shared_of(size)) * p.all_tiles);
       };
       // From an even share up in steps, which end at the latest where every cache is one piece
       // (lr_attention_prefix gives as many places).
@@ -87,33 +70,12 @@ struct Cut {
     }
     size = __builtin_amdgcn_readfirstlane(size);
     prefix = ceil_div(tiles, max(1, __builtin_amdgcn_readfirstlane(shared_of(size))));
-    shared = even(tiles, prefix);
+    shared = Pieces::even(tiles, prefix);
   }
-  // Tiles of a piece where `all` are cut into `count`: even ones, the last at most smaller.
-  static __device__ __forceinline__ int even(int all, int count) { return count > 1 ? ceil_div(all, count) : all; }
   // What has piece `place` of the caches: the sequence (-1: none) and its first piece.
   __device__ __forceinline__ void find(const PrefixArgs& p, int place, int& seq, int& first) const {
-    const int lane = threadIdx.x & 63;
-    seq = -1;
-    if (!p.places) {   // a piece each
-      seq = place < p.n ? place : -1;
-      first = seq;
-      return;
-    }
-    int before = 0;
-#pragma unroll
-    for (int g = 0; g < kListed / 64; ++g) {
-      if (g >= groups || seq >= 0) continue;
-      const int n = ceil_div(mine[g], size);
-      const int upto = wave_prefix_sum(n);
-      const uint64_t hit = __ballot(before + upto > place && 64 * g + lane < p.n);
-      if (hit) {
-        const int l = __builtin_ctzll(hit);
-        seq = 64 * g + l;
-        first = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
-      }
-      before += __builtin_amdgcn_readlane(upto, 63);
-    }
+    if (p.places) own.find(p.n, size, place, seq, first);
+    else seq = first = place < p.n ? place : -1;   // a piece each
   }
   // Each sequence's first piece and how many there are, and behind them the pieces of the prefix,
   // by one wave for the kernel that joins them.
@@ -123,8 +85,8 @@ struct Cut {
     if (p.places) {
 #pragma unroll
       for (int g = 0; g < kListed / 64; ++g) {
-        if (g >= groups) continue;
-        const int n = ceil_div(mine[g], size), upto = wave_prefix_sum(n);
+        if (g >= own.groups) continue;
+        const int n = ceil_div(own.tiles[g], size), upto = wave_prefix_sum(n);
         if (64 * g + lane < p.n) table[64 * g + lane] = make_int2(before + upto - n, n);
         before += __builtin_amdgcn_readlane(upto, 63);
       }
@@ -220,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
     const Row row(p, r0 + wave * 32 + col, rows, hd, w.kn);
     qoff = seq * p.qb + row.tok * p.qt + row.head * p.qh;
     keys = own_cache(p, seq, hd, w, row.seen);
-    const int all = key_tiles(w.kn), size = p.places ? Cut::even(all, ceil_div(all, cut.size)) : all;
+    const int all = key_tiles(w.kn), size = p.places ? Pieces::even(all, ceil_div(all, cut.size)) : all;
     t0 = min(w.tiles, (piece - first) * size);
     t1 = min(w.tiles, t0 + size);
     part = own_part(p, piece) + (int64_t)row.tok * p.heads + row.head;

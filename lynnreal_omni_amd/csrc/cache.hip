@@ -12,6 +12,7 @@
 // Eviction reads the weights, finds for every cache and head the keys that stay, and moves
 // their rows to another cache, in their order.
 #include "lr_attention.h"
+#include "lr_pieces.h"
 #include "lr_runtime.h"
 
 namespace lr {
@@ -41,6 +42,7 @@ struct WeighArgs {
   int n, q_rows, k_rows, heads, kv_heads, group;
   int causal, splits;     // splits: of the rows, `chunk` tiles of 64 each
   int chunk;
+  int places;             // few rows: pieces of all caches for a key head
   float c;                // scale * log2(e)
   Divisor by_group;
 };
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
   const int seq = (int)(id % (uint32_t)p.n);
   id /= (uint32_t)p.n;
   const int split = (int)(id % (uint32_t)p.splits), key0 = (int)(id / (uint32_t)p.splits) * KEYS;
-  const int kn = p.lengths ? (int)clamp64(p.lengths[seq], 0, p.k_rows) : p.k_rows;
+  const int kn = keys_of(p.lengths, seq, p.k_rows);
   const int hidden = kn - p.q_rows;   // causal: token t sees keys up to hidden + t
   const int rows = p.q_rows * p.group;
   const int first = p.causal ? (int)min((int64_t)rows, max(0, key0 - hidden) * (int64_t)p.group) : 0;
@@ -252,6 +254,99 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
   }
 }
 
+// At most 32 rows per key head: what counts is the stream of keys. They are cut into pieces
+// over all caches (lr_pieces.h); a wave has 32 keys of each 128 of them, through 32 rows of
+// LDS of its own, and the queries in registers, so that no wave waits for another. The next
+// keys are on their way while these are worked on.
+// (Eight caches of 16152 keys in all, places for 65536, 40 heads over 8: 17.2 us with a workgroup
+// for every 128 places of every cache.)
+constexpr int kGroup = 128;
+constexpr int kCopied = 1024;   // places behind the caches' keys that a workgroup copies at a time
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 4) void weigh_few(WeighArgs p) {
+  typedef typename Mfma<T>::V V8;
+  constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32, KD = D / 16, DMAS = 32 * ROW / 1024;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * 32 * ROW];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, col = lane & 31;
+  const int place = (int)(blockIdx.x / (uint32_t)p.kv_heads), hd = (int)(blockIdx.x - place * p.kv_heads);
+  Pieces caches;
+  caches.load(p.lengths, p.n, p.k_rows, kGroup);
+  // The smallest pieces that all have a place (there are n at least).
+  int size = max(1, (int)(caches.count(1) / (float)p.places));
+  while (caches.count(size) > (float)p.places) size += max(1, size >> 4);
+  int seq, first = 0;
+  caches.find(p.n, size, place, seq, first);
+  if (seq >= 0) {
+    const int kn = keys_of(p.lengths, seq, p.k_rows), hidden = kn - p.q_rows, all = ceil_div(kn, kGroup);
+    const int each = Pieces::even(all, ceil_div(all, size));
+    const int g0 = (place - first) * each, g1 = min(all, g0 + each);
+    const uint16_t* const kbase = p.k + seq * p.kb + hd * p.kh;
+    char* const mine = smem + wave * 32 * ROW;
+    auto issue = [&](int g) {
+      const int key = g * kGroup + wave * 32, left = min(32, kn - key);   // keys past the last read as zero
+      const __amdgpu_buffer_rsrc_t r =
+          row_rsrc(kbase + (left > 0 ? (int64_t)key * p.kt : 0), left > 0 ? ((int64_t)(left - 1) * p.kt + D) * 2 : 0);
+#pragma unroll
+      for (int i = 0; i < DMAS; ++i) {
+        const int row = (i * 64 + lane) / CH, ch = (i * 64 + lane) % CH ^ (row / RPB % PAIRS) * 2;
+        dma16(r, mine + i * 1024, (uint32_t)(row * p.kt * 2 + ch * 16));
+      }
+    };
+    if (g0 < g1) issue(g0);
+    // The lane's row; lanes past the last one repeat it and see nothing.
+    const int rows = p.q_rows * p.group, r = min(col, rows - 1), tok = p.by_group.of(r), h = hd * p.group + r - tok * p.group;
+    const uint16_t* const q = p.q + seq * p.qb + tok * p.qt + h * p.qh;
+    V8 qf[KD];
+#pragma unroll
+    for (int d = 0; d < KD; ++d) qf[d] = *reinterpret_cast<const V8*>(q + 16 * d + 8 * half);
+    const float l2 = p.lse[((int64_t)seq * p.q_rows + tok) * p.heads + h] * kLog2e;
+    const int lim = col >= rows ? 0 : (p.causal ? hidden + tok + 1 : kn);
+    const float* const w = p.w + ((int64_t)seq * p.kv_heads + hd) * p.k_rows;
+    float* const out = p.out + ((int64_t)seq * p.kv_heads + hd) * p.k_rows;
+    for (int g = g0; g < g1; ++g) {
+      const int key0 = g * kGroup + wave * 32;
+      // Lane col < 16 of a half has this key in the end.
+      const int key = key0 + 8 * (col >> 2) + 4 * half + (col & 3);
+      const float had = col < 16 && key < kn ? w[key] : 0.0f;
+      __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);   // vmcnt(0): this wave's keys are there
+      asm volatile("" ::: "memory");
+      V8 kf[KD];
+#pragma unroll
+      for (int d = 0; d < KD; ++d)
+        kf[d] = *reinterpret_cast<const V8*>(mine + col * ROW + ((2 * d + half) ^ (col / RPB % PAIRS) * 2) * 16);
+      __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): and in registers
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      if (g + 1 < g1) issue(g + 1);
+      v16f s = {};
+#pragma unroll
+      for (int d = 0; d < KD; ++d) s = Mfma<T>::mul(kf[d], qf[d], s);
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.c, -l2));
+        const float v = half_sum(key0 + 8 * (e >> 2) + 4 * half + (e & 3) < lim ? x : 0.0f);
+        sum = col == e ? v : sum;
+      }
+      if (col < 16 && key < kn) out[key] = had + sum;
+    }
+  }
+  if (p.out == p.w) return;
+  // Places behind the caches' keys stay as they were.
+  const int runs = ceil_div(p.k_rows, kCopied);
+  for (int64_t i = blockIdx.x; i < (int64_t)p.n * p.kv_heads * runs; i += gridDim.x) {
+    const int64_t row = i / runs;
+    const int kn = keys_of(p.lengths, (int)(row / p.kv_heads), p.k_rows), from = (int)(i - row * runs) * kCopied;
+#pragma unroll
+    for (int j = 0; j < kCopied / 256; ++j) {
+      const int key = from + 256 * j + (int)threadIdx.x;
+      if (key >= kn && key < p.k_rows) p.out[row * p.k_rows + key] = p.w[row * p.k_rows + key];
+    }
+  }
+}
+
 // out = w + the splits' sums, in order.
 __global__ __launch_bounds__(256) void add_splits(const float* part, const float* w, float* out, int64_t n, int splits) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -320,7 +415,7 @@ __global__ __launch_bounds__(kSelect) void choose_keys(EvictArgs p) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int part = blockIdx.x % (uint32_t)p.parts, row = blockIdx.x / (uint32_t)p.parts;
   const int head = row % (uint32_t)p.heads, seq = row / (uint32_t)p.heads;
-  const int n = p.lengths ? (int)clamp64(p.lengths[seq], 0, p.size) : p.size;
+  const int n = keys_of(p.lengths, seq, p.size);
   const int stay = min(n, p.budget);
   const float* const w = p.w + (int64_t)row * p.size;
   float* const w_out = p.w_out + (int64_t)row * p.capacity;
@@ -502,6 +597,7 @@ __global__ __launch_bounds__(256) void move_rows(EvictArgs p) {
 
 struct WeighPlan {
   int blocks, splits, chunk;   // of 32 keys per wave; of the rows, and their tiles
+  int places;                  // of pieces for a key head (few rows), else 0
   int64_t grid;
 };
 
@@ -524,12 +620,21 @@ WeighPlan weigh_plan(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int k
   pl.chunk = (int)((tiles + s - 1) / s);
   pl.splits = pl.chunk > 0 ? (int)((tiles + pl.chunk - 1) / pl.chunk) : 1;
   pl.grid = groups * pl.splits;
+  pl.places = 0;
+  if (rows > 0 && rows <= 32 && n <= kListed && n > 0) {
+    // Four workgroups per CU are resident; each cache has a piece at least.
+    const int64_t places = 4 * cus / kv_heads;
+    pl.places = (int)(places < n ? n : places);
+    pl.splits = 1;
+    pl.grid = (int64_t)pl.places * kv_heads;
+  }
   return pl;
 }
 
 template <typename T, int D>
 void weigh(const WeighArgs& p, const WeighPlan& pl, hipStream_t s) {
-  if (pl.blocks == 1) weigh_keys<T, D, 1><<<(unsigned)pl.grid, 256, 0, s>>>(p);
+  if (pl.places) weigh_few<T, D><<<(unsigned)pl.grid, 256, 0, s>>>(p);
+  else if (pl.blocks == 1) weigh_keys<T, D, 1><<<(unsigned)pl.grid, 256, 0, s>>>(p);
   else weigh_keys<T, D, 2><<<(unsigned)pl.grid, 256, 0, s>>>(p);
 }
 
@@ -594,7 +699,7 @@ extern "C" int lr_attention_weights(const void* q, const void* k, const float* l
   const WeighArgs p = {static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), lse, weights, out,
                        static_cast<float*>(workspace), strides[0], strides[1], strides[2], strides[3], strides[4],
                        strides[5], key_lengths, (int)sequences, (int)q_rows, (int)k_rows, heads, kv_heads, group,
-                       causal != 0, pl.splits, pl.chunk, scale * 1.4426950408889634f, Divisor((uint32_t)group)};
+                       causal != 0, pl.splits, pl.chunk, pl.places, scale * 1.4426950408889634f, Divisor((uint32_t)group)};
   LR_REQUIRE(p.c > 0.0f && isfinite(p.c), "attention_weights: the scale must be positive and finite");
   const int64_t all = sequences * kv_heads * k_rows;
   LR_REQUIRE(pl.grid <= kMaxBlocks && (pl.splits == 1 || all <= kMaxBlocks * 256),

@@ -144,10 +144,141 @@ __device__ __forceinline__ OneCache prefix_cache(const PrefixArgs& p, int hd) {
   return {p.pk + hd * p.pkh, p.pv + hd * p.pvh, p.pkt, p.pvt, p.prefix, p.prefix, p.prefix};
 }
 
+// attend for at most 32 rows, the same for all waves: what counts is the stream of keys. A wave
+// takes 32 keys of each 128 by itself, through LDS of its own: they are all read into
+// registers before they are worked on, and the next ones are on their way meanwhile, so that the
+// whole workgroup's LDS is in flight (twice what the tiles of attend have) and no wave waits
+// for another. Weights are kept as a rounded number and its rest, as there. The waves' rows
+// are joined in LDS at the end, in their order: wave w is left with columns 16 w .. of each 64
+// of the lane's row (D / 8 of o, in all of its D / 2), l and the exponent.
+template <typename T, int D>
+__device__ __forceinline__ void attend_few(char* smem, float2* stats, const OneCache& keys, const uint16_t* qrow, const float c,
+                                           const int t0, const int t1, float& l, float& off, float (&mine)[D / 8]) {
+  typedef typename Mfma<T>::V V8;
+  constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32, KD = D / 16, DB = D / 32;
+  constexpr int HALF = 32 * ROW, DMAS = HALF / 1024;   // a wave's keys, its values behind them
+  static_assert(4 * 2 * HALF == kTileBytes<D>, "LDS");
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, col = lane & 31;
+  char* const ks = smem + wave * 2 * HALF;
+  char* const vs = ks + HALF;
+  V8 q[KD];
+#pragma unroll
+  for (int d = 0; d < KD; ++d) q[d] = *reinterpret_cast<const V8*>(qrow + 16 * d + 8 * half);
+  uint32_t koff[DMAS], voff[DMAS];
+#pragma unroll
+  for (int i = 0; i < DMAS; ++i) {
+    const int at = i * 64 + lane, row = at / CH, ch = at % CH ^ (row / RPB % PAIRS) * 2;
+    koff[i] = (uint32_t)(row * keys.kt * 2 + ch * 16);
+    voff[i] = (uint32_t)(row * keys.vt * 2 + ch * 16);
+  }
+  auto issue = [&](int s) {   // keys 32 s ..; those past the last read as zero
+    const int left = min(32, keys.kn - 32 * s);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const int64_t stride = v ? keys.vt : keys.kt;
+      const __amdgpu_buffer_rsrc_t r = row_rsrc((v ? keys.v : keys.k) + (left > 0 ? 32 * (int64_t)s * stride : 0),
+                                                left > 0 ? ((int64_t)(left - 1) * stride + D) * 2 : 0);
+#pragma unroll
+      for (int i = 0; i < DMAS; ++i) dma16(r, (v ? vs : ks) + i * 1024, v ? voff[i] : koff[i]);
+    }
+  };
+  v16f o[DB];
+  float m = -INFINITY, unused = 0.0f;
+  l = off = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  const int i16 = lane & 15, vr = 4 * half + (i16 >> 2);
+  const int s1 = 2 * t1;
+  int s = 2 * t0 + wave;
+  if (s < s1) issue(s);
+#pragma unroll 1
+  for (; s < s1; s += 4) {
+    __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);   // vmcnt(0): this wave's keys and values are there
+    asm volatile("" ::: "memory");
+    V8 kf[KD], vf[2][DB];
+#pragma unroll
+    for (int d = 0; d < KD; ++d)
+      kf[d] = *reinterpret_cast<const V8*>(ks + col * ROW + ((2 * d + half) ^ (col / RPB % PAIRS) * 2) * 16);
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const int ch = 4 * d + 2 * ((lane >> 4) & 1) + (i16 >> 1 & 1), r0 = 16 * kc + vr, r1 = r0 + 8;
+        vf[kc][d] = tr_pair<V8>(vs + r0 * ROW + (ch ^ (r0 / RPB % PAIRS) * 2) * 16 + (i16 & 1) * 8,
+                                vs + r1 * ROW + (ch ^ (r1 / RPB % PAIRS) * 2) * 16 + (i16 & 1) * 8);
+      }
+    __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): and in registers
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (s + 4 < s1) issue(s + 4);
+    v16f sc = {};
+#pragma unroll
+    for (int d = 0; d < KD; ++d) sc = Mfma<T>::mul(kf[d], q[d], sc);
+    if (32 * s + 32 > keys.sure) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = 32 * s + 8 * (e >> 2) + 4 * half + (e & 3) < keys.seen ? sc[e] : -INFINITY;
+    }
+    float x = sc[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) x = fmaxf(x, sc[e]);
+    off = move_max<DB, false>(max_with_partner(x), m, l, unused, o, c, Mfma<T>::kShift);
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+      uint4 hi, lo;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * kc + 2 * w], c, -off));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * kc + 2 * w + 1], c, -off));
+        const uint32_t h = Mfma<T>::pack(p0, p1);
+        set_word(hi, w, h);
+        set_word(lo, w, Mfma<T>::pack(p0 - Mfma<T>::first(h), p1 - Mfma<T>::second(h)));
+        l += p0 + p1;
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        o[d] = Mfma<T>::mul(vf[kc][d], __builtin_bit_cast(V8, hi), o[d]);
+        o[d] = Mfma<T>::mul(vf[kc][d], __builtin_bit_cast(V8, lo), o[d]);
+      }
+    }
+  }
+  // (Nothing is on its way to the LDS: the last keys have been waited for.)
+  l = add_partner(l);
+  __syncthreads();
+  float* const parts = reinterpret_cast<float*>(smem);   // [wave][D / 2][lane]
+  stats[wave * 64 + lane] = make_float2(off, l);
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) parts[(wave * (D / 2) + 16 * d + e) * 64 + lane] = o[d][e];
+  __syncthreads();
+  float2 st[4];
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    st[w] = stats[w * 64 + lane];
+    if (st[w].y != 0.0f) top = fmaxf(top, st[w].x);
+  }
+  off = top == -INFINITY ? 0.0f : top;
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) mine[i] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (st[w].y == 0.0f) continue;
+    const float f = __builtin_amdgcn_exp2f(st[w].x - off);
+    l += f * st[w].y;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) mine[i] += f * parts[(w * (D / 2) + wave * (D / 8) + i) * 64 + lane];
+  }
+}
+
 // One piece of the prefix or of a cache for at most 128 rows.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[kTileBytes<D>];
+  __shared__ __attribute__((aligned(1024))) char smem[kTileBytes<D> + 256 * 8];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = lane >> 5, col = lane & 31;
   // All key heads of the same keys, which lie side by side, come first.
@@ -155,15 +286,17 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
   const Cut cut(p);
   if (blockIdx.x == 0 && wave == 0) cut.publish(p, pieces_of<D>(p));
   OneCache keys;
-  int t0, t1, rows, r0;
+  int t0, t1, rows, r0, r;   // r: the lane's row
   int64_t part, qoff;
-  bool sees;
+  bool sees, few;
   if (item < cut.prefix * p.all_tiles) {
     // The row tiles of a piece lie side by side, so that they share its keys in a cache.
     const int piece = (int)((uint32_t)item / (uint32_t)p.all_tiles);
     rows = p.n * p.q_rows * p.group;
     r0 = (item - piece * p.all_tiles) * kRows;
-    const Row row(p, r0 + wave * 32 + col, rows, hd, 0);
+    few = rows - r0 <= 32;
+    r = r0 + (few ? 0 : wave * 32) + col;
+    const Row row(p, r, rows, hd, 0);
     const int seq = (int)((uint32_t)row.tok / (uint32_t)p.q_rows);
     qoff = seq * p.qb + (row.tok - seq * p.q_rows) * p.qt + row.head * p.qh;
     keys = prefix_cache(p, hd);
@@ -179,7 +312,9 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
     const OwnRows w(p, seq, place - piece * p.seq_tiles);
     rows = w.rows;
     r0 = w.r0;
-    const Row row(p, r0 + wave * 32 + col, rows, hd, w.kn);
+    few = rows - r0 <= 32;
+    r = r0 + (few ? 0 : wave * 32) + col;
+    const Row row(p, r, rows, hd, w.kn);
     qoff = seq * p.qb + row.tok * p.qt + row.head * p.qh;
     keys = own_cache(p, seq, hd, w, row.seen);
     const int all = key_tiles(w.kn), size = p.places ? Pieces::even(all, ceil_div(all, cut.size)) : all;
@@ -188,17 +323,31 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
     part = own_part(p, piece) + (int64_t)row.tok * p.heads + row.head;
     sees = row.seen > t0 * kKeys;
   }
+  float* const po = p.part + part * D;
+  float4* const stat = reinterpret_cast<float4*>(p.part + all_parts(p) * D) + part;
+  float l, off;
+  if (few) {
+    float o[D / 8];
+    attend_few<T, D>(smem, reinterpret_cast<float2*>(smem + kTileBytes<D>), keys, p.q + qoff, p.c, t0, t1, l, off, o);
+    if (r >= rows) return;
+    if (half == 0 && wave == 0) *stat = make_float4(off, l, l, sees);
+    if (l == 0.0f) return;   // left out of the join by its l
+#pragma unroll
+    for (int g = 0; g < D / 32; ++g) {
+      const int at = wave * (D / 32) + g;   // of the lane's D / 8 groups of four columns
+      *reinterpret_cast<float4*>(po + 32 * (at / 4) + 8 * (at % 4) + 4 * half) =
+          make_float4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
+    }
+    return;
+  }
   v16f o[D / 32];
-  float m, l, exact, off;
-  const bool idle = r0 + wave * 32 >= rows;
-  if (rows - r0 <= 32) attend<T, D, true, true>(smem, keys, p.q + qoff, p.c, t0, t1, idle, m, l, exact, off, o);
-  else attend<T, D, false, true>(smem, keys, p.q + qoff, p.c, t0, t1, idle, m, l, exact, off, o);
+  float m, exact;
+  attend<T, D, false, true>(smem, keys, p.q + qoff, p.c, t0, t1, r0 + wave * 32 >= rows, m, l, exact, off, o);
   l = add_partner(l);
   exact = add_partner(exact);
-  if (r0 + wave * 32 + col >= rows) return;
-  float* const po = p.part + part * D;
-  if (half == 0) reinterpret_cast<float4*>(p.part + all_parts(p) * D)[part] = make_float4(off, l, exact, sees);
-  if (l == 0.0f) return;   // left out of the join by its l
+  if (r >= rows) return;
+  if (half == 0) *stat = make_float4(off, l, exact, sees);
+  if (l == 0.0f) return;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll

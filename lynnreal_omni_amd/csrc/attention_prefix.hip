@@ -22,6 +22,7 @@ namespace lr {
 namespace {
 
 constexpr int kMaxPieces = 256;   // of a cache, and of the prefix
+constexpr int kMaxCuts = 8;       // of the rows that a walk leaves behind its rounds
 
 struct PrefixArgs {
   const uint16_t *q, *pk, *pv, *k, *v;
@@ -359,11 +360,21 @@ __global__ __launch_bounds__(256, 2) void prefix_pieces(PrefixArgs p) {
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kMaxParts = 2 * kMaxPieces;
 
-// Joins the parts of a row, at(0) .. at(n - 1): weights 2^(exponent - the largest). A workgroup
-// per row: D / 4 threads hold a part's columns, and the groups of them take every G-th part,
-// then are added in order, so that the result does not depend on timing.
-template <typename T, int D, class At>
-__device__ __forceinline__ void join_row(const float* part, const float4* stats, int n, const At& at, uint16_t* out, float* lse) {
+// Joins a row's pieces of the prefix and of its cache: weights 2^(exponent - the largest). A
+// workgroup per row: D / 4 threads hold a part's columns, and the groups of them take every
+// G-th part, then are added in order, so that the result does not depend on timing.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_join(PrefixArgs p) {
+  const int64_t row = blockIdx.x;
+  const int each = p.q_rows * p.heads, seq = (int)(blockIdx.x / (uint32_t)each);
+  const int2 mine = pieces_of<D>(p)[seq];
+  const int shared = pieces_of<D>(p)[p.n].x, n = shared + mine.y;
+  const int64_t own = own_part(p, mine.x) + (row - (int64_t)seq * each);
+  auto at = [&](int i) __attribute__((always_inline)) {
+    return i < shared ? row + (int64_t)i * p.n * each : own + (int64_t)(i - shared) * each;
+  };
+  const float* const part = p.part;
+  const float4* const stats = reinterpret_cast<const float4*>(p.part + all_parts(p) * D);
   constexpr int LANES = D / 4, G = 256 / LANES, NV = kMaxParts / 64;
   __shared__ float weight[kMaxParts];
   __shared__ float4 sums[G][LANES];
@@ -419,24 +430,9 @@ __device__ __forceinline__ void join_row(const float* part, const float4* stats,
     o.w += y.w;
   }
   const float inv = l == 0.0f ? (seen != 0.0f ? NAN : 0.0f) : 1.0f / l;
-  *reinterpret_cast<uint2*>(out + 4 * x) =
+  *reinterpret_cast<uint2*>(p.out + row * D + 4 * x) =
       make_uint2(Mfma<T>::pack(o.x * inv, o.y * inv), Mfma<T>::pack(o.z * inv, o.w * inv));
-  if (lse && x == 0) *lse = l == 0.0f ? -INFINITY : kLn2 * (top + __builtin_amdgcn_logf(exact));
-}
-
-// A row's pieces of the prefix and of its cache.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void prefix_join(PrefixArgs p) {
-  const int64_t row = blockIdx.x;
-  const int each = p.q_rows * p.heads, seq = (int)(blockIdx.x / (uint32_t)each);
-  const int2 mine = pieces_of<D>(p)[seq];
-  const int shared = pieces_of<D>(p)[p.n].x;
-  const int64_t own = own_part(p, mine.x) + (row - (int64_t)seq * each);
-  auto at = [&](int i) __attribute__((always_inline)) {
-    return i < shared ? row + (int64_t)i * p.n * each : own + (int64_t)(i - shared) * each;
-  };
-  join_row<T, D>(p.part, reinterpret_cast<const float4*>(p.part + all_parts(p) * D), shared + mine.y, at, p.out + row * D,
-                 p.lse ? p.lse + row : nullptr);
+  if (p.lse && x == 0) p.lse[row] = l == 0.0f ? -INFINITY : kLn2 * (top + __builtin_amdgcn_logf(exact));
 }
 
 // The prefix, then the own cache. (Both sides of a choice are values: chosen between by
@@ -527,19 +523,65 @@ __global__ __launch_bounds__(256, 2) void prefix_walk(PrefixArgs p) {
                      Mfma<T>::pack(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
 }
 
-// The cut workgroups' rows.
+// Joins the cut workgroups' rows, as prefix_join does: a wave per row, and all of its at most
+// eight parts at once.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void walk_join(PrefixArgs p) {
-  const int run = (int)(blockIdx.x / kRows), at0 = (int)(blockIdx.x % kRows);
+  constexpr int LANES = D / 4, G = 64 / LANES, PER = kMaxCuts / G;
+  const int lane = threadIdx.x & 63, x = lane % LANES, g = lane / LANES;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int run = (int)(id / kRows), at0 = (int)(id % kRows);
   const WalkItem it(p, (uint32_t)(p.whole + run));
   const int rows = p.q_rows * p.group, r = it.tile * kRows + at0;
   if (r >= rows) return;
   const Row row(p, r, rows, it.hd, 0);
   const int64_t to = ((int64_t)it.seq * p.q_rows + row.tok) * p.heads + row.head;
-  const int64_t parts = (int64_t)p.left * p.cuts * kRows;
-  auto at = [&](int i) __attribute__((always_inline)) { return ((int64_t)run * p.cuts + i) * kRows + at0; };
-  join_row<T, D>(p.part, reinterpret_cast<const float4*>(p.part + parts * D), p.cuts, at, p.out + to * D,
-                 p.lse ? p.lse + to : nullptr);
+  const float4* const stats = reinterpret_cast<const float4*>(p.part + (int64_t)p.left * p.cuts * kRows * D);
+  const int64_t first = (int64_t)run * p.cuts * kRows + at0;
+  float4 v[kMaxCuts], y[PER];
+#pragma unroll
+  for (int i = 0; i < kMaxCuts; ++i) v[i] = i < p.cuts ? stats[first + i * kRows] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < PER; ++i)   // (what a part without keys has not written has no weight)
+    y[i] = *reinterpret_cast<const float4*>(p.part + (first + min(i * G + g, p.cuts - 1) * kRows) * D + 4 * x);
+  float top = -INFINITY, l = 0.0f, exact = 0.0f, seen = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMaxCuts; ++i) {
+    if (v[i].y != 0.0f) top = fmaxf(top, v[i].x);
+    seen = fmaxf(seen, v[i].w);
+  }
+#pragma unroll
+  for (int i = 0; i < kMaxCuts; ++i) {
+    v[i].x = v[i].y != 0.0f ? __builtin_amdgcn_exp2f(v[i].x - top) : 0.0f;
+    l += v[i].x * v[i].y;
+    exact += v[i].x * v[i].z;
+  }
+  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    float w = 0.0f;
+#pragma unroll
+    for (int j = 0; j < G; ++j) w = g == j ? v[i * G + j].x : w;
+    if (w == 0.0f) continue;
+    o[0] += w * y[i].x;
+    o[1] += w * y[i].y;
+    o[2] += w * y[i].z;
+    o[3] += w * y[i].w;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    o[e] = add_partner(o[e]);
+    if (LANES <= 16) {
+      const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(o[e]), __float_as_uint(o[e]), false, false);
+      o[e] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    if (LANES <= 8) o[e] += xor_partner<8>(o[e]);
+  }
+  if (g != 0) return;
+  const float inv = l == 0.0f ? (seen != 0.0f ? NAN : 0.0f) : 1.0f / l;
+  *reinterpret_cast<uint2*>(p.out + to * D + 4 * x) =
+      make_uint2(Mfma<T>::pack(o[0] * inv, o[1] * inv), Mfma<T>::pack(o[2] * inv, o[3] * inv));
+  if (p.lse && x == 0) p.lse[to] = l == 0.0f ? -INFINITY : kLn2 * (top + __builtin_amdgcn_logf(exact));
 }
 
 // How a call is laid over the GPU.
@@ -568,8 +610,8 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, 
   const int64_t least = pl.all_tiles + pl.seq_tiles * n, round = 2 * cus / kv_heads > 0 ? 2 * cus / kv_heads : 1;
   const int64_t places = (least * 7 / 5 + round - 1) / round * round;
   // The most pieces of the prefix, and the least tiles of one, by the cost of joining: 1 us per
-  // tile of keys against 0.15 ns per row and piece, as in attention.hip.
-  const double s = fmin(fmin(sqrt(tiles_p / (0.00015 * (double)rows)), (double)(places / pl.all_tiles)), kMaxPieces);
+  // tile of keys against 0.4 ns per row and piece.
+  const double s = fmin(fmin(sqrt(tiles_p / (0.0004 * (double)rows)), (double)(places / pl.all_tiles)), kMaxPieces);
   pl.shares = s > 1.0 ? (int)s : 1;
   const double each = fmax(1.0, fmin(sqrt(tiles_k / (0.0003 * (double)rows)), tiles_k));
   pl.piece = (int)ceil(tiles_k / each);
@@ -578,16 +620,24 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, 
   pl.own = (int)(n > kListed ? n : places / pl.seq_tiles);
   pl.parts = (pl.shares * n + pl.own) * q_rows * heads;
   pl.table = n + 1;
-  const double walk = fmax(1.0, (double)(n * pl.seq_tiles * kv_heads) / (double)cus) * (tiles_p + tiles_k);
+  // Either way in us: a tile of a row tile and head takes one, a part of a row 0.15 ns to join
+  // (2 x 400 tokens behind 3000, 40 heads over 8: 79 us cut into pieces, walked 116 us).
+  constexpr double kJoin = 0.00015;
+  const double tiles = tiles_p + tiles_k;
   const double pieces = ((double)pl.all_tiles * tiles_p + (double)(n * pl.seq_tiles) * tiles_k) * kv_heads / (double)cus +
-                        2.8 + (double)rows * (0.0006 + 0.00015 * pl.shares);
-  pl.walk = walk <= pieces || rows > kMaxBlocks;
+                        2.8 + (double)rows * (0.0006 + kJoin * pl.shares);
+  // A walk: two workgroups per CU are resident, for which a tile takes twice as long as for one.
+  // What is left behind full rounds is cut so that it fills the GPU once more, for a part
+  // of a round (at most eight, for what is written and read again).
+  const int64_t items = n * pl.seq_tiles * kv_heads, slots = 2 * cus, left = items % slots;
+  const int64_t cuts = left > 0 ? slots / left : 1;
+  pl.cuts = cuts > kMaxCuts ? kMaxCuts : (int)cuts;
+  double walk = (double)(items / slots) * tiles * 2.0;
+  if (pl.cuts > 1) walk += ceil(tiles / pl.cuts) * 2.0 + 2.8 + (double)(left * kRows) * (0.0002 + kJoin * pl.cuts);
+  else if (left > 0) walk += tiles * (left > cus ? 2.0 : 1.0);
+  // (One wave's rows are not walked: the walk has its matrix instructions for four.)
+  pl.walk = (q_rows * group > 32 && walk <= pieces) || rows > kMaxBlocks;
   if (pl.walk) {
-    // Two workgroups per CU are resident. What is left behind full rounds is cut so that it fills
-    // the GPU once more, for a part of a round (8 at most, for what is written and read again).
-    const int64_t items = n * pl.seq_tiles * kv_heads, slots = 2 * cus, left = items % slots;
-    const int64_t cuts = left > 0 ? slots / left : 1;
-    pl.cuts = cuts > 8 ? 8 : (int)cuts;
     pl.left = pl.cuts > 1 ? left : 0;
     pl.whole = items - pl.left;
     pl.parts = pl.left * pl.cuts * kRows;
@@ -605,7 +655,7 @@ int launch(const PrefixArgs& p, const Plan& pl, hipStream_t s) {
     else prefix_walk<T, D, false><<<(unsigned)grid, 256, 0, s>>>(p);
     if (int rc = check_launch("attention_prefix")) return rc;
     if (pl.left == 0) return LR_OK;
-    walk_join<T, D><<<(unsigned)(pl.left * kRows), 256, 0, s>>>(p);
+    walk_join<T, D><<<(unsigned)(pl.left * kRows / 4), 256, 0, s>>>(p);
     return check_launch("attention_prefix");
   }
   const int64_t grid = (p.places ? p.places : pl.shares * pl.all_tiles + p.n * pl.seq_tiles) * p.kv_heads;

@@ -131,6 +131,37 @@ def test_weights_of_views(new):
     assert torch.equal(cache.accumulate_weights(w, *odd, lse), want)
 
 
+@pytest.mark.parametrize("batch", [512, 513])
+@pytest.mark.parametrize("new", [1, 4])
+def test_weights_of_many_caches(batch, new):
+    w, q, k = make(batch, new, 150, 4, 2, 32, torch.bfloat16, batch)
+    lengths = [(37 * i) % 152 for i in range(batch)]
+    lse = sums_of(q, k, lengths, True)
+    got = cache.accumulate_weights(w, q, k, lse, causal=True, key_lengths=torch.tensor(lengths, device="cuda"))
+    check(got, w, q, k, lse, lengths, True, 32 ** -0.5)
+
+
+@pytest.mark.parametrize("new,heads", [(1, 32), (1, 33), (16, 2), (32, 1), (33, 1)])
+def test_weights_around_32_rows(new, heads):
+    w, q, k = make(2, new, 1500, heads, 1, 64, torch.float16, new + heads)
+    lengths = [1500, 700]
+    lse = sums_of(q, k, lengths, True)
+    got = cache.accumulate_weights(w, q, k, lse, causal=True, key_lengths=torch.tensor(lengths, device="cuda"))
+    check(got, w, q, k, lse, lengths, True, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_weights_of_far_keys(new):
+    """Keys past 2^31 elements of the first."""
+    size, step = 300, 2 ** 23 - 64
+    k = torch.empty(size * step, dtype=torch.bfloat16, device="cuda").as_strided((1, size, 1, 64), (size * step, step, 64, 1))
+    assert (size - 1) * step > 2 ** 31
+    w, q, near = make(1, new, size, 3, 1, 64, torch.bfloat16, new)
+    k.copy_(near)
+    lse = sums_of(q, near, None, False)
+    assert torch.equal(cache.accumulate_weights(w, q, k, lse), cache.accumulate_weights(w, q, near, lse))
+
+
 def kept_of(weights, length, budget, recent):
     """The rule, for one head: the places that stay."""
     if length <= budget:

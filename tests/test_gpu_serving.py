@@ -135,3 +135,39 @@ def test_requests_over_a_shared_prefix():
         check_adapters(out.view(batch * new, -1), x.view(batch * new, -1), layer.out.layer(x).view(batch * new, -1),
                        picks.repeat_interleave(new), *layer.weights[1])
     assert evictions == 2
+
+
+@torch.inference_mode()
+def test_two_streams_at_once():
+    """Two batches on streams of their own, whose calls run beside each other: each has what it has alone."""
+    heads, kv_heads, dim, batch = 8, 2, 64, 3
+
+    def make(seed):
+        g = torch.Generator().manual_seed(seed)
+        q, k, v = (torch.randn(batch, n, h, dim, generator=g).bfloat16().cuda()
+                   for n, h in ((1, heads), (40000, kv_heads), (40000, kv_heads)))
+        prefix = torch.randn(5000, kv_heads, dim, generator=g).bfloat16().cuda()
+        weights = torch.rand(batch, kv_heads, 40000, generator=g).cuda()
+        x = torch.randn(700, 512, generator=g).bfloat16().cuda()
+        base = torch.randn(700, 1024, generator=g).bfloat16().cuda()
+        adapters = L.LowRankAdapters(*some_adapters(5, 32, 1024, 512, torch.bfloat16, seed))
+        return q, k, v, prefix, weights, x, base, adapters, torch.randint(-1, 5, (700,), generator=g).cuda()
+
+    def run(q, k, v, prefix, weights, x, base, adapters, picks):
+        out, lse = attention_shared_prefix(q, prefix, prefix, k, v, return_lse=True)
+        weights = cache.accumulate_weights(weights, q, k, lse)
+        return out, lse, weights, *cache.evict(k, v, weights, None, 9000, recent=9), adapters(x, base, L.AdapterPlan(picks, 5))
+
+    given = [make(seed) for seed in (1, 2)]
+    want = [run(*args) for args in given]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in given]
+    got = [[] for _ in given]
+    for _ in range(6):
+        for stream, args, results in zip(streams, given, got):
+            with torch.cuda.stream(stream):
+                results.append(run(*args))
+    torch.cuda.synchronize()
+    for results, alone in zip(got, want):
+        for result in results:
+            assert all(torch.equal(a, b) for a, b in zip(result, alone))

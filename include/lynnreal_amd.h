@@ -420,7 +420,7 @@ int lr_attention_prefix(const void* q, const void* prefix_k, const void* prefix_
  * lr_attention, for dense batches; strides, six: of q (token, head, sequence), then k.
  * workspace of the bytes that lr_attention_weights_workspace gives (0: it may be NULL). */
 int lr_attention_weights_workspace(int64_t sequences, int64_t q_rows, int64_t k_rows, int heads, int kv_heads,
-                                   int head_dim, int causal, int64_t* bytes);
+                                   int head_dim, int64_t* bytes);
 int lr_attention_weights(const void* q, const void* k, const float* lse, const float* weights, float* out, int dtype,
                          int64_t sequences, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int head_dim,
                          const int64_t* strides, const int32_t* key_lengths, int causal, int scale_bits,

@@ -74,7 +74,7 @@ SIGNATURES = {
     "lr_attention_prefix_workspace": [_I64, _I64, _I64, _I64, _I32, _I32, _I32, _P],
     "lr_attention_prefix": [_P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32,
                             _I32, _P, _I64, _P],
-    "lr_attention_weights_workspace": [_I64, _I64, _I64, _I32, _I32, _I32, _I32, _P],
+    "lr_attention_weights_workspace": [_I64, _I64, _I64, _I32, _I32, _I32, _P],
     "lr_attention_weights": [_P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32, _I32, _P, _I64,
                              _P],
     "lr_cache_evict_workspace": [_I64, _I64, _I32, _P],

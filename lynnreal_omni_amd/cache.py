@@ -43,11 +43,10 @@ def _no_gradients(*tensors):
 
 
 @functools.lru_cache(maxsize=4096)
-def _weights_workspace(device, batch, tokens, keys, heads, kv_heads, dim, causal):
+def _weights_workspace(device, batch, tokens, keys, heads, kv_heads, dim):
     nbytes = array("q", [0])
     with torch.cuda.device(device):
-        _lib.call("lr_attention_weights_workspace", batch, tokens, keys, heads, kv_heads, dim, causal,
-                  nbytes.buffer_info()[0])
+        _lib.call("lr_attention_weights_workspace", batch, tokens, keys, heads, kv_heads, dim, nbytes.buffer_info()[0])
     return nbytes[0]
 
 
@@ -105,7 +104,7 @@ def accumulate_weights(weights, query, key, lse, *, causal=False, scale=None, ke
     if strides is None:
         query, key = query.clone(memory_format=torch.contiguous_format), _attention._rows(key)
         strides = _six_strides(query.stride(), key.stride(), True, query.shape, key.shape)
-    nbytes = _weights_workspace(query.get_device(), batch, tokens, keys, heads, kv_heads, dim, int(bool(causal)))
+    nbytes = _weights_workspace(query.get_device(), batch, tokens, keys, heads, kv_heads, dim)
     ws = _lib.workspace(query, nbytes) if nbytes else None   # held until the launch
     _lib.launch(query, "lr_attention_weights", query.data_ptr(), key.data_ptr(), lse.data_ptr(), weights.data_ptr(),
                 out.data_ptr(), _attention._DTYPES[query.dtype], batch, tokens, keys, heads, kv_heads, dim,

@@ -7,7 +7,9 @@
 // transpose of what attention does, so a workgroup keeps keys, in registers, and the
 // queries go by: S^T = K Q^T on the 32x32x16 MFMA leaves a lane with 16 keys of one query,
 // each added to its own fp32 sum; the sums over the 32 lanes come once at the end. Every
-// key is read once, and the order of additions does not depend on timing.
+// key is read once, and the order of additions does not depend on timing. With few rows the keys'
+// stream bounds it; with many the exponentials and the matrix instructions do (a prompt of 3683
+// tokens, 40 heads over 8: 115 us causal, 169 where every row sees every key).
 //
 // Eviction reads the weights, finds for every cache and head the keys that stay, and moves
 // their rows to another cache, in their order.
@@ -36,14 +38,15 @@ struct WeighArgs {
   const uint16_t *q, *k;
   const float *lse, *w;   // lse [n][q_rows][heads]; w, out [n][kv_heads][k_rows]
   float* out;
-  float* part;            // sums of splits of the rows [splits][n][kv_heads][k_rows]
+  float* part;            // sums of a share's first and last keys [kv_heads][shares][2][256]
   int64_t qt, qh, qb, kt, kh, kb;
   const int32_t* lengths;
   int n, q_rows, k_rows, heads, kv_heads, group;
-  int causal, splits;     // splits: of the rows, `chunk` tiles of 64 each
-  int chunk;
+  int causal;
+  int shares;             // of a key head's work; 0: a workgroup for every 128 keys
   int places;             // few rows: pieces of all caches for a key head
   float c;                // scale * log2(e)
+  float one_by_group;
   Divisor by_group;
 };
 
@@ -63,42 +66,98 @@ __device__ __forceinline__ float half_sum(float v) {
   return v + xor_partner<1>(v);
 }
 
+constexpr int kGroup = 128;        // keys
+constexpr int kDealt = 256;        // keys of a group that is dealt out
+constexpr int kShared = 64;        // caches at most that are dealt out in shares: one per lane
+constexpr int kLeastShare = 256;   // rows
+
+// A cache's keys in groups of KEYS, each with the rows that see any of it: from `first` on.
+template <int KEYS>
+struct Seen {
+  int kn, rows, hidden, group, causal;   // causal: token t sees keys up to hidden + t
+  __device__ __forceinline__ Seen(const WeighArgs& p, int seq)
+      : kn(keys_of(p.lengths, seq, p.k_rows)), rows(p.q_rows * p.group), hidden(kn - p.q_rows), group(p.group), causal(p.causal) {}
+  __device__ __forceinline__ int groups() const { return ceil_div(kn, KEYS); }
+  __device__ __forceinline__ int first(int g) const { return causal ? max(0, g * KEYS - hidden) * group : 0; }   // < rows
+  // The rows of groups 0 .. g - 1, one group's behind the other's. `whole` of them have all rows.
+  __device__ __forceinline__ int64_t before(int g) const {
+    const int whole = causal ? (hidden < 0 ? 0 : min(g, hidden / KEYS + 1)) : g;
+    const int64_t m = g - whole;
+    return (int64_t)g * rows - group * (m * (whole * KEYS - hidden) + KEYS / 2 * m * (m - 1));
+  }
+  // The group that has row x of them.
+  __device__ __forceinline__ int find(int64_t x) const {
+    int lo = 0, hi = groups() - 1;
+    while (lo < hi) {
+      const int mid = lo + (hi - lo + 1) / 2;
+      if (before(mid) <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+};
+
+// All caches' rows, one cache's behind the other's, dealt out in even shares. Every wave works it
+// out from the lengths by itself.
+struct Deal {
+  int64_t upto;   // the caches 0 .. lane
+  int64_t all, each;
+  static __device__ __forceinline__ int64_t of_lane(int64_t v, int lane) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+  }
+  __device__ __forceinline__ explicit Deal(const WeighArgs& p) {
+    const int lane = threadIdx.x & 63;
+    const Seen<kDealt> mine(p, min(lane, p.n - 1));
+    upto = lane < p.n ? mine.before(mine.groups()) : 0;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int64_t y = __shfl_up(upto, o);
+      upto += lane >= o ? y : 0;
+    }
+    all = of_lane(upto, 63);
+    each = ((all + p.shares - 1) / p.shares + kKeys - 1) / kKeys * kKeys;
+    each = of_lane(each < kLeastShare ? kLeastShare : each, 0);   // (a division is a vector's work)
+  }
+  __device__ __forceinline__ explicit Deal(int64_t known) : upto(known), all(0), each(0) {}
+  __device__ __forceinline__ int cache_of(int64_t x) const { return __builtin_ctzll(__ballot(upto > x)); }
+  __device__ __forceinline__ int64_t before(int seq) const { return seq ? of_lane(upto, seq - 1) : 0; }
+};
+
 // Four waves with KB blocks of 32 keys each; queries in tiles of 64 rows, with their sums,
-// through a ring in the LDS that first holds the keys on their way to the registers. Swizzle as
-// in lr_attention.h.
+// through a ring in the LDS that first holds the keys on their way to the registers. Swizzle as in
+// lr_attention.h. KB = 1: a workgroup for every 128 keys. KB = 2, which halves what the
+// queries' fragments take of the LDS: a workgroup has a share of its key head's work, rows of one
+// group of keys after the other, and sums of a group that is not its alone go to `part`. (Equal
+// runs of each group's rows instead left a third of the CUs idle where causal: the prompt of
+// 3683 tokens 138 us. Tokens and heads of a tile's rows by whole divisions in every tile: 8% more.)
 template <typename T, int D, int KB>
-__global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
+__global__ __launch_bounds__(256, 4 / KB) void weigh_keys(WeighArgs p) {
   typedef typename Mfma<T>::V V8;
   constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32, KD = D / 16;
-  constexpr int WAVES = 4, TILE = kKeys * ROW, DMAS = TILE / 1024 / WAVES, KEYS = 32 * WAVES * KB;
+  constexpr int WAVES = 4, TILE = kKeys * ROW, DMAS = TILE / 1024 / WAVES, KEYS = 128 * KB;
+  constexpr bool DEALT = KB == 2;
   constexpr int RING = KEYS / kKeys, LOADS = DMAS + 1;   // slots that fit into the keys' LDS; DMAs per wave and tile
   // (One array for all of it: between two the compiler waits for every DMA before any read.)
-  __shared__ __attribute__((aligned(1024))) char smem[KEYS * (ROW + 4) + RING * WAVES * kKeys * 4];
+  __shared__ __attribute__((aligned(1024))) char smem[KEYS * (ROW + 4) + RING * WAVES * kKeys * 4 + (DEALT ? kShared * 8 : 0)];
   float* const sums = reinterpret_cast<float*>(smem + KEYS * ROW);
   char* const lses = smem + KEYS * (ROW + 4);   // [RING][WAVES][64], each wave's own
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int half = lane >> 5, col = lane & 31;
-  // Heads, which lie side by side, first; then sequences, so that the first keys, which
-  // the most rows see where causal, come first.
-  uint32_t id = blockIdx.x;
-  const int hd = (int)(id % (uint32_t)p.kv_heads);
-  id /= (uint32_t)p.kv_heads;
-  const int seq = (int)(id % (uint32_t)p.n);
-  id /= (uint32_t)p.n;
-  const int split = (int)(id % (uint32_t)p.splits), key0 = (int)(id / (uint32_t)p.splits) * KEYS;
-  const int kn = keys_of(p.lengths, seq, p.k_rows);
-  const int hidden = kn - p.q_rows;   // causal: token t sees keys up to hidden + t
-  const int rows = p.q_rows * p.group;
-  const int first = p.causal ? (int)min((int64_t)rows, max(0, key0 - hidden) * (int64_t)p.group) : 0;
-  const int tiles = key0 < kn ? (rows - first + kKeys - 1) / kKeys : 0;
-  // Splits of one size, whatever the keys' own number of rows: causal ones are then as long.
-  const int t0 = min(tiles, split * p.chunk), t1 = min(tiles, t0 + p.chunk);
-  float acc[KB][16];
+  int64_t* const uptos = reinterpret_cast<int64_t*>(lses + RING * WAVES * kKeys * 4);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Heads, which lie side by side, first.
+  const int share = (int)(blockIdx.x / (uint32_t)p.kv_heads), hd = (int)(blockIdx.x - share * p.kv_heads);
+  // Adds rows r_from .. rows - 1 to group g's sums, which are then in `sums`.
+  auto weigh = [&](int seq, int g, int r_from, int rows) __attribute__((always_inline)) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));   // what follows from it does not stay in registers between groups
+    const int half = lane >> 5, col = lane & 31;
+    const int kn = keys_of(p.lengths, seq, p.k_rows), hidden = kn - p.q_rows;
+    const int key0 = g * KEYS, tiles = (rows - r_from + kKeys - 1) / kKeys;
+    float acc[KB][16];
 #pragma unroll
-  for (int b = 0; b < KB; ++b)
+    for (int y = 0; y < KB; ++y)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[b][e] = 0.0f;
-  if (t0 < t1) {
+      for (int e = 0; e < 16; ++e) acc[y][e] = 0.0f;
     auto publish = [&](auto left) __attribute__((always_inline)) {   // loads that may still be on their way
       constexpr int N = decltype(left)::value;
       __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x70 | 0xf00);
@@ -114,54 +173,57 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
     };
     const uint16_t* const kbase = p.k + seq * p.kb + hd * p.kh;
 #pragma unroll
-    for (int g = 0; g < KEYS / kKeys; ++g) {
-      const int left = min(kKeys, kn - key0 - g * kKeys);   // keys past the last read as zero
-      const __amdgpu_buffer_rsrc_t r = row_rsrc(kbase + (key0 + (int64_t)g * kKeys) * p.kt,
+    for (int x = 0; x < KEYS / kKeys; ++x) {
+      const int left = min(kKeys, kn - key0 - x * kKeys);   // keys past the last read as zero
+      const __amdgpu_buffer_rsrc_t r = row_rsrc(kbase + (left > 0 ? (key0 + (int64_t)x * kKeys) * p.kt : 0),
                                                 left > 0 ? ((int64_t)(left - 1) * p.kt + D) * 2 : 0);
 #pragma unroll
       for (int i = 0; i < DMAS; ++i)
-        dma16(r, smem + g * TILE + (wave * DMAS + i) * 1024, (uint32_t)(slot_row(i) * p.kt * 2 + slot_chunk(i) * 16));
+        dma16(r, smem + x * TILE + (wave * DMAS + i) * 1024, (uint32_t)(slot_row(i) * p.kt * 2 + slot_chunk(i) * 16));
     }
     publish(std::integral_constant<int, 0>{});
     V8 kf[KB][KD];
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      const int row = (wave * KB + b) * 32 + col;
+    for (int y = 0; y < KB; ++y) {
+      const int row = (wave * KB + y) * 32 + col;
 #pragma unroll
       for (int d = 0; d < KD; ++d)
-        kf[b][d] = *reinterpret_cast<const V8*>(smem + row * ROW + ((2 * d + half) ^ (row / RPB % PAIRS) * 2) * 16);
+        kf[y][d] = *reinterpret_cast<const V8*>(smem + row * ROW + ((2 * d + half) ^ (row / RPB % PAIRS) * 2) * 16);
     }
     __syncthreads();   // the keys are in registers: the queries may take their place
     const uint16_t* const qbase = p.q + seq * p.qb + (int64_t)hd * p.group * p.qh;
     const float* const lbase = p.lse + (int64_t)seq * p.q_rows * p.heads + hd * p.group;
-    // Rows past the last one repeat it and are masked; tiles past the last one, which keep
-    // the count of loads the same, repeat that.
+    // The token, from r0's on, and the head that row r0 + i is of, where r0 is `ph` rows behind its
+    // token's first: quotient and rest by `group` of a number below group + 64, in fp32 (its error
+    // of 2^-17 at most is less than the half that keeps it from a whole number, 0.5 / group).
+    auto token_of = [&](int i, int ph) __attribute__((always_inline)) { return (int)(((float)(ph + i) + 0.5f) * p.one_by_group); };
+    uint32_t qoff[DMAS];   // as if of one token
+#pragma unroll
+    for (int i = 0; i < DMAS; ++i) qoff[i] = (uint32_t)(slot_row(i) * p.qh * 2 + slot_chunk(i) * 16);
+    const uint32_t turn_q = (uint32_t)((p.qt - p.group * p.qh) * 2), turn_l = (uint32_t)(p.heads - p.group);
+    // Rows past the last one, which are masked, read others between the first and the last, or
+    // zero; tiles past the last one, which keep the count of loads the same, repeat that.
     auto issue = [&](int t) {
-      const int slot = (t - t0) % RING, r0 = first + min(t, t1 - 1) * kKeys, tok0 = p.by_group.of(r0);
+      const int slot = t % RING, r0 = r_from + min(t, tiles - 1) * kKeys, tok0 = p.by_group.of(r0), ph = r0 - tok0 * p.group;
       const int toks = min(kKeys, p.q_rows - tok0);   // that 64 rows from r0 on can have
       const __amdgpu_buffer_rsrc_t rs =
           row_rsrc(qbase + (int64_t)tok0 * p.qt, ((toks - 1) * p.qt + (p.group - 1) * p.qh + D) * 2);
+      const uint32_t at = (uint32_t)(ph * p.qh * 2);
 #pragma unroll
-      for (int i = 0; i < DMAS; ++i) {
-        const int r = min(r0 + slot_row(i), rows - 1), tok = p.by_group.of(r);
-        dma16(rs, smem + slot * TILE + (wave * DMAS + i) * 1024,
-              (uint32_t)((tok - tok0) * p.qt * 2 + (r - tok * p.group) * p.qh * 2 + slot_chunk(i) * 16));
-      }
+      for (int i = 0; i < DMAS; ++i)
+        dma16(rs, smem + slot * TILE + (wave * DMAS + i) * 1024, qoff[i] + at + token_of(slot_row(i), ph) * turn_q);
       const __amdgpu_buffer_rsrc_t ls =
           row_rsrc(lbase + (int64_t)tok0 * p.heads, ((int64_t)(toks - 1) * p.heads + p.group) * 4);
-      const int r = min(r0 + lane, rows - 1), tok = p.by_group.of(r);
-      dma4(ls, lses + (slot * WAVES + wave) * kKeys * 4, (uint32_t)(((tok - tok0) * p.heads + r - tok * p.group) * 4));
+      dma4(ls, lses + (slot * WAVES + wave) * kKeys * 4, (ph + lane + token_of(lane, ph) * turn_l) * 4);
     };
-    // Adds a block's shares, which are those of keys past `lim` too where WHOLE. lim counts from
-    // the lane's first key on.
-    const int own = key0 + wave * KB * 32 + 4 * half;
-    auto add = [&](const v16f (&s)[KB], float l2, int lim, int x, int e, auto whole) __attribute__((always_inline)) {
-      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], p.c, -l2));
-      acc[x][e] += decltype(whole)::value || 32 * x + 8 * (e >> 2) + (e & 3) < lim ? w : 0.0f;
+    float l2 = INFINITY;   // of the block before: its row's lse * log2(e)
+    auto add = [&](const v16f (&s)[KB], int i, bool sees) __attribute__((always_inline)) {
+      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 16][i % 16], p.c, -l2));
+      acc[i / 16][i % 16] += sees ? w : 0.0f;
     };
-    // The scores of block b of a tile, while the exponentials of the block before, which every
-    // row sees whole, run between the matrix instructions.
-    auto product = [&](v16f (&s)[KB], const char* qs, int b, const v16f (&before)[KB], float l2) __attribute__((always_inline)) {
+    // The scores of block b of a tile, while the exponentials of the block before run between the
+    // matrix instructions.
+    auto product = [&](v16f (&s)[KB], const char* qs, int b, const v16f (&before)[KB]) __attribute__((always_inline)) {
       constexpr int AHEAD = KD < 3 ? KD : 3;
       V8 qf[4];
       // (2 d + half) ^ turn, hidden so that its values for every d do not stay in registers.
@@ -177,81 +239,126 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
       for (int d = 0; d < KD; ++d) {
         if (d + AHEAD < KD) qf[(d + AHEAD) & 3] = read(d + AHEAD);
 #pragma unroll
-        for (int x = 0; x < KB; ++x) s[x] = Mfma<T>::mul(kf[x][d], qf[d & 3], d ? s[x] : zero);
+        for (int y = 0; y < KB; ++y) s[y] = Mfma<T>::mul(kf[y][d], qf[d & 3], d ? s[y] : zero);
 #pragma unroll
-        for (int i = 16 * KB * d / KD; i < 16 * KB * (d + 1) / KD; ++i) add(before, l2, 0, i / 16, i % 16, std::true_type{});
+        for (int i = 16 * KB * d / KD; i < 16 * KB * (d + 1) / KD; ++i) {
+          add(before, i, true);
+          asm volatile("" : "+v"(acc[i / 16][i % 16]));   // here, not behind the branch that follows
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    // A block without shares, for the start and behind one that was not whole.
     v16f s0[KB] = {}, s1[KB] = {};
-    float l2 = INFINITY;   // of the block before
-    auto block = [&](v16f (&s)[KB], v16f (&before)[KB], const char* qs, int t, int b, float sum2, int lim) __attribute__((always_inline)) {
-      product(s, qs, b, before, l2);
+    auto block = [&](v16f (&s)[KB], v16f (&before)[KB], const char* qs, int t, int b, float sum2) __attribute__((always_inline)) {
+      product(s, qs, b, before);
       l2 = sum2;
-      const int r0 = first + t * kKeys + 32 * b;
-      if (r0 + 32 <= rows && (!p.causal || hidden + p.by_group.of(r0) + 1 >= key0 + KEYS)) return;
+      const int wave0 = key0 + wave * KB * 32, r0 = r_from + t * kKeys + 32 * b, tok0 = p.by_group.of(r0);
+      if (r0 + 32 <= rows && (!p.causal || hidden + tok0 + 1 >= wave0 + 32 * KB)) return;
+      // The keys that the lane's row sees, from the lane's first one on. A score of -infinity
+      // stands for the others, or an infinite sum for all of them.
+      const int own = wave0 + 4 * half;
+      const int lim = r0 + col >= rows ? 0 : (p.causal ? hidden + tok0 + token_of(col, r0 - tok0 * p.group) + 1 : kn) - own;
+      auto sees = [&](int i) __attribute__((always_inline)) { return 32 * (i / 16) + 8 * (i % 16 >> 2) + (i & 3) < lim; };
+      if (__ballot(lim > 0 && l2 == -INFINITY) == 0) {
 #pragma unroll
-      for (int x = 0; x < KB; ++x)
+        for (int i = 0; i < 16 * KB; ++i) s[i / 16][i % 16] = sees(i) ? s[i / 16][i % 16] : -INFINITY;
+        if (lim <= 0) l2 = INFINITY;
+        return;
+      }
+      // (Rows whose scores are all -infinity, whose shares are NaN, but not those of keys they do not see.)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          add(s, l2, lim, x, e, std::false_type{});
-          s[x][e] = 0.0f;
-        }
+      for (int i = 0; i < 16 * KB; ++i) {
+        add(s, i, sees(i));
+        s[i / 16][i % 16] = 0.0f;
+      }
       l2 = INFINITY;
     };
 #pragma unroll
-    for (int i = 0; i < RING - 1; ++i) issue(t0 + i);
+    for (int i = 0; i < RING - 1; ++i) issue(i);
 #pragma unroll 1
-    for (int t = t0; t < t1; ++t) {
+    for (int t = 0; t < tiles; ++t) {
       publish(std::integral_constant<int, (RING - 2) * LOADS>{});   // tile t; every wave is done with tile t - 1
       issue(t + RING - 1);
-      const int slot = (t - t0) % RING;
+      const int slot = t % RING;
       const char* const qs = smem + slot * TILE;
-      // Of the lane's row in each block: lse * log2(e), and the keys that it sees.
+      // lse * log2(e) of the lane's row in each block.
       float now[2];
-      int lim[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b)
         now[b] = reinterpret_cast<const float*>(lses)[(slot * WAVES + wave) * kKeys + 32 * b + col] * kLog2e;
-        const int r = first + t * kKeys + 32 * b + col;
-        lim[b] = r >= rows ? 0 : (p.causal ? hidden + p.by_group.of(r) + 1 : kn) - own;
-      }
-      block(s0, s1, qs, t, 0, now[0], lim[0]);
-      if (first + t * kKeys + 32 >= rows) {   // the last tile, without a second block
+      block(s0, s1, qs, t, 0, now[0]);
+      if (r_from + t * kKeys + 32 >= rows) {   // the last tile, without a second block
 #pragma unroll
-        for (int x = 0; x < KB; ++x)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            add(s0, l2, 0, x, e, std::true_type{});
-            s1[x][e] = 0.0f;
-          }
-        l2 = INFINITY;
+        for (int i = 0; i < 16 * KB; ++i) s1[i / 16][i % 16] = s0[i / 16][i % 16];
         break;
       }
-      block(s1, s0, qs, t, 1, now[1], lim[1]);
+      block(s1, s0, qs, t, 1, now[1]);
     }
 #pragma unroll
-    for (int x = 0; x < KB; ++x)
+    for (int i = 0; i < 16 * KB; ++i) add(s1, i, true);
+    __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);   // the last DMAs have landed before the LDS goes to another
 #pragma unroll
-      for (int e = 0; e < 16; ++e) add(s1, l2, 0, x, e, std::true_type{});
-  }
-  __builtin_amdgcn_s_waitcnt(0x70 | 0xf00);   // the last DMAs have landed before the LDS goes to another
-#pragma unroll
-  for (int x = 0; x < KB; ++x)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float v = half_sum(acc[x][e]);
-      if (col == 0) sums[(wave * KB + x) * 32 + 8 * (e >> 2) + 4 * half + (e & 3)] = v;
+    for (int i = 0; i < 16 * KB; ++i) {
+      const int y = i / 16, e = i % 16;
+      const float v = half_sum(acc[y][e]);
+      if (col == 0) sums[(wave * KB + y) * 32 + 8 * (e >> 2) + 4 * half + (e & 3)] = v;
     }
-  __syncthreads();
-  const int64_t at = ((int64_t)seq * p.kv_heads + hd) * p.k_rows + key0;
-  for (int i = threadIdx.x; i < KEYS; i += 256) {
-    if (key0 + i >= p.k_rows) return;
-    // Places behind the cache's keys stay as they were.
-    if (p.splits > 1) p.part[(int64_t)split * p.n * p.kv_heads * p.k_rows + at + i] = key0 + i < kn ? sums[i] : 0.0f;
-    else p.out[at + i] = key0 + i < kn ? p.w[at + i] + sums[i] : p.w[at + i];
+    __syncthreads();
+  };
+  const int i = (int)threadIdx.x;
+  if constexpr (!DEALT) {
+    const int seq = share % p.n, g = share / p.n, key = g * KEYS + i;
+    const Seen<KEYS> seen(p, seq);
+    const bool any = g < seen.groups() && seen.rows > 0;
+    if (any) weigh(seq, g, seen.first(g), seen.rows);
+    if (i >= KEYS || key >= p.k_rows) return;
+    const int64_t at = ((int64_t)seq * p.kv_heads + hd) * p.k_rows + key;
+    p.out[at] = any && key < seen.kn ? p.w[at] + sums[i] : p.w[at];   // places behind the keys stay as they were
+  } else {
+    const Deal deal(p);
+    uptos[i & 63] = deal.upto;   // the same from every wave
+    const int64_t begin = share * deal.each, end = min(deal.all, begin + deal.each);
+    for (int64_t x = begin; x < end;) {
+      const Deal known(uptos[i & 63]);
+      const int seq = known.cache_of(x);
+      const Seen<KEYS> seen(p, seq);
+      const int64_t here = x - known.before(seq);
+      const int g = __builtin_amdgcn_readfirstlane(seen.find(here)), key = g * KEYS + i, first = seen.first(g);
+      const int r_from = first + (int)(here - seen.before(g)), to = (int)min((int64_t)seen.rows, r_from + (end - x));
+      weigh(seq, g, r_from, to);
+      if (key < keys_of(p.lengths, seq, p.k_rows)) {
+        const int64_t at = ((int64_t)seq * p.kv_heads + hd) * p.k_rows + key;
+        if (r_from == first && to == p.q_rows * p.group) p.out[at] = p.w[at] + sums[i];
+        else p.part[(((int64_t)hd * p.shares + share) * 2 + (x != begin)) * KEYS + i] = sums[i];
+      }
+      x += to - r_from;
+    }
   }
+}
+
+// Adds to the keys of a group that several shares have what each of them found, in order. Places
+// behind the caches' keys stay as they were.
+__global__ __launch_bounds__(kDealt) void join_shares(WeighArgs p) {
+  const int hd = (int)(blockIdx.x % (uint32_t)p.kv_heads), rest = (int)(blockIdx.x / (uint32_t)p.kv_heads);
+  const int seq = rest % p.n, g = rest / p.n, i = (int)threadIdx.x, key = g * kDealt + i;
+  const Seen<kDealt> seen(p, seq);
+  const Deal deal(p);
+  if (key >= p.k_rows) return;
+  const int64_t at = ((int64_t)seq * p.kv_heads + hd) * p.k_rows + key;
+  if (key >= seen.kn || deal.all == 0) {
+    if (p.out != p.w) p.out[at] = p.w[at];
+    return;
+  }
+  const int64_t from = deal.before(seq) + seen.before(g), to = deal.before(seq) + seen.before(g + 1);
+  const int s0 = (int)(from / deal.each), s1 = (int)((to - 1) / deal.each);
+  if (s0 == s1) return;   // that share has written it
+  float v = 0.0f;
+  for (int s = s0; s <= s1; ++s) {
+    // It is the first of a share's groups where the share begins inside of it.
+    const float* const part = p.part + (((int64_t)hd * p.shares + s) * 2 + (s * deal.each < from)) * kDealt;
+    v += part[i];
+  }
+  p.out[at] = p.w[at] + v;
 }
 
 // At most 32 rows per key head: what counts is the stream of keys. They are cut into pieces
@@ -260,7 +367,6 @@ __global__ __launch_bounds__(256, 2) void weigh_keys(WeighArgs p) {
 // keys are on their way while these are worked on.
 // (Eight caches of 16152 keys in all, places for 65536, 40 heads over 8: 17.2 us with a workgroup
 // for every 128 places of every cache.)
-constexpr int kGroup = 128;
 constexpr int kCopied = 1024;   // places behind the caches' keys that a workgroup copies at a time
 
 template <typename T, int D>
@@ -345,15 +451,6 @@ __global__ __launch_bounds__(256, 4) void weigh_few(WeighArgs p) {
       if (key >= kn && key < p.k_rows) p.out[row * p.k_rows + key] = p.w[row * p.k_rows + key];
     }
   }
-}
-
-// out = w + the splits' sums, in order.
-__global__ __launch_bounds__(256) void add_splits(const float* part, const float* w, float* out, int64_t n, int splits) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float v = part[i];
-  for (int s = 1; s < splits; ++s) v += part[s * n + i];
-  out[i] = w[i] + v;
 }
 
 // ------------------------------------------------------------- eviction ----
@@ -596,37 +693,30 @@ __global__ __launch_bounds__(256) void move_rows(EvictArgs p) {
 }
 
 struct WeighPlan {
-  int blocks, splits, chunk;   // of 32 keys per wave; of the rows, and their tiles
-  int places;                  // of pieces for a key head (few rows), else 0
-  int64_t grid;
+  int shares;   // of a key head's work (0: a workgroup for every 128 keys)
+  int places;   // of pieces for a key head (few rows), else 0
+  int64_t grid, join;
+  int64_t bytes(int kv_heads) const { return (int64_t)shares * kv_heads * 2 * kDealt * 4; }
 };
 
-WeighPlan weigh_plan(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, bool causal) {
-  WeighPlan pl;
-  const int64_t rows = q_rows * (heads / kv_heads), tiles = (rows + kKeys - 1) / kKeys, cus = compute_units();
-  auto groups_of = [&](int blocks) { return n * kv_heads * ((k_rows + 128 * blocks - 1) / (128 * blocks)); };
-  // 64 keys per wave halve what the queries' fragments take of the LDS. With a tile or two of
-  // queries the keys' stream counts, and smaller workgroups; so with too few to fill the GPU.
-  pl.blocks = tiles > 2 && groups_of(2) * ((tiles + 3) / 4) >= cus ? 2 : 1;
-  const int64_t groups = groups_of(pl.blocks);
-  // Rows are split, in runs of four tiles and more, for four workgroups per CU, of which two
-  // are resident; where causal, half of the runs have no rows and the others differ, for twelve
-  // (3683 tokens, 40 heads over 8: 153 us with twelve, 183 with four; all keys 179 with
-  // four, 200 with twelve).
-  int64_t s = groups > 0 ? (causal ? 12 : 4) * cus / groups : 1;
-  if (s > tiles / 4) s = tiles / 4;
-  if (s < 1) s = 1;
-  if (s > 64) s = 64;
-  pl.chunk = (int)((tiles + s - 1) / s);
-  pl.splits = pl.chunk > 0 ? (int)((tiles + pl.chunk - 1) / pl.chunk) : 1;
-  pl.grid = groups * pl.splits;
-  pl.places = 0;
+WeighPlan weigh_plan(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int kv_heads) {
+  WeighPlan pl = {};
+  const int64_t rows = q_rows * (heads / kv_heads), cus = compute_units(), groups = n * kv_heads * ((k_rows + kGroup - 1) / kGroup);
   if (rows > 0 && rows <= 32 && n <= kListed && n > 0) {
     // Four workgroups per CU are resident; each cache has a piece at least.
     const int64_t places = 4 * cus / kv_heads;
     pl.places = (int)(places < n ? n : places);
-    pl.splits = 1;
     pl.grid = (int64_t)pl.places * kv_heads;
+  } else if (rows > 23 * kKeys && groups <= 2 * cus && n <= kShared) {
+    // Few workgroups, of 24 tiles of rows and more: dealt out, two resident per CU (40 heads over
+    // 8, causal: 1024 tokens 26 us, a workgroup for every 128 keys 79; four times 300 over 2000
+    // keys 34 and 36; 256 tokens over 8192 keys, 20 tiles, 39 and 35. 2048 tokens of 40 key
+    // heads, 640 workgroups of 32 tiles, 48 and 45; 8 x 2048 tokens, 1024 of 160, 241 and 248).
+    pl.shares = 2 * cus / kv_heads > 0 ? (int)(2 * cus / kv_heads) : 1;
+    pl.grid = (int64_t)pl.shares * kv_heads;
+    pl.join = n * ((k_rows + kDealt - 1) / kDealt) * kv_heads;
+  } else {
+    pl.grid = groups;
   }
   return pl;
 }
@@ -634,8 +724,8 @@ WeighPlan weigh_plan(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int k
 template <typename T, int D>
 void weigh(const WeighArgs& p, const WeighPlan& pl, hipStream_t s) {
   if (pl.places) weigh_few<T, D><<<(unsigned)pl.grid, 256, 0, s>>>(p);
-  else if (pl.blocks == 1) weigh_keys<T, D, 1><<<(unsigned)pl.grid, 256, 0, s>>>(p);
-  else weigh_keys<T, D, 2><<<(unsigned)pl.grid, 256, 0, s>>>(p);
+  else if (pl.shares) weigh_keys<T, D, 2><<<(unsigned)pl.grid, 256, 0, s>>>(p);
+  else weigh_keys<T, D, 1><<<(unsigned)pl.grid, 256, 0, s>>>(p);
 }
 
 template <typename T>
@@ -666,11 +756,10 @@ int check_weigh(int64_t n, int64_t q_rows, int64_t k_rows, int heads, int kv_hea
 using namespace lr;
 
 extern "C" int lr_attention_weights_workspace(int64_t sequences, int64_t q_rows, int64_t k_rows, int heads, int kv_heads,
-                                              int head_dim, int causal, int64_t* bytes) {
+                                              int head_dim, int64_t* bytes) {
   if (int rc = check_weigh(sequences, q_rows, k_rows, heads, kv_heads, head_dim)) return rc;
   LR_REQUIRE(bytes, "attention_weights: null pointer");
-  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads, causal != 0);
-  *bytes = pl.splits > 1 ? pl.splits * sequences * kv_heads * k_rows * 4 : 0;
+  *bytes = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads).bytes(kv_heads);
   return LR_OK;
 }
 
@@ -695,24 +784,22 @@ extern "C" int lr_attention_weights(const void* q, const void* k, const float* l
   float scale;
   static_assert(sizeof scale == sizeof scale_bits, "fp32");
   __builtin_memcpy(&scale, &scale_bits, sizeof scale);
-  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads, causal != 0);
+  const WeighPlan pl = weigh_plan(sequences, q_rows, k_rows, heads, kv_heads);
   const WeighArgs p = {static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), lse, weights, out,
                        static_cast<float*>(workspace), strides[0], strides[1], strides[2], strides[3], strides[4],
                        strides[5], key_lengths, (int)sequences, (int)q_rows, (int)k_rows, heads, kv_heads, group,
-                       causal != 0, pl.splits, pl.chunk, pl.places, scale * 1.4426950408889634f, Divisor((uint32_t)group)};
+                       causal != 0, pl.shares, pl.places, scale * 1.4426950408889634f, 1.0f / (float)group, Divisor((uint32_t)group)};
   LR_REQUIRE(p.c > 0.0f && isfinite(p.c), "attention_weights: the scale must be positive and finite");
-  const int64_t all = sequences * kv_heads * k_rows;
-  LR_REQUIRE(pl.grid <= kMaxBlocks && (pl.splits == 1 || all <= kMaxBlocks * 256),
-             "attention_weights: %lld workgroups are not supported", (long long)pl.grid);
-  if (pl.splits > 1)
-    LR_REQUIRE(workspace && aligned(workspace, 4) && workspace_bytes >= pl.splits * all * 4,
-               "attention_weights: needs a workspace of %lld bytes", (long long)(pl.splits * all * 4));
+  LR_REQUIRE(pl.grid <= kMaxBlocks && pl.join <= kMaxBlocks, "attention_weights: %lld workgroups are not supported",
+             (long long)(pl.grid > pl.join ? pl.grid : pl.join));
+  LR_REQUIRE(pl.shares == 0 || (workspace && aligned(workspace, 4) && workspace_bytes >= pl.bytes(kv_heads)),
+             "attention_weights: needs a workspace of %lld bytes", (long long)pl.bytes(kv_heads));
   hipStream_t s = as_stream(stream);
   if (dtype == LR_DTYPE_BF16) weigh_by_dim<__bf16>(p, head_dim, pl, s);
   else weigh_by_dim<_Float16>(p, head_dim, pl, s);
   if (int rc = check_launch("attention_weights")) return rc;
-  if (pl.splits == 1) return LR_OK;
-  add_splits<<<(unsigned)((all + 255) / 256), 256, 0, s>>>(p.part, weights, out, all, pl.splits);
+  if (pl.shares == 0) return LR_OK;
+  join_shares<<<(unsigned)pl.join, kDealt, 0, s>>>(p);
   return check_launch("attention_weights");
 }
 

@@ -132,9 +132,9 @@ def test_entry_point_refusals_without_a_gpu():
         assert call(**bad) == _lib.LR_EINVAL, bad
     out = array("q", [0])
     size = lambda *shape: lib.lr_attention_weights_workspace(*shape, out.buffer_info()[0])  # noqa: E731
-    assert size(1, 4096, 64, 8, 8, 128, 0) == _lib.LR_OK and out[0] > 0
-    assert size(64, 1, 8192, 40, 8, 128, 1) == _lib.LR_OK and out[0] == 0
-    assert size(1, 1, 1, 3, 2, 64, 0) == _lib.LR_EINVAL
+    assert size(1, 4096, 64, 8, 8, 128) == _lib.LR_OK and out[0] > 0
+    assert size(64, 1, 8192, 40, 8, 128) == _lib.LR_OK and out[0] == 0
+    assert size(1, 1, 1, 3, 2, 64) == _lib.LR_EINVAL
 
     size = lambda *shape: lib.lr_cache_evict_workspace(*shape, out.buffer_info()[0])  # noqa: E731
     assert size(4, 16384, 8) == _lib.LR_OK and out[0] == 0

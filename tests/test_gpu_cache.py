@@ -150,6 +150,38 @@ def test_weights_around_32_rows(new, heads):
     check(got, w, q, k, lse, lengths, True, 64 ** -0.5)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("batch,new,size,heads,kv_heads,dim", [
+    (64, 400, 300, 4, 1, 32), (65, 400, 300, 4, 1, 32), (7, 310, 1100, 5, 1, 64), (3, 1600, 700, 2, 2, 128),
+    (2, 1473, 256, 1, 1, 64)])
+def test_weights_dealt_out(batch, new, size, heads, kv_heads, dim, causal):
+    """Many rows over few keys, whose work is dealt out over the GPU: empty and short caches between
+    long ones, and more tokens than keys."""
+    w, q, k = make(batch, new, size, heads, kv_heads, dim, torch.bfloat16, batch)
+    lengths = [(0, size, 1, 257, size - 1, 128, 0, 77)[i % 8] for i in range(batch)]
+    lengths = [min(n, size) for n in lengths]
+    lse = sums_of(q, k, lengths, causal)
+    given = torch.tensor(lengths, device="cuda")
+    got = cache.accumulate_weights(w, q, k, lse, causal=causal, key_lengths=given)
+    check(got, w, q, k, lse, lengths, causal, dim ** -0.5)
+    assert torch.equal(cache.accumulate_weights(w, q, k, lse, causal=causal, key_lengths=given, out=w), got)
+
+
+@pytest.mark.parametrize("new", [20, 40, 2000])
+def test_weights_of_infinite_sums(new):
+    """A token whose lse is -infinity, as where all of its scores are: infinity for the keys that it
+    sees, as the formula's exp(s + inf), and nothing for the others."""
+    size = new + 200
+    w, q, k = make(1, new, size, 1, 1, 64, torch.float16, new)
+    lse = sums_of(q, k, None, True)
+    lse[:, 5] = float("inf")   # exp(s - inf) = 0
+    want = cache.accumulate_weights(w, q, k, lse, causal=True)
+    lse[:, 5] = -float("inf")
+    got = cache.accumulate_weights(w, q, k, lse, causal=True)
+    assert (got[..., :206] == float("inf")).all()
+    assert torch.equal(got[..., 206:], want[..., 206:]) and want.isfinite().all()
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_weights_of_far_keys(new):
     """Keys past 2^31 elements of the first."""
@@ -271,9 +303,10 @@ def test_far_caches():
     assert (keys[0, 0] == 2).all() and (keys[0, 1] == 1).all() and torch.equal(keys, values)
 
 
-def test_graph():
+@pytest.mark.parametrize("new", [1, 500])
+def test_graph(new):
     """The attention, the weights and an eviction in one graph, replayed as the caches change."""
-    w, q, k = make(3, 1, 300, 8, 2, 64, torch.bfloat16, 3)
+    w, q, k = make(3, new, 300, 8, 2, 64, torch.bfloat16, 3)
     v = k.flip(1).contiguous()
     prefix = k[0, :100].contiguous()
     lengths = torch.full((3,), 300, device="cuda", dtype=torch.int32)

@@ -450,7 +450,8 @@ int lr_cache_evict(const void* k, const void* v, const float* weights, const int
  *   out[t] = base[t] where index[t] is not in [0, adapters).
  * lr_adapter_plan sorts the tokens by adapter, once for all products of a batch: order
  * int32 [tokens], tiles int32 [lr_adapter_tiles(tokens, adapters)][4] (adapter, first
- * place in order, tokens, 0), 16-byte aligned. At most 1000 adapters, 2^24 - 1 tokens.
+ * place in order, tokens, and the first tile of a pair or -1: a list of its own), 16-byte
+ * aligned. At most 1000 adapters, 2^24 - 1 tokens.
  * lr_adapter_add: x [tokens, k], base and out [tokens, n] (rows x_stride, .. elements
  * apart; out may be base, and may not overlap x or base otherwise), down [adapters, rank, k8] and up [adapters, n,
  * rank8], all of one 16-bit type, k8 and rank8 being k and rank rounded up to multiples of 8; what

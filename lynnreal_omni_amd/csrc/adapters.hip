@@ -3,7 +3,7 @@
 //   out[t] = base[t] + scale[a] (x[t] down[a]^T) up[a]^T,   a = index[t], or base[t] without one
 //
 // with down[a] [rank, k] and up[a] [n, rank]. A plan, made once for a batch and used by
-// every layer, lists the tokens by adapter in tiles of at most 64. Two kernels:
+// every layer, lists the tokens by adapter in tiles of at most 64, and the tiles in pairs. Two kernels:
 //   shrink   inner[t] = x[t] down[a]^T, fp32, a tile of tokens and a share of k per workgroup
 //   expand   adds up a token's shares in order, scales them, and adds the product with up
 //            to the projection, a tile of tokens and a run of columns per workgroup
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(kPlan) void plan_adapters(const int32_t* index, int
                                                        int4* tiles, int max_tiles) {
   constexpr int WAVES = kPlan / 64;
   extern __shared__ int counts[];   // [WAVES][adapters + 1]: tokens, then their next place
-  __shared__ int sums[2][WAVES];
+  __shared__ int sums[3][WAVES];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, kinds = adapters + 1;
   for (int i = t; i < WAVES * kinds; i += kPlan) counts[i] = 0;
   __syncthreads();
@@ -54,27 +54,33 @@ __global__ __launch_bounds__(kPlan) void plan_adapters(const int32_t* index, int
   const int i0 = min(tokens, wave * stretch), i1 = min(tokens, i0 + stretch);
   for (int i = i0 + lane; i < i1; i += 64) atomicAdd(&mine[kind_of(i)], 1);
   __syncthreads();
-  // Thread t has kinds 2 t and 2 t + 1: their tokens and tiles, and those before them.
-  int n[2] = {0, 0}, need[2];
+  // Thread t has kinds 2 t and 2 t + 1: their tokens, tiles and pairs of tiles, and those before them.
+  int n[2] = {0, 0}, need[2], pairs[2];
   for (int j = 0; j < 2; ++j) {
     const int a = 2 * t + j;
     if (a < kinds)
       for (int w = 0; w < WAVES; ++w) n[j] += counts[w * kinds + a];
     need[j] = (n[j] + kTokens - 1) / kTokens;
+    pairs[j] = a < adapters ? (need[j] + 1) / 2 : 0;
   }
   const int upto_n = wave_prefix_sum(n[0] + n[1]), upto_t = wave_prefix_sum(need[0] + need[1]);
+  const int upto_p = wave_prefix_sum(pairs[0] + pairs[1]);
   if (lane == 63) {
     sums[0][wave] = upto_n;
     sums[1][wave] = upto_t;
+    sums[2][wave] = upto_p;
   }
   __syncthreads();
   int place = upto_n - n[0] - n[1], tile = upto_t - need[0] - need[1], all = 0;
+  int pair = upto_p - pairs[0] - pairs[1], all_pairs = 0;
   for (int w = 0; w < WAVES; ++w) {
     if (w < wave) {
       place += sums[0][w];
       tile += sums[1][w];
+      pair += sums[2][w];
     }
     all += sums[1][w];
+    all_pairs += sums[2][w];
   }
   for (int j = 0; j < 2; ++j) {
     const int a = 2 * t + j;
@@ -85,12 +91,22 @@ __global__ __launch_bounds__(kPlan) void plan_adapters(const int32_t* index, int
       counts[w * kinds + a] = at;
       at += c;
     }
-    for (int i = 0; i < need[j]; ++i)
-      tiles[tile + i] = make_int4(a < adapters ? a : -1, place + i * kTokens, min(kTokens, n[j] - i * kTokens), 0);
+    for (int i = 0; i < need[j]; ++i) {
+      int4& to = tiles[tile + i];
+      to.x = a < adapters ? a : -1;
+      to.y = place + i * kTokens;
+      to.z = min(kTokens, n[j] - i * kTokens);
+    }
+    for (int i = 0; i < pairs[j]; ++i) tiles[pair + i].w = tile + 2 * i;
+    pair += pairs[j];
     place += n[j];
     tile += need[j];
   }
-  for (int i = all + t; i < max_tiles; i += kPlan) tiles[i] = make_int4(-1, 0, 0, 0);
+  for (int i = all + t; i < max_tiles; i += kPlan) {
+    tiles[i].x = -1;
+    tiles[i].y = tiles[i].z = 0;
+  }
+  for (int i = all_pairs + t; i < max_tiles; i += kPlan) tiles[i].w = -1;
   __syncthreads();
   for (int i = i0; i < i1; i += 64) {
     const int at = i + lane, a = at < i1 ? kind_of(at) : -1;
@@ -117,7 +133,7 @@ struct AdapterArgs {
   int64_t xs, bs, os;    // row strides in elements
   int64_t first;         // token of this window of x, and how many: what 32-bit offsets reach
   int window;
-  int tokens, n, k, rank, max_tiles;
+  int tokens, n, k, rank, max_tiles, max_pairs;
   int k8, rank8;         // rows of down and up, in elements
   int splits;            // of k
   int columns;           // of a workgroup of expand
@@ -142,8 +158,8 @@ __device__ __forceinline__ void wait_loads() {   // all but the last COUNT
 }
 
 // Slots of the rings: three, two and one workgroups per CU.
-template <int RP>
-constexpr int kRingX = RP == 32 ? 5 : (RP == 64 ? 6 : 8);
+template <int RP, bool PAIR>
+constexpr int kRingX = RP == 32 ? 5 : (RP == 64 ? 6 : (PAIR ? 4 : 8));
 template <int RP>
 constexpr int kRingD = RP == 32 ? 3 : 4;
 
@@ -155,21 +171,32 @@ constexpr int kRingD = RP == 32 ? 3 : 4;
 // (One array holds all of a kernel's LDS: between two the compiler cannot tell which a DMA
 // writes, and waits for all of them before any read. With a second one 12605 x 14336 at
 // rank 128 took 285 us.)
-template <typename T, int RP>
+// A CU takes in 35 KB/us, from wherever: of that x is the smaller part at rank 128. PAIR: two
+// tiles of an adapter at a time, so that down comes half as often (12605 tokens of four adapters,
+// 14336 columns at rank 128, with an expand of 128 columns: 117 us, 138 a tile at a time).
+template <typename T, int RP, bool PAIR>
 __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
   typedef typename Mfma<T>::V V8;
-  constexpr int RB = RP / 32, TB = kTokens / 32, ROW = 2 * kStep, RX = kRingX<RP>, RD = kRingD<RP>, CH = ROW / 16, PER = 1024 / ROW;
-  constexpr int SX = kTokens * ROW, SD = RP * ROW, LDS = RX * SX + RD * SD, XD = kTokens / PER / 4, DD = RP / PER / 4;   // DMAs of a wave
+  constexpr int TOKENS = PAIR ? 2 * kTokens : kTokens;
+  constexpr int RB = RP / 32, TB = TOKENS / 32, ROW = 2 * kStep, RX = kRingX<RP, PAIR>, RD = kRingD<RP>, CH = ROW / 16, PER = 1024 / ROW;
+  constexpr int SX = TOKENS * ROW, SD = RP * ROW, LDS = RX * SX + RD * SD, XD = TOKENS / PER / 4, DD = RP / PER / 4;   // DMAs of a wave
   constexpr int GROUP = 4 < TB * RB ? 4 : TB * RB;   // blocks that are added at a time
   static_assert(LDS >= 4 * GROUP * 4096, "the sums take the rings' place");
   __shared__ __attribute__((aligned(1024))) char smem[LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = lane >> 5, col = lane & 31;
-  const uint32_t id = run_of_xcd();
-  const int tile = (int)(id % (uint32_t)p.max_tiles), split = (int)(id / (uint32_t)p.max_tiles);
+  const uint32_t id = run_of_xcd(), places = (uint32_t)(PAIR ? p.max_pairs : p.max_tiles);
+  const int place = (int)(id % places), split = (int)(id / places), tile = PAIR ? p.tiles[place].w : place;
+  if (PAIR && tile < 0) return;
   const int4 info = p.tiles[tile];
-  const int a = info.x, count = info.z;
+  const int a = info.x, start = info.y;
+  int count = info.z;
   if (a < 0 || count == 0) return;
+  if (PAIR && tile + 1 < p.max_tiles) {
+    // (The first of two is full, so that their tokens, and their rows of inner, are in line.)
+    const int4 next = p.tiles[tile + 1];
+    count += next.x == a ? next.z : 0;
+  }
   const int steps = (p.k + kStep - 1) / kStep, chunk = (steps + p.splits - 1) / p.splits;
   const int s0 = min(steps, split * chunk), s1 = min(steps, s0 + chunk);
   const __amdgpu_buffer_rsrc_t xr = row_rsrc(p.x + p.first * p.xs, ((int64_t)(p.window - 1) * p.xs + p.k8) * 2);
@@ -180,7 +207,7 @@ __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
 #pragma unroll
   for (int i = 0; i < XD; ++i) {
     const int r = (wave * XD + i) * PER + lane / CH;
-    const int64_t tok = r < count ? p.order[info.y + r] - p.first : -1;
+    const int64_t tok = r < count ? p.order[start + r] - p.first : -1;
     const bool in = tok >= 0 && tok < p.window;
     xo[i] = in ? (uint32_t)(tok * p.xs * 2) : kOutside;
   }
@@ -277,7 +304,7 @@ __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
     }
     if (s < s1) step(df[0], xf[0], df[1], xf[1], s);
   };
-  if (count <= 32) steps_of(std::integral_constant<int, 1>{});
+  if (!PAIR && count <= TOKENS / 2) steps_of(std::integral_constant<int, TB / 2>{});
   else steps_of(std::integral_constant<int, TB>{});
   float4* const sums = reinterpret_cast<float4*>(smem);
   float* const part = p.part + ((int64_t)split * p.max_tiles + tile) * kTokens * RP;
@@ -308,7 +335,7 @@ __global__ __launch_bounds__(256) void shrink(AdapterArgs p) {
       const int tok = (g0 + g) / RB * 32 + col, r = (g0 + g) % RB * 32 + 8 * wave + 4 * half;
       if (tok >= count) continue;
       if (p.window < p.tokens) {   // rows of other windows are theirs to write
-        const int64_t of = p.order[info.y + tok] - p.first;
+        const int64_t of = p.order[start + tok] - p.first;
         if (of < 0 || of >= p.window) continue;
       }
       *reinterpret_cast<float4*>(part + tok * RP + r) = v;
@@ -683,8 +710,8 @@ __global__ __launch_bounds__(256) void expand(AdapterArgs p) {
 struct AddPlan {
   int rank;      // padded
   int splits, columns;
-  bool few;
-  int64_t tiles, bytes;
+  bool few, pair;
+  int64_t tiles, pairs, bytes;
 };
 
 AddPlan add_plan(int64_t tokens, int64_t n, int64_t k, int rank, int64_t adapters) {
@@ -703,11 +730,16 @@ AddPlan add_plan(int64_t tokens, int64_t n, int64_t k, int rank, int64_t adapter
   // 45 KB/us for each CU and six of them to fill the ring, against a launch to add the shares
   // and their way through memory.
   const int per_cu = pl.rank == 32 ? 3 : (pl.rank == 64 ? 2 : 1);
-  const double step = per_cu * (kTokens + pl.rank) * 2.0 * kStep / 45e3;
+  // Pairs of tiles where an adapter has many and the CUs have 94 steps and more (4 adapters of
+  // 12605 tokens: level at 5376 columns, 52 us; 24 us without and 27 so for 16 of 4096, 2048).
+  pl.pair = pl.rank == 128 && tokens >= 16 * kTokens * adapters && pl.tiles * steps >= 94 * cus;
+  pl.pairs = tokens / (2 * kTokens) + (adapters < tokens ? adapters : tokens);
+  const int64_t tiles = pl.pair ? pl.pairs : pl.tiles;
+  const double step = per_cu * ((pl.pair ? 2 : 1) * kTokens + pl.rank) * 2.0 * kStep / 45e3;
   const double share = (double)pl.tiles * kTokens * pl.rank * 4 * 2.0 / 5e6;
   double least = 0.0;
   for (int s = 1; s <= 16 && (s == 1 || s <= steps / 4); ++s) {
-    const double rounds = ceil((double)(pl.tiles * s) / (double)(cus * per_cu));
+    const double rounds = ceil((double)(tiles * s) / (double)(cus * per_cu));
     const double us = rounds * ((double)((steps + s - 1) / s) + 6.0) * step + (s > 1 ? 2.5 + s * share : 0.0);
     if (s == 1 || us < least) {
       least = us;
@@ -724,7 +756,8 @@ int add(AdapterArgs p, const AddPlan& pl, bool vector, hipStream_t s) {
   for (int64_t first = 0; first < p.tokens; first += rows) {
     p.first = first;
     p.window = (int)(p.tokens - first < rows ? p.tokens - first : rows);
-    shrink<T, RP><<<(unsigned)(pl.tiles * pl.splits), 256, 0, s>>>(p);
+    if (RP == 128 && pl.pair) shrink<T, RP, RP == 128><<<(unsigned)(pl.pairs * pl.splits), 256, 0, s>>>(p);
+    else shrink<T, RP, false><<<(unsigned)(pl.tiles * pl.splits), 256, 0, s>>>(p);
     if (int rc = check_launch("adapter_add")) return rc;
   }
   const unsigned grid = (unsigned)(pl.tiles * ((p.n + pl.columns - 1) / pl.columns));
@@ -824,6 +857,7 @@ extern "C" int lr_adapter_add(const void* x, int64_t x_stride, const void* down,
   p.k = (int)k;
   p.rank = rank;
   p.max_tiles = (int)pl.tiles;
+  p.max_pairs = (int)pl.pairs;
   p.k8 = (int)k8;
   p.rank8 = (rank + 7) & ~7;
   p.splits = pl.splits;

@@ -86,6 +86,20 @@ def test_cases(indices, count, rank, n, k, dtype):
     run(indices, count, rank, n, k, dtype, rank + n)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,rank,k", [
+    ((6000, -100, 6100), 128, 8008), ((9000, 1, 65), 100, 12000), ((-1000, 4000, 64, 4036), 128, 12120)])
+def test_pairs_of_tiles(sizes, rank, k, dtype):
+    """Many tokens of few adapters at a high rank: pairs of tiles, odd numbers of them, adapters of a
+    tile or less, and tokens of none (negative sizes)."""
+    indices, at = [], 0
+    for n in sizes:
+        indices += [at if n > 0 else -1] * abs(n)
+        at += n > 0
+    order = torch.randperm(len(indices), generator=torch.Generator().manual_seed(rank)).tolist()
+    run([indices[i] for i in order], at, rank, 40, k, dtype, rank)
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_plans(seed):
     """A plan lists every token once, in tiles of one adapter, in order."""

@@ -469,7 +469,8 @@ struct EvictArgs {
   int n, heads, size, budget, recent, capacity;
   int chunks;              // 16-byte pieces of a row
   int clear;               // whether rows behind a cache's last are set to zero
-  uint32_t* hist;          // counts of three digits [3][n][heads][parts][2048], where parts > 1
+  uint32_t* hist;          // where parts > 1: counts of three digits [3][n][heads][parts][2048],
+  uint4* found;            // and [n][heads][parts] what is known of the border (choose_keys)
   int parts;               // of kPart keys
 };
 
@@ -491,10 +492,11 @@ constexpr int kDigitShift[3] = {21, 10, 0}, kDigitBits[3] = {11, 11, 10};
 // value of it; then every weight's place among those that stay is a count of the ones before
 // it. A workgroup has 16384 weights, in registers; a wave's are next to each other.
 //   WHOLE   a cache of one workgroup: all of it in one kernel
-//   0, 1, 2 counts of that digit, for each workgroup's part, into p.hist
-//   PLACE   the border and the parts before this one from those counts, then the places
+//   0, 1, 2 the border's digit before from its counts, then the counts of this digit, for each
+//           workgroup's part
+//   PLACE   the last digit, then the places
 // (Four caches of 40000 to 131072 keys, 8 heads: a workgroup for each, that went through its weights
-// five times, took 159 us.)
+// five times, took 159 us; the four kernels take 42.)
 constexpr int kPlace = 3, kWhole = 4;
 
 // Sum of the waves' numbers v[0], v[2], .. before wave `end`.
@@ -591,31 +593,44 @@ __global__ __launch_bounds__(kSelect) void choose_keys(EvictArgs p) {
       settle(d, bins[kBins - 1 - 2 * t], bins[kBins - 2 - 2 * t]);
     }
   } else {
-    // All digits' counts first: their loads wait for none of them.
-    constexpr int DIGITS = STEP < kPlace ? STEP : 3, COUNT = 8;   // parts on their way at a time
-    uint32_t c0[DIGITS + 1] = {}, c1[DIGITS + 1] = {}, mine0[DIGITS + 1] = {}, mine1[DIGITS + 1] = {};
-    for (int q = 0; q < p.parts; q += COUNT) {
-      uint2 c[DIGITS + 1][COUNT];
+    // What the steps before have found: the border's digits, how many on it are left to stay, and
+    // the keys of the parts before this one that are above it.
+    uint4& known = p.found[(int64_t)row * p.parts + part];
+    if constexpr (STEP > 1) {
+      border = known.x;
+      equals = known.y;
+    }
+    if constexpr (STEP > 0) {
+      constexpr int DIGIT = STEP - 1, COUNT = 8;   // parts on their way at a time
+      uint32_t c0 = 0, c1 = 0, mine0 = 0, mine1 = 0;
+      for (int q = 0; q < p.parts; q += COUNT) {
+        uint2 c[COUNT];
 #pragma unroll
-      for (int d = 0; d < DIGITS; ++d)
-#pragma unroll
-        for (int i = 0; i < COUNT; ++i) c[d][i] = q + i < p.parts ? counted(d, q + i) : make_uint2(0, 0);
-#pragma unroll
-      for (int d = 0; d < DIGITS; ++d)
+        for (int i = 0; i < COUNT; ++i) c[i] = q + i < p.parts ? counted(DIGIT, q + i) : make_uint2(0, 0);
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
-          c0[d] += c[d][i].y;
-          c1[d] += c[d][i].x;
-          mine0[d] += q + i < part ? c[d][i].y : 0;
-          mine1[d] += q + i < part ? c[d][i].x : 0;
+          c0 += c[i].y;
+          c1 += c[i].x;
+          mine0 += q + i < part ? c[i].y : 0;
+          mine1 += q + i < part ? c[i].x : 0;
         }
-    }
-#pragma unroll
-    for (int d = 0; d < DIGITS; ++d) {
-      settle(d, c0[d], c1[d]);
-      const int digit = (int)found[0], mine = kBins - 1 - 2 * t;
-      before[0] += (mine > digit ? mine0[d] : 0) + (mine - 1 > digit ? mine1[d] : 0);
-      if (d == 2) before[1] = (mine == digit ? mine0[d] : 0) + (mine - 1 == digit ? mine1[d] : 0);
+      }
+      settle(DIGIT, c0, c1);
+      const int digit = (int)found[0], upper = kBins - 1 - 2 * t;   // this thread's bins: upper and the one below
+      const uint32_t above = (upper > digit ? mine0 : 0) + (upper - 1 > digit ? mine1 : 0);
+      const uint32_t same = (upper == digit ? mine0 : 0) + (upper - 1 == digit ? mine1 : 0);
+      // The sums over the threads' bins.
+      const uint32_t a = (uint32_t)wave_prefix_sum((int)above), b = (uint32_t)wave_prefix_sum((int)same);
+      __syncthreads();
+      if (lane == 63) {
+        counts[wave][0] = a;
+        counts[wave][1] = b;
+      }
+      __syncthreads();
+      before[0] = sum_before(&counts[0][0], WAVES) + (STEP > 1 ? known.z : 0);
+      before[1] = sum_before(&counts[0][1], WAVES);
+      __syncthreads();   // known has been read
+      if (STEP < kPlace && t == 0) known = make_uint4(border, equals, before[0], 0);
     }
     if (STEP < kPlace) {
       count(STEP);
@@ -623,16 +638,6 @@ __global__ __launch_bounds__(kSelect) void choose_keys(EvictArgs p) {
       for (int i = t; i < kBins; i += kSelect) to[i] = bins[i];
       return;
     }
-    // The sums over the threads' bins.
-    const uint32_t a = (uint32_t)wave_prefix_sum((int)before[0]), b = (uint32_t)wave_prefix_sum((int)before[1]);
-    __syncthreads();
-    if (lane == 63) {
-      counts[wave][0] = a;
-      counts[wave][1] = b;
-    }
-    __syncthreads();
-    before[0] = sum_before(&counts[0][0], WAVES);
-    before[1] = sum_before(&counts[0][1], WAVES);
   }
   uint32_t larger = 0, on = 0;
 #pragma unroll
@@ -804,7 +809,7 @@ extern "C" int lr_attention_weights(const void* q, const void* k, const float* l
 }
 
 static int64_t evict_bytes(int64_t sequences, int64_t size, int kv_heads) {
-  return size > kPart ? 3 * sequences * kv_heads * ((size + kPart - 1) / kPart) * kBins * 4 : 0;
+  return size > kPart ? sequences * kv_heads * ((size + kPart - 1) / kPart) * (3 * kBins * 4 + 16) : 0;
 }
 
 extern "C" int lr_cache_evict_workspace(int64_t sequences, int64_t size, int kv_heads, int64_t* bytes) {
@@ -852,6 +857,7 @@ extern "C" int lr_cache_evict(const void* k, const void* v, const float* weights
                        strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8],
                        strides[9], strides[10], strides[11], (int)sequences, kv_heads, (int)size, (int)budget,
                        (int)recent, (int)capacity, (int)chunks, clear != 0, static_cast<uint32_t*>(workspace),
+                       reinterpret_cast<uint4*>(static_cast<uint32_t*>(workspace) + 3 * sequences * kv_heads * parts * kBins),
                        (int)parts};
   hipStream_t s = as_stream(stream);
   const unsigned grid = (unsigned)(sequences * kv_heads * parts);

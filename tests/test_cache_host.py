@@ -138,7 +138,7 @@ def test_entry_point_refusals_without_a_gpu():
 
     size = lambda *shape: lib.lr_cache_evict_workspace(*shape, out.buffer_info()[0])  # noqa: E731
     assert size(4, 16384, 8) == _lib.LR_OK and out[0] == 0
-    assert size(4, 16385, 8) == _lib.LR_OK and out[0] == 3 * 4 * 8 * 2 * 2048 * 4
+    assert size(4, 16385, 8) == _lib.LR_OK and out[0] == 4 * 8 * 2 * (3 * 2048 * 4 + 16)
     assert size(1 << 24, 1, 8) == _lib.LR_EINVAL and size(1, 1, 0) == _lib.LR_EINVAL
 
     twelve = (256, 128, 1280) * 4

@@ -15,7 +15,10 @@ Drop-in modules with the reference's call surface:
 Beside them, without a counterpart there:
   mxfp4               Mxfp4Linear, quantize_transformer (4-bit projections)
   mxfp4_gemm          mxfp4_matmul, tile_scales; kernels.quantize_rows_mxfp4
-  attention           attention, attention_packed, block_attention
+  attention           attention, attention_packed, attention_shared_prefix,
+                      block_attention
+  cache               accumulate_weights, evict (caches of bounded size)
+  adapters            AdapterPlan, LowRankAdapters, AdaptedLinear, adapt_transformer
 All compute runs in liblynnreal_amd.so (hand-written HIP for gfx950, C ABI in
 include/lynnreal_amd.h); there is no CPU or Triton fallback.
 """

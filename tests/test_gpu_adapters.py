@@ -209,6 +209,18 @@ def test_inputs_past_32_bits():
     assert torch.equal(got, layer(small, base, plan))
 
 
+def test_pairs_of_tiles_past_32_bits():
+    k, n, tokens, step = 8064, 16, 12605, 180000
+    big = torch.empty((tokens - 1) * step + k, dtype=torch.bfloat16, device="cuda")
+    x = big.as_strided((tokens, k), (step, 1))
+    small, base = rows(tokens, n, k, torch.bfloat16, 5)
+    x.copy_(small)
+    weights = make(2, 128, n, k, torch.bfloat16, 6)
+    indices = torch.tensor(spread(tokens, 2)).cuda()
+    layer, plan = L.LowRankAdapters(*weights), L.AdapterPlan(indices, 2)
+    assert torch.equal(layer(x, base, plan), layer(small, base, plan))
+
+
 @pytest.mark.parametrize("kind", ["int8", "mxfp4", "linear"])
 def test_adapted_layers(kind):
     g = torch.Generator().manual_seed(2)

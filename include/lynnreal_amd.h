@@ -455,12 +455,14 @@ int lr_cache_evict(const void* k, const void* v, const float* weights, const int
  * lr_adapter_add: x [tokens, k], base and out [tokens, n] (rows x_stride, .. elements
  * apart; out may be base, and may not overlap x or base otherwise), down [adapters, rank, k8] and up [adapters, n,
  * rank8], all of one 16-bit type, k8 and rank8 being k and rank rounded up to multiples of 8; what
- * lies behind k in the rows of x (x_stride >= k8) and of down, and behind rank in those of up,
- * must be 0. scale fp32 [adapters]. rank at most 128. Sums are fp32 in a fixed order, rounded
- * once. workspace: 16-byte aligned, of the bytes that lr_adapter_workspace gives. */
+ * lies behind k in the rows of down, and behind rank in those of up, must be 0. scale fp32
+ * [adapters]. rank at most 128. Sums are fp32 in a fixed order, rounded once. workspace:
+ * 16-byte aligned, of the bytes that lr_adapter_workspace gives: with copies where x has to be
+ * copied, unless its rows have a multiple of 8 columns, begin at 16 bytes and are a multiple of 8
+ * elements apart, below 2^30, none or k at least. */
 int lr_adapter_tiles(int64_t tokens, int adapters);
 int lr_adapter_plan(const int32_t* index, int64_t tokens, int adapters, int32_t* order, int32_t* tiles, void* stream);
-int lr_adapter_workspace(int64_t tokens, int64_t n, int64_t k, int rank, int adapters, int64_t* bytes);
+int lr_adapter_workspace(int64_t tokens, int64_t n, int64_t k, int rank, int adapters, int copies, int64_t* bytes);
 int lr_adapter_add(const void* x, int64_t x_stride, const void* down, const void* up, const float* scale,
                    const void* base, int64_t base_stride, void* out, int64_t out_stride, int dtype, int64_t tokens,
                    int64_t n, int64_t k, int rank, int adapters, const int32_t* order, const int32_t* tiles,

@@ -82,7 +82,7 @@ SIGNATURES = {
                        _P],
     "lr_adapter_tiles": [_I64, _I32],
     "lr_adapter_plan": [_P, _I64, _I32, _P, _P, _P],
-    "lr_adapter_workspace": [_I64, _I64, _I64, _I32, _I32, _P],
+    "lr_adapter_workspace": [_I64, _I64, _I64, _I32, _I32, _I32, _P],
     "lr_adapter_add": [_P, _I64, _P, _P, _P, _P, _I64, _P, _I64, _I32, _I64, _I64, _I64, _I32, _I32, _P, _P, _P, _I64, _P],
     "lr_device_supported": [_I32],
     "lr_abi_version": [],

@@ -67,21 +67,19 @@ class AdapterPlan:
         return self
 
 
+def _copies(k, step, odd):
+    """Whether the kernels copy rows of k columns `step` elements apart first: not whole ones, or 16
+    bytes or a multiple apart, or ones that overlap, or of an x that lies at an odd place."""
+    return bool(odd or k % 8 or step % 8 or step >= 1 << 30 or 0 < step < k)
+
+
 @functools.lru_cache(maxsize=4096)
-def _workspace(device, tokens, n, k, rank, adapters):
+def _workspace(device, tokens, n, k, rank, adapters, step, odd):
     nbytes = array("q", [0])
     with torch.cuda.device(device):
-        _lib.call("lr_adapter_workspace", tokens, n, k, rank, adapters, nbytes.buffer_info()[0])
+        _lib.call("lr_adapter_workspace", tokens, n, k, rank, adapters, int(_copies(k, step, odd)),
+                  nbytes.buffer_info()[0])
     return nbytes[0]
-
-
-@functools.lru_cache(maxsize=4096)
-def _row_step(stride, rows, width):
-    """Elements from one row of x to the next as the kernel reads them: dense rows, 16 bytes
-    apart or a multiple, that are one or do not overlap; None where they are not so."""
-    step = stride[0] if rows > 1 else width
-    dense = stride[1] == 1 or width == 1
-    return step if dense and not step % 8 and step < 1 << 30 and (step >= width or step == 0) else None
 
 
 class LowRankAdapters(nn.Module):
@@ -153,21 +151,23 @@ class LowRankAdapters(nn.Module):
         _lib.same_device(x, base=base, down=down, plan=plan.order, out=out)
         rows = x if len(x_shape) == 2 else x.reshape(tokens, self.in_features)
         onto = base if len(base_shape) == 2 else base.reshape(tokens, self.out_features)
-        if self.in_features % 8:
-            rows = nn.functional.pad(rows, (0, -self.in_features % 8))
-        x_step = _row_step(rows.stride(), tokens, rows.shape[1])
-        if x_step is None or rows.data_ptr() & 15:
-            rows = rows.clone(memory_format=torch.contiguous_format)
-            x_step = rows.shape[1]
+        x_step, column = rows.stride()
+        if column != 1 and self.in_features > 1:
+            rows = rows.contiguous()
+            x_step = self.in_features
+        elif tokens == 1:
+            x_step = self.in_features   # (any stride; it is not used)
         base_step, column = onto.stride()
         if column != 1 and self.out_features > 1:
             onto = onto.contiguous()
             base_step = self.out_features
         if out is None:
             out = base.new_empty(base_shape)
-        nbytes = _workspace(x.get_device(), tokens, self.out_features, self.in_features, self.rank, self.adapters)
+        x_at = rows.data_ptr()
+        nbytes = _workspace(x.get_device(), tokens, self.out_features, self.in_features, self.rank, self.adapters, x_step,
+                            x_at & 15)
         ws = _lib.workspace(x, nbytes) if nbytes else None   # held until the launch
-        _lib.launch(x, "lr_adapter_add", rows.data_ptr(), x_step, down.data_ptr(), up.data_ptr(),
+        _lib.launch(x, "lr_adapter_add", x_at, x_step, down.data_ptr(), up.data_ptr(),
                     scale.data_ptr(), onto.data_ptr(), base_step, out.data_ptr(), self.out_features,
                     _DTYPES[down.dtype], tokens, self.out_features, self.in_features, self.rank, self.adapters,
                     plan.order.data_ptr(), plan.tiles.data_ptr(), _lib.ptr(ws), nbytes)

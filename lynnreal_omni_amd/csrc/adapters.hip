@@ -31,6 +31,29 @@ int64_t plan_tiles(int64_t tokens, int64_t adapters) {
   return tokens / kTokens + (adapters + 1 < tokens ? adapters + 1 : tokens);
 }
 
+// Rows of x that the DMAs cannot fetch (of any 2-byte alignment, or that end inside 16 bytes), with
+// zeros behind them. A thread per 16 bytes of the copy.
+__global__ __launch_bounds__(256) void copy_rows(const uint16_t* x, int64_t stride, int64_t tokens, int k, int k8, uint16_t* to) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int chunks = k8 / 8;
+  const int64_t row = i / chunks;
+  if (row >= tokens) return;
+  const int c = (int)(i - row * chunks) * 8;
+  const uint16_t* const from = x + row * stride + c;
+  uint4 v;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const uint32_t low = c + e < k ? from[e] : 0, high = c + e + 1 < k ? from[e + 1] : 0;
+    set_word(v, e / 2, low | high << 16);
+  }
+  *reinterpret_cast<uint4*>(to + row * k8 + c) = v;
+}
+
+// Whether rows of x, `stride` elements apart, have to be copied.
+bool copied(const void* x, int64_t stride, int64_t k) {
+  return k % 8 || stride % 8 || !aligned(x, 16) || stride >= (1LL << 30) || (stride > 0 && stride < k);
+}
+
 // -------------------------------------------------------------------- plan ----
 constexpr int kPlan = 1024;   // threads
 
@@ -812,10 +835,11 @@ extern "C" int lr_adapter_plan(const int32_t* index, int64_t tokens, int adapter
   return check_launch("adapter_plan");
 }
 
-extern "C" int lr_adapter_workspace(int64_t tokens, int64_t n, int64_t k, int rank, int adapters, int64_t* bytes) {
+extern "C" int lr_adapter_workspace(int64_t tokens, int64_t n, int64_t k, int rank, int adapters, int copies,
+                                    int64_t* bytes) {
   if (int rc = check_add(tokens, n, k, rank, adapters)) return rc;
   LR_REQUIRE(bytes, "adapter_add: null pointer");
-  *bytes = tokens ? add_plan(tokens, n, k, rank, adapters).bytes : 0;
+  *bytes = tokens ? add_plan(tokens, n, k, rank, adapters).bytes + (copies ? tokens * ((k + 7) & ~7LL) * 2 : 0) : 0;
   return LR_OK;
 }
 
@@ -827,21 +851,20 @@ extern "C" int lr_adapter_add(const void* x, int64_t x_stride, const void* down,
   if (int rc = check_add(tokens, n, k, rank, adapters)) return rc;
   if (tokens == 0) return LR_OK;
   LR_REQUIRE(x && down && up && scale && base && out && order && tiles, "adapter_add: null pointer");
-  LR_REQUIRE(aligned(x, 16) && aligned(down, 16) && aligned(up, 16) && aligned(scale, 4) && aligned(order, 4) &&
+  LR_REQUIRE(aligned(x, 2) && aligned(down, 16) && aligned(up, 16) && aligned(scale, 4) && aligned(order, 4) &&
                  aligned(tiles, 16) && aligned(base, 2) && aligned(out, 2),
-             "adapter_add: inputs and adapters must be 16-byte aligned");
+             "adapter_add: adapters and plans must be 16-byte aligned");
   const int64_t k8 = (k + 7) & ~7LL;
-  LR_REQUIRE(x_stride >= 0 && x_stride % 8 == 0 && (x_stride >= k8 || tokens == 1 || x_stride == 0),
-             "adapter_add: rows of x %lld elements apart, not a multiple of 8 of at least %lld", (long long)x_stride,
-             (long long)k8);
-  LR_REQUIRE(x_stride < (1LL << 30) && base_stride >= 0 && (out_stride >= n || tokens == 1),
+  LR_REQUIRE(x_stride >= 0 && base_stride >= 0 && (out_stride >= n || tokens == 1),
              "adapter_add: rows of %lld columns %lld apart", (long long)n, (long long)out_stride);
+  const bool copies = copied(x, x_stride, k);
   const AddPlan pl = add_plan(tokens, n, k, rank, adapters);
   const int64_t runs = (n + pl.columns - 1) / pl.columns;
   LR_REQUIRE(pl.tiles * pl.splits <= kMaxBlocks && pl.tiles * runs <= kMaxBlocks,
              "adapter_add: %lld tiles of tokens are not supported", (long long)pl.tiles);
-  LR_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= pl.bytes,
-             "adapter_add: needs a workspace of %lld bytes", (long long)pl.bytes);
+  const int64_t needs = pl.bytes + (copies ? tokens * k8 * 2 : 0);
+  LR_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= needs,
+             "adapter_add: needs a workspace of %lld bytes", (long long)needs);
   AdapterArgs p = {};
   p.x = static_cast<const uint16_t*>(x);
   p.down = static_cast<const uint16_t*>(down);
@@ -867,5 +890,14 @@ extern "C" int lr_adapter_add(const void* x, int64_t x_stride, const void* down,
   p.columns = pl.columns;
   const bool vector = n % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned(base, 16) && aligned(out, 16);
   hipStream_t s = as_stream(stream);
+  if (copies) {
+    const int64_t blocks = (tokens * (k8 / 8) + 255) / 256;
+    LR_REQUIRE(blocks <= kMaxBlocks, "adapter_add: %lld x %lld inputs to copy are not supported", (long long)tokens, (long long)k);
+    uint16_t* const to = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + pl.bytes);
+    copy_rows<<<(unsigned)blocks, 256, 0, s>>>(p.x, p.xs, tokens, p.k, p.k8, to);
+    if (int rc = check_launch("adapter_add")) return rc;
+    p.x = to;
+    p.xs = k8;
+  }
   return dtype == LR_DTYPE_BF16 ? add_by_rank<__bf16>(p, pl, vector, s) : add_by_rank<_Float16>(p, pl, vector, s);
 }

@@ -97,11 +97,12 @@ def test_out_is_base_or_other_memory():
 
 def test_rows_are_read_as_they_are_where_they_can():
     wide = torch.zeros(9, 64, dtype=BF16)
-    step = lambda t: L._row_step(t.stride(), *t.shape)  # noqa: E731
-    assert step(wide) == 64 and step(wide[:, 8:32]) == 64 and step(wide[::2]) == 128 and step(wide[3:4, :24]) == 24
-    assert step(wide[:1].expand(9, -1)) == 0
-    assert step(wide.t()) is None and step(torch.zeros(9, 65, dtype=BF16)[:, :64]) is None
-    assert step(torch.zeros(100, dtype=BF16).as_strided((5, 64), (8, 1))) is None
+    copies = lambda t: L._copies(t.shape[1], t.stride(0), t.data_ptr() & 15)  # noqa: E731
+    assert not copies(wide) and not copies(wide[:, 8:32]) and not copies(wide[::2]) and not copies(wide[3:4, :24])
+    assert not copies(wide[:1].expand(9, -1))
+    assert copies(wide[:, 4:36]) and copies(wide[:, :60]) and copies(torch.zeros(9, 65, dtype=BF16)[:, :64])
+    assert copies(torch.zeros(100, dtype=BF16).as_strided((5, 64), (8, 1)))
+    assert L._copies(64, 1 << 30, 0) and not L._copies(64, (1 << 30) - 8, 0)
 
 
 def test_adapted_transformer():
@@ -138,16 +139,19 @@ def test_entry_point_refusals_without_a_gpu():
         assert call(**bad) == _lib.LR_EINVAL, bad
     out = array("q", [0])
     size = lambda *shape: lib.lr_adapter_workspace(*shape, out.buffer_info()[0])  # noqa: E731
-    assert size(5, 40, 24, 4, 3) == _lib.LR_OK and out[0] > 0
-    assert size(0, 40, 24, 4, 3) == _lib.LR_OK and out[0] == 0
-    assert size(5, 40, 24, 129, 3) == _lib.LR_EUNSUPPORTED and size(5, 0, 24, 4, 3) == _lib.LR_EINVAL
+    assert size(0, 40, 24, 4, 3, 1) == _lib.LR_OK and out[0] == 0
+    assert size(5, 40, 24, 129, 3, 0) == _lib.LR_EUNSUPPORTED and size(5, 0, 24, 4, 3, 0) == _lib.LR_EINVAL
+    assert size(5, 40, 23, 4, 3, 0) == _lib.LR_OK and out[0] > 0
+    plain = out[0]
+    assert size(5, 40, 23, 4, 3, 1) == _lib.LR_OK and out[0] == plain + 5 * 24 * 2
     good = dict(x=p, xs=24, down=p, up=p, scale=p, base=p, bs=40, out=p, os=40, dtype=0, tokens=5, n=40, k=24, rank=4,
                 adapters=3, order=p, tiles=p, ws=p, wsb=1 << 30, stream=None)
     call = lambda **kw: lib.lr_adapter_add(*{**good, **kw}.values())  # noqa: E731
     assert call(tokens=0) == _lib.LR_OK
     assert call(rank=129) == _lib.LR_EUNSUPPORTED and call(adapters=1001) == _lib.LR_EUNSUPPORTED
     for bad in [dict(x=None), dict(down=None), dict(up=None), dict(scale=None), dict(base=None), dict(out=None), dict(order=None),
-                dict(tiles=None), dict(ws=None), dict(wsb=8), dict(x=p + 8), dict(up=p + 2), dict(base=p + 1), dict(tiles=p + 4),
-                dict(xs=16), dict(xs=25), dict(xs=1 << 30), dict(os=39), dict(bs=-8), dict(dtype=2), dict(tokens=-1),
+                dict(tiles=None), dict(ws=None), dict(wsb=8), dict(x=p + 1), dict(up=p + 2), dict(base=p + 1), dict(tiles=p + 4),
+                dict(xs=-8), dict(xs=25, wsb=plain), dict(xs=16, wsb=plain), dict(xs=1 << 30, wsb=plain),
+                dict(x=p + 8, wsb=plain), dict(k=23, wsb=plain), dict(os=39), dict(bs=-8), dict(dtype=2), dict(tokens=-1),
                 dict(tokens=1 << 24), dict(n=0), dict(n=1 << 24), dict(k=(1 << 23) + 8), dict(rank=0)]:
         assert call(**bad) == _lib.LR_EINVAL, bad

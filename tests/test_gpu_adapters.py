@@ -148,6 +148,25 @@ def test_views():
     assert torch.equal(layer(same, base, plan), layer(same.contiguous(), base, plan))
 
 
+@pytest.mark.parametrize("k", [1, 40, 33, 4969])
+@pytest.mark.parametrize("tokens", [1, 70, 300])
+def test_copied_rows(tokens, k):
+    """Rows of x at any place, and ones that overlap."""
+    n = 24
+    weights = make(3, 20, n, k, torch.float16, 1)
+    layer = L.LowRankAdapters(*weights)
+    g = torch.Generator().manual_seed(k)
+    flat = torch.randn(tokens * (k + 8) + 16, generator=g).half().cuda()
+    base = torch.randn(tokens, n, generator=g).half().cuda()
+    indices = torch.tensor(spread(tokens, 3)).cuda()
+    plan = L.AdapterPlan(indices, 3)
+    for first, step in ((0, k), (3, k), (8, k + 5), (1, 1), (0, 8), (5, 0)):
+        x = flat[first:].as_strided((tokens, k), (step, 1), first)
+        got = layer(x, base, plan)
+        check(got, x, base, indices, *weights)
+        assert torch.equal(layer(x.clone(memory_format=torch.contiguous_format), base, plan), got)
+
+
 def test_rows_do_not_depend_on_the_batch():
     """A token gives the same bits in whatever tile it lies, and an infinity or NaN of another
     token stays there."""

@@ -15,6 +15,7 @@
 // Many rows per sequence: a workgroup's 128 rows walk the prefix and then the own cache
 // in one pass. The prefix comes out of the caches, since the matrix units, not the keys, are
 // what bounds it (878 tokens of four sequences behind 12605, 56 heads: 1.3 ms, 1.05 PFLOP/s).
+// Few rows are walked too where there are few keys, for a kernel less.
 #include "lr_attention.h"
 #include "lr_pieces.h"
 #include "lr_runtime.h"
@@ -154,8 +155,8 @@ __device__ __forceinline__ OneCache prefix_cache(const PrefixArgs& p, int hd) {
 // are joined in LDS at the end, in their order: wave w is left with columns 16 w .. of each 64
 // of the lane's row (D / 8 of o, in all of its D / 2), l and the exponent. (16 sequences of 40
 // key heads behind 8192: 59 us, 4.4 TB/s; 68 with the tiles of attend.)
-template <typename T, int D>
-__device__ __forceinline__ void attend_few(char* smem, float2* stats, const OneCache& keys, const uint16_t* qrow, const float c,
+template <typename T, int D, class Keys>
+__device__ __forceinline__ void attend_few(char* smem, float2* stats, const Keys& keys, const uint16_t* qrow, const float c,
                                            const int t0, const int t1, float& l, float& off, float (&mine)[D / 8]) {
   typedef typename Mfma<T>::V V8;
   constexpr int ROW = 2 * D, CH = ROW / 16, RPB = 256 / ROW, PAIRS = ROW / 32, KD = D / 16, DB = D / 32;
@@ -168,22 +169,29 @@ __device__ __forceinline__ void attend_few(char* smem, float2* stats, const OneC
   V8 q[KD];
 #pragma unroll
   for (int d = 0; d < KD; ++d) q[d] = *reinterpret_cast<const V8*>(qrow + 16 * d + 8 * half);
-  uint32_t koff[DMAS], voff[DMAS];
-#pragma unroll
-  for (int i = 0; i < DMAS; ++i) {
+  // The 16 bytes of a tile that this lane fetches.
+  auto offset = [&](int i, uint32_t stride) __attribute__((always_inline)) {
     const int at = i * 64 + lane, row = at / CH, ch = at % CH ^ (row / RPB % PAIRS) * 2;
-    koff[i] = (uint32_t)(row * keys.kt * 2 + ch * 16);
-    voff[i] = (uint32_t)(row * keys.vt * 2 + ch * 16);
+    return row * stride * 2 + ch * 16;
+  };
+  uint32_t koff[DMAS], voff[DMAS];
+  if constexpr (Keys::kOneStride) {
+#pragma unroll
+    for (int i = 0; i < DMAS; ++i) {
+      koff[i] = offset(i, (uint32_t)keys.stride(0, 0));
+      voff[i] = offset(i, (uint32_t)keys.stride(0, 1));
+    }
   }
-  auto issue = [&](int s) {   // keys 32 s ..; those past the last read as zero
-    const int left = min(32, keys.kn - 32 * s);
+  auto issue = [&](int s) {   // half s % 2 of tile s / 2; keys past the last read as zero
+    const int t = s >> 1, left = min(32, keys.left(t) - 32 * (s & 1));
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      const int64_t stride = v ? keys.vt : keys.kt;
-      const __amdgpu_buffer_rsrc_t r = row_rsrc((v ? keys.v : keys.k) + (left > 0 ? 32 * (int64_t)s * stride : 0),
+      const int64_t stride = keys.stride(t, v);
+      const __amdgpu_buffer_rsrc_t r = row_rsrc(keys.at(t, v) + (left > 0 ? 32 * (s & 1) * stride : 0),
                                                 left > 0 ? ((int64_t)(left - 1) * stride + D) * 2 : 0);
 #pragma unroll
-      for (int i = 0; i < DMAS; ++i) dma16(r, (v ? vs : ks) + i * 1024, v ? voff[i] : koff[i]);
+      for (int i = 0; i < DMAS; ++i)
+        dma16(r, (v ? vs : ks) + i * 1024, Keys::kOneStride ? (v ? voff[i] : koff[i]) : offset(i, (uint32_t)stride));
     }
   };
   v16f o[DB];
@@ -220,9 +228,10 @@ __device__ __forceinline__ void attend_few(char* smem, float2* stats, const OneC
     v16f sc = {};
 #pragma unroll
     for (int d = 0; d < KD; ++d) sc = Mfma<T>::mul(kf[d], q[d], sc);
-    if (32 * s + 32 > keys.sure) {
+    if (!keys.whole(s >> 1)) {
+      const int lim = keys.limit(s >> 1) - keys.first(s >> 1) - 32 * (s & 1) - 4 * half;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = 32 * s + 8 * (e >> 2) + 4 * half + (e & 3) < keys.seen ? sc[e] : -INFINITY;
+      for (int e = 0; e < 16; ++e) sc[e] = 8 * (e >> 2) + (e & 3) < lim ? sc[e] : -INFINITY;
     }
     float x = sc[0];
 #pragma unroll
@@ -525,6 +534,30 @@ __global__ __launch_bounds__(256, 2) void prefix_walk(PrefixArgs p) {
                      Mfma<T>::pack(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
 }
 
+// At most 32 rows per sequence and key head: all keys of them, without pieces and joins.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void prefix_walk_few(PrefixArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[kTileBytes<D> + 256 * 8];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
+  const int seq = (int)(blockIdx.x / (uint32_t)p.kv_heads), hd = (int)(blockIdx.x - seq * p.kv_heads), r = lane & 31;
+  const OwnRows w(p, seq, 0);
+  const Row row(p, r, w.rows, hd, w.kn);
+  const TwoCaches keys = {prefix_cache(p, hd), own_cache(p, seq, hd, w, row.seen), key_tiles(p.prefix)};
+  float l, off, o[D / 8];
+  attend_few<T, D>(smem, reinterpret_cast<float2*>(smem + kTileBytes<D>), keys, p.q + seq * p.qb + row.tok * p.qt + row.head * p.qh,
+                   p.c, 0, keys.tiles + w.tiles, l, off, o);
+  if (r >= w.rows) return;
+  const int64_t to = ((int64_t)seq * p.q_rows + row.tok) * p.heads + row.head;
+  if (p.lse && half == 0 && wave == 0) p.lse[to] = l == 0.0f ? -INFINITY : kLn2 * (off + __builtin_amdgcn_logf(l));
+  const float inv = l == 0.0f ? (p.prefix + row.seen > 0 ? NAN : 0.0f) : 1.0f / l;
+#pragma unroll
+  for (int g = 0; g < D / 32; ++g) {
+    const int at = wave * (D / 32) + g;   // of the lane's D / 8 groups of four columns
+    *reinterpret_cast<uint2*>(p.out + to * D + 32 * (at / 4) + 8 * (at % 4) + 4 * half) =
+        make_uint2(Mfma<T>::pack(o[4 * g] * inv, o[4 * g + 1] * inv), Mfma<T>::pack(o[4 * g + 2] * inv, o[4 * g + 3] * inv));
+  }
+}
+
 // Joins the cut workgroups' rows, as prefix_join does: a wave per row, and all of its at most
 // eight parts at once.
 template <typename T, int D>
@@ -588,7 +621,7 @@ __global__ __launch_bounds__(256) void walk_join(PrefixArgs p) {
 
 // How a call is laid over the GPU.
 struct Plan {
-  bool walk;
+  bool walk, few;   // all keys of a workgroup's rows; those of at most 32 rows
   int64_t seq_tiles, all_tiles;
   int places, shares, own, piece;
   int64_t whole, left;
@@ -637,9 +670,17 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, 
   double walk = (double)(items / slots) * tiles * 2.0;
   if (pl.cuts > 1) walk += ceil(tiles / pl.cuts) * 2.0 + 2.8 + (double)(left * kRows) * (0.0002 + kJoin * pl.cuts);
   else if (left > 0) walk += tiles * (left > cus ? 2.0 : 1.0);
-  // (One wave's rows are not walked: the walk has its matrix instructions for four.)
-  pl.walk = (q_rows * group > 32 && walk <= pieces) || rows > kMaxBlocks;
-  if (pl.walk) {
+  // At most 32 rows take their keys in half a tile's time and nothing is joined, for the cost of a
+  // kernel less, 10 us with its launch (one token of 32 sequences over 1024 own keys at most, 40
+  // heads over 8: 16.5 us, 23.4 in pieces; of 57 behind 164 shared and 157 own ones, 56 heads: 11.1
+  // and 22.5; of 64 behind 4096: 66 and 35).
+  pl.few = q_rows * group <= 32;
+  if (pl.few)
+    walk = ceil((double)items / (double)slots) * (tiles * (items <= cus ? 0.55 : 0.85) + 3.5) + 1.0 - 10.0;
+  pl.walk = walk <= pieces || rows > kMaxBlocks;
+  if (pl.walk && pl.few) {
+    pl.parts = pl.table = 0;
+  } else if (pl.walk) {
     pl.left = pl.cuts > 1 ? left : 0;
     pl.whole = items - pl.left;
     pl.parts = pl.left * pl.cuts * kRows;
@@ -650,6 +691,12 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, 
 
 template <typename T, int D>
 int launch(const PrefixArgs& p, const Plan& pl, hipStream_t s) {
+  if (pl.walk && pl.few) {
+    const int64_t grid = (int64_t)p.n * p.kv_heads;
+    LR_REQUIRE(grid <= kMaxBlocks, "attention_prefix: %lld workgroups are not supported", (long long)grid);
+    prefix_walk_few<T, D><<<(unsigned)grid, 256, 0, s>>>(p);
+    return check_launch("attention_prefix");
+  }
   if (pl.walk) {
     const int64_t grid = pl.whole + pl.left * pl.cuts;
     LR_REQUIRE(grid <= kMaxBlocks, "attention_prefix: %lld workgroups are not supported", (long long)grid);

@@ -80,17 +80,19 @@ def test_cases(batch, new, prefix, size, heads, kv_heads, dim, lengths, causal, 
 
 
 @pytest.mark.parametrize("batch", [512, 513, 700])
-def test_many_sequences(batch):
+@pytest.mark.parametrize("prefix", [300, 9000])
+def test_many_sequences(batch, prefix):
     """On both sides of the most sequences that a list of pieces holds."""
     lengths = [(i * 37) % 90 for i in range(batch)]
     lengths[3] = 400
-    check_all(make(batch, 1, 300, 400, 4, 2, 32, torch.bfloat16, batch), lengths, True)
+    check_all(make(batch, 1, prefix, 400, 4, 2, 32, torch.bfloat16, batch), lengths, True)
 
 
 @pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("more", [0, 6000])   # keys, which are cut into pieces where few tokens have many
 @pytest.mark.parametrize("scale", [1e-3, 1.0, 20.0])
-def test_scales(scale, new):
-    check_all(make(2, new, 200, 150, 4, 2, 64, torch.bfloat16, 3), [150, 150], True, scale)
+def test_scales(scale, more, new):
+    check_all(make(2, new, 200 + more, 150, 4, 2, 64, torch.bfloat16, 3), [150, 150], True, scale)
 
 
 @pytest.mark.parametrize("new", [1, 3, 140])
@@ -104,10 +106,11 @@ def test_nothing_shared_is_plain_attention(new):
 
 
 @pytest.mark.parametrize("new", [1, 100])
-def test_unused_places_are_not_read(new):
+@pytest.mark.parametrize("more", [0, 6000])   # keys, which are cut into pieces where few tokens have many
+def test_unused_places_are_not_read(new, more):
     """NaN and infinities behind a cache's keys and in keys that causality hides."""
-    lengths = [new, new + 70, new + 1]
-    q, pk, pv, k, v = make(3, new, 100, new + 200, 4, 2, 64, torch.float16, 9)
+    lengths = [new, new + 70 + more, new + 1]
+    q, pk, pv, k, v = make(3, new, 100, new + more + 200, 4, 2, 64, torch.float16, 9)
     want = A.attention_shared_prefix(q, pk, pv, k, v, causal=True, key_lengths=torch.tensor(lengths, device="cuda"))
     for i, n in enumerate(lengths):
         k[i, n:], v[i, n:] = float("nan"), float("inf")
@@ -117,17 +120,18 @@ def test_unused_places_are_not_read(new):
 
 
 @pytest.mark.parametrize("new", [1, 100])
-def test_scores_of_minus_infinity(new):
+@pytest.mark.parametrize("more", [0, 6000])   # keys, which are cut into pieces where few tokens have many
+def test_scores_of_minus_infinity(new, more):
     """A row that sees only such scores is NaN (0 / 0), one that also sees others leaves them out;
     the logarithm of the sum is -inf and finite."""
-    q, pk, pv, k, v = make(2, new, 70, 40, 2, 2, 64, torch.bfloat16, 5)
+    q, pk, pv, k, v = make(2, new, 70 + more, 40 + more, 2, 2, 64, torch.bfloat16, 5)
     q[..., 0] = 1.0
     pk[..., 0] = -math.inf
     got, lse = A.attention_shared_prefix(q, pk, pv, k, v, return_lse=True)
     assert torch.isfinite(got).all() and torch.isfinite(lse).all()
     for i in range(2):
-        check(got[i], *formula(q[i], k[i], v[i], 64 ** -0.5, mask(new, 40, False)))
-        check_lse(lse[i], q[i], k[i], 64 ** -0.5, mask(new, 40, False))
+        check(got[i], *formula(q[i], k[i], v[i], 64 ** -0.5, mask(new, 40 + more, False)))
+        check_lse(lse[i], q[i], k[i], 64 ** -0.5, mask(new, 40 + more, False))
     k[..., 0] = -math.inf
     got, lse = A.attention_shared_prefix(q, pk, pv, k, v, return_lse=True)
     assert got.isnan().all() and (lse == -math.inf).all()
@@ -137,16 +141,17 @@ def test_scores_of_minus_infinity(new):
 
 
 @pytest.mark.parametrize("new", [1, 140])
-def test_layouts(new):
+@pytest.mark.parametrize("more", [0, 6000])   # keys, which are cut into pieces where few tokens have many
+def test_layouts(new, more):
     """Slices of a fused projection, heads outside, an expanded batch, a prefix inside a
     larger buffer whose rows are further apart than the caches': read as they are. Odd ones
     are copied."""
-    dim, lengths = 64, torch.tensor([new, new + 9, 150], device="cuda")
+    dim, lengths = 64, torch.tensor([new, new + 9 + more, 150], device="cuda")
     g = torch.Generator().manual_seed(new)
     fused = torch.randn(3, new, 8 * dim, generator=g).bfloat16().cuda()
     q = fused[..., :4 * dim].unflatten(-1, (4, dim))
-    k = torch.randn(3, 2, 200, dim, generator=g).bfloat16().cuda().transpose(1, 2)
-    v = torch.randn(1, 200, 2, dim, generator=g).bfloat16().cuda().expand(3, -1, -1, -1)
+    k = torch.randn(3, 2, 200 + more, dim, generator=g).bfloat16().cuda().transpose(1, 2)
+    v = torch.randn(1, 200 + more, 2, dim, generator=g).bfloat16().cuda().expand(3, -1, -1, -1)
     pk = torch.randn(300, 5, dim, generator=g).bfloat16().cuda()[10:190, 1:3]
     pv = torch.randn(2, 180, dim, generator=g).bfloat16().cuda().transpose(0, 1)
     views = (q, pk, pv, k, v)

@@ -671,12 +671,17 @@ Plan plan(int64_t n, int64_t q_rows, int64_t k_rows, int64_t prefix, int heads, 
   if (pl.cuts > 1) walk += ceil(tiles / pl.cuts) * 2.0 + 2.8 + (double)(left * kRows) * (0.0002 + kJoin * pl.cuts);
   else if (left > 0) walk += tiles * (left > cus ? 2.0 : 1.0);
   // At most 32 rows take their keys in half a tile's time and nothing is joined, for the cost of a
-  // kernel less, 10 us with its launch (one token of 32 sequences over 1024 own keys at most, 40
-  // heads over 8: 16.5 us, 23.4 in pieces; of 57 behind 164 shared and 157 own ones, 56 heads: 11.1
-  // and 22.5; of 64 behind 4096: 66 and 35).
+  // kernel less, 10 us with its launch, and 3 more for every round of pieces past two (one token
+  // of 32 sequences over 1024 own keys at most, 40 heads over 8: 16.5 us, 23.4 in pieces; of 57
+  // behind 164 shared and 157 own ones, 56 heads: 11.1 and 22.5; four of 39 behind 216, 56 key heads:
+  // 39 and 51; one of 64 behind 4096, 40 heads: 66 and 35).
   pl.few = q_rows * group <= 32;
-  if (pl.few)
-    walk = ceil((double)items / (double)slots) * (tiles * (items <= cus ? 0.55 : 0.85) + 3.5) + 1.0 - 10.0;
+  if (pl.few) {
+    const int64_t grid = (pl.places ? pl.places : pl.shares * pl.all_tiles + n * pl.seq_tiles) * kv_heads;
+    const double rounds = ceil((double)grid / (double)slots);
+    walk = ceil((double)items / (double)slots) * (tiles * (items <= cus ? 0.55 : 0.85) + 3.5) + 1.0 - 10.0 -
+           3.0 * fmax(0.0, rounds - 2.0);
+  }
   pl.walk = walk <= pieces || rows > kMaxBlocks;
   if (pl.walk && pl.few) {
     pl.parts = pl.table = 0;

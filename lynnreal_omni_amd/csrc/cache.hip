@@ -259,13 +259,14 @@ __global__ __launch_bounds__(256, 4 / KB) void weigh_keys(WeighArgs p) {
       const int own = wave0 + 4 * half;
       const int lim = r0 + col >= rows ? 0 : (p.causal ? hidden + tok0 + token_of(col, r0 - tok0 * p.group) + 1 : kn) - own;
       auto sees = [&](int i) __attribute__((always_inline)) { return 32 * (i / 16) + 8 * (i % 16 >> 2) + (i & 3) < lim; };
-      if (__ballot(lim > 0 && l2 == -INFINITY) == 0) {
+      if (__ballot(lim > 0 && !(l2 > -INFINITY)) == 0) {
 #pragma unroll
         for (int i = 0; i < 16 * KB; ++i) s[i / 16][i % 16] = sees(i) ? s[i / 16][i % 16] : -INFINITY;
         if (lim <= 0) l2 = INFINITY;
         return;
       }
-      // (Rows whose scores are all -infinity, whose shares are NaN, but not those of keys they do not see.)
+      // A row whose sum is -infinity (all of its scores are) or NaN: a score of -infinity would give
+      // NaN there, so that what it does not see is left out by a choice.
 #pragma unroll
       for (int i = 0; i < 16 * KB; ++i) {
         add(s, i, sees(i));

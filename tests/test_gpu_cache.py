@@ -182,6 +182,29 @@ def test_weights_of_infinite_sums(new):
     assert torch.equal(got[..., 206:], want[..., 206:]) and want.isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("at", [0, 5, -1])
+@pytest.mark.parametrize("new,size,heads", [(20, 220, 1), (40, 240, 1), (40, 240, 3), (2000, 2200, 1), (700, 700, 3)])
+def test_weights_of_nan_sums(new, size, heads, at, dtype):
+    """A token whose lse is NaN, as the attention leaves it for a query of NaN: NaN for the keys
+    that it sees, and nothing for the others, which keep the bits of a run where it counts for nothing."""
+    w, q, k = make(1, new, size, heads, 1, 64, dtype, new + heads)
+    at %= new
+    lse = sums_of(q, k, None, True)
+    lse[:, at] = float("inf")   # exp(s - inf) = 0
+    want = cache.accumulate_weights(w, q, k, lse, causal=True)
+    assert want.isfinite().all()
+    seen = size - new + at + 1
+    lse[:, at, heads // 2] = float("nan")
+    got = cache.accumulate_weights(w, q, k, lse, causal=True)
+    assert got[..., :seen].isnan().all() and torch.equal(got[..., seen:], want[..., seen:])
+    q[:, at] = float("nan")
+    lse = sums_of(q, k, None, True)
+    assert lse[:, at].isnan().all()
+    got = cache.accumulate_weights(w, q, k, lse, causal=True)
+    assert got[..., :seen].isnan().all() and torch.equal(got[..., seen:], want[..., seen:])
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_weights_of_far_keys(new):
     """Keys past 2^31 elements of the first."""

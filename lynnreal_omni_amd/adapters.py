@@ -24,6 +24,8 @@ from torch import nn
 from . import _lib
 from .attention import _DTYPES
 from .cache import _overlap
+from .int8 import Int8Linear
+from .mxfp4 import Mxfp4Linear
 
 MAX_ADAPTERS, MAX_RANK = 1000, 128
 
@@ -182,10 +184,23 @@ class Requests:
         self.plan = plan
 
 
+_global_hooks = nn.modules.module._global_forward_hooks
+
+
+def _gives_new_memory(layer):
+    """Whether what a call of the layer returns is memory that nothing else holds: a layer whose
+    forward is known, with no hook that could keep the result or put its own in its place."""
+    own = layer.__dict__
+    return (type(layer) in (Int8Linear, Mxfp4Linear, nn.Linear) and not own["_forward_hooks"] and not _global_hooks
+            and "forward" not in own and "forward_quantized" not in own)
+
+
 class AdaptedLinear(nn.Module):
     """A projection with adapters beside it: layer(value), plus the products of the adapters
     that requests.plan gives the tokens. Layers that quantize their input do so as without
-    adapters, which see the input itself: fused blocks pass it to this layer unquantized."""
+    adapters, which see the input itself: fused blocks pass it to this layer unquantized.
+    The products are added in the memory of the layer's result where nothing else can hold
+    it (an Int8Linear, Mxfp4Linear or nn.Linear without forward hooks), else in new memory."""
 
     def __init__(self, layer, adapters, requests):
         super().__init__()
@@ -206,8 +221,10 @@ class AdaptedLinear(nn.Module):
     def forward(self, value):
         y = self.layer(value)
         plan = self.requests.plan
-        # y is this layer's own memory, so the products are added in place.
-        return y if plan is None else self.adapters(value, y, plan, out=y)
+        if plan is None:
+            return y
+        # In place where nothing else holds y: tokens without an adapter then cost nothing.
+        return self.adapters(value, y, plan, out=y if _gives_new_memory(self.layer) and y.is_contiguous() else None)
 
 
 def adapt_transformer(transformer, adapters):

@@ -127,6 +127,71 @@ def test_adapted_transformer():
         L.adapt_transformer(model, {"0": some()})
 
 
+class Beside:
+    """Stands for the adapters of a layer: adds one, where it is told to, and remembers where that was."""
+    in_features, out_features = 24, 40
+
+    def __call__(self, x, base, plan, out=None):
+        self.out = out
+        return out.copy_(base + 1) if out is not None else base + 1
+
+
+def adapted(layer):
+    beside, requests = Beside(), L.Requests(Plan())
+    return L.AdaptedLinear(layer, beside, requests), beside
+
+
+@torch.no_grad()
+def test_products_go_into_memory_of_the_layer_alone():
+    """What a hook keeps of the layer's result stays as it was, and so does a buffer that it puts in its place."""
+    x = torch.randn(5, 24, dtype=BF16)
+    layer = nn.Linear(24, 40, dtype=BF16)
+    want = layer(x)
+    model, beside = adapted(layer)
+    assert torch.equal(model(x), want + 1) and beside.out is not None
+    seen = []
+    handle = layer.register_forward_hook(lambda m, args, y: seen.append(y))
+    assert torch.equal(model(x), want + 1) and torch.equal(seen[0], want)
+    handle.remove()
+    buffer = torch.zeros(5, 40, dtype=BF16)
+    handle = layer.register_forward_hook(lambda m, args, y: buffer)
+    assert torch.equal(model(x), torch.ones(5, 40, dtype=BF16)) and not buffer.any()
+    handle.remove()
+    seen.clear()
+    handle = nn.modules.module.register_module_forward_hook(lambda m, args, y: seen.append((m, y)))
+    try:
+        got = model(x)
+    finally:
+        handle.remove()
+    assert torch.equal(got, want + 1) and torch.equal(next(y for m, y in seen if m is layer), want)
+    assert torch.equal(model(x), want + 1) and beside.out is not None   # no hook is left
+
+
+@torch.no_grad()
+def test_layers_that_keep_their_result():
+    x = torch.randn(5, 24, dtype=BF16)
+
+    class Keeps(nn.Linear):
+        def forward(self, value):
+            self.kept = super().forward(value)
+            return self.kept
+
+    layer = Keeps(24, 40, dtype=BF16)
+    got = adapted(layer)[0](x)
+    assert torch.equal(got, layer.kept + 1)
+    # One whose rows are not next to each other.
+    class Columns(nn.Linear):
+        def forward(self, value):
+            return super().forward(value).t().contiguous().t()
+
+    layer = Columns(24, 40, dtype=BF16)
+    assert torch.equal(adapted(layer)[0](x), layer(x) + 1)
+    # A forward put in the place of the layer's own.
+    layer, kept = nn.Linear(24, 40, dtype=BF16), torch.zeros(5, 40, dtype=BF16)
+    layer.forward = lambda value: kept
+    assert torch.equal(adapted(layer)[0](x), torch.ones(5, 40, dtype=BF16)) and not kept.any()
+
+
 def test_entry_point_refusals_without_a_gpu():
     lib, p = _lib.load(), 4096
     assert lib.lr_adapter_tiles(0, 3) == 0 and lib.lr_adapter_tiles(5, 1001) == 0 and lib.lr_adapter_tiles(-1, 3) == 0

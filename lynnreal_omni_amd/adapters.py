@@ -68,6 +68,13 @@ class AdapterPlan:
                     self.tiles.data_ptr())
         return self
 
+    def rows(self, keep, batch=1):
+        """The plan of the tokens `keep` (numbers on the GPU) of each of `batch` sequences that this one is of."""
+        # The adapter of each place of the order, then of each token.
+        sorted_by = torch.repeat_interleave(self.tiles[:, 0], self.tiles[:, 2], output_size=self.tokens)
+        indices = torch.empty_like(sorted_by).scatter_(0, self.order.long(), sorted_by)
+        return AdapterPlan(indices.view(batch, self.tokens // batch)[:, keep], self.adapters)
+
 
 def _copies(k, step, odd):
     """Whether the kernels copy rows of k columns `step` elements apart first: not whole ones, or 16
@@ -178,10 +185,19 @@ class LowRankAdapters(nn.Module):
 
 class Requests:
     """What the adapted projections of a transformer share: the plan of the batch that goes
-    through it, or None for none of their adapters."""
+    through it, or None for none of their adapters. Blocks that Flash runs on selected rows
+    have the plan of those rows meanwhile (flash.configure_flash)."""
 
     def __init__(self, plan=None):
         self.plan = plan
+
+
+def requests_of(modules):
+    """The Requests of the adapted projections in some modules, each once."""
+    if not AdaptedLinear.any_made:
+        return []
+    found = (m.requests for module in modules for m in module.modules() if isinstance(m, AdaptedLinear))
+    return list({id(requests): requests for requests in found}.values())
 
 
 _global_hooks = nn.modules.module._global_forward_hooks
@@ -201,6 +217,12 @@ class AdaptedLinear(nn.Module):
     adapters, which see the input itself: fused blocks pass it to this layer unquantized.
     The products are added in the memory of the layer's result where nothing else can hold
     it (an Int8Linear, Mxfp4Linear or nn.Linear without forward hooks), else in new memory."""
+
+    any_made = False   # in this process, also by copy or unpickling
+
+    def __new__(cls, *args, **kwargs):
+        AdaptedLinear.any_made = True
+        return super().__new__(cls)
 
     def __init__(self, layer, adapters, requests):
         super().__init__()

@@ -27,6 +27,7 @@ import math
 import torch
 
 from . import _lib
+from .adapters import requests_of
 
 VIDEO_TAG = 0
 
@@ -160,15 +161,17 @@ def _compressed_span(blocks, config):
 class _FlashForward:
     """Hook state of one Flash transformer: the layout of the current forward
     (cached across forwards with equal positions and tags) and, between the
-    first compressed block and the restore, the full-resolution hidden rows
-    and the compressed rows that entered the compressed span."""
+    first compressed block and the restore, the full-resolution hidden rows,
+    the compressed rows that entered the compressed span, and the plans of
+    all rows that its adapted projections have otherwise."""
 
-    def __init__(self, transformer, gain):
+    def __init__(self, transformer, span, gain):
         self.signature = inspect.signature(transformer.forward)
-        self.gain = gain
+        self.span, self.gain = span, gain
         self.layout = None          # (positions, tags, keep, inverse) of the last layout built
         self.current = None         # (keep, inverse) while a forward runs
         self.full = self.entered = None
+        self.plans = []             # (requests, plan of all rows)
 
     def begin(self, module, args, kwargs):
         if module.training or torch.is_grad_enabled():
@@ -188,17 +191,34 @@ class _FlashForward:
         if self.full is None:           # the first compressed block: drop rows once
             self.full, hidden = hidden, gather_rows(hidden, keep, 1)
             self.entered = hidden
+            self.select_plans(*self.full.shape[:2])
         return (hidden, temb, gather_rows(indices, keep, 0),
                 tuple(gather_rows(value, keep, -2) for value in rotary),
                 None if mask is None else gather_rows(mask, keep, -1))
 
+    def select_plans(self, batch, tokens):
+        """Plans of all rows become plans of the kept ones; those of other rows (of the kept
+        ones already) are their owner's matter."""
+        for requests in requests_of(self.span):
+            plan = requests.plan
+            if plan is not None and plan.tokens == batch * tokens:
+                self.plans.append((requests, plan))
+                requests.plan = plan.rows(self.current[0], batch)
+
+    def restore_plans(self):
+        for requests, plan in self.plans:
+            requests.plan = plan
+        self.plans = []
+
     def restore(self, module, args):
         hidden = restore(self.full, args[0], self.entered, self.current[1], self.gain)
         self.full = self.entered = None
+        self.restore_plans()
         return (hidden, *args[1:])
 
     def finish(self, *_):
         self.current = self.full = self.entered = None
+        self.restore_plans()
 
 
 def configure_flash(transformer, config):
@@ -208,14 +228,16 @@ def configure_flash(transformer, config):
     restored full sequence. The block pre-hook arguments are (hidden, temb,
     adaLN indices, rotary (cos, sin), attention mask), as in the reference;
     hidden/indices/rotary/mask are gathered on their token dimension (1, 0,
-    -2, -1). One forward runs at a time.
+    -2, -1). The adapters of the middle blocks (adapters.adapt_transformer, before
+    or after) follow the kept rows: a plan of all rows gives way to one of those
+    until the restore. One forward runs at a time.
     """
     blocks = transformer.transformer_blocks
     start, end, gain = _compressed_span(blocks, config)
     if hasattr(transformer, "_lynnreal_flash_hooks"):
         raise ValueError("Flash is already configured")
     transformer.h3_token_compression = None
-    run = _FlashForward(transformer, gain)
+    run = _FlashForward(transformer, blocks[start:end], gain)
     handles = [transformer.register_forward_pre_hook(run.begin, with_kwargs=True)]
     handles += [block.register_forward_pre_hook(run.compress) for block in blocks[start:end]]
     handles += [blocks[end].register_forward_pre_hook(run.restore),

@@ -437,7 +437,7 @@ int lr_attention_weights(const void* q, const void* k, const float* lse, const f
  *   stay as they were where not.
  * weights fp32 [sequences, kv_heads, size]. strides, twelve, in bytes, multiples of 16: from
  * one key, head and sequence of k to the next, then of v, k_out and v_out; a row has
- * row_bytes, a multiple of 16. The outputs must not overlap the inputs. workspace: 16-byte
+ * row_bytes, a multiple of 16. The outputs must not overlap the inputs, nor each other. workspace: 16-byte
  * aligned, of the bytes that lr_cache_evict_workspace gives (0: it may be NULL). */
 int lr_cache_evict_workspace(int64_t sequences, int64_t size, int kv_heads, int64_t* bytes);
 int lr_cache_evict(const void* k, const void* v, const float* weights, const int32_t* key_lengths, void* k_out,

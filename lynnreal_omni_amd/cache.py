@@ -113,16 +113,81 @@ def accumulate_weights(weights, query, key, lse, *, causal=False, scale=None, ke
 
 
 def _span(t):
-    """First and last byte (exclusive) of what a tensor's elements lie in."""
-    first = t.data_ptr()
-    return first, first + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+    """First and last byte (exclusive) of what a tensor's elements lie in; nothing where it has none."""
+    first, size = t.data_ptr(), t.element_size()
+    if t.is_contiguous():
+        return first, first + t.numel() * size
+    shape = t.shape
+    return first, first if 0 in shape else first + (sum([(n - 1) * st for n, st in zip(shape, t.stride())]) + 1) * size
 
 
 def _overlap(a, b):
-    if a.numel() == 0 or b.numel() == 0:
+    """Whether a and b have memory in common: rows between each other's are apart."""
+    return _clash((a,), (b,))
+
+
+def _clash(written, read):
+    """Whether one of the tensors in `written` has memory in common with another of them or with one
+    in `read` (None is skipped)."""
+    spans = [(t, *_span(t)) for t in written]
+    for i, (a, a0, a1) in enumerate(spans):
+        for b, b0, b1 in spans[:i]:
+            if a0 < b1 and b0 < a1 and _share(_layout(a), _layout(b), b0 - a0):
+                return True
+    for b in read:
+        if b is not None:
+            b0, b1 = _span(b)
+            for a, a0, a1 in spans:
+                if a0 < b1 and b0 < a1 and _share(_layout(a), _layout(b), b0 - a0):
+                    return True
+    return False
+
+
+def _layout(t):
+    return t.shape, t.stride(), t.element_size()
+
+
+@functools.lru_cache(maxsize=4096)
+def _share(a, b, apart):
+    return _meet(_runs(*a), _runs(*b), apart, [10000])
+
+
+def _runs(shape, stride, size):
+    """A tensor's memory as (bytes between, number of) runs from the outermost on, the last one
+    of single bytes."""
+    runs = [(1, size)]
+    for st, n in sorted((st * size, n) for st, n in zip(stride, shape) if n > 1 and st > 0):
+        step, count = runs[-1]
+        if st == step * count:
+            runs[-1] = (step, count * n)   # behind each other
+        else:
+            runs.append((st, n))
+    return tuple(reversed(runs))
+
+
+def _meet(a, b, apart, budget):
+    """Whether runs a and b, which begin `apart` bytes behind a's, have a byte in common. Exact,
+    but for strides so unlike each other that the budget of steps ends: those are taken to have."""
+    reach_a, reach_b = (sum((n - 1) * st for st, n in runs) + 1 for runs in (a, b))
+    if apart >= reach_a or -apart >= reach_b:
         return False
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+    if len(a) == 1 and len(b) == 1:
+        return True
+    budget[0] -= 1
+    if budget[0] < 0:
+        return True
+    if a[0][0] < b[0][0]:
+        a, b, reach_a, reach_b, apart = b, a, reach_b, reach_a, -apart
+    (step, n), inner = a[0], a[1:]
+    reach = reach_a - (n - 1) * step
+    if b[0][0] == step:
+        # Only how many steps a's run lies before b's matters.
+        others, reach_b, low = b[1:], reach_b - (b[0][1] - 1) * step, 1 - b[0][1]
+    else:
+        others, low = b, 0
+    # The run i of a begins i steps behind its first and has to reach others, from `apart` to there + reach_b.
+    first, last = max(low, -((reach - apart - 1) // step)), min(n - 1, (apart + reach_b - 1) // step)
+    return any(_meet(inner, others, apart - i * step, budget) for i in range(first, last + 1))
 
 
 def _distinct(t):
@@ -161,9 +226,10 @@ def evict(key, value, weights, key_lengths, budget, *, recent=0, out=None):
     weights [batch, kv_heads, budget], 0 behind; lengths int32 [batch]; and kept int32
     [batch, kv_heads, budget], the places that the keys had, -1 behind the last.
 
-    out = (key, value, weights): caches of any number of places from `budget` on, on
-    whose memory the inputs do not lie, written instead of new ones; rows of theirs
-    behind the last key stay as they were, weights there become 0.
+    out = (key, value, weights): caches of any number of places from `budget` on, of
+    memory that neither the inputs nor another of them have (rows between each other's are
+    fine), written instead of new ones; rows of theirs behind the last key stay as they
+    were, weights there become 0.
     """
     if key.dim() != 4 or value.shape != key.shape or value.dtype != key.dtype:
         raise ValueError("key and value must be [batch, keys, kv_heads, head_dim], of one shape and dtype")
@@ -183,7 +249,7 @@ def evict(key, value, weights, key_lengths, budget, *, recent=0, out=None):
         key_lengths = _attention._lengths(key_lengths, batch, keys)
     if out is not None:
         key_out, value_out, weights_out = out
-        _check_out(key, value, weights, key_out, value_out, weights_out, budget)
+        _check_out(key, value, weights, key_lengths, key_out, value_out, weights_out, budget)
     _lib.check_device(key)
     _lib.same_device(key, value=value, weights=weights, key_lengths=key_lengths)
     if out is None:
@@ -218,7 +284,7 @@ def _evict_workspace(batch, keys, kv_heads):
     return nbytes[0]
 
 
-def _check_out(key, value, weights, key_out, value_out, weights_out, budget):
+def _check_out(key, value, weights, key_lengths, key_out, value_out, weights_out, budget):
     batch, _, kv_heads, dim = key.shape
     if (key_out.dim() != 4 or key_out.shape[1] < budget or key_out.shape != (batch, key_out.shape[1], kv_heads, dim)
             or value_out.shape != key_out.shape or key_out.dtype != key.dtype or value_out.dtype != key.dtype):
@@ -230,7 +296,5 @@ def _check_out(key, value, weights, key_out, value_out, weights_out, budget):
             t.data_ptr() & 15 or not _attention._dense(t.stride(), t.shape) or not _distinct(t)
             for t in (key_out, value_out)):
         raise ValueError("out must be caches whose rows are dense, 16-byte aligned and distinct, and contiguous weights")
-    if any(_overlap(a, b) for a in (key_out, value_out, weights_out) for b in (key, value, weights)):
-        raise ValueError("out must not overlap the caches that are cut down")
-    if key_out.numel() and key_out.data_ptr() == value_out.data_ptr():
-        raise ValueError("out's keys and values must be different memory")
+    if _clash((key_out, value_out, weights_out), (key, value, weights, key_lengths)):
+        raise ValueError("out's keys, values and weights must not overlap each other, nor the caches that are cut down")

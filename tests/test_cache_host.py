@@ -1,4 +1,6 @@
 """What the operators of bounded caches refuse, on the CPU."""
+import itertools
+import random
 import struct
 from array import array
 
@@ -105,6 +107,65 @@ def test_eviction_into_given_caches():
     for good in (new(), [both[:, :, 0], both[:, :, 1], torch.zeros(2, 2, 4)]):
         with pytest.raises(ValueError, match="GPU"):
             cache.evict(key, value, weights, None, 3, out=good)
+
+
+def test_outputs_of_an_eviction_are_memory_of_their_own():
+    """Of each other's, of the inputs', and of nothing that only lies between their rows."""
+    key, value, weights, _ = caches()
+    buffer = torch.zeros(2 * 40 * 2 * 64, dtype=BF16)
+    rows = buffer.view(2, 40, 2, 64)
+    other = lambda: torch.zeros(2, 4, 2, 64, dtype=BF16)  # noqa: E731
+    sums = lambda: torch.zeros(2, 2, 4)  # noqa: E731
+    shared = torch.zeros(4096, dtype=torch.int32)
+    as_floats, as_rows = shared[:16].view(torch.float32).view(2, 2, 4), shared[:512].view(BF16).view(2, 4, 2, 64)
+    for bad in ([rows[:, :4], rows[:, 3:7], sums()], [rows[:, 3:7], rows[:, :4], sums()], [rows[:, :4], rows[:, 1:5], sums()],
+                [rows[:, 0:8:2], rows[:, 2:10:2], sums()], [rows[:, 0:8:2], rows[:, 0:4], sums()],
+                # Keys and values with their tokens and heads the other way round, in one place.
+                [buffer[:1024].view(2, 4, 2, 64), buffer[:1024].view(2, 2, 4, 64).transpose(1, 2), sums()],
+                [as_rows, other(), as_floats], [other(), as_rows, as_floats]):
+        with pytest.raises(ValueError, match="out"):
+            cache.evict(key, value, weights, None, 3, out=bad)
+    lengths = torch.zeros(18, dtype=torch.int32)
+    with pytest.raises(ValueError, match="out"):
+        cache.evict(key, value, weights, lengths[15:17], 3, out=[other(), other(), lengths[:16].view(torch.float32).view(2, 2, 4)])
+    inside = rows[:, 5:10], rows[:, 20:25]
+    for bad in ([rows[:, 9:13], other(), sums()], [other(), rows[:, 17:21], sums()]):
+        with pytest.raises(ValueError, match="out"):
+            cache.evict(*inside, weights, None, 3, out=bad)
+    # Rows between each other's, and between those of the inputs.
+    halves = torch.zeros(2, 16 * 64, dtype=BF16)
+    heads_outside = halves[:, 8 * 64:].view(2, 2, 4, 64).transpose(1, 2)
+    for good in ([rows[:, 10:18:2], rows[:, 11:19:2], sums()], [rows[:, 10:14], rows[:, 25:29], sums()], [rows[:, 30:34], rows[:, 34:38], sums()],
+                 [halves[:, :8 * 64].view(2, 4, 2, 64), heads_outside, sums()]):
+        with pytest.raises(ValueError, match="GPU"):
+            cache.evict(*inside, weights, None, 3, out=good)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_overlap(seed):
+    """Whether two strided tensors share memory, against the sets of their bytes."""
+    g = random.Random(seed)
+    memory = torch.zeros(600, dtype=torch.int16)
+
+    def some():
+        dtype = g.choice([torch.int16, torch.float32])
+        base = memory.view(dtype)
+        if g.random() < 0.5:   # a slice with its dimensions in any order
+            shape = [g.randint(1, 5) for _ in range(3)]
+            at = g.randint(0, 20)
+            t = base[at:at + shape[0] * shape[1] * shape[2]].view(shape).permute(*g.sample(range(3), 3))
+            return t[::g.randint(1, 3), g.randint(0, t.shape[1] - 1):]
+        shape, stride = [g.randint(0, 4) for _ in range(3)], [g.randint(0, 30) for _ in range(3)]
+        return base.as_strided(shape, stride, g.randint(0, 20))
+
+    def places(t):
+        first, size = (t.data_ptr() - memory.data_ptr()), t.element_size()
+        return {first + size * sum(i * st for i, st in zip(at, t.stride())) + b
+                for at in itertools.product(*(range(n) for n in t.shape)) for b in range(size)}
+
+    for _ in range(20):
+        a, b = some(), some()
+        assert cache._overlap(a, b) == bool(places(a) & places(b)), (a.shape, a.stride(), b.shape, b.stride())
 
 
 def test_entry_point_refusals_without_a_gpu():

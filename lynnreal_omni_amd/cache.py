@@ -90,7 +90,7 @@ def accumulate_weights(weights, query, key, lse, *, causal=False, scale=None, ke
         _check_weights(out, key, "out")
         _no_gradients(out)
         same = out.data_ptr() == weights.data_ptr() and weights.is_contiguous()
-        if not out.is_contiguous() or _overlap(out, lse) or (not same and _overlap(out, weights)):
+        if not out.is_contiguous() or _clash((out,), (None if same else weights, query, key, lse, key_lengths)):
             raise ValueError("out must be contiguous, and weights themselves or memory of its own")
     scale = _attention._scale_bits(float(dim ** -0.5 if scale is None else scale))
     _lib.check_device(query)
@@ -134,12 +134,14 @@ def _clash(written, read):
         for b, b0, b1 in spans[:i]:
             if a0 < b1 and b0 < a1 and _share(_layout(a), _layout(b), b0 - a0):
                 return True
+    last = max([a1 for _, _, a1 in spans])
     for b in read:
-        if b is not None:
-            b0, b1 = _span(b)
-            for a, a0, a1 in spans:
-                if a0 < b1 and b0 < a1 and _share(_layout(a), _layout(b), b0 - a0):
-                    return True
+        if b is None or b.data_ptr() >= last:   # behind them all, as half of what is looked at
+            continue
+        b0, b1 = _span(b)
+        for a, a0, a1 in spans:
+            if a0 < b1 and b0 < a1 and _share(_layout(a), _layout(b), b0 - a0):
+                return True
     return False
 
 

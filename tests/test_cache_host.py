@@ -109,6 +109,22 @@ def test_eviction_into_given_caches():
             cache.evict(key, value, weights, None, 3, out=good)
 
 
+def test_weights_out_is_apart_from_all_that_is_read():
+    memory = torch.zeros(4096, dtype=torch.int32)
+    out = memory[8:28].view(torch.float32).view(2, 2, 5)
+    _, q, k, lse = weigh()
+    w = torch.zeros(2, 2, 5)
+    halves = memory.view(BF16)
+    for bad in (dict(query=halves[:q.numel()].view(q.shape)), dict(key=halves[48:48 + k.numel()].view(k.shape)),
+                dict(lse=memory[:24].view(torch.float32).view(2, 3, 4)), dict(key_lengths=memory[27:29])):
+        with pytest.raises(ValueError, match="out must"):
+            cache.accumulate_weights(**{**dict(weights=w, query=q, key=k, lse=lse, out=out), **bad})
+    # Behind and before them; lengths of 64 bits, which are copied first.
+    for lengths in (memory[6:8], memory[26:30].view(torch.int64)):
+        with pytest.raises(ValueError, match="GPU"):
+            cache.accumulate_weights(w, halves[56:56 + q.numel()].view(q.shape), k, lse, out=out, key_lengths=lengths)
+
+
 def test_outputs_of_an_eviction_are_memory_of_their_own():
     """Of each other's, of the inputs', and of nothing that only lies between their rows."""
     key, value, weights, _ = caches()

@@ -453,7 +453,7 @@ int lr_cache_evict(const void* k, const void* v, const float* weights, const int
  * place in order, tokens, and the first tile of a pair or -1: a list of its own), 16-byte
  * aligned. At most 1000 adapters, 2^24 - 1 tokens.
  * lr_adapter_add: x [tokens, k], base and out [tokens, n] (rows x_stride, .. elements
- * apart; out may be base, and may not overlap x or base otherwise), down [adapters, rank, k8] and up [adapters, n,
+ * apart; out may be base, and may not overlap x, base otherwise, or any other input), down [adapters, rank, k8] and up [adapters, n,
  * rank8], all of one 16-bit type, k8 and rank8 being k and rank rounded up to multiples of 8; what
  * lies behind k in the rows of down, and behind rank in those of up, must be 0. scale fp32
  * [adapters]. rank at most 128. Sums are fp32 in a fixed order, rounded once. workspace:

@@ -23,7 +23,7 @@ from torch import nn
 
 from . import _lib
 from .attention import _DTYPES
-from .cache import _overlap
+from .cache import _clash
 from .int8 import Int8Linear
 from .mxfp4 import Mxfp4Linear
 
@@ -154,7 +154,7 @@ class LowRankAdapters(nn.Module):
             if out.shape != base.shape or out.dtype != base.dtype or not out.is_contiguous():
                 raise ValueError("out must be contiguous, like base")
             same = out.data_ptr() == base.data_ptr() and base.is_contiguous()
-            if _overlap(out, x) or (not same and _overlap(out, base)):
+            if _clash((out,), (None if same else base, x)):   # (adapters and plan: by the call)
                 raise ValueError("out must be base itself or memory of its own")
         _lib.check_device(x)
         _lib.same_device(x, base=base, down=down, plan=plan.order, out=out)

@@ -857,6 +857,15 @@ extern "C" int lr_adapter_add(const void* x, int64_t x_stride, const void* down,
   const int64_t k8 = (k + 7) & ~7LL;
   LR_REQUIRE(x_stride >= 0 && base_stride >= 0 && (out_stride >= n || tokens == 1),
              "adapter_add: rows of %lld columns %lld apart", (long long)n, (long long)out_stride);
+  // What is read by all of the tokens may not change under them.
+  auto apart = [&](const void* p, int64_t bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), o = reinterpret_cast<uintptr_t>(out);
+    return a + bytes <= o || o + ((tokens - 1) * out_stride + n) * 2 <= a;
+  };
+  const int64_t rank8 = (rank + 7) & ~7;
+  LR_REQUIRE(apart(down, adapters * rank * k8 * 2) && apart(up, adapters * n * rank8 * 2) && apart(scale, adapters * 4) &&
+                 apart(order, tokens * 4) && apart(tiles, plan_tiles(tokens, adapters) * 16),
+             "adapter_add: out must not overlap the adapters or the plan");
   const bool copies = copied(x, x_stride, k);
   const AddPlan pl = add_plan(tokens, n, k, rank, adapters);
   const int64_t runs = (n + pl.columns - 1) / pl.columns;
@@ -885,7 +894,7 @@ extern "C" int lr_adapter_add(const void* x, int64_t x_stride, const void* down,
   p.max_tiles = (int)pl.tiles;
   p.max_pairs = (int)pl.pairs;
   p.k8 = (int)k8;
-  p.rank8 = (rank + 7) & ~7;
+  p.rank8 = (int)rank8;
   p.splits = pl.splits;
   p.columns = pl.columns;
   const bool vector = n % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned(base, 16) && aligned(out, 16);

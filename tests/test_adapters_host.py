@@ -220,3 +220,20 @@ def test_entry_point_refusals_without_a_gpu():
                 dict(x=p + 8, wsb=plain), dict(k=23, wsb=plain), dict(os=39), dict(bs=-8), dict(dtype=2), dict(tokens=-1),
                 dict(tokens=1 << 24), dict(n=0), dict(n=1 << 24), dict(k=(1 << 23) + 8), dict(rank=0)]:
         assert call(**bad) == _lib.LR_EINVAL, bad
+
+
+def test_entry_point_refuses_outputs_over_its_inputs():
+    lib = _lib.load()
+    at = lambda i, by=0: (i + 1 << 20) + by  # noqa: E731
+    sizes = dict(down=3 * 4 * 24 * 2, up=3 * 40 * 8 * 2, scale=3 * 4, order=5 * 4, tiles=lib.lr_adapter_tiles(5, 3) * 16)
+    good = dict(x=at(0), xs=24, down=at(1), up=at(2), scale=at(3), base=at(6), bs=40, out=at(7), os=40, dtype=0, tokens=5, n=40,
+                k=24, rank=4, adapters=3, order=at(4), tiles=at(5), ws=None, wsb=0, stream=None)
+    call = lambda **kw: lib.lr_adapter_add(*{**good, **kw}.values())  # noqa: E731
+    error = lambda: lib.lr_last_error().decode()  # noqa: E731
+    for name, size in sizes.items():
+        first = good[name]
+        for out in (first, first - 5 * 40 * 2 + 2, first + size - 2):
+            assert call(out=out) == _lib.LR_EINVAL and "overlap" in error(), (name, out)
+        # Behind and before it the call gets as far as the workspace, which is missing.
+        for out in (first - 5 * 40 * 2, first + size):
+            assert call(out=out) == _lib.LR_EINVAL and "workspace" in error(), (name, out)

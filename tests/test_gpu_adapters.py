@@ -304,3 +304,18 @@ def test_no_tokens():
     got = L.LowRankAdapters(*weights)(torch.zeros(0, 8, dtype=torch.bfloat16, device="cuda"),
                                       torch.zeros(0, 16, dtype=torch.bfloat16, device="cuda"), L.AdapterPlan(empty, 2))
     assert got.shape == (0, 16)
+
+
+@pytest.mark.parametrize("name", ["down", "up", "scale", "order", "tiles"])
+def test_out_is_apart_from_adapters_and_plan(name):
+    layer = L.LowRankAdapters(*make(2, 4, 16, 8, torch.bfloat16, 0))
+    x, base = rows(60, 16, 8, torch.bfloat16, 1)
+    plan = L.AdapterPlan(torch.zeros(60, dtype=torch.int32, device="cuda"), 2)
+    owner = plan if hasattr(plan, name) else layer
+    want, read = layer(x, base, plan), getattr(owner, name)
+    memory = torch.zeros(8192, dtype=torch.uint8, device="cuda")
+    setattr(owner, name, memory[:read.nbytes].view(read.dtype).view(read.shape).copy_(read))
+    with pytest.raises(ValueError, match="out must"):
+        layer(x, base, plan, out=memory[:base.nbytes].view(torch.bfloat16).view(60, 16))
+    out = memory[-base.nbytes:].view(torch.bfloat16).view(60, 16)
+    assert torch.equal(layer(x, base, plan, out=out), want)

@@ -756,9 +756,12 @@ AddPlan add_plan(int64_t tokens, int64_t n, int64_t k, int rank, int64_t adapter
   // 45 KB/us for each CU and six of them to fill the ring, against a launch to add the shares
   // and their way through memory.
   const int per_cu = pl.rank == 32 ? 3 : (pl.rank == 64 ? 2 : 1);
-  // Pairs of tiles where an adapter has many and the CUs have 94 steps and more (4 adapters of
-  // 12605 tokens: level at 5376 columns, 52 us; 24 us without and 27 so for 16 of 4096, 2048).
-  pl.pair = pl.rank == 128 && tokens >= 16 * kTokens * adapters && pl.tiles * steps >= 94 * cus;
+  // Pairs of tiles where an adapter has seven and more on average, and each CU 30 steps and more.
+  // With 640 outputs, a tile at a time and so: 12605 tokens of 4 adapters, 2048 columns (25 steps
+  // per CU) 43 and 48 us, 5376 (66) 68 and 65, 7168 (88) 82 and 77, 14336 (176) 142 and 121; 4096 of
+  // 4, 5376 (23) level, 7168 (30) 38 and 37, 14336 (60) 53 and 47; 3683 of 8, 7 tiles each, 7168
+  // (29) 38 and 37, 20480 (82) 75 and 61; 4096 of 16, 4 tiles each, 10240 (51) 45 and 46, 20480 (101) level.
+  pl.pair = pl.rank == 128 && tokens >= 7 * kTokens * adapters && pl.tiles * steps >= 30 * cus;
   pl.pairs = tokens / (2 * kTokens) + (adapters < tokens ? adapters : tokens);
   const int64_t tiles = pl.pair ? pl.pairs : pl.tiles;
   const double step = per_cu * ((pl.pair ? 2 : 1) * kTokens + pl.rank) * 2.0 * kStep / 45e3;

@@ -100,6 +100,21 @@ def test_pairs_of_tiles(sizes, rank, k, dtype):
     run([indices[i] for i in order], at, rank, 40, k, dtype, rank)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,rank,k", [
+    ((3000, 1090), 128, 8008), ((64, 1, 1500, 63, 65, 128, 129, -7, 1900), 70, 12000), ((2049, -2051), 127, 8000),
+    ((900,), 128, 33000)])
+def test_pairs_of_fewer_tiles(sizes, rank, k, dtype):
+    """Around the fewest tokens and steps that are taken in pairs of tiles: shares of k, and adapters of one
+    tile, of a tile and a token, and of none."""
+    indices, at = [], 0
+    for n in sizes:
+        indices += [at if n > 0 else -1] * abs(n)
+        at += n > 0
+    order = torch.randperm(len(indices), generator=torch.Generator().manual_seed(rank)).tolist()
+    run([indices[i] for i in order], at, rank, 40, k, dtype, rank)
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_plans(seed):
     """A plan lists every token once, in tiles of one adapter, in order."""

@@ -94,10 +94,12 @@ def _workspace(device, tokens, n, k, rank, adapters, step, odd):
 class LowRankAdapters(nn.Module):
     """The adapters of a projection from in_features to out_features: down [adapters, rank,
     in_features], up [adapters, out_features, rank], bf16 or fp16, and scale, a number or
-    [adapters]. Adapters of lower rank than the others have zeros in down behind theirs.
+    [adapters]. Adapters of lower rank than the others have zeros in down behind theirs. How a
+    call is laid over the GPU follows from the number of adapters held, not of those in use.
 
     Buffers: `down` and `up` with their rows filled up with zeros to multiples of 8, and
-    `scale` float32 [adapters].
+    `scale` float32 [adapters]. Calls after a move to another type (model.to(torch.bfloat16), which
+    takes scale along) are refused: make the adapters of the type they are to have, last.
     """
 
     def __init__(self, down, up, scale=1.0):

@@ -16,6 +16,11 @@ x query heads of a key head) they keep the rest of that rounding as a second num
 so that the output's own rounding is all that remains. attention_packed rounds them
 once whatever its number of tokens, so that a sequence gives the same bits whatever
 lies around it: the same token may differ by the weights' rounding between the two.
+In attention_shared_prefix a sequence's rows over its own keys keep the rest where they are
+at most 32, and the rows of all sequences together over the prefix where they are at most 32, or where
+the keys are so few that a sequence's rows take them all in one kernel. With more rows the weights
+are rounded once: a token's last bits depend on how many others share its prefix (bf16
+outputs are off by 2.3e-3 of their size then, 1.66e-3 else).
 
 Tensors whose last dimension is dense, whose other strides are multiples of 8 elements
 (those between tokens below 2^23) and whose memory is 16-byte aligned are read as

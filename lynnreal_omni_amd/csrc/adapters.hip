@@ -59,7 +59,7 @@ constexpr int kPlan = 1024;   // threads
 
 // A counting sort by one workgroup: every wave counts its stretch of the tokens, then puts
 // them in their places in order. Tokens without an adapter (an index outside 0 .. adapters - 1)
-// come last, as those of adapter -1. Latency bounds it, once per batch: 4 us for one token, 24 for 12605.
+// come last, as those of adapter -1. Latency bounds it, once per batch: 4 us for one token, 25 for 12605.
 __global__ __launch_bounds__(kPlan) void plan_adapters(const int32_t* index, int tokens, int adapters, int32_t* order,
                                                        int4* tiles, int max_tiles) {
   constexpr int WAVES = kPlan / 64;
@@ -564,7 +564,7 @@ __global__ __launch_bounds__(256, VECTOR && RP < 128 ? (RP == 32 ? 3 : 2) : 1) v
 // Four waves: 32 tokens x 64 columns each of a step of 128 columns. up's rows come through
 // LDS like the keys of lr_attention.h (a row holds RP numbers); the sums leave through LDS
 // too, so that base and out are read and written in whole lines. VECTOR: 16 bytes at a time.
-// (3683 tokens, 28672 columns at rank 64: 94 us, 5 TB/s.)
+// (3683 tokens, 28672 columns at rank 64: 93-97 us, 4.6 TB/s.)
 template <typename T, int RP, bool VECTOR>
 __global__ __launch_bounds__(256) void expand(AdapterArgs p) {
   typedef typename Mfma<T>::V V8;

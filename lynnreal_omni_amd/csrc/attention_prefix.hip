@@ -10,12 +10,19 @@
 // sequences, 128 of them per workgroup, cut into pieces over the GPU; so are the own
 // caches, each for its own rows; a second kernel joins a row's pieces in order.
 // What that reads is the floor: the prefix once, not once per sequence (one token of 16
-// sequences behind 131072 keys, 56 heads over 8: 142 us, 4.7 TB/s in the first kernel, 7 in the second).
+// sequences behind 131072 keys, 56 heads over 8: 144 us, 4.5 TB/s in the first kernel, 7.5 in the second).
 //
 // Many rows per sequence: a workgroup's 128 rows walk the prefix and then the own cache
 // in one pass. The prefix comes out of the caches, since the matrix units, not the keys, are
-// what bounds it (878 tokens of four sequences behind 12605, 56 heads: 1.3 ms, 1.05 PFLOP/s).
+// what bounds it (878 tokens of four sequences behind 12605, 56 heads: 1.3 ms, 1.04 PFLOP/s).
 // Few rows are walked too where there are few keys, for a kernel less.
+//
+// The softmax weights are rounded to the inputs' type for the product with v. At most 32 rows of a
+// piece keep the rest of that rounding as a second number, so that the output's own rounding is all
+// that is left. Other walks and pieces of more rows do without: their outputs' error against 64 bits is 1.40 times
+// as large (bf16: 2.3e-3 of their size, of which rounding the output alone is 1.66e-3). The second number
+// in those pieces too was measured: one token of 32 sequences behind 12605, 43 -> 47 us; of 16 behind
+// 131072, 56 heads over 8, 143 -> 164; of 48, 40 heads over 8, 247 -> 295; 4 tokens of 16 behind 12605, 52 -> 67.
 #include "lr_attention.h"
 #include "lr_pieces.h"
 #include "lr_runtime.h"

@@ -9,7 +9,7 @@
 // each added to its own fp32 sum; the sums over the 32 lanes come once at the end. Every
 // key is read once, and the order of additions does not depend on timing. With few rows the keys'
 // stream bounds it; with many the exponentials and the matrix instructions do (a prompt of 3683
-// tokens, 40 heads over 8: 115 us causal, 169 where every row sees every key).
+// tokens, 40 heads over 8: 105 us causal, 157 where every row sees every key).
 //
 // Eviction reads the weights, finds for every cache and head the keys that stay, and moves
 // their rows to another cache, in their order.
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(kDealt) void join_shares(WeighArgs p) {
 // over all caches (lr_pieces.h); a wave has 32 keys of each 128 of them, through 32 rows of
 // LDS of its own, and the queries in registers, so that no wave waits for another. The next
 // keys are on their way while these are worked on.
-// (Eight caches of 16152 keys in all, places for 65536, 40 heads over 8: 10.7 us; 17.2 with a
+// (Eight caches of 16152 keys in all, places for 65536, 40 heads over 8: 11-12 us; 17.2 with a
 // workgroup for every 128 places of every cache. One of 131072 keys: 45 us, 6 TB/s, part of it out of the caches.)
 constexpr int kCopied = 1024;   // places behind the caches' keys that a workgroup copies at a time
 

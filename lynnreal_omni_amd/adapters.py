@@ -207,10 +207,13 @@ _global_hooks = nn.modules.module._global_forward_hooks
 
 def _gives_new_memory(layer):
     """Whether what a call of the layer returns is memory that nothing else holds: a layer whose
-    forward is known, with no hook that could keep the result or put its own in its place."""
-    own = layer.__dict__
-    return (type(layer) in (Int8Linear, Mxfp4Linear, nn.Linear) and not own["_forward_hooks"] and not _global_hooks
-            and "forward" not in own and "forward_quantized" not in own)
+    forward is known, with no hook or replaced function that could keep the result or put its own
+    in its place."""
+    if type(layer) not in (Int8Linear, Mxfp4Linear, nn.Linear):
+        return False
+    if layer._forward_hooks or _global_hooks or "forward" in layer.__dict__:
+        return False
+    return type(layer) is not Int8Linear or layer._fused_call() is not None
 
 
 class AdaptedLinear(nn.Module):

@@ -5,7 +5,7 @@ import pytest
 import torch
 from torch import nn
 
-from lynnreal_omni_amd import _lib, adapters as L
+from lynnreal_omni_amd import _lib, adapters as L, int8
 
 BF16 = torch.bfloat16
 
@@ -190,6 +190,22 @@ def test_layers_that_keep_their_result():
     layer, kept = nn.Linear(24, 40, dtype=BF16), torch.zeros(5, 40, dtype=BF16)
     layer.forward = lambda value: kept
     assert torch.equal(adapted(layer)[0](x), torch.ones(5, 40, dtype=BF16)) and not kept.any()
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("wrapped", ["int8_matmul", "forward_quantized", "class"])
+def test_products_of_replaced_functions_stay(wrapped, monkeypatch):
+    """What a caller's own int8_matmul or forward_quantized has returned may be the caller's to keep."""
+    x, kept = torch.randn(5, 24, dtype=BF16), torch.zeros(5, 40, dtype=BF16)
+    layer = int8.Int8Linear(nn.Linear(24, 40, dtype=BF16), "hip")
+    if wrapped == "int8_matmul":
+        monkeypatch.setattr(int8.int8_gemm, "int8_matmul", lambda *args, **kwargs: kept)
+    elif wrapped == "class":
+        monkeypatch.setattr(int8.Int8Linear, "forward_quantized", lambda self, *args: kept)
+    else:
+        layer.forward_quantized = lambda *args: kept
+    model, beside = adapted(layer)
+    assert torch.equal(model(x), torch.ones(5, 40, dtype=BF16)) and not kept.any() and beside.out is None
 
 
 def test_entry_point_refusals_without_a_gpu():

@@ -121,14 +121,9 @@ def _span(t):
     return first, first if 0 in shape else first + (sum([(n - 1) * st for n, st in zip(shape, t.stride())]) + 1) * size
 
 
-def _overlap(a, b):
-    """Whether a and b have memory in common: rows between each other's are apart."""
-    return _clash((a,), (b,))
-
-
 def _clash(written, read):
     """Whether one of the tensors in `written` has memory in common with another of them or with one
-    in `read` (None is skipped)."""
+    in `read` (None is skipped). Rows between each other's are apart."""
     spans = [(t, *_span(t)) for t in written]
     for i, (a, a0, a1) in enumerate(spans):
         for b, b0, b1 in spans[:i]:

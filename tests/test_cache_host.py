@@ -181,7 +181,7 @@ def test_overlap(seed):
 
     for _ in range(20):
         a, b = some(), some()
-        assert cache._overlap(a, b) == bool(places(a) & places(b)), (a.shape, a.stride(), b.shape, b.stride())
+        assert cache._clash((a,), (b,)) == bool(places(a) & places(b)), (a.shape, a.stride(), b.shape, b.stride())
 
 
 def test_entry_point_refusals_without_a_gpu():
